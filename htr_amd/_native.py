@@ -14,6 +14,7 @@ _CSRC = os.path.join(os.path.dirname(os.path.abspath(__file__)), "csrc")
 LIB_PATH = os.environ.get("HTR_GFX950_LIB") or os.path.join(_CSRC, "libhtr_gfx950.so")
 
 BF16, F16, F32 = 0, 1, 2
+E4M3 = 3
 MAX_BATCH = 2048
 MAX_ROWS_PER_TILE = 128
 MAX_GROUP_ROWS = 32
@@ -52,6 +53,11 @@ SIGNATURES = {
     "htr_decode_raw": (_i, [_vp, _vp, _i64, _i, _vp]),
     "htr_dequant_q": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp]),
     "htr_dequant_w": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp]),
+    "htr_rms_norm": (_i, [_vp, _i64, _vp, _i64, _vp, _i64, _i, ctypes.c_double, _i, _vp, _vp, _vp, _vp]),
+    "htr_quantize_e4m3": (_i, [_vp, _i64, _i64, _i, _i, _vp, _vp, _vp]),
+    "htr_product": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _i, _i, _vp]),
+    "htr_moe_stacked_scratch_bytes": (_sz, [_i64, _i, _i, _i, _i, _i]),
+    "htr_moe_stacked": (_i, [_vp, _i, _vp, _i, _vp, _i64, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _sz, _vp]),
 }
 
 

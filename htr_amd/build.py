@@ -10,9 +10,10 @@ import sys
 
 CSRC = os.path.join(os.path.dirname(os.path.abspath(__file__)), "csrc")
 LIB = os.path.join(CSRC, "libhtr_gfx950.so")
-SOURCES = [os.path.join(CSRC, "htr_gfx950.hip")]          # one translation unit; the kernels live in the parts it includes
+# two translation units, compiled side by side; the kernels live in the parts they include
+SOURCES = [os.path.join(CSRC, "htr_gfx950.hip"), os.path.join(CSRC, "unpacked.hip")]
 PARTS = [os.path.join(CSRC, f) for f in ("decode.hpp", "linear.hpp", "linear_batch.hpp", "linear_tile.hpp", "linear_gemm.hpp", "linear_wide.hpp", "moe.hpp", "dequant.hpp",
-                                         "viterbi.hpp", "anchors.hpp", "plan.hpp")]
+                                         "viterbi.hpp", "anchors.hpp", "plan.hpp", "norm.hpp", "product.hpp", "experts.hpp")]
 BINDING_SOURCE = os.path.join(CSRC, "torch_binding.cpp")
 BINDING = os.path.join(os.path.dirname(CSRC), "_fast.so")
 HEADER = os.path.join(os.path.dirname(CSRC), os.pardir, "include", "htr_gfx950.h")
@@ -42,7 +43,14 @@ def binding_command():
 
 
 def build(verbose=False, extra=()):
-    cmds = [[hipcc()] + HIPCC_FLAGS + list(extra) + ["-o", LIB] + SOURCES, binding_command()]
+    objects = [source[:-4] + ".o" for source in SOURCES]
+    flags = [f for f in HIPCC_FLAGS if f != "-shared"]
+    _run([[hipcc()] + flags + list(extra) + ["-c", source, "-o", obj] for source, obj in zip(SOURCES, objects)] + [binding_command()], verbose)
+    _run([[hipcc(), "--offload-arch=gfx950", "-shared", "-o", LIB] + objects], verbose)
+    return LIB
+
+
+def _run(cmds, verbose):
     if verbose:
         for cmd in cmds:
             print(" ".join(cmd), flush=True)
@@ -54,7 +62,6 @@ def build(verbose=False, extra=()):
             raise RuntimeError(os.path.basename(cmd[0]) + " failed:\n" + out)
         if verbose and out.strip():
             print(out)
-    return LIB
 
 
 def is_stale():

@@ -65,11 +65,14 @@ const char* htr_strerror(int status) {
     case HTR_ERR_LAUNCH: return "HIP launch failed";
     case HTR_ERR_SPLIT: return "explicit split count does not fit this shape";
     case HTR_ERR_COUNT: return "problem count out of range";
+    case HTR_ERR_SIZE: return "a size is out of range, or not a multiple of 128 (e4m3) or of 8 (16-bit rows)";
     default: return "unknown status";
   }
 }
 
 int htr_last_hip_error(void) { return g_last_hip_error; }
+// for the library's other translation unit
+__attribute__((visibility("hidden"))) int htr_note_hip_error(int e) { g_last_hip_error = e; return HTR_ERR_LAUNCH; }
 int htr_abi_version(void) { return HTR_ABI_VERSION; }
 float htr_cbscale(void) { return (float)(1.0 / __builtin_sqrt(MEAN_SQ)); }
 

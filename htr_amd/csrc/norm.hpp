@@ -1,0 +1,276 @@
+// Part of unpacked.hip, included inside its anonymous namespace: root-mean-square norm with the residual's addition, and rows in e4m3 with a
+// scale for each 128 columns.
+//
+//   t = round(x + r),   y_c = t_c w_c / sqrt(mean_c t_c^2 + eps)
+//   e4m3: s_b = the least power of two from max_b |y| / 448 up,   q_c = e4m3(y_c / s_b)      for each block b of 128 columns
+//
+// Scales are powers of two: the division is then exact, and the values of a 16-bit row reach e4m3 in one rounding.  With amax / 448 as the scale,
+// x / s falls on ties of e4m3 for one block in seven (448 = 7 2^6), where the rounding of s itself decides: results then differ by
+// several thousandths between machines, and by 2 % behind a second quantization.  A power of two costs no precision but at the lower
+// end, where values below 2^-15 of the block's largest lose a bit more.
+// Bound: HBM (x, r and w read once, t and y or q and s written once).  A workgroup takes one row and keeps it in registers between the two passes.
+
+// ---- e4m3
+// the scale of a block whose largest finite magnitude is `amax`: amax = f 2^e with f in [1/2, 1), 448 = 0.875 2^9.  A block of zeros (or of
+// values below 2^-100) counts as 2^-100, so that neither the scale nor its inverse leaves float32.
+__device__ __forceinline__ int e4m3_exponent(double amax) {
+  amax = fmax(amax, 0x1p-100);
+  const unsigned long long u = __builtin_bit_cast(unsigned long long, amax);
+  const int e = (int)(u >> 52) - 1022;                                // frexp's exponent
+  return e - 9 + ((u & 0xFFFFFFFFFFFFFull) > 0xC000000000000ull);     // mantissa beyond 1.75
+}
+__device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }      // -126 <= e <= 127
+// what e4m3 has no value for becomes NaN there, and takes no part in the scale
+__device__ __forceinline__ float finite_or_nan(float v) { return fabsf(v) < INFINITY ? v : __builtin_nanf(""); }
+__device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d) {
+  int v = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, v, true);
+}
+// largest of 16 neighbouring lanes, in all of them
+__device__ __forceinline__ float max16(float v) {
+  v = fmaxf(v, dpp_mov<0xB1>(v)); v = fmaxf(v, dpp_mov<0x4E>(v));
+  v = fmaxf(v, dpp_mov<0x141>(v)); return fmaxf(v, dpp_mov<0x140>(v));
+}
+__device__ __forceinline__ double max16(double v) {
+#pragma unroll
+  for (int off = 1; off < 16; off <<= 1) v = fmax(v, __shfl_xor(v, off));
+  return v;
+}
+
+// ---- two floats to 16 bits each, rounded to nearest
+typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) { return __builtin_bit_cast(uint32_t, b2{(__bf16)a, (__bf16)b}); }
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) { return __builtin_bit_cast(uint32_t, h2{(_Float16)a, (_Float16)b}); }
+
+// ---- eight consecutive elements
+template <int T> struct Eight;      // T: HTR_BF16, HTR_F16 or HTR_F32
+template <> struct Eight<HTR_BF16> {
+  u4 v;
+  __device__ __forceinline__ void load(const void* p, size_t i) { v = *(const HTR_GLOBAL u4*)((const HTR_GLOBAL uint16_t*)p + i); }
+  __device__ __forceinline__ void store(void* p, size_t i) const { *(HTR_GLOBAL u4*)((HTR_GLOBAL uint16_t*)p + i) = v; }
+  __device__ __forceinline__ float get(int k) const { return __uint_as_float(k & 1 ? v[k >> 1] & 0xFFFF0000u : v[k >> 1] << 16); }
+  __device__ __forceinline__ void set(const float (&f)[8]) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = pack_bf16(f[2 * k], f[2 * k + 1]);
+  }
+};
+template <> struct Eight<HTR_F16> {
+  u4 v;
+  __device__ __forceinline__ void load(const void* p, size_t i) { v = *(const HTR_GLOBAL u4*)((const HTR_GLOBAL uint16_t*)p + i); }
+  __device__ __forceinline__ void store(void* p, size_t i) const { *(HTR_GLOBAL u4*)((HTR_GLOBAL uint16_t*)p + i) = v; }
+  __device__ __forceinline__ float get(int k) const { return f16_bits_to_float((uint16_t)(k & 1 ? v[k >> 1] >> 16 : v[k >> 1])); }
+  __device__ __forceinline__ void set(const float (&f)[8]) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = pack_f16(f[2 * k], f[2 * k + 1]);
+  }
+};
+template <> struct Eight<HTR_F32> {
+  f4 v[2];
+  __device__ __forceinline__ void load(const void* p, size_t i) {
+    v[0] = *(const HTR_GLOBAL f4*)((const HTR_GLOBAL float*)p + i); v[1] = *(const HTR_GLOBAL f4*)((const HTR_GLOBAL float*)p + i + 4);
+  }
+  __device__ __forceinline__ void store(void* p, size_t i) const {
+    *(HTR_GLOBAL f4*)((HTR_GLOBAL float*)p + i) = v[0]; *(HTR_GLOBAL f4*)((HTR_GLOBAL float*)p + i + 4) = v[1];
+  }
+  __device__ __forceinline__ float get(int k) const { return v[k >> 2][k & 3]; }
+  __device__ __forceinline__ void set(const float (&f)[8]) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k >> 2][k & 3] = f[k];
+  }
+};
+
+// Eight finite products (t w) r of a row, 16 neighbouring lanes holding a block of 128: their e4m3 values and the block's scale.
+// p = t w is exact in float32 for 16-bit types (22 bits); the factor r of the row is kept in 64 bits, so that the scale is the right one also
+// where the block's largest value lies next to 448 times a power of two.  For float32 rows p is a 64-bit product.
+template <int T>
+__device__ __forceinline__ u2 quantize8(const Eight<T>& t, const Eight<T>& w, double r, float& scale) {
+  double y[8];
+  double amax;
+  if constexpr (T == HTR_F32) {
+    amax = 0.0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      y[k] = (double)finite_or_nan(t.get(k)) * (double)w.get(k) * r;
+      if (fabs(y[k]) > (double)__FLT_MAX__) y[k] = __builtin_nan("");
+      amax = fmax(amax, fabs(y[k]));
+    }
+    amax = max16(amax);
+  } else {
+    float m = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float p = finite_or_nan(t.get(k) * w.get(k));
+      m = fmaxf(m, fabsf(p));
+      y[k] = (double)p * r;
+    }
+    amax = (double)max16(m) * r;
+  }
+  const int e = min(e4m3_exponent(amax), 120);      // beyond: larger than float32 can hold
+  const double inv = __builtin_bit_cast(double, (unsigned long long)(1023 - e) << 52);
+  scale = exp2i(e);
+  u2 q;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float f[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) f[k] = (float)(y[4 * h + k] * inv);
+    q[h] = pack_e4m3(f[0], f[1], f[2], f[3]);
+  }
+  return q;
+}
+// The same for eight values in float32 as they are
+__device__ __forceinline__ u2 quantize8(const float (&v)[8], float& scale) {
+  float f[8], m = 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) { f[k] = finite_or_nan(v[k]); m = fmaxf(m, fabsf(f[k])); }
+  const int e = e4m3_exponent((double)max16(m));
+  const float inv = exp2i(-e);
+  scale = exp2i(e);
+  u2 q;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) q[h] = pack_e4m3(f[4 * h] * inv, f[4 * h + 1] * inv, f[4 * h + 2] * inv, f[4 * h + 3] * inv);
+  return q;
+}
+
+struct NormArgs {
+  const void *x, *residual, *weight;
+  void *y, *sum;                    // y: of x's type, or e4m3; sum: t, where there is a residual
+  float* scales;                    // e4m3: [rows][n / 128]
+  long long x_stride, residual_stride;      // elements between rows
+  long long rows;
+  int n;
+  double eps;
+};
+
+// sum over the workgroup, the same in every thread
+__device__ __forceinline__ double block_sum(double v, double* lds) {
+#pragma unroll
+  for (int off = 32; off; off >>= 1) v += __shfl_xor(v, off);
+  const int waves = (blockDim.x + 63) >> 6;
+  if (waves == 1) return v;
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  double s = 0.0;
+  for (int k = 0; k < waves; ++k) s += lds[k];
+  return s;
+}
+
+// NV runs of eight columns to a thread; n <= 8 NV threads, every row on a 16-byte boundary.
+// The squares are summed in 64 bits: a row's mean of many of them keeps what float32 holds, for two instructions to an element
+// that the memory hides.
+template <int T, int NV, bool RES, bool QUANT>
+__global__ __launch_bounds__(1024) void k_rms_norm(const NormArgs a) {
+  __shared__ double s_sum[16];
+  const long long row = blockIdx.x;
+  const int n = a.n;
+  Eight<T> t[NV], w[NV];
+  double sq = 0.0;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = 8 * (threadIdx.x + i * blockDim.x);
+    if (c < n) {
+      t[i].load(a.x, (size_t)(row * a.x_stride) + c);
+      w[i].load(a.weight, c);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = 8 * (threadIdx.x + i * blockDim.x);
+    if (c >= n) continue;
+    if constexpr (RES) {
+      Eight<T> r;
+      float f[8];
+      r.load(a.residual, (size_t)(row * a.residual_stride) + c);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f[k] = t[i].get(k) + r.get(k);
+      t[i].set(f);
+      t[i].store(a.sum, (size_t)(row * n) + c);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) { const double v = t[i].get(k); sq += v * v; }
+  }
+  const double mean = block_sum(sq, s_sum) / n + a.eps;
+  const double r = 1.0 / sqrt(mean);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = 8 * (threadIdx.x + i * blockDim.x);
+    if constexpr (QUANT) {
+      // n is a multiple of 128 and blockDim.x of 64: 16 neighbouring lanes are inside or outside together
+      if (c >= n) continue;
+      float scale;
+      const u2 q = quantize8<T>(t[i], w[i], r, scale);
+      *(HTR_GLOBAL u2*)((HTR_GLOBAL uint8_t*)a.y + (size_t)(row * n) + c) = q;
+      if ((threadIdx.x & 15) == 0) ((HTR_GLOBAL float*)a.scales)[(size_t)row * (n >> 7) + (c >> 7)] = scale;
+    } else {
+      if (c >= n) continue;
+      float f[8];
+      const float rf = (float)r;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f[k] = t[i].get(k) * rf * w[i].get(k);
+      Eight<T> y;
+      y.set(f);
+      y.store(a.y, (size_t)(row * n) + c);
+    }
+  }
+}
+
+// Any width, alignment and stride, element by element; a row is read twice (the second time from the cache)
+template <bool QUANT>
+__global__ __launch_bounds__(256) void k_rms_norm_any(const NormArgs a, int dtype) {
+  __shared__ double s_sum[4];
+  const long long row = blockIdx.x;
+  const int n = a.n, lane = threadIdx.x & 63;
+  auto at = [&](int c) {
+    const float v = load_elem_g(a.x, dtype, (size_t)(row * a.x_stride) + c);
+    if (a.residual == nullptr) return v;
+    const float s = v + load_elem_g(a.residual, dtype, (size_t)(row * a.residual_stride) + c);
+    return dtype == HTR_BF16 ? bf16_bits_to_float(float_to_bf16_bits(s)) : dtype == HTR_F16 ? (float)(_Float16)s : s;
+  };
+  double sq = 0.0;
+  for (int c = threadIdx.x; c < n; c += 256) {
+    const double t = at(c);
+    sq += t * t;
+    if (a.residual != nullptr) store_elem_g(a.sum, dtype, (size_t)(row * n) + c, (float)t);
+  }
+  const double r = 1.0 / sqrt(block_sum(sq, s_sum) / n + a.eps);
+  if constexpr (QUANT) {
+    for (int b = threadIdx.x >> 6; b < n >> 7; b += 4) {            // a wave takes a block of 128 columns, two to a lane
+      double y[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int c = b * 128 + 2 * lane + k;
+        y[k] = (double)finite_or_nan(at(c)) * (double)load_elem_g(a.weight, dtype, c) * r;
+        if (!(fabs(y[k]) <= (double)__FLT_MAX__)) y[k] = __builtin_nan("");
+      }
+      double amax = fmax(fmax(0.0, fabs(y[0])), fabs(y[1]));        // fmax passes over NaN
+#pragma unroll
+      for (int off = 32; off; off >>= 1) amax = fmax(amax, __shfl_xor(amax, off));
+      const int e = min(e4m3_exponent(amax), 120);
+      const double inv = __builtin_bit_cast(double, (unsigned long long)(1023 - e) << 52);
+      const uint32_t q = pack_e4m3((float)(y[0] * inv), (float)(y[1] * inv), 0.f, 0.f);
+      HTR_GLOBAL uint8_t* out = (HTR_GLOBAL uint8_t*)a.y + (size_t)(row * n) + b * 128 + 2 * lane;
+      out[0] = (uint8_t)q; out[1] = (uint8_t)(q >> 8);
+      if (lane == 0) ((HTR_GLOBAL float*)a.scales)[(size_t)row * (n >> 7) + b] = exp2i(e);
+    }
+  } else {
+    const float rf = (float)r;
+    for (int c = threadIdx.x; c < n; c += 256) store_elem_g(a.y, dtype, (size_t)(row * n) + c, at(c) * rf * load_elem_g(a.weight, dtype, c));
+  }
+}
+
+// Rows to e4m3 as they are: 16 lanes to a block of 128 columns
+template <int T>
+__global__ __launch_bounds__(256) void k_quantize(const void* __restrict__ x, long long stride, long long blocks, int per_row, uint8_t* __restrict__ q,
+                                                  float* __restrict__ scales) {
+  const long long b = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
+  if (b >= blocks) return;
+  const long long row = b / per_row;
+  const int c = (int)(b - row * per_row) * 128 + 8 * (threadIdx.x & 15);
+  Eight<T> v;
+  v.load(x, (size_t)(row * stride) + c);
+  float f[8], scale;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) f[k] = v.get(k);
+  *(HTR_GLOBAL u2*)((HTR_GLOBAL uint8_t*)q + (size_t)row * per_row * 128 + c) = quantize8(f, scale);
+  if ((threadIdx.x & 15) == 0) ((HTR_GLOBAL float*)scales)[b] = scale;
+}

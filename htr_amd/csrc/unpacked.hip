@@ -1,0 +1,233 @@
+// Kernels for MI355X (gfx950) around the packed linears, behind the same C ABI: the norm in front of them, and products with matrices that a
+// checkpoint keeps in 16 bits or in e4m3 with block scales, whole or by expert.  Own translation unit: the packed kernels take two minutes to
+// compile, these a few seconds.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+#include <string.h>
+#include <stdlib.h>
+#include <atomic>
+#include <type_traits>
+
+#include "../../include/htr_gfx950.h"
+
+// keeps the runtime's error for htr_last_hip_error (htr_gfx950.hip)
+extern "C" __attribute__((visibility("hidden"))) int htr_note_hip_error(int e);
+
+namespace {
+#include "decode.hpp"
+#include "norm.hpp"
+#include "product.hpp"
+#include "experts.hpp"
+
+#define TRY_HIP(EXPR) do { const hipError_t e_ = (EXPR); if (e_ != hipSuccess) return htr_note_hip_error((int)e_); } while (0)
+
+// one launch with the runtime's own return value, as in plan.hpp
+template <typename T> struct same { typedef T type; };
+template <typename... K>
+hipError_t launch(void (*kernel)(K...), dim3 grid, unsigned threads, size_t lds, hipStream_t st, typename same<K>::type... args) {
+  void* argv[] = {(void*)&args...};
+  return hipLaunchKernel((const void*)kernel, grid, dim3(threads), argv, lds, st);
+}
+// more dynamic LDS than the default 64 KB, once per device and kernel
+template <auto Kernel> hipError_t allow_lds(size_t bytes) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return e;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_acquire) & bit) return hipSuccess;
+  e = hipFuncSetAttribute((const void*)Kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == hipSuccess) done.fetch_or(bit, std::memory_order_release);
+  return e;
+}
+
+bool is_16bit(int dtype) { return dtype == HTR_BF16 || dtype == HTR_F16; }
+bool is_dtype(int dtype) { return is_16bit(dtype) || dtype == HTR_F32; }
+size_t element_bytes(int dtype) { return dtype == HTR_F32 ? 4 : dtype == HTR_E4M3 ? 1 : 2; }
+bool aligned(const void* p, size_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
+
+// ---- norm
+template <int T, bool RES, bool QUANT>
+hipError_t launch_norm(const NormArgs& a, hipStream_t st) {
+  const int eights = (a.n + 7) / 8;
+  const dim3 grid((unsigned)a.rows);
+  // a thread takes one run of eight columns where that is a workgroup, so that a row's loads are all in flight at once; two or four beyond
+  const int nv = eights <= 1024 ? 1 : eights <= 2048 ? 2 : 4;
+  const unsigned threads = ((eights + nv - 1) / nv + 63) / 64 * 64;
+  switch (nv) {
+    case 1: return launch(k_rms_norm<T, 1, RES, QUANT>, grid, threads, 0, st, a);
+    case 2: return launch(k_rms_norm<T, 2, RES, QUANT>, grid, threads, 0, st, a);
+    default: return launch(k_rms_norm<T, 4, RES, QUANT>, grid, threads, 0, st, a);
+  }
+}
+template <int T> hipError_t launch_norm(const NormArgs& a, bool quant, hipStream_t st) {
+  if (a.residual) return quant ? launch_norm<T, true, true>(a, st) : launch_norm<T, true, false>(a, st);
+  return quant ? launch_norm<T, false, true>(a, st) : launch_norm<T, false, false>(a, st);
+}
+
+hipError_t launch_quantize(const void* x, int dtype, long long rows, int n, long long stride, void* q, float* scales, hipStream_t st) {
+  const int per_row = n / 128;
+  const long long blocks = rows * per_row;
+  const dim3 grid((unsigned)((blocks + 15) / 16));
+  if (dtype == HTR_BF16) return launch(k_quantize<HTR_BF16>, grid, 256, 0, st, x, stride, blocks, per_row, (uint8_t*)q, scales);
+  if (dtype == HTR_F16) return launch(k_quantize<HTR_F16>, grid, 256, 0, st, x, stride, blocks, per_row, (uint8_t*)q, scales);
+  return launch(k_quantize<HTR_F32>, grid, 256, 0, st, x, stride, blocks, per_row, (uint8_t*)q, scales);
+}
+
+// ---- products
+template <int T, int R, int TT> hipError_t launch_stream(const ProductArgs& a, hipStream_t st) {
+  const long long tiles = span_bound(a.rows, a.experts, a.ends != nullptr, 16 * TT);
+  return launch(k_product_stream<T, R, TT>, dim3((a.m + 16 * R - 1) / (16 * R), (unsigned)tiles), STREAM_WAVES * 64, 0, st, a);
+}
+template <int T, int WM, int WN, int AT, int BT> hipError_t launch_tile(const ProductArgs& a, hipStream_t st) {
+  constexpr int TM = 16 * AT * WM, TN = 16 * BT * WN;
+  constexpr size_t LDS = 2 * (TM + TN) * 128;
+  const long long mtiles = (a.m + TM - 1) / TM, ttiles = span_bound(a.rows, a.experts, a.ends != nullptr, TN);
+  const hipError_t e = allow_lds<k_product_tile<T, WM, WN, AT, BT>>(LDS);
+  if (e != hipSuccess) return e;
+  return launch(k_product_tile<T, WM, WN, AT, BT>, dim3((unsigned)((mtiles * ttiles + 7) / 8 * 8)), WM * WN * 64, LDS, st, a, (int)mtiles, (int)ttiles, 8);
+}
+template <int T> hipError_t launch_product(const ProductArgs& a, hipStream_t st) {
+  const int mean = (int)((a.rows + (long long)a.experts - 1) / a.experts);
+  if (mean <= 64 && span_bound(a.rows, a.experts, a.ends != nullptr, 16) <= 65535) {
+    if (mean <= 8 || (mean <= 16 && a.ends == nullptr)) return a.m <= 4096 ? launch_stream<T, 1, 1>(a, st) : launch_stream<T, 2, 1>(a, st);
+    if (mean <= 32) return launch_stream<T, 2, 2>(a, st);
+    return launch_stream<T, 2, 4>(a, st);
+  }
+  if (mean <= 192) return launch_tile<T, 2, 2, 4, 4>(a, st);
+  return launch_tile<T, 2, 4, 8, 4>(a, st);
+}
+hipError_t launch_product(const ProductArgs& a, int type, hipStream_t st) {
+  return type == HTR_E4M3 ? launch_product<P_F8>(a, st) : type == HTR_BF16 ? launch_product<HTR_BF16>(a, st) : launch_product<HTR_F16>(a, st);
+}
+// what launch_product takes: HTR_OK or the status to refuse with
+int product_shape(long long rows, int m, int n, int experts, int type, bool grouped) {
+  if (type != HTR_E4M3 && !is_16bit(type)) return HTR_ERR_DTYPE;
+  if (rows < 0 || rows > (1ll << 31) - (1 << 20) || m < 1 || n < 1 || experts < 1 || experts > 65535 || n % (type == HTR_E4M3 ? 128 : 8)) return HTR_ERR_SIZE;
+  if (m > (1 << 30) || n > (1 << 28)) return HTR_ERR_SIZE;
+  const long long tiles = span_bound(rows, experts, grouped, 128) * ((m + 127) / 128);
+  return tiles > (1ll << 31) - 8 ? HTR_ERR_SIZE : HTR_OK;
+}
+
+// ---- a routed-expert layer: scratch laid out one after the other, every part on a 256-byte boundary
+struct StackedScratch {
+  size_t ends, token, pos_of, xq, xs, h, a, as, out, bytes;
+  StackedScratch(long long tokens, int top, int experts, int hidden, int inter, int type) {
+    size_t at = 0;
+    auto take = [&](size_t n) { const size_t here = at; at += (n + 255) / 256 * 256; return here; };
+    const size_t pairs = (size_t)tokens * top;
+    const bool f8 = type == HTR_E4M3;
+    ends = take((size_t)experts * 4);
+    token = take(pairs * 4);
+    pos_of = take(pairs * 4);
+    xq = take(f8 ? (size_t)tokens * hidden : 0);
+    xs = take(f8 ? (size_t)tokens * (hidden / 128) * 4 : 0);
+    h = take(pairs * 2 * inter * 4);
+    a = take(pairs * inter * (f8 ? 1 : 2));
+    as = take(f8 ? pairs * (inter / 128) * 4 : 0);
+    out = take(pairs * hidden * 4);
+    bytes = at;
+  }
+};
+int stacked_shape(long long tokens, int top, int experts, int hidden, int inter, int type) {
+  if (tokens < 1 || top < 1 || experts < 1 || hidden < 1 || inter < 1 || top > 4096 || tokens > (1 << 24) || inter > (1 << 28)) return HTR_ERR_SIZE;
+  if (type != HTR_E4M3 && !is_16bit(type)) return HTR_ERR_DTYPE;
+  if (hidden % 8 || inter % (type == HTR_E4M3 ? 128 : 8)) return HTR_ERR_SIZE;
+  if (tokens * top > (1 << 30)) return HTR_ERR_SIZE;
+  const int rc = product_shape(tokens * top, 2 * inter, hidden, experts, type, true);
+  return rc != HTR_OK ? rc : product_shape(tokens * top, hidden, inter, experts, type, true);
+}
+}  // namespace
+
+// ================================================================================================ C ABI
+extern "C" {
+
+int htr_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, const void* weight, int64_t rows, int n, double eps,
+                 int dtype, void* y, void* scales, void* sum, void* stream) {
+  if (rows < 0 || rows > 0x7FFFFFFF || n < 1) return HTR_ERR_SIZE;
+  if (!is_dtype(dtype)) return HTR_ERR_DTYPE;
+  if (rows == 0) return HTR_OK;
+  if (!x || !weight || !y || (residual != nullptr) != (sum != nullptr)) return HTR_ERR_NULL;
+  const size_t size = element_bytes(dtype);
+  if (!aligned(x, size) || !aligned(residual, size) || !aligned(weight, size) || !aligned(sum, size) || !aligned(scales, 4) || (!scales && !aligned(y, size)))
+    return HTR_ERR_ALIGN;
+  if (scales && n % 128) return HTR_ERR_SIZE;
+  const NormArgs a{x, residual, weight, y, sum, (float*)scales, x_stride, residual_stride, rows, n, eps};
+  hipStream_t st = (hipStream_t)stream;
+  const bool vector = n % 8 == 0 && n <= 32768 && aligned(x, 16) && aligned(residual, 16) && aligned(weight, 16) && aligned(y, 16) && aligned(sum, 16) &&
+                      x_stride % 8 == 0 && residual_stride % 8 == 0;
+  if (!vector) {
+    TRY_HIP(scales ? launch(k_rms_norm_any<true>, dim3((unsigned)rows), 256, 0, st, a, dtype) : launch(k_rms_norm_any<false>, dim3((unsigned)rows), 256, 0, st, a, dtype));
+  } else {
+    TRY_HIP(dtype == HTR_BF16 ? launch_norm<HTR_BF16>(a, scales != nullptr, st) : dtype == HTR_F16 ? launch_norm<HTR_F16>(a, scales != nullptr, st)
+                                                                                               : launch_norm<HTR_F32>(a, scales != nullptr, st));
+  }
+  return HTR_OK;
+}
+
+int htr_quantize_e4m3(const void* x, int64_t stride, int64_t rows, int n, int dtype, void* q, void* scales, void* stream) {
+  if (rows < 0 || n < 1 || n % 128 || rows > (1ll << 34) / (n / 128)) return HTR_ERR_SIZE;
+  if (!is_dtype(dtype)) return HTR_ERR_DTYPE;
+  if (rows == 0) return HTR_OK;
+  if (!x || !q || !scales) return HTR_ERR_NULL;
+  if (!aligned(x, 16) || stride % 8 || !aligned(q, 8) || !aligned(scales, 4)) return HTR_ERR_ALIGN;
+  TRY_HIP(launch_quantize(x, dtype, rows, n, stride, q, (float*)scales, (hipStream_t)stream));
+  return HTR_OK;
+}
+
+int htr_product(const void* x, const void* x_scales, const void* w, const void* w_scales, const void* bias, const int32_t* ends, void* y, int64_t rows,
+                int m, int n, int experts, int type, int y_dtype, void* stream) {
+  const int rc = product_shape(rows, m, n, experts, type, ends != nullptr);
+  if (rc != HTR_OK) return rc;
+  if (!is_dtype(y_dtype)) return HTR_ERR_DTYPE;
+  if (ends == nullptr && experts != 1) return HTR_ERR_NULL;
+  if (rows == 0) return HTR_OK;
+  if (!x || !w || !y || (type == HTR_E4M3 && (!x_scales || !w_scales))) return HTR_ERR_NULL;
+  if (!aligned(x, 16) || !aligned(w, 16) || !aligned(y, 16) || !aligned(x_scales, 4) || !aligned(w_scales, 4) || !aligned(ends, 4) ||
+      !aligned(bias, element_bytes(y_dtype)))
+    return HTR_ERR_ALIGN;
+  const ProductArgs a{x, (const float*)x_scales, w, (const float*)w_scales, bias, y, ends, nullptr, (int)rows, m, n, experts, y_dtype};
+  TRY_HIP(launch_product(a, type, (hipStream_t)stream));
+  return HTR_OK;
+}
+
+size_t htr_moe_stacked_scratch_bytes(int64_t tokens, int top, int experts, int hidden, int inter, int type) {
+  return stacked_shape(tokens, top, experts, hidden, inter, type) == HTR_OK ? StackedScratch(tokens, top, experts, hidden, inter, type).bytes : 0;
+}
+
+int htr_moe_stacked(const void* x, int dtype, const void* ids, int ids_int64, const float* weights, int64_t tokens, int top, const void* gate_up,
+                    const void* gate_up_scales, const void* down, const void* down_scales, int experts, int hidden, int inter, int type, void* y,
+                    void* scratch, size_t scratch_bytes, void* stream) {
+  const int rc = stacked_shape(tokens, top, experts, hidden, inter, type);
+  if (rc != HTR_OK) return rc;
+  if (!is_16bit(dtype) || (type != HTR_E4M3 && type != dtype)) return HTR_ERR_DTYPE;
+  const bool f8 = type == HTR_E4M3;
+  if (!x || !ids || !weights || !gate_up || !down || !y || (f8 && (!gate_up_scales || !down_scales))) return HTR_ERR_NULL;
+  if (!aligned(x, 16) || !aligned(gate_up, 16) || !aligned(down, 16) || !aligned(y, 16) || !aligned(ids, ids_int64 ? 8 : 4) || !aligned(weights, 4) ||
+      !aligned(gate_up_scales, 4) || !aligned(down_scales, 4))
+    return HTR_ERR_ALIGN;
+  const StackedScratch at(tokens, top, experts, hidden, inter, type);
+  if (!scratch || !aligned(scratch, 256) || scratch_bytes < at.bytes) return HTR_ERR_WORKSPACE;
+  hipStream_t st = (hipStream_t)stream;
+  uint8_t* s = (uint8_t*)scratch;
+  const int pairs = (int)(tokens * top);
+  int *ends = (int*)(s + at.ends), *token = (int*)(s + at.token), *pos_of = (int*)(s + at.pos_of);
+  float *h = (float*)(s + at.h), *out = (float*)(s + at.out);
+  TRY_HIP(launch(k_expert_order, dim3(experts), ORDER_THREADS, 0, st, ids, ids_int64, pairs, top, experts, ends, token, pos_of));
+  ProductArgs a{x, nullptr, gate_up, (const float*)gate_up_scales, nullptr, h, ends, token, pairs, 2 * inter, hidden, experts, HTR_F32};
+  if (f8) {
+    TRY_HIP(launch_quantize(x, dtype, tokens, hidden, hidden, s + at.xq, (float*)(s + at.xs), st));
+    a.x = s + at.xq; a.xs = (const float*)(s + at.xs);
+  }
+  TRY_HIP(launch_product(a, type, st));
+  TRY_HIP(f8 ? launch(k_gated<P_F8>, dim3(pairs), 256, 0, st, h, ends, experts, inter, s + at.a, (float*)(s + at.as))
+             : dtype == HTR_BF16 ? launch(k_gated<HTR_BF16>, dim3(pairs), 256, 0, st, h, ends, experts, inter, s + at.a, nullptr)
+                                 : launch(k_gated<HTR_F16>, dim3(pairs), 256, 0, st, h, ends, experts, inter, s + at.a, nullptr));
+  const ProductArgs d{s + at.a, (const float*)(s + at.as), down, (const float*)down_scales, nullptr, out, ends, nullptr, pairs, hidden, inter, experts, HTR_F32};
+  TRY_HIP(launch_product(d, type, st));
+  const dim3 grid((unsigned)tokens, (hidden + 2047) / 2048);
+  TRY_HIP(dtype == HTR_BF16 ? launch(k_weighted_sum<HTR_BF16>, grid, 256, 0, st, out, pos_of, weights, top, hidden, y)
+                            : launch(k_weighted_sum<HTR_F16>, grid, 256, 0, st, out, pos_of, weights, top, hidden, y));
+  return HTR_OK;
+}
+}  // extern "C"

@@ -12,6 +12,8 @@ import os
 import torch
 
 from . import _native, wire
+from .unpacked import (dequantize_fp8, grouped_mm, linear_fp8, moe_experts_stacked, quantize_fp8, quantize_weight_fp8,  # noqa: F401
+                       rms_norm)
 
 CB = wire.cbscale()
 _DTYPE_CODE = {torch.bfloat16: _native.BF16, torch.float16: _native.F16, torch.float32: _native.F32}

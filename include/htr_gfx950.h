@@ -37,11 +37,14 @@ typedef enum {
   HTR_ERR_ALIGN = 7,      /* a tensor pointer is not aligned as required */
   HTR_ERR_LAUNCH = 8,     /* the HIP runtime refused the launch (see htr_last_hip_error) */
   HTR_ERR_SPLIT = 9,      /* explicit split count not usable for this shape */
-  HTR_ERR_COUNT = 10      /* grouped call: count outside 1..HTR_MAX_GROUP */
+  HTR_ERR_COUNT = 10,     /* grouped call: count outside 1..HTR_MAX_GROUP */
+  HTR_ERR_SIZE = 11       /* a size that an operator on matrices outside HTR-W1 does not take */
 } htr_status;
 
 /* element type codes; same numbering as the reference's out-dtype map (htr/ops.py:79,94) */
 enum { HTR_BF16 = 0, HTR_F16 = 1, HTR_F32 = 2 };
+/* operands of the products outside HTR-W1: OCP e4m3 (one byte, no infinities) */
+enum { HTR_E4M3 = 3 };
 
 #define HTR_ABI_VERSION 2      /* what htr_abi_version returns */
 #define HTR_MAX_BATCH 2048      /* activation rows one htr_linear launch accepts */
@@ -302,6 +305,54 @@ int htr_dequant_q(const void* qweight, const void* scales, void* out_f32, int mt
  */
 int htr_dequant_w(const void* qweight, const void* scales, const void* su, const void* sv, void* out_bf16,
                   int m, int n, int K, void* stream);
+
+/*
+ * ---- Around the packed linears: the norm in front of them, and linears and experts that a checkpoint leaves out of HTR-W1.  The reference
+ * leaves both to its caller (its plugin returns UnquantizedLinearMethod for such modules, htr/vllm_plugin.py:49-69).
+ *
+ * e4m3 rows carry a float32 scale for each 128 columns, [rows][n / 128]; e4m3 matrices one for each 128x128 block, [ceil(m / 128)][n / 128].
+ * The scales that these calls make are powers of two, the least from amax / 448 up (amax: the block's largest finite magnitude, at least
+ * 2^-100); scales they are given may be any float32.  Infinities and NaN become NaN.
+ *
+ * htr_rms_norm: t = round(x + residual), y = t weight / sqrt(mean(t^2) + eps), the mean in 64 bits.
+ *   x, residual  [rows][n] of dtype with that many elements from row to row; residual may be NULL (then sum is, too: t = x)
+ *   weight       [n] of dtype
+ *   y            [rows][n]: of dtype where scales is NULL, otherwise e4m3 with scales [rows][n / 128], n a multiple of 128
+ *   sum          [rows][n] of dtype: t.  Nothing written may overlap anything read.
+ * 0 <= rows < 2^31.  Any alignment of the elements; multiples of 16 bytes (and of 8 columns) are faster.
+ */
+int htr_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, const void* weight, int64_t rows, int n, double eps,
+                 int dtype, void* y, void* scales, void* sum, void* stream);
+
+/* Rows [rows][n] of dtype, `stride` elements apart, to e4m3 [rows][n] with scales [rows][n / 128].  n a multiple of 128, x on a 16-byte boundary,
+ * stride a multiple of 8. */
+int htr_quantize_e4m3(const void* x, int64_t stride, int64_t rows, int n, int dtype, void* q, void* scales, void* stream);
+
+/*
+ * y[r] = W_e x[r] (+ bias), e the expert of row r, sums in float32.
+ *   type    HTR_E4M3 (x and w with their scales), HTR_BF16 or HTR_F16 (scales NULL)
+ *   x       [rows][n], w [experts][m][n], 16-byte aligned; n a multiple of 128 (e4m3) or of 8 (16 bits), any m
+ *   ends    device int32 [experts]: expert e has rows ends[e - 1] .. ends[e] - 1 (from 0); rows from the last end on become zeros.  An end below
+ *           an earlier one, or beyond rows, counts as that one, or as rows.  NULL: one matrix (experts = 1) for all rows
+ *   bias    [m] of y_dtype or NULL;  y [rows][m], y_dtype any of the three, 16-byte aligned; it may overlap nothing that is read
+ * The result does not depend on which rows come together but for the rounding of sums in another order.
+ */
+int htr_product(const void* x, const void* x_scales, const void* w, const void* w_scales, const void* bias, const int32_t* ends, void* y, int64_t rows,
+                int m, int n, int experts, int type, int y_dtype, void* stream);
+
+/*
+ * A routed-expert layer on stacked matrices: y_t = sum_j w[t, j] Down_e( silu(Gate_e x_t) * Up_e x_t ), e = ids[t, j], sums in float32 and in
+ * ascending j, y of dtype (bf16 or f16).  The hidden values between the products are rounded to dtype, or to e4m3 with scales.
+ *   type     dtype, or HTR_E4M3 (x is then rounded to e4m3 as well)
+ *   gate_up  [experts][2 inter][hidden], gate rows first;  down [experts][hidden][inter];  scales as in htr_product, or NULL
+ *   ids      [tokens][top] int32 or int64 and weights [tokens][top] float32, on the device; an expert out of range makes its token NaN
+ *   scratch  htr_moe_stacked_scratch_bytes() bytes (0: sizes that are not taken), 256-byte aligned, of any content, used until the launches are done
+ * hidden a multiple of 8 (e4m3: 128), inter too.  htr_moe_experts is this layer on HTR-W1 matrices.
+ */
+size_t htr_moe_stacked_scratch_bytes(int64_t tokens, int top, int experts, int hidden, int inter, int type);
+int htr_moe_stacked(const void* x, int dtype, const void* ids, int ids_int64, const float* weights, int64_t tokens, int top, const void* gate_up,
+                    const void* gate_up_scales, const void* down, const void* down_scales, int experts, int hidden, int inter, int type, void* y,
+                    void* scratch, size_t scratch_bytes, void* stream);
 
 /*
  * Timing anchors: measurement only, the results they leave in y are meaningless.  No reference counterpart (the
