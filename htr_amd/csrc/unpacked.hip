@@ -81,11 +81,11 @@ template <int T, int R, int TT> hipError_t launch_stream(const ProductArgs& a, h
 }
 template <int T, int WM, int WN, int AT, int BT> hipError_t launch_tile(const ProductArgs& a, hipStream_t st) {
   constexpr int TM = 16 * AT * WM, TN = 16 * BT * WN;
-  constexpr size_t LDS = 2 * (TM + TN) * 128;
+  constexpr size_t LDS = 2 * ((TM + TN) * 128 + (T == P_F8 ? TN * 4 + 256 : 0));
   const long long mtiles = (a.m + TM - 1) / TM, ttiles = span_bound(a.rows, a.experts, a.ends != nullptr, TN);
   const hipError_t e = allow_lds<k_product_tile<T, WM, WN, AT, BT>>(LDS);
   if (e != hipSuccess) return e;
-  return launch(k_product_tile<T, WM, WN, AT, BT>, dim3((unsigned)((mtiles * ttiles + 7) / 8 * 8)), WM * WN * 64, LDS, st, a, (int)mtiles, (int)ttiles, 8);
+  return launch(k_product_tile<T, WM, WN, AT, BT>, dim3((unsigned)((mtiles * ttiles + 255) / 256 * 256)), WM * WN * 64, LDS, st, a, (int)mtiles, (int)ttiles, 8);
 }
 template <int T> hipError_t launch_product(const ProductArgs& a, hipStream_t st) {
   const int mean = (int)((a.rows + (long long)a.experts - 1) / a.experts);
@@ -106,7 +106,7 @@ int product_shape(long long rows, int m, int n, int experts, int type, bool grou
   if (rows < 0 || rows > (1ll << 31) - (1 << 20) || m < 1 || n < 1 || experts < 1 || experts > 65535 || n % (type == HTR_E4M3 ? 128 : 8)) return HTR_ERR_SIZE;
   if (m > (1 << 30) || n > (1 << 28)) return HTR_ERR_SIZE;
   const long long tiles = span_bound(rows, experts, grouped, 128) * ((m + 127) / 128);
-  return tiles > (1ll << 31) - 8 ? HTR_ERR_SIZE : HTR_OK;
+  return tiles > (1ll << 31) - 256 ? HTR_ERR_SIZE : HTR_OK;
 }
 
 // ---- a routed-expert layer: scratch laid out one after the other, every part on a 256-byte boundary
