@@ -192,151 +192,178 @@ __global__ __launch_bounds__(STREAM_WAVES * 64) void k_product_stream(const Prod
 }
 
 // ------------------------------------------------------------------------------------------------ many rows
-// A workgroup of WM x WN waves owns TM = 16 AT WM rows of a matrix and TN = 16 BT WN rows of x; slabs go from memory straight to LDS, two stages.
+// A workgroup of WM x WN waves takes tiles of TM = 16 AT WM rows of a matrix by TN = 16 BT WN rows of x, one after the other, their slabs one stream: slabs go
+// from memory straight to LDS, two stages.  While one slab is multiplied from registers, the next one lands and is read, and the one after it is asked for;
+// a tile's last products run while the next tile's first slabs arrive, and its results go out during the next one's products.
 // LDS rows are 128 bytes in eight chunks of 16; chunk c of row r lies at place c ^ swizzle(r).  A 16-byte read serves 16 lanes at a time: lanes 0-3, 12-15,
 // 20-23, 24-27, then 4-11, 16-19, 28-31, and the same of the upper half (measured: which pairs of lanes slow each other down on one bank), that is
 // four fours of rows; two rows lie side by side in the banks, and the swizzles put the fours on different pairs of places.
-// Row number 4 q + j of a wave's MFMA tile i is its row 4 AT q + 4 i + j: a lane then holds 4 AT consecutive outputs.
-template <int AT> __device__ __forceinline__ int swizzle_w(int r) { return ((r >> 1) & 1) | ((r / (4 * AT) & 3) << 1); }
+// Row number 4 q + j of a wave's MFMA tiles 2 h and 2 h + 1 are its rows 32 h + 8 q + j and + 4: a lane then holds eight consecutive outputs, and four
+// lanes 64 bytes of a row in 16 bits.
+__device__ __forceinline__ int swizzle_w(int r) { return ((r >> 1) & 1) | ((r >> 3 & 3) << 1); }
 __device__ __forceinline__ int swizzle_x(int r) { return (r >> 1) & 7; }
+constexpr int TILE_XCDS = 8;
 
-#ifndef SPREAD
-#define SPREAD 4
-#endif
-#define SPREAD_AT(k) ((k) >= SPREAD ? L : (k) * L / SPREAD)
+// eight consecutive outputs of a row, from i on, as far as the row goes
+template <int Y> __device__ __forceinline__ void store8(const ProductArgs& a, float (&f)[8], size_t at, int i) {
+  if (a.bias != nullptr) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] += load_elem_g(a.bias, Y, min(i + k, a.m - 1));
+  }
+  if ((a.m & 7) == 0) {
+    Eight<Y> v;
+    v.set(f);
+    v.store(a.y, at);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) if (i + k < a.m) store_elem_g(a.y, Y, at + k, f[k]);
+  }
+}
+
 template <int T, int WM, int WN, int AT, int BT>
-__global__ __launch_bounds__(WM * WN * 64) void k_product_tile(const ProductArgs a, int mtiles, int ttiles, int together) {
+__global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductArgs a, int mtiles, int ttiles, int together) {
   constexpr int WAVES = WM * WN, TM = 16 * AT * WM, TN = 16 * BT * WN;
   constexpr int SCALES = T == P_F8 ? TN * 4 + 256 : 0, STAGE = (TM + TN) * 128 + SCALES;      // e4m3: the rows' scales, then the matrix's
   constexpr int LW = TM / 8 / WAVES, LX = TN / 8 / WAVES, L = LW + LX;        // 1 KB loads of a wave to a stage
-  constexpr int RA = T == P_F8 ? 2 : 4;                          // tiles of the matrix in registers
+  constexpr int RA = T == P_F8 ? 2 : 4;                          // MFMA tiles of the matrix in registers
+  constexpr int BARRIER = AT - RA + 1;                           // the tile of products before which the next slab has landed
   static_assert(T != P_F8 || TN / 64 < WAVES, "a wave for the matrix's scales");
-  static_assert(TM % (8 * WAVES) == 0 && TN % (8 * WAVES) == 0 && AT % RA == 0, "whole loads, registers in turn");
+  static_assert(AT % 4 == 0 && TM % (8 * WAVES) == 0 && TN % (8 * WAVES) == 0 && AT % RA == 0, "whole loads, registers in turn");
   extern __shared__ __align__(16) uint8_t lds[];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
   const int wm = wv / WN, wn = wv % WN;
-  // Workgroups go to the eight XCDs in turn: 32 neighbouring tiles to one XCD (a tile for each of its compute units, `together` tiles of x by a few of
-  // the matrix, whose rows its L2 serves to several of them), the next 32 to the next.  Tiles without rows, which are the last, fall on all alike.
-  const int id = ((blockIdx.x >> 8) << 8) + (blockIdx.x & 7) * 32 + ((blockIdx.x >> 3) & 31);
-  if (id >= mtiles * ttiles) return;
-  const int strip = id / (mtiles * together), t0 = strip * together, high = min(together, ttiles - t0);
-  const int rest = id - strip * mtiles * together, mt = rest / high, tt = t0 + rest % high;
-  const int m0 = mt * TM;
-  const Span s = find_span(a, TN, tt);
-  if (s.e < 0) return;
-  if (s.e == a.experts) { zero_rows(a, s, m0, TM); return; }
   const size_t row_bytes = (size_t)a.n * bytes_of<T>;
   const int slabs = (int)((row_bytes + 127) >> 7);
-  // what the lane loads: 32-bit distances from the tile's first row of either operand (from x where rows are gathered), so that a load takes one
-  // register of address
-  const HTR_GLOBAL uint8_t* wb = (const HTR_GLOBAL uint8_t*)a.w + ((size_t)s.e * a.m + m0) * row_bytes;
-  const HTR_GLOBAL uint8_t* xb = (const HTR_GLOBAL uint8_t*)a.x + (a.gather != nullptr ? 0 : (size_t)s.first * row_bytes);
-  uint32_t src[L];
-  auto chunk_of = [&](int j) {
-    const int r = ((j < LW ? j : j - LW) * WAVES + wv) * 8 + (lane >> 3);
-    return (lane & 7) ^ (j < LW ? swizzle_w<AT>(r) : swizzle_x(r));
-  };
-#pragma unroll
-  for (int j = 0; j < L; ++j) {
-    int r = ((j < LW ? j : j - LW) * WAVES + wv) * 8 + (lane >> 3);
-    if (j < LW) {
-      r = min(r, a.m - 1 - m0);
-    } else {
-      r = min(r, s.count - 1);
-      if (a.gather != nullptr) r = a.gather[s.first + r];
+  // Workgroups go to the eight XCDs in turn: neighbouring tiles to one XCD, one for each of its workgroups, `together` tiles of x by a few of the matrix, whose
+  // rows its L2 serves to several of them; the next run to the next XCD.  Tiles without rows, which are the last, fall on all alike.
+  const int run = gridDim.x / TILE_XCDS;
+  int id = (int)(blockIdx.x % TILE_XCDS) * run + (int)(blockIdx.x / TILE_XCDS);
+
+  // The tile in hand, and the next one that has products, if there is one; rows behind the last expert's become zeros on the way
+  struct Tile { Span s; int m0; };
+  Tile mine, then;
+  auto find = [&](Tile& t) {
+    for (; id < mtiles * ttiles; id += gridDim.x) {
+      const int strip = id / (mtiles * together), t0 = strip * together, high = min(together, ttiles - t0);
+      const int rest = id - strip * mtiles * together;
+      t.m0 = rest / high * TM;
+      t.s = find_span(a, TN, t0 + rest % high);
+      if (t.s.e == a.experts) zero_rows(a, t.s, t.m0, TM);
+      else if (t.s.e >= 0) return true;
     }
-    src[j] = (uint32_t)r * (uint32_t)row_bytes + 16 * chunk_of(j);
-  }
+    return false;
+  };
+  if (!find(mine)) return;
+  // Where a lane's loads of a tile start: 32-bit distances from the tile's first row of either operand (from x where rows are gathered), so that a load takes
+  // one register of address
+  struct Source {
+    const HTR_GLOBAL uint8_t *w, *x;
+    const HTR_GLOBAL float* scales;
+    uint32_t off[L], scale;
+  };
+  auto row_of = [&](int j) { return ((j < LW ? j : j - LW) * WAVES + wv) * 8 + (lane >> 3); };
+  auto chunk_of = [&](int j) { return (lane & 7) ^ (j < LW ? swizzle_w(row_of(j)) : swizzle_x(row_of(j))); };
+  auto source = [&](const Tile& t, Source& to) {
+    to.w = (const HTR_GLOBAL uint8_t*)a.w + ((size_t)t.s.e * a.m + t.m0) * row_bytes;
+    to.x = (const HTR_GLOBAL uint8_t*)a.x + (a.gather != nullptr ? 0 : (size_t)t.s.first * row_bytes);
+#pragma unroll
+    for (int j = 0; j < L; ++j) {
+      int r = row_of(j);
+      if (j < LW) {
+        r = min(r, a.m - 1 - t.m0);      // beyond the matrix, or the expert's rows: the last row, whose results are not stored
+      } else {
+        r = min(r, t.s.count - 1);
+        if (a.gather != nullptr) r = a.gather[t.s.first + r];
+      }
+      to.off[j] = (uint32_t)r * (uint32_t)row_bytes + 16 * chunk_of(j);
+    }
+    // A slab's scales come with it, through LDS: as loads into registers they would make the wave wait for all the loads issued after them.  Waves
+    // 0 .. TN / 64 - 1 take 64 rows' each, the others the matrix's (one for each 128 rows; all the same, since a branch costs registers all over the loop).
+    if constexpr (T == P_F8) {
+      if (wv < TN / 64) {
+        int r = min(wv * 64 + lane, t.s.count - 1);
+        if (a.gather != nullptr) r = a.gather[t.s.first + r];
+        to.scales = (const HTR_GLOBAL float*)a.xs + (a.gather != nullptr ? 0 : (size_t)t.s.first * (a.n >> 7));
+        to.scale = (uint32_t)r * (uint32_t)(a.n >> 7);
+      } else {
+        const int blocks = (a.m + 127) >> 7;
+        to.scales = (const HTR_GLOBAL float*)a.ws + ((size_t)t.s.e * blocks + (t.m0 >> 7)) * (a.n >> 7);
+        to.scale = (uint32_t)min(lane, blocks - 1 - (t.m0 >> 7)) * (uint32_t)(a.n >> 7);
+      }
+    }
+  };
+  Source src, src2;
+  source(mine, src);
   // 16-bit rows may end inside the last slab, at a multiple of 16 bytes: chunks from there on are loaded as the slab's first, and zeroed in LDS
   const int tail = (int)(row_bytes & 127) >> 4;
   auto place = [&](int j, int stage) { return stage * STAGE + (j < LW ? (j * WAVES + wv) * 1024 : TM * 128 + ((j - LW) * WAVES + wv) * 1024); };
-  auto issue = [&](int slab, int stage, int from, int to) {      // behind the last slab it is loaded again, for nothing
-    slab = min(slab, slabs - 1);
+  auto issue = [&](Source& src, int slab, int stage, int from, int to) {
 #pragma unroll
     for (int j = from; j < to; ++j) {
-      asm volatile("" : "+v"(src[j]));                           // or the compiler keeps 64-bit addresses
-      uint32_t off = src[j];
-      if (T != P_F8 && tail != 0 && slab == slabs - 1) { const int ch = chunk_of(j); off -= ch >= tail ? 16 * ch : 0; }      // src holds 16 ch
-      const HTR_GLOBAL uint8_t* p = (j < LW ? wb : xb) + ((size_t)slab << 7) + off;
+      asm volatile("" : "+v"(src.off[j]));                         // or the compiler keeps 64-bit addresses
+      uint32_t off = src.off[j];
+      if (T != P_F8 && tail != 0 && slab == slabs - 1) { const int ch = chunk_of(j); off -= ch >= tail ? 16 * ch : 0; }      // it holds 16 ch
+      const HTR_GLOBAL uint8_t* p = (j < LW ? src.w : src.x) + ((size_t)slab << 7) + off;
       __builtin_amdgcn_global_load_lds((const HTR_GLOBAL void*)p, (__attribute__((address_space(3))) void*)(lds + place(j, stage)), 16, 0, 0);
     }
+  };
+  auto issue_scales = [&](const Source& src, int slab, int stage) {
+    if constexpr (T == P_F8)
+      __builtin_amdgcn_global_load_lds((const HTR_GLOBAL void*)(src.scales + slab + src.scale),
+                                       (__attribute__((address_space(3))) void*)(lds + stage * STAGE + (TM + TN) * 128 + min(wv, TN / 64) * 256), 4, 0, 0);
+  };
+  // The stage is there for every wave, and every wave has read all of the other one.  `behind`: loads of this wave that may still be on their way (they arrive in
+  // order); `last`: the stage holds its tile's last slab
+  auto landed = [&](int stage, bool last, auto behind) {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(decltype(behind)::value) : "memory");
+    if (T != P_F8 && tail != 0 && last) {
+#pragma unroll
+      for (int j = 0; j < L; ++j) if (chunk_of(j) >= tail) *(u4*)(lds + place(j, stage) + 16 * lane) = u4{0u, 0u, 0u, 0u};
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
   };
   // where a lane reads its first chunk of each tile of either operand; the second lies at place ^ 4
   int ra[AT], rb[BT];
 #pragma unroll
   for (int i = 0; i < AT; ++i) {
-    const int r = wm * 16 * AT + (c >> 2) * 4 * AT + 4 * i + (c & 3);
-    ra[i] = r * 128 + 16 * (g ^ swizzle_w<AT>(r));
+    const int r = wm * 16 * AT + 32 * (i >> 1) + 8 * (c >> 2) + 4 * (i & 1) + (c & 3);
+    ra[i] = r * 128 + 16 * (g ^ swizzle_w(r));
   }
 #pragma unroll
   for (int t = 0; t < BT; ++t) {
     const int r = wn * 16 * BT + 16 * t + c;
     rb[t] = TM * 128 + r * 128 + 16 * (g ^ swizzle_x(r));
   }
-  // A slab's scales come with it, through LDS: as loads into registers they would make the wave wait for all the loads issued after them.  Waves 0 .. TN / 64 - 1
-  // take 64 rows' each, the others the matrix's (one for each 128 rows; all the same, since a branch here costs registers all over the loop).
-  const HTR_GLOBAL float* sb = nullptr;
-  uint32_t so = 0u;
-  if constexpr (T == P_F8) {
-    if (wv < TN / 64) {
-      int r = min(wv * 64 + lane, s.count - 1);
-      if (a.gather != nullptr) r = a.gather[s.first + r];
-      sb = (const HTR_GLOBAL float*)a.xs + (a.gather != nullptr ? 0 : (size_t)s.first * (a.n >> 7));
-      so = (uint32_t)r * (uint32_t)(a.n >> 7);
-    } else {
-      const int blocks = (a.m + 127) >> 7;
-      sb = (const HTR_GLOBAL float*)a.ws + ((size_t)s.e * blocks + (m0 >> 7)) * (a.n >> 7);
-      so = (uint32_t)min(lane, blocks - 1 - (m0 >> 7)) * (uint32_t)(a.n >> 7);
-    }
-  }
-  auto issue_scales = [&](int slab, int stage) {
-    if constexpr (T == P_F8)
-      __builtin_amdgcn_global_load_lds((const HTR_GLOBAL void*)(sb + min(slab, slabs - 1) + so),
-                                       (__attribute__((address_space(3))) void*)(lds + stage * STAGE + (TM + TN) * 128 + min(wv, TN / 64) * 256), 4, 0, 0);
+  u4 A[RA][2], B[BT][2];
+  float sx[BT], sw = 0.f;
+  auto read_a = [&](int i, int stage) {
+    const uint8_t* base = lds + stage * STAGE;
+    A[i % RA][0] = *(const u4*)(base + ra[i]); A[i % RA][1] = *(const u4*)(base + (ra[i] ^ 64));
+  };
+  auto read_b = [&](int t, int stage) {
+    const uint8_t* base = lds + stage * STAGE;
+    B[t][0] = *(const u4*)(base + rb[t]); B[t][1] = *(const u4*)(base + (rb[t] ^ 64));
+  };
+  auto read_scales = [&](int stage) {
+    const float* base = (const float*)(lds + stage * STAGE + (TM + TN) * 128);
+#pragma unroll
+    for (int t = 0; t < BT; ++t) sx[t] = base[wn * 16 * BT + 16 * t + c];
+    sw = base[TN + ((wm * 16 * AT) >> 7)];
   };
   f4 acc[AT][BT];
 #pragma unroll
   for (int i = 0; i < AT; ++i)
 #pragma unroll
     for (int t = 0; t < BT; ++t) acc[i][t] = f4{0.f, 0.f, 0.f, 0.f};
-  issue_scales(0, 0);
-  issue(0, 0, 0, L);
-  issue_scales(1, 1);
-  issue(1, 1, 0, SPREAD_AT(RA - 1));
-  // the stage of `slab` is there for every wave; `behind`: loads of this wave that may still be on their way (they arrive in order)
-  auto landed = [&](int slab, auto behind) {
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(decltype(behind)::value) : "memory");
-    if (T != P_F8 && tail != 0 && slab == slabs - 1) {
-#pragma unroll
-      for (int j = 0; j < L; ++j) if (chunk_of(j) >= tail) *(u4*)(lds + place(j, slab & 1) + 16 * lane) = u4{0u, 0u, 0u, 0u};
-    }
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  int stage = 0;                                                 // of the slab in registers
+  constexpr int PIECES = 4;                                      // MFMA tiles over which the loads of a slab are spread
+  auto issue_piece = [&](Source& from, int slab, int to, int piece) {
+    if (piece < PIECES) issue(from, slab, to, piece * L / PIECES, (piece + 1) * L / PIECES);
   };
-  u4 A[RA][2], B[BT][2];
-  float sx[BT], sw = 0.f;
-  auto read_scales = [&](int slab) {
-    const float* base = (const float*)(lds + (slab & 1) * STAGE + (TM + TN) * 128);
-#pragma unroll
-    for (int t = 0; t < BT; ++t) sx[t] = base[wn * 16 * BT + 16 * t + c];
-    sw = base[TN + ((wm * 16 * AT) >> 7)];
-  };
-  auto read_a = [&](int i, int slab) {
-    const uint8_t* base = lds + (slab & 1) * STAGE;
-    A[i % RA][0] = *(const u4*)(base + ra[i]); A[i % RA][1] = *(const u4*)(base + (ra[i] ^ 64));
-  };
-  auto read_b = [&](int t, int slab) {
-    const uint8_t* base = lds + (slab & 1) * STAGE;
-    B[t][0] = *(const u4*)(base + rb[t]); B[t][1] = *(const u4*)(base + (rb[t] ^ 64));
-  };
-  // A slab's operands are in registers before its products begin: the barrier lies where every wave has read all of the slab before, RA - 1 tiles ahead
-  // of its last product, so its stage can be loaded again at once, and the last tiles' products cover the first reads
-  landed(0, std::integral_constant<int, SPREAD_AT(RA - 1)>());
-#pragma unroll
-  for (int i = 0; i < RA - 1; ++i) read_a(i, 0);
-#pragma unroll
-  for (int t = 0; t < BT; ++t) read_b(t, 0);
-  if constexpr (T == P_F8) read_scales(0);
-  for (int slab = 0; slab < slabs; ++slab) {
+  // The products of the slab in registers, while the operands of the next one are read.  Every wave has read all of this slab RA - 1 MFMA tiles ahead of
+  // its last product; there lies the barrier, behind which the slab after the next, `ask`, is asked for, into this one's stage: a few loads with each
+  // MFMA tile, the first of the next call's among them (`asked`); all at once they would keep the wave from its products for as long as they take to issue
+  auto multiply = [&](int asked, Source& from, int ask, Source& from2, bool last_lands) {
     float sc[BT];
     f4 part[3];
     if constexpr (T == P_F8) {
@@ -345,14 +372,13 @@ __global__ __launch_bounds__(WM * WN * 64) void k_product_tile(const ProductArgs
     }
 #pragma unroll
     for (int i = 0; i < AT; ++i) {
-      if (i == AT - RA + 1) {
-        landed(slab + 1, std::integral_constant<int, 0>());
-        issue_scales(slab + 2, slab & 1);
-        if constexpr (T == P_F8) read_scales(slab + 1);
+      if (i == BARRIER) {
+        landed(stage ^ 1, last_lands, std::integral_constant<int, 0>());
+        issue_scales(from2, ask, stage);
+        if constexpr (T == P_F8) read_scales(stage ^ 1);
       }
-      if (i >= AT - RA + 1) issue(slab + 2, slab & 1, SPREAD_AT(i - (AT - RA + 1)), SPREAD_AT(i - (AT - RA + 1) + 1));
-      else issue(slab + 1, (slab + 1) & 1, SPREAD_AT(i + RA - 1), SPREAD_AT(i + RA));
-      if (i + RA - 1 < AT) read_a(i + RA - 1, slab); else read_a(i + RA - 1 - AT, slab + 1);
+      if (i < BARRIER) issue_piece(from, asked, stage ^ 1, i + AT - BARRIER); else issue_piece(from2, ask, stage, i - BARRIER);
+      if (i + RA - 1 < AT) read_a(i + RA - 1, stage); else read_a(i + RA - 1 - AT, stage ^ 1);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int t = 0; t < BT; ++t) {
@@ -365,7 +391,7 @@ __global__ __launch_bounds__(WM * WN * 64) void k_product_tile(const ProductArgs
           acc[i][t] = mfma_16<T>(A[i % RA][0], B[t][0], acc[i][t]);
           acc[i][t] = mfma_16<T>(A[i % RA][1], B[t][1], acc[i][t]);
         }
-        if (i == AT - 1) read_b(t, slab + 1);
+        if (i == AT - 1) read_b(t, stage ^ 1);
       }
       if constexpr (T == P_F8) {
         // a product, then the four sums of the one two before it: left to itself the compiler waits for results just asked for
@@ -378,24 +404,59 @@ __global__ __launch_bounds__(WM * WN * 64) void k_product_tile(const ProductArgs
 #pragma unroll
       for (int l = AT * BT - 2; l < AT * BT; ++l) acc[l / BT][l % BT] += part[l % 3] * sc[l % BT];
     }
-  }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // the last loads again: they write to LDS
-  // results: 16 rows of x at a time through the wave's own part of LDS, four consecutive outputs to a lane, so that a row's go out in whole lines
-  __syncthreads();
-  constexpr int PITCH = 16 * AT + 4, ACROSS = 4 * AT;            // floats of a row there, lanes to a row
-  static_assert(WAVES * 16 * PITCH * 4 <= 2 * STAGE, "room");
-  float* mine = (float*)lds + wv * 16 * PITCH;
-  const int i0 = m0 + wm * 16 * AT + (lane % ACROSS) * 4;        // first of the lane's outputs
+    stage ^= 1;
+  };
+  issue_scales(src, 0, 0);
+  issue(src, 0, 0, 0, L);
+  landed(0, slabs == 1, std::integral_constant<int, 0>());
 #pragma unroll
-  for (int t = 0; t < BT; ++t) {
+  for (int i = 0; i < RA - 1; ++i) read_a(i, 0);
 #pragma unroll
-    for (int i = 0; i < AT; ++i) *(f4*)(mine + c * PITCH + g * ACROSS + 4 * i) = acc[i][t];
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    for (int r = lane / ACROSS; r < 16; r += 64 / ACROSS) {
-      const f4 v = *(const f4*)(mine + r * PITCH + (lane % ACROSS) * 4);
-      const int row = wn * 16 * BT + 16 * t + r;
-      if (row < s.count && i0 < a.m) store4(a, v, s.first + row, i0);
+  for (int t = 0; t < BT; ++t) read_b(t, 0);
+  if constexpr (T == P_F8) read_scales(0);
+  int asked = min(1, slabs - 1);
+  issue_scales(src, asked, 1);
+#pragma unroll
+  for (int piece = 0; piece < AT - BARRIER; ++piece) issue_piece(src, asked, 1, piece);
+  bool more = true;
+  src2 = src;
+  for (int slab = 0;;) {
+    // the last two slabs of a tile ask for the next one's first two; where there is no next tile, for their own tile's again, for nothing
+    if (slab + 2 == slabs || slabs == 1) {
+      id += gridDim.x;
+      more = find(then);
+      if (more) source(then, src2);
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const int ask = slab + 2 < slabs ? slab + 2 : slabs == 1 ? 0 : slab + 2 - slabs;
+    multiply(asked, src, ask, src2, slab + 2 == slabs || slabs == 1);
+    asked = ask;
+    src = src2;
+    if (++slab < slabs) continue;
+    slab = 0;
+    const int i0 = mine.m0 + wm * 16 * AT + 8 * g;               // first of the lane's outputs
+    auto put = [&](auto type) {
+      constexpr int Y = decltype(type)::value;
+#pragma unroll
+      for (int t = 0; t < BT; ++t) {
+        const int r = wn * 16 * BT + 16 * t + c;
+#pragma unroll
+        for (int h = 0; h < AT / 2; ++h) {
+          float f[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) f[k] = acc[2 * h + (k >> 2)][t][k & 3];
+          if (r < mine.s.count && i0 + 32 * h < a.m) store8<Y>(a, f, (size_t)(mine.s.first + r) * a.m + i0 + 32 * h, i0 + 32 * h);
+        }
+      }
+    };
+    if (a.y_dtype == HTR_BF16) put(std::integral_constant<int, HTR_BF16>());
+    else if (a.y_dtype == HTR_F16) put(std::integral_constant<int, HTR_F16>());
+    else put(std::integral_constant<int, HTR_F32>());
+#pragma unroll
+    for (int i = 0; i < AT; ++i)
+#pragma unroll
+      for (int t = 0; t < BT; ++t) acc[i][t] = f4{0.f, 0.f, 0.f, 0.f};
+    if (!more) break;
+    mine = then;
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // loads for nothing: they write to LDS
 }

@@ -82,10 +82,13 @@ template <int T, int R, int TT> hipError_t launch_stream(const ProductArgs& a, h
 template <int T, int WM, int WN, int AT, int BT> hipError_t launch_tile(const ProductArgs& a, hipStream_t st) {
   constexpr int TM = 16 * AT * WM, TN = 16 * BT * WN;
   constexpr size_t LDS = 2 * ((TM + TN) * 128 + (T == P_F8 ? TN * 4 + 256 : 0));
-  const long long mtiles = (a.m + TM - 1) / TM, ttiles = span_bound(a.rows, a.experts, a.ends != nullptr, TN);
+  const long long mtiles = (a.m + TM - 1) / TM, ttiles = span_bound(a.rows, a.experts, a.ends != nullptr, TN), tiles = mtiles * ttiles;
   const hipError_t e = allow_lds<k_product_tile<T, WM, WN, AT, BT>>(LDS);
   if (e != hipSuccess) return e;
-  return launch(k_product_tile<T, WM, WN, AT, BT>, dim3((unsigned)((mtiles * ttiles + 255) / 256 * 256)), WM * WN * 64, LDS, st, a, (int)mtiles, (int)ttiles, 8);
+  // as many workgroups as run at once (an MI355X has 256 compute units), a multiple of the XCDs; rows of one slab have no stream to run on from tile to tile
+  const bool stream = (long long)a.n * bytes_of<T> > 128;
+  const long long wgs = 256 * (160 * 1024 / LDS), up = (tiles + TILE_XCDS - 1) / TILE_XCDS * TILE_XCDS;
+  return launch(k_product_tile<T, WM, WN, AT, BT>, dim3((unsigned)(stream && wgs < up ? wgs : up)), WM * WN * 64, LDS, st, a, (int)mtiles, (int)ttiles, 8);
 }
 template <int T> hipError_t launch_product(const ProductArgs& a, hipStream_t st) {
   const int mean = (int)((a.rows + (long long)a.experts - 1) / a.experts);
