@@ -193,7 +193,7 @@ __global__ __launch_bounds__(STREAM_WAVES * 64) void k_product_stream(const Prod
 
 // ------------------------------------------------------------------------------------------------ many rows
 // A workgroup of WM x WN waves takes tiles of TM = 16 AT WM rows of a matrix by TN = 16 BT WN rows of x, one after the other, their slabs one stream: slabs go
-// from memory straight to LDS, two stages.  While one slab is multiplied from registers, the next one lands and is read, and the one after it is asked for;
+// from memory straight to LDS, a ring of NS stages.  While one slab is multiplied from registers, the next one is read, and the one NS behind is asked for;
 // a tile's last products run while the next tile's first slabs arrive, and its results go out during the next one's products.
 // LDS rows are 128 bytes in eight chunks of 16; chunk c of row r lies at place c ^ swizzle(r).  A 16-byte read serves 16 lanes at a time: lanes 0-3, 12-15,
 // 20-23, 24-27, then 4-11, 16-19, 28-31, and the same of the upper half (measured: which pairs of lanes slow each other down on one bank), that is
@@ -220,7 +220,7 @@ template <int Y> __device__ __forceinline__ void store8(const ProductArgs& a, fl
   }
 }
 
-template <int T, int WM, int WN, int AT, int BT>
+template <int T, int WM, int WN, int AT, int BT, int NS>
 __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductArgs a, int mtiles, int ttiles, int together) {
   constexpr int WAVES = WM * WN, TM = 16 * AT * WM, TN = 16 * BT * WN;
   constexpr int SCALES = T == P_F8 ? TN * 4 + 256 : 0, STAGE = (TM + TN) * 128 + SCALES;      // e4m3: the rows' scales, then the matrix's
@@ -312,8 +312,8 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
       __builtin_amdgcn_global_load_lds((const HTR_GLOBAL void*)(src.scales + slab + src.scale),
                                        (__attribute__((address_space(3))) void*)(lds + stage * STAGE + (TM + TN) * 128 + min(wv, TN / 64) * 256), 4, 0, 0);
   };
-  // The stage is there for every wave, and every wave has read all of the other one.  `behind`: loads of this wave that may still be on their way (they arrive in
-  // order); `last`: the stage holds its tile's last slab
+  // The stage is there for every wave, and every wave has read all of the one before.  `behind`: later loads of this wave, which may still be on their way (they
+  // arrive in order; results being stored in between only make the wait longer); `last`: the stage holds its tile's last slab
   auto landed = [&](int stage, bool last, auto behind) {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(decltype(behind)::value) : "memory");
     if (T != P_F8 && tail != 0 && last) {
@@ -356,16 +356,18 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
 #pragma unroll
     for (int t = 0; t < BT; ++t) acc[i][t] = f4{0.f, 0.f, 0.f, 0.f};
   int stage = 0;                                                 // of the slab in registers
+  auto after = [](int st, int by) { const int to = st + by; return to >= NS ? to - NS : to; };
   constexpr int PIECES = 4;                                      // MFMA tiles over which the loads of a slab are spread
   auto issue_piece = [&](Source& from, int slab, int to, int piece) {
     if (piece < PIECES) issue(from, slab, to, piece * L / PIECES, (piece + 1) * L / PIECES);
   };
   // The products of the slab in registers, while the operands of the next one are read.  Every wave has read all of this slab RA - 1 MFMA tiles ahead of
-  // its last product; there lies the barrier, behind which the slab after the next, `ask`, is asked for, into this one's stage: a few loads with each
+  // its last product; there lies the barrier, behind which the slab NS after this one, `ask`, is asked for, into this one's stage: a few loads with each
   // MFMA tile, the first of the next call's among them (`asked`); all at once they would keep the wave from its products for as long as they take to issue
   auto multiply = [&](int asked, Source& from, int ask, Source& from2, bool last_lands) {
     float sc[BT];
     f4 part[3];
+    const int next = after(stage, 1), prev = after(stage, NS - 1);
     if constexpr (T == P_F8) {
 #pragma unroll
       for (int t = 0; t < BT; ++t) sc[t] = sx[t] * sw;
@@ -373,12 +375,12 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
 #pragma unroll
     for (int i = 0; i < AT; ++i) {
       if (i == BARRIER) {
-        landed(stage ^ 1, last_lands, std::integral_constant<int, 0>());
+        landed(next, last_lands, std::integral_constant<int, (NS - 2) * (L + (T == P_F8))>());
         issue_scales(from2, ask, stage);
-        if constexpr (T == P_F8) read_scales(stage ^ 1);
+        if constexpr (T == P_F8) read_scales(next);
       }
-      if (i < BARRIER) issue_piece(from, asked, stage ^ 1, i + AT - BARRIER); else issue_piece(from2, ask, stage, i - BARRIER);
-      if (i + RA - 1 < AT) read_a(i + RA - 1, stage); else read_a(i + RA - 1 - AT, stage ^ 1);
+      if (i < BARRIER) issue_piece(from, asked, prev, i + AT - BARRIER); else issue_piece(from2, ask, stage, i - BARRIER);
+      if (i + RA - 1 < AT) read_a(i + RA - 1, stage); else read_a(i + RA - 1 - AT, next);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int t = 0; t < BT; ++t) {
@@ -391,7 +393,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
           acc[i][t] = mfma_16<T>(A[i % RA][0], B[t][0], acc[i][t]);
           acc[i][t] = mfma_16<T>(A[i % RA][1], B[t][1], acc[i][t]);
         }
-        if (i == AT - 1) read_b(t, stage ^ 1);
+        if (i == AT - 1) read_b(t, next);
       }
       if constexpr (T == P_F8) {
         // a product, then the four sums of the one two before it: left to itself the compiler waits for results just asked for
@@ -404,31 +406,35 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
 #pragma unroll
       for (int l = AT * BT - 2; l < AT * BT; ++l) acc[l / BT][l % BT] += part[l % 3] * sc[l % BT];
     }
-    stage ^= 1;
+    stage = next;
   };
-  issue_scales(src, 0, 0);
-  issue(src, 0, 0, 0, L);
-  landed(0, slabs == 1, std::integral_constant<int, 0>());
+  // slabs behind the last one: the last one again, for nothing
+#pragma unroll
+  for (int st = 0; st < NS - 1; ++st) {
+    issue_scales(src, min(st, slabs - 1), st);
+    issue(src, min(st, slabs - 1), st, 0, L);
+  }
+  int asked = min(NS - 1, slabs - 1);
+  issue_scales(src, asked, NS - 1);
+#pragma unroll
+  for (int piece = 0; piece < AT - BARRIER; ++piece) issue_piece(src, asked, NS - 1, piece);
+  landed(0, slabs == 1, std::integral_constant<int, (NS - 2) * (L + (T == P_F8))>());
 #pragma unroll
   for (int i = 0; i < RA - 1; ++i) read_a(i, 0);
 #pragma unroll
   for (int t = 0; t < BT; ++t) read_b(t, 0);
   if constexpr (T == P_F8) read_scales(0);
-  int asked = min(1, slabs - 1);
-  issue_scales(src, asked, 1);
-#pragma unroll
-  for (int piece = 0; piece < AT - BARRIER; ++piece) issue_piece(src, asked, 1, piece);
-  bool more = true;
+  bool more = false;
   src2 = src;
   for (int slab = 0;;) {
-    // the last two slabs of a tile ask for the next one's first two; where there is no next tile, for their own tile's again, for nothing
-    if (slab + 2 == slabs || slabs == 1) {
+    // the last NS slabs of a tile ask for the next one's first; where there is no next tile, for their own tile's again, for nothing
+    if (slab + NS == slabs) {
       id += gridDim.x;
       more = find(then);
       if (more) source(then, src2);
     }
-    const int ask = slab + 2 < slabs ? slab + 2 : slabs == 1 ? 0 : slab + 2 - slabs;
-    multiply(asked, src, ask, src2, slab + 2 == slabs || slabs == 1);
+    const int ask = slab + NS < slabs ? slab + NS : slabs >= NS ? slab + NS - slabs : slabs - 1;
+    multiply(asked, src, ask, src2, slab + 2 == slabs);
     asked = ask;
     src = src2;
     if (++slab < slabs) continue;

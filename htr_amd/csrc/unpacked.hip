@@ -79,16 +79,18 @@ template <int T, int R, int TT> hipError_t launch_stream(const ProductArgs& a, h
   const long long tiles = span_bound(a.rows, a.experts, a.ends != nullptr, 16 * TT);
   return launch(k_product_stream<T, R, TT>, dim3((a.m + 16 * R - 1) / (16 * R), (unsigned)tiles), STREAM_WAVES * 64, 0, st, a);
 }
-template <int T, int WM, int WN, int AT, int BT> hipError_t launch_tile(const ProductArgs& a, hipStream_t st) {
+template <int T, int WM, int WN, int AT, int BT, int NS> hipError_t launch_tile(const ProductArgs& a, hipStream_t st) {
   constexpr int TM = 16 * AT * WM, TN = 16 * BT * WN;
-  constexpr size_t LDS = 2 * ((TM + TN) * 128 + (T == P_F8 ? TN * 4 + 256 : 0));
+  constexpr size_t LDS = NS * ((TM + TN) * 128 + (T == P_F8 ? TN * 4 + 256 : 0));
+  static_assert(LDS <= 160 * 1024, "a compute unit's LDS");
   const long long mtiles = (a.m + TM - 1) / TM, ttiles = span_bound(a.rows, a.experts, a.ends != nullptr, TN), tiles = mtiles * ttiles;
-  const hipError_t e = allow_lds<k_product_tile<T, WM, WN, AT, BT>>(LDS);
+  const hipError_t e = allow_lds<k_product_tile<T, WM, WN, AT, BT, NS>>(LDS);
   if (e != hipSuccess) return e;
-  // as many workgroups as run at once (an MI355X has 256 compute units), a multiple of the XCDs; rows of one slab have no stream to run on from tile to tile
-  const bool stream = (long long)a.n * bytes_of<T> > 128;
+  // as many workgroups as run at once (an MI355X has 256 compute units), a multiple of the XCDs; rows of fewer slabs than stages have no stream to run on from
+  // tile to tile
+  const bool stream = (long long)a.n * bytes_of<T> > 128 * (NS - 1);
   const long long wgs = 256 * (160 * 1024 / LDS), up = (tiles + TILE_XCDS - 1) / TILE_XCDS * TILE_XCDS;
-  return launch(k_product_tile<T, WM, WN, AT, BT>, dim3((unsigned)(stream && wgs < up ? wgs : up)), WM * WN * 64, LDS, st, a, (int)mtiles, (int)ttiles, 8);
+  return launch(k_product_tile<T, WM, WN, AT, BT, NS>, dim3((unsigned)(stream && wgs < up ? wgs : up)), WM * WN * 64, LDS, st, a, (int)mtiles, (int)ttiles, 8);
 }
 template <int T> hipError_t launch_product(const ProductArgs& a, hipStream_t st) {
   const int mean = (int)((a.rows + (long long)a.experts - 1) / a.experts);
@@ -97,8 +99,8 @@ template <int T> hipError_t launch_product(const ProductArgs& a, hipStream_t st)
     if (mean <= 32) return launch_stream<T, 2, 2>(a, st);
     return launch_stream<T, 2, 4>(a, st);
   }
-  if (mean <= 192) return launch_tile<T, 2, 2, 4, 4>(a, st);
-  return launch_tile<T, 2, 4, 8, 4>(a, st);
+  if (mean <= 192) return launch_tile<T, 2, 2, 4, 4, 2>(a, st);
+  return launch_tile<T, 2, 4, 8, 4, 2>(a, st);
 }
 hipError_t launch_product(const ProductArgs& a, int type, hipStream_t st) {
   return type == HTR_E4M3 ? launch_product<P_F8>(a, st) : type == HTR_BF16 ? launch_product<HTR_BF16>(a, st) : launch_product<HTR_F16>(a, st);
