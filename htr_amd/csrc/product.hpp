@@ -98,11 +98,10 @@ __device__ __forceinline__ void store4(const ProductArgs& a, f4 v, int row, int 
 }
 
 // ------------------------------------------------------------------------------------------------ few rows
-// A workgroup owns 16 R rows of a matrix and up to 16 TT rows of x; its eight waves take the slabs in turn, straight from memory into registers
+// A workgroup owns 16 R rows of a matrix and up to 16 TT rows of x; its waves take the slabs in turn, straight from memory into registers
 // (every byte of the matrix is used by one wave once: LDS would only be a detour), and add up through LDS.
 // Bound: HBM, the matrix read once.
-constexpr int STREAM_WAVES = 8;
-template <int T, int R, int TT>
+template <int T, int R, int TT, int STREAM_WAVES>
 __global__ __launch_bounds__(STREAM_WAVES * 64) void k_product_stream(const ProductArgs a) {
   constexpr int P = R + TT <= 3 ? 4 : 2;                       // slabs in flight
   __shared__ float red[STREAM_WAVES][R * TT * 256];
@@ -223,12 +222,13 @@ template <int Y> __device__ __forceinline__ void store8(const ProductArgs& a, fl
 template <int T, int WM, int WN, int AT, int BT, int NS>
 __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductArgs a, int mtiles, int ttiles, int together) {
   constexpr int WAVES = WM * WN, TM = 16 * AT * WM, TN = 16 * BT * WN;
-  constexpr int SCALES = T == P_F8 ? TN * 4 + 256 : 0, STAGE = (TM + TN) * 128 + SCALES;      // e4m3: the rows' scales, then the matrix's
+  constexpr int XW = (TN + 63) / 64;                             // waves that load rows' scales
+  constexpr int SCALES = T == P_F8 ? XW * 256 + 256 : 0, STAGE = (TM + TN) * 128 + SCALES;    // e4m3: the rows' scales, then the matrix's
   constexpr int LW = TM / 8 / WAVES, LX = TN / 8 / WAVES, L = LW + LX;        // 1 KB loads of a wave to a stage
-  constexpr int RA = T == P_F8 ? 2 : 4;                          // MFMA tiles of the matrix in registers
+  constexpr int RA = T == P_F8 || AT < 4 ? 2 : 4;                // MFMA tiles of the matrix in registers
   constexpr int BARRIER = AT - RA + 1;                           // the tile of products before which the next slab has landed
-  static_assert(T != P_F8 || TN / 64 < WAVES, "a wave for the matrix's scales");
-  static_assert(AT % 4 == 0 && TM % (8 * WAVES) == 0 && TN % (8 * WAVES) == 0 && AT % RA == 0, "whole loads, registers in turn");
+  static_assert(T != P_F8 || XW < WAVES, "a wave for the matrix's scales");
+  static_assert(AT % 2 == 0 && TM % (8 * WAVES) == 0 && TN % (8 * WAVES) == 0 && AT % RA == 0, "whole loads, registers in turn");
   extern __shared__ __align__(16) uint8_t lds[];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
   const int wm = wv / WN, wn = wv % WN;
@@ -278,9 +278,9 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
       to.off[j] = (uint32_t)r * (uint32_t)row_bytes + 16 * chunk_of(j);
     }
     // A slab's scales come with it, through LDS: as loads into registers they would make the wave wait for all the loads issued after them.  Waves
-    // 0 .. TN / 64 - 1 take 64 rows' each, the others the matrix's (one for each 128 rows; all the same, since a branch costs registers all over the loop).
+    // 0 .. XW - 1 take 64 rows' each, the others the matrix's (one for each 128 rows; all the same, since a branch costs registers all over the loop).
     if constexpr (T == P_F8) {
-      if (wv < TN / 64) {
+      if (wv < XW) {
         int r = min(wv * 64 + lane, t.s.count - 1);
         if (a.gather != nullptr) r = a.gather[t.s.first + r];
         to.scales = (const HTR_GLOBAL float*)a.xs + (a.gather != nullptr ? 0 : (size_t)t.s.first * (a.n >> 7));
@@ -310,7 +310,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
   auto issue_scales = [&](const Source& src, int slab, int stage) {
     if constexpr (T == P_F8)
       __builtin_amdgcn_global_load_lds((const HTR_GLOBAL void*)(src.scales + slab + src.scale),
-                                       (__attribute__((address_space(3))) void*)(lds + stage * STAGE + (TM + TN) * 128 + min(wv, TN / 64) * 256), 4, 0, 0);
+                                       (__attribute__((address_space(3))) void*)(lds + stage * STAGE + (TM + TN) * 128 + min(wv, XW) * 256), 4, 0, 0);
   };
   // The stage is there for every wave, and every wave has read all of the one before.  `behind`: later loads of this wave, which may still be on their way (they
   // arrive in order; results being stored in between only make the wait longer); `last`: the stage holds its tile's last slab
@@ -348,7 +348,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
     const float* base = (const float*)(lds + stage * STAGE + (TM + TN) * 128);
 #pragma unroll
     for (int t = 0; t < BT; ++t) sx[t] = base[wn * 16 * BT + 16 * t + c];
-    sw = base[TN + ((wm * 16 * AT) >> 7)];
+    sw = base[XW * 64 + ((wm * 16 * AT) >> 7)];
   };
   f4 acc[AT][BT];
 #pragma unroll
@@ -357,7 +357,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
     for (int t = 0; t < BT; ++t) acc[i][t] = f4{0.f, 0.f, 0.f, 0.f};
   int stage = 0;                                                 // of the slab in registers
   auto after = [](int st, int by) { const int to = st + by; return to >= NS ? to - NS : to; };
-  constexpr int PIECES = 4;                                      // MFMA tiles over which the loads of a slab are spread
+  constexpr int PIECES = AT < 4 ? AT : 4;                        // MFMA tiles over which the loads of a slab are spread
   auto issue_piece = [&](Source& from, int slab, int to, int piece) {
     if (piece < PIECES) issue(from, slab, to, piece * L / PIECES, (piece + 1) * L / PIECES);
   };

@@ -5,6 +5,7 @@
 #include <stdint.h>
 #include <string.h>
 #include <stdlib.h>
+#include <math.h>
 #include <atomic>
 #include <type_traits>
 
@@ -75,13 +76,13 @@ hipError_t launch_quantize(const void* x, int dtype, long long rows, int n, long
 }
 
 // ---- products
-template <int T, int R, int TT> hipError_t launch_stream(const ProductArgs& a, hipStream_t st) {
+template <int T, int R, int TT, int WAVES> hipError_t launch_stream(const ProductArgs& a, hipStream_t st) {
   const long long tiles = span_bound(a.rows, a.experts, a.ends != nullptr, 16 * TT);
-  return launch(k_product_stream<T, R, TT>, dim3((a.m + 16 * R - 1) / (16 * R), (unsigned)tiles), STREAM_WAVES * 64, 0, st, a);
+  return launch(k_product_stream<T, R, TT, WAVES>, dim3((a.m + 16 * R - 1) / (16 * R), (unsigned)tiles), WAVES * 64, 0, st, a);
 }
 template <int T, int WM, int WN, int AT, int BT, int NS> hipError_t launch_tile(const ProductArgs& a, hipStream_t st) {
   constexpr int TM = 16 * AT * WM, TN = 16 * BT * WN;
-  constexpr size_t LDS = NS * ((TM + TN) * 128 + (T == P_F8 ? TN * 4 + 256 : 0));
+  constexpr size_t LDS = NS * ((TM + TN) * 128 + (T == P_F8 ? (TN + 63) / 64 * 256 + 256 : 0));
   static_assert(LDS <= 160 * 1024, "a compute unit's LDS");
   const long long mtiles = (a.m + TM - 1) / TM, ttiles = span_bound(a.rows, a.experts, a.ends != nullptr, TN), tiles = mtiles * ttiles;
   const hipError_t e = allow_lds<k_product_tile<T, WM, WN, AT, BT, NS>>(LDS);
@@ -92,15 +93,51 @@ template <int T, int WM, int WN, int AT, int BT, int NS> hipError_t launch_tile(
   const long long wgs = 256 * (160 * 1024 / LDS), up = (tiles + TILE_XCDS - 1) / TILE_XCDS * TILE_XCDS;
   return launch(k_product_tile<T, WM, WN, AT, BT, NS>, dim3((unsigned)(stream && wgs < up ? wgs : up)), WM * WN * 64, LDS, st, a, (int)mtiles, (int)ttiles, 8);
 }
+// Which tiles for many rows: the ones whose rounds take the least time by what a slab of a tile takes where the compute units have little else to do
+// and where all are at work (measured on 64 .. 8192 rows of 4096 .. 14336 columns, ns; both types: their slabs have the same bytes).  A larger tile multiplies
+// more for what it loads, a smaller one leaves fewer compute units idle: 333 rows on 6144x4096 in e4m3 52 us by 256x256, 27 by 128x128, 25 by 128x64;
+// 1000 on 14336x4096 68, 99, 109; 100 on 6144x4096 51, 28, 22 and 15 by 64x64.
+struct TileChoice { int tm, tn, at_once; float light, full; };
+constexpr TileChoice TILES[] = {{256, 256, 1, 1450.f, 1950.f}, {256, 128, 1, 950.f, 1300.f}, {128, 128, 1, 700.f, 800.f},
+                                {128, 64, 2, 550.f, 850.f},    {64, 64, 2, 420.f, 600.f},    {64, 32, 3, 290.f, 450.f}};
+int best_tile(const ProductArgs& a, size_t row_bytes) {
+  int best = 0;
+  float least = 0.f;
+  for (int k = 0; k < (int)(sizeof(TILES) / sizeof(TILES[0])); ++k) {
+    const TileChoice& c = TILES[k];
+    const float mtiles = (float)((a.m + c.tm - 1) / c.tm), full = (float)a.rows / c.tn;
+    const float experts = (float)(a.rows < a.experts ? a.rows : a.experts);
+    // an expert's last tile is half full on average
+    const float tiles = mtiles * (a.ends == nullptr ? ceilf(full) : fmaxf(experts, full + 0.5f * experts));
+    const float rounds = tiles / (256.f * c.at_once), whole = floorf(rounds), part = rounds - whole;
+    const float ns = (4000.f + (float)((row_bytes + 127) >> 7) * (whole * c.full + (part > 0.f ? c.light + part * (c.full - c.light) : 0.f)));
+    if (k == 0 || ns < least) { least = ns; best = k; }
+  }
+  return best;
+}
+// Few rows of a matrix are a matter of reading it.  k_product_stream has the most loads on their way where a matrix's rows alone make enough workgroups;
+// k_product_tile goes on from tile to tile without a pause where there is more (e4m3, us):
+//   one row: 1024x4096 5.0 (16 rows to a workgroup of 8 waves; 4 waves 6.4, tiles of 64x32 10.9), 4096x4096 5.9 (7.4, 12.0), 14336x4096 15.5 (17.2, 16.9),
+//   28672x4096 25.7 (27.2, 29.5); 32 rows: 4096x4096 10.3 (tiles of 64x32 12.4, of 128x32 16.6), 28672x4096 64 (33, 31)
+//   96 rows of 64 experts: 2816x2048 56 (64 rows to a workgroup of 4 waves; 16 rows to one of 8 86; tiles of 128x32 59), 2048x1408 34 (52; 35)
 template <int T> hipError_t launch_product(const ProductArgs& a, hipStream_t st) {
   const int mean = (int)((a.rows + (long long)a.experts - 1) / a.experts);
-  if (mean <= 64 && span_bound(a.rows, a.experts, a.ends != nullptr, 16) <= 65535) {
-    if (mean <= 8 || (mean <= 16 && a.ends == nullptr)) return a.m <= 4096 ? launch_stream<T, 1, 1>(a, st) : launch_stream<T, 2, 1>(a, st);
-    if (mean <= 32) return launch_stream<T, 2, 2>(a, st);
-    return launch_stream<T, 2, 4>(a, st);
+  const bool grouped = a.ends != nullptr, narrow = span_bound(a.rows, a.experts, grouped, 16) <= 65535;
+  if (!grouped) {
+    if (mean <= 16) return launch_stream<T, 1, 1, 8>(a, st);
+    if (mean <= 32) return a.m < 8192 ? launch_stream<T, 1, 2, 8>(a, st) : a.m < 16384 ? launch_tile<T, 2, 2, 2, 1, 4>(a, st) : launch_tile<T, 4, 1, 2, 2, 4>(a, st);
+  } else {
+    if (mean <= 4 && narrow) return launch_stream<T, 4, 1, 4>(a, st);
+    if (mean <= 24) return launch_tile<T, 4, 1, 2, 2, 4>(a, st);
   }
-  if (mean <= 192) return launch_tile<T, 2, 2, 4, 4, 2>(a, st);
-  return launch_tile<T, 2, 4, 8, 4, 2>(a, st);
+  switch (best_tile(a, (size_t)a.n * bytes_of<T>)) {
+    case 0: return launch_tile<T, 2, 4, 8, 4, 2>(a, st);
+    case 1: return launch_tile<T, 4, 2, 4, 4, 3>(a, st);
+    case 2: return launch_tile<T, 2, 2, 4, 4, 3>(a, st);
+    case 3: return launch_tile<T, 2, 2, 4, 2, 3>(a, st);
+    case 4: return launch_tile<T, 2, 2, 2, 2, 4>(a, st);
+    default: return launch_tile<T, 2, 2, 2, 1, 4>(a, st);
+  }
 }
 hipError_t launch_product(const ProductArgs& a, int type, hipStream_t st) {
   return type == HTR_E4M3 ? launch_product<P_F8>(a, st) : type == HTR_BF16 ? launch_product<HTR_BF16>(a, st) : launch_product<HTR_F16>(a, st);
@@ -110,7 +147,7 @@ int product_shape(long long rows, int m, int n, int experts, int type, bool grou
   if (type != HTR_E4M3 && !is_16bit(type)) return HTR_ERR_DTYPE;
   if (rows < 0 || rows > (1ll << 31) - (1 << 20) || m < 1 || n < 1 || experts < 1 || experts > 65535 || n % (type == HTR_E4M3 ? 128 : 8)) return HTR_ERR_SIZE;
   if (m > (1 << 30) || n > (1 << 28)) return HTR_ERR_SIZE;
-  const long long tiles = span_bound(rows, experts, grouped, 128) * ((m + 127) / 128);
+  const long long tiles = span_bound(rows, experts, grouped, 32) * ((m + 63) / 64);
   return tiles > (1ll << 31) - 256 ? HTR_ERR_SIZE : HTR_OK;
 }
 
