@@ -20,6 +20,7 @@ struct ProductArgs {
   const int* ends;                       // [experts]: expert e has rows ends[e - 1] .. ends[e] - 1; NULL: one expert, all rows
   const int* gather;                     // row r of the product is row gather[r] of x; NULL: r
   int rows, m, n, experts, y_dtype;
+  float* ys;                             // k_product_tile<GATED> with y in e4m3: its scales, [rows][m / 256]
 };
 
 // Rows first .. first + count - 1 of expert e are tile number t of tiles of `height` rows, expert by expert; e = experts: rows behind the last
@@ -81,21 +82,7 @@ template <int T> __device__ __forceinline__ f4 mfma_16(const u4& a, const u4& b,
   else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
 }
 
-// four consecutive outputs of a row, from i on, as far as the row goes
-__device__ __forceinline__ void store4(const ProductArgs& a, f4 v, int row, int i) {
-  const size_t at = (size_t)row * a.m + i;
-  if (a.bias != nullptr) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] += load_elem_g(a.bias, a.y_dtype, min(i + k, a.m - 1));
-  }
-  if ((a.m & 3) == 0) {
-    if (a.y_dtype == HTR_F32) *(HTR_GLOBAL f4*)((HTR_GLOBAL float*)a.y + at) = v;
-    else *(HTR_GLOBAL u2*)((HTR_GLOBAL uint16_t*)a.y + at) = a.y_dtype == HTR_BF16 ? u2{pack_bf16(v.x, v.y), pack_bf16(v.z, v.w)} : u2{pack_f16(v.x, v.y), pack_f16(v.z, v.w)};
-  } else {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) if (i + k < a.m) store_elem_g(a.y, a.y_dtype, at + k, v[k]);
-  }
-}
+__device__ __forceinline__ float silu(float g) { return g / (1.f + __expf(-g)); }
 
 // ------------------------------------------------------------------------------------------------ few rows
 // A workgroup owns 16 R rows of a matrix and up to 16 TT rows of x; its waves take the slabs in turn, straight from memory into registers
@@ -199,6 +186,8 @@ __global__ __launch_bounds__(STREAM_WAVES * 64) void k_product_stream(const Prod
 // four fours of rows; two rows lie side by side in the banks, and the swizzles put the fours on different pairs of places.
 // Row number 4 q + j of a wave's MFMA tiles 2 h and 2 h + 1 are its rows 32 h + 8 q + j and + 4: a lane then holds eight consecutive outputs, and four
 // lanes 64 bytes of a row in 16 bits.
+// GATED: the matrix is gate over up, m / 2 rows each; a tile takes TM / 2 of either, 32 by 32 in turn, so that a lane holds gate and up of eight consecutive
+// hidden columns; y [rows][m / 2] is silu(gate) up, in 16 bits or in e4m3 (then TM / 2 = 128 columns share a scale; rows behind the last expert's are left).
 __device__ __forceinline__ int swizzle_w(int r) { return ((r >> 1) & 1) | ((r >> 3 & 3) << 1); }
 __device__ __forceinline__ int swizzle_x(int r) { return (r >> 1) & 7; }
 constexpr int TILE_XCDS = 8;
@@ -219,7 +208,7 @@ template <int Y> __device__ __forceinline__ void store8(const ProductArgs& a, fl
   }
 }
 
-template <int T, int WM, int WN, int AT, int BT, int NS>
+template <int T, int WM, int WN, int AT, int BT, int NS, bool GATED>
 __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductArgs a, int mtiles, int ttiles, int together) {
   constexpr int WAVES = WM * WN, TM = 16 * AT * WM, TN = 16 * BT * WN;
   constexpr int XW = (TN + 63) / 64;                             // waves that load rows' scales
@@ -229,6 +218,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
   constexpr int BARRIER = AT - RA + 1;                           // the tile of products before which the next slab has landed
   static_assert(T != P_F8 || XW < WAVES, "a wave for the matrix's scales");
   static_assert(AT % 2 == 0 && TM % (8 * WAVES) == 0 && TN % (8 * WAVES) == 0 && AT % RA == 0, "whole loads, registers in turn");
+  static_assert(!GATED || (AT % 4 == 0 && (T != P_F8 || TM == 256)), "32 gates and 32 ups to a wave; whole blocks of 128");
   extern __shared__ __align__(16) uint8_t lds[];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
   const int wm = wv / WN, wn = wv % WN;
@@ -248,7 +238,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
       const int rest = id - strip * mtiles * together;
       t.m0 = rest / high * TM;
       t.s = find_span(a, TN, t0 + rest % high);
-      if (t.s.e == a.experts) zero_rows(a, t.s, t.m0, TM);
+      if (t.s.e == a.experts) { if constexpr (!GATED) zero_rows(a, t.s, t.m0, TM); }
       else if (t.s.e >= 0) return true;
     }
     return false;
@@ -264,12 +254,14 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
   auto row_of = [&](int j) { return ((j < LW ? j : j - LW) * WAVES + wv) * 8 + (lane >> 3); };
   auto chunk_of = [&](int j) { return (lane & 7) ^ (j < LW ? swizzle_w(row_of(j)) : swizzle_x(row_of(j))); };
   auto source = [&](const Tile& t, Source& to) {
-    to.w = (const HTR_GLOBAL uint8_t*)a.w + ((size_t)t.s.e * a.m + t.m0) * row_bytes;
+    to.w = (const HTR_GLOBAL uint8_t*)a.w + ((size_t)t.s.e * a.m + (GATED ? 0 : t.m0)) * row_bytes;
     to.x = (const HTR_GLOBAL uint8_t*)a.x + (a.gather != nullptr ? 0 : (size_t)t.s.first * row_bytes);
 #pragma unroll
     for (int j = 0; j < L; ++j) {
       int r = row_of(j);
-      if (j < LW) {
+      if (GATED && j < LW) {
+        r = min((t.m0 >> 1) + (r >> 6 << 5) + (r & 31), (a.m >> 1) - 1) + (r & 32 ? a.m >> 1 : 0);
+      } else if (j < LW) {
         r = min(r, a.m - 1 - t.m0);      // beyond the matrix, or the expert's rows: the last row, whose results are not stored
       } else {
         r = min(r, t.s.count - 1);
@@ -287,8 +279,9 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
         to.scale = (uint32_t)r * (uint32_t)(a.n >> 7);
       } else {
         const int blocks = (a.m + 127) >> 7;
-        to.scales = (const HTR_GLOBAL float*)a.ws + ((size_t)t.s.e * blocks + (t.m0 >> 7)) * (a.n >> 7);
-        to.scale = (uint32_t)min(lane, blocks - 1 - (t.m0 >> 7)) * (uint32_t)(a.n >> 7);
+        const int block = t.m0 >> (GATED ? 8 : 7);      // GATED: the gates' in the first place, the ups' in the second
+        to.scales = (const HTR_GLOBAL float*)a.ws + ((size_t)t.s.e * blocks + block) * (a.n >> 7);
+        to.scale = (uint32_t)(GATED ? (lane & 1) * (blocks >> 1) : min(lane, blocks - 1 - block)) * (uint32_t)(a.n >> 7);
       }
     }
   };
@@ -335,7 +328,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
     rb[t] = TM * 128 + r * 128 + 16 * (g ^ swizzle_x(r));
   }
   u4 A[RA][2], B[BT][2];
-  float sx[BT], sw = 0.f;
+  float sx[BT], sw[GATED ? 2 : 1];
   auto read_a = [&](int i, int stage) {
     const uint8_t* base = lds + stage * STAGE;
     A[i % RA][0] = *(const u4*)(base + ra[i]); A[i % RA][1] = *(const u4*)(base + (ra[i] ^ 64));
@@ -348,7 +341,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
     const float* base = (const float*)(lds + stage * STAGE + (TM + TN) * 128);
 #pragma unroll
     for (int t = 0; t < BT; ++t) sx[t] = base[wn * 16 * BT + 16 * t + c];
-    sw = base[XW * 64 + ((wm * 16 * AT) >> 7)];
+    if constexpr (GATED) { sw[0] = base[XW * 64]; sw[1] = base[XW * 64 + 1]; } else sw[0] = base[XW * 64 + ((wm * 16 * AT) >> 7)];
   };
   f4 acc[AT][BT];
 #pragma unroll
@@ -365,12 +358,15 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
   // its last product; there lies the barrier, behind which the slab NS after this one, `ask`, is asked for, into this one's stage: a few loads with each
   // MFMA tile, the first of the next call's among them (`asked`); all at once they would keep the wave from its products for as long as they take to issue
   auto multiply = [&](int asked, Source& from, int ask, Source& from2, bool last_lands) {
-    float sc[BT];
+    float sc[GATED ? 2 : 1][BT];
     f4 part[3];
     const int next = after(stage, 1), prev = after(stage, NS - 1);
     if constexpr (T == P_F8) {
 #pragma unroll
-      for (int t = 0; t < BT; ++t) sc[t] = sx[t] * sw;
+      for (int t = 0; t < BT; ++t) {
+        sc[0][t] = sx[t] * sw[0];
+        if constexpr (GATED) sc[1][t] = sx[t] * sw[1];
+      }
     }
 #pragma unroll
     for (int i = 0; i < AT; ++i) {
@@ -388,7 +384,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
           // the sums two products behind the matrix unit
           const int k = i * BT + t, l = k - 2;
           part[k % 3] = mfma_f8(A[i % RA][0], A[i % RA][1], B[t][0], B[t][1]);
-          if (l >= 0) acc[l / BT][l % BT] += part[l % 3] * sc[l % BT];
+          if (l >= 0) acc[l / BT][l % BT] += part[l % 3] * sc[GATED ? l / BT >> 1 & 1 : 0][l % BT];
         } else {
           acc[i][t] = mfma_16<T>(A[i % RA][0], B[t][0], acc[i][t]);
           acc[i][t] = mfma_16<T>(A[i % RA][1], B[t][1], acc[i][t]);
@@ -404,7 +400,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
     }
     if constexpr (T == P_F8) {
 #pragma unroll
-      for (int l = AT * BT - 2; l < AT * BT; ++l) acc[l / BT][l % BT] += part[l % 3] * sc[l % BT];
+      for (int l = AT * BT - 2; l < AT * BT; ++l) acc[l / BT][l % BT] += part[l % 3] * sc[GATED ? l / BT >> 1 & 1 : 0][l % BT];
     }
     stage = next;
   };
@@ -439,24 +435,81 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
     src = src2;
     if (++slab < slabs) continue;
     slab = 0;
-    const int i0 = mine.m0 + wm * 16 * AT + 8 * g;               // first of the lane's outputs
-    auto put = [&](auto type) {
-      constexpr int Y = decltype(type)::value;
+    if constexpr (GATED) {
+      const int F = a.m >> 1, i0 = (mine.m0 >> 1) + wm * 8 * AT + 8 * g;      // hidden columns; first of the lane's
+      float amax[BT];
 #pragma unroll
       for (int t = 0; t < BT; ++t) {
-        const int r = wn * 16 * BT + 16 * t + c;
+        amax[t] = 0.f;
 #pragma unroll
-        for (int h = 0; h < AT / 2; ++h) {
-          float f[8];
+        for (int h = 0; h < AT / 4; ++h)
 #pragma unroll
-          for (int k = 0; k < 8; ++k) f[k] = acc[2 * h + (k >> 2)][t][k & 3];
-          if (r < mine.s.count && i0 + 32 * h < a.m) store8<Y>(a, f, (size_t)(mine.s.first + r) * a.m + i0 + 32 * h, i0 + 32 * h);
+          for (int k = 0; k < 8; ++k) {
+            float v = silu(acc[4 * h + (k >> 2)][t][k & 3]) * acc[4 * h + 2 + (k >> 2)][t][k & 3];
+            if constexpr (T == P_F8) { v = finite_or_nan(v); amax[t] = fmaxf(amax[t], fabsf(v)); }
+            acc[4 * h + (k >> 2)][t][k & 3] = v;
+          }
+      }
+      if constexpr (T == P_F8) {
+        // the waves' largest of each row; the last reads of the place lie a barrier of the main loop back
+        float* place = (float*)(lds + NS * STAGE);
+#pragma unroll
+        for (int t = 0; t < BT; ++t) {
+          amax[t] = fmaxf(amax[t], __shfl_xor(amax[t], 16));
+          amax[t] = fmaxf(amax[t], __shfl_xor(amax[t], 32));
+          if (g == 0) place[wm * TN + wn * 16 * BT + 16 * t + c] = amax[t];
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+        for (int t = 0; t < BT; ++t) {
+          const int r = wn * 16 * BT + 16 * t + c;
+          float m = place[r];
+#pragma unroll
+          for (int k = 1; k < WM; ++k) m = fmaxf(m, place[k * TN + r]);
+          const int e = e4m3_exponent((double)m);
+          const float inv = exp2i(-e);
+          if (r >= mine.s.count) continue;
+          const size_t row = (size_t)(mine.s.first + r);
+          if (wm == 0 && g == 0) ((HTR_GLOBAL float*)a.ys)[row * (F >> 7) + (mine.m0 >> 8)] = exp2i(e);
+#pragma unroll
+          for (int h = 0; h < AT / 4; ++h) {
+            const f4 lo = acc[4 * h][t] * inv, hi = acc[4 * h + 1][t] * inv;
+            *(HTR_GLOBAL u2*)((HTR_GLOBAL uint8_t*)a.y + row * F + i0 + 32 * h) = u2{pack_e4m3(lo.x, lo.y, lo.z, lo.w), pack_e4m3(hi.x, hi.y, hi.z, hi.w)};
+          }
+        }
+      } else {
+#pragma unroll
+        for (int t = 0; t < BT; ++t) {
+          const int r = wn * 16 * BT + 16 * t + c;
+#pragma unroll
+          for (int h = 0; h < AT / 4; ++h) {
+            float f[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) f[k] = acc[4 * h + (k >> 2)][t][k & 3];
+            if (r < mine.s.count && i0 + 32 * h < F) { Eight<T> v; v.set(f); v.store(a.y, (size_t)(mine.s.first + r) * F + i0 + 32 * h); }
+          }
         }
       }
-    };
-    if (a.y_dtype == HTR_BF16) put(std::integral_constant<int, HTR_BF16>());
-    else if (a.y_dtype == HTR_F16) put(std::integral_constant<int, HTR_F16>());
-    else put(std::integral_constant<int, HTR_F32>());
+    } else {
+      const int i0 = mine.m0 + wm * 16 * AT + 8 * g;               // first of the lane's outputs
+      auto put = [&](auto type) {
+        constexpr int Y = decltype(type)::value;
+#pragma unroll
+        for (int t = 0; t < BT; ++t) {
+          const int r = wn * 16 * BT + 16 * t + c;
+#pragma unroll
+          for (int h = 0; h < AT / 2; ++h) {
+            float f[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) f[k] = acc[2 * h + (k >> 2)][t][k & 3];
+            if (r < mine.s.count && i0 + 32 * h < a.m) store8<Y>(a, f, (size_t)(mine.s.first + r) * a.m + i0 + 32 * h, i0 + 32 * h);
+          }
+        }
+      };
+      if (a.y_dtype == HTR_BF16) put(std::integral_constant<int, HTR_BF16>());
+      else if (a.y_dtype == HTR_F16) put(std::integral_constant<int, HTR_F16>());
+      else put(std::integral_constant<int, HTR_F32>());
+    }
 #pragma unroll
     for (int i = 0; i < AT; ++i)
 #pragma unroll

@@ -80,18 +80,18 @@ template <int T, int R, int TT, int WAVES> hipError_t launch_stream(const Produc
   const long long tiles = span_bound(a.rows, a.experts, a.ends != nullptr, 16 * TT);
   return launch(k_product_stream<T, R, TT, WAVES>, dim3((a.m + 16 * R - 1) / (16 * R), (unsigned)tiles), WAVES * 64, 0, st, a);
 }
-template <int T, int WM, int WN, int AT, int BT, int NS> hipError_t launch_tile(const ProductArgs& a, hipStream_t st) {
+template <int T, int WM, int WN, int AT, int BT, int NS, bool GATED = false> hipError_t launch_tile(const ProductArgs& a, hipStream_t st) {
   constexpr int TM = 16 * AT * WM, TN = 16 * BT * WN;
-  constexpr size_t LDS = NS * ((TM + TN) * 128 + (T == P_F8 ? (TN + 63) / 64 * 256 + 256 : 0));
+  constexpr size_t LDS = NS * ((TM + TN) * 128 + (T == P_F8 ? (TN + 63) / 64 * 256 + 256 : 0)) + (GATED && T == P_F8 ? WM * TN * 4 : 0);
   static_assert(LDS <= 160 * 1024, "a compute unit's LDS");
   const long long mtiles = (a.m + TM - 1) / TM, ttiles = span_bound(a.rows, a.experts, a.ends != nullptr, TN), tiles = mtiles * ttiles;
-  const hipError_t e = allow_lds<k_product_tile<T, WM, WN, AT, BT, NS>>(LDS);
+  const hipError_t e = allow_lds<k_product_tile<T, WM, WN, AT, BT, NS, GATED>>(LDS);
   if (e != hipSuccess) return e;
   // as many workgroups as run at once (an MI355X has 256 compute units), a multiple of the XCDs; rows of fewer slabs than stages have no stream to run on from
   // tile to tile
   const bool stream = (long long)a.n * bytes_of<T> > 128 * (NS - 1);
   const long long wgs = 256 * (160 * 1024 / LDS), up = (tiles + TILE_XCDS - 1) / TILE_XCDS * TILE_XCDS;
-  return launch(k_product_tile<T, WM, WN, AT, BT, NS>, dim3((unsigned)(stream && wgs < up ? wgs : up)), WM * WN * 64, LDS, st, a, (int)mtiles, (int)ttiles, 8);
+  return launch(k_product_tile<T, WM, WN, AT, BT, NS, GATED>, dim3((unsigned)(stream && wgs < up ? wgs : up)), WM * WN * 64, LDS, st, a, (int)mtiles, (int)ttiles, 8);
 }
 // Which tiles for many rows: the ones whose rounds take the least time by what a slab of a tile takes where the compute units have little else to do
 // and where all are at work (measured on 64 .. 8192 rows of 4096 .. 14336 columns, ns; both types: their slabs have the same bytes).  A larger tile multiplies
@@ -100,11 +100,13 @@ template <int T, int WM, int WN, int AT, int BT, int NS> hipError_t launch_tile(
 struct TileChoice { int tm, tn, at_once; float light, full; };
 constexpr TileChoice TILES[] = {{256, 256, 1, 1450.f, 1950.f}, {256, 128, 1, 950.f, 1300.f}, {128, 128, 1, 700.f, 800.f},
                                 {128, 64, 2, 550.f, 850.f},    {64, 64, 2, 420.f, 600.f},    {64, 32, 3, 290.f, 450.f}};
-int best_tile(const ProductArgs& a, size_t row_bytes) {
+// gate and up in one: 128 hidden columns to a tile
+constexpr TileChoice GATED_TILES[] = {{256, 256, 1, 1450.f, 1950.f}, {256, 128, 1, 950.f, 1300.f}, {256, 64, 1, 750.f, 950.f}, {256, 32, 1, 600.f, 700.f}};
+template <int N> int best_tile(const TileChoice (&choices)[N], const ProductArgs& a, size_t row_bytes) {
   int best = 0;
   float least = 0.f;
-  for (int k = 0; k < (int)(sizeof(TILES) / sizeof(TILES[0])); ++k) {
-    const TileChoice& c = TILES[k];
+  for (int k = 0; k < N; ++k) {
+    const TileChoice& c = choices[k];
     const float mtiles = (float)((a.m + c.tm - 1) / c.tm), full = (float)a.rows / c.tn;
     const float experts = (float)(a.rows < a.experts ? a.rows : a.experts);
     // an expert's last tile is half full on average
@@ -130,7 +132,7 @@ template <int T> hipError_t launch_product(const ProductArgs& a, hipStream_t st)
     if (mean <= 4 && narrow) return launch_stream<T, 4, 1, 4>(a, st);
     if (mean <= 24) return launch_tile<T, 4, 1, 2, 2, 4>(a, st);
   }
-  switch (best_tile(a, (size_t)a.n * bytes_of<T>)) {
+  switch (best_tile(TILES, a, (size_t)a.n * bytes_of<T>)) {
     case 0: return launch_tile<T, 2, 4, 8, 4, 2>(a, st);
     case 1: return launch_tile<T, 4, 2, 4, 4, 3>(a, st);
     case 2: return launch_tile<T, 2, 2, 4, 4, 3>(a, st);
@@ -138,6 +140,19 @@ template <int T> hipError_t launch_product(const ProductArgs& a, hipStream_t st)
     case 4: return launch_tile<T, 2, 2, 2, 2, 4>(a, st);
     default: return launch_tile<T, 2, 2, 2, 1, 4>(a, st);
   }
+}
+// silu(gate) up of rows by expert, where one launch is the better way (few rows to an expert: the matrices are read by k_product_stream, k_gated follows)
+bool gates_in_one(long long rows, int experts) { return rows > 4ll * experts; }
+template <int T> hipError_t launch_gated_product(const ProductArgs& a, hipStream_t st) {
+  switch (best_tile(GATED_TILES, a, (size_t)a.n * bytes_of<T>)) {
+    case 0: return launch_tile<T, 2, 4, 8, 4, 2, true>(a, st);
+    case 1: return launch_tile<T, 4, 2, 4, 4, 3, true>(a, st);
+    case 2: return launch_tile<T, 2, 2, 8, 2, 3, true>(a, st);
+    default: return launch_tile<T, 4, 1, 4, 2, 4, true>(a, st);
+  }
+}
+hipError_t launch_gated_product(const ProductArgs& a, int type, hipStream_t st) {
+  return type == HTR_E4M3 ? launch_gated_product<P_F8>(a, st) : type == HTR_BF16 ? launch_gated_product<HTR_BF16>(a, st) : launch_gated_product<HTR_F16>(a, st);
 }
 hipError_t launch_product(const ProductArgs& a, int type, hipStream_t st) {
   return type == HTR_E4M3 ? launch_product<P_F8>(a, st) : type == HTR_BF16 ? launch_product<HTR_BF16>(a, st) : launch_product<HTR_F16>(a, st);
@@ -164,7 +179,7 @@ struct StackedScratch {
     pos_of = take(pairs * 4);
     xq = take(f8 ? (size_t)tokens * hidden : 0);
     xs = take(f8 ? (size_t)tokens * (hidden / 128) * 4 : 0);
-    h = take(pairs * 2 * inter * 4);
+    h = take(gates_in_one(pairs, experts) ? 0 : pairs * 2 * inter * 4);
     a = take(pairs * inter * (f8 ? 1 : 2));
     as = take(f8 ? pairs * (inter / 128) * 4 : 0);
     out = take(pairs * hidden * 4);
@@ -175,7 +190,9 @@ int stacked_shape(long long tokens, int top, int experts, int hidden, int inter,
   if (tokens < 1 || top < 1 || experts < 1 || hidden < 1 || inter < 1 || top > 4096 || tokens > (1 << 24) || inter > (1 << 28)) return HTR_ERR_SIZE;
   if (type != HTR_E4M3 && !is_16bit(type)) return HTR_ERR_DTYPE;
   if (hidden % 8 || inter % (type == HTR_E4M3 ? 128 : 8)) return HTR_ERR_SIZE;
-  if (tokens * top > (1 << 30)) return HTR_ERR_SIZE;
+  // loads go by 32-bit distances from x, from the gathered rows' scales and from an expert's matrices
+  const unsigned long long size = type == HTR_E4M3 ? 1 : 2, most = 1ull << 32;
+  if (tokens * top > (1 << 30) || (unsigned long long)tokens * hidden * size >= most || 2ull * inter * hidden * size >= most) return HTR_ERR_SIZE;
   const int rc = product_shape(tokens * top, 2 * inter, hidden, experts, type, true);
   return rc != HTR_OK ? rc : product_shape(tokens * top, hidden, inter, experts, type, true);
 }
@@ -228,7 +245,7 @@ int htr_product(const void* x, const void* x_scales, const void* w, const void* 
   if (!aligned(x, 16) || !aligned(w, 16) || !aligned(y, 16) || !aligned(x_scales, 4) || !aligned(w_scales, 4) || !aligned(ends, 4) ||
       !aligned(bias, element_bytes(y_dtype)))
     return HTR_ERR_ALIGN;
-  const ProductArgs a{x, (const float*)x_scales, w, (const float*)w_scales, bias, y, ends, nullptr, (int)rows, m, n, experts, y_dtype};
+  const ProductArgs a{x, (const float*)x_scales, w, (const float*)w_scales, bias, y, ends, nullptr, (int)rows, m, n, experts, y_dtype, nullptr};
   TRY_HIP(launch_product(a, type, (hipStream_t)stream));
   return HTR_OK;
 }
@@ -255,17 +272,22 @@ int htr_moe_stacked(const void* x, int dtype, const void* ids, int ids_int64, co
   const int pairs = (int)(tokens * top);
   int *ends = (int*)(s + at.ends), *token = (int*)(s + at.token), *pos_of = (int*)(s + at.pos_of);
   float *h = (float*)(s + at.h), *out = (float*)(s + at.out);
-  TRY_HIP(launch(k_expert_order, dim3(experts), ORDER_THREADS, 0, st, ids, ids_int64, pairs, top, experts, ends, token, pos_of));
-  ProductArgs a{x, nullptr, gate_up, (const float*)gate_up_scales, nullptr, h, ends, token, pairs, 2 * inter, hidden, experts, HTR_F32};
+  TRY_HIP(launch(k_expert_order, dim3(experts), ORDER_WAVES * 64, 0, st, ids, ids_int64, pairs, top, experts, ends, token, pos_of));
+  ProductArgs a{x, nullptr, gate_up, (const float*)gate_up_scales, nullptr, h, ends, token, pairs, 2 * inter, hidden, experts, HTR_F32, nullptr};
   if (f8) {
     TRY_HIP(launch_quantize(x, dtype, tokens, hidden, hidden, s + at.xq, (float*)(s + at.xs), st));
     a.x = s + at.xq; a.xs = (const float*)(s + at.xs);
   }
-  TRY_HIP(launch_product(a, type, st));
-  TRY_HIP(f8 ? launch(k_gated<P_F8>, dim3(pairs), 256, 0, st, h, ends, experts, inter, s + at.a, (float*)(s + at.as))
-             : dtype == HTR_BF16 ? launch(k_gated<HTR_BF16>, dim3(pairs), 256, 0, st, h, ends, experts, inter, s + at.a, nullptr)
-                                 : launch(k_gated<HTR_F16>, dim3(pairs), 256, 0, st, h, ends, experts, inter, s + at.a, nullptr));
-  const ProductArgs d{s + at.a, (const float*)(s + at.as), down, (const float*)down_scales, nullptr, out, ends, nullptr, pairs, hidden, inter, experts, HTR_F32};
+  if (gates_in_one(pairs, experts)) {
+    a.y = s + at.a; a.ys = (float*)(s + at.as); a.y_dtype = type;
+    TRY_HIP(launch_gated_product(a, type, st));
+  } else {
+    TRY_HIP(launch_product(a, type, st));
+    TRY_HIP(f8 ? launch(k_gated<P_F8>, dim3(pairs), 256, 0, st, h, ends, experts, inter, s + at.a, (float*)(s + at.as))
+               : dtype == HTR_BF16 ? launch(k_gated<HTR_BF16>, dim3(pairs), 256, 0, st, h, ends, experts, inter, s + at.a, nullptr)
+                                   : launch(k_gated<HTR_F16>, dim3(pairs), 256, 0, st, h, ends, experts, inter, s + at.a, nullptr));
+  }
+  const ProductArgs d{s + at.a, (const float*)(s + at.as), down, (const float*)down_scales, nullptr, out, ends, nullptr, pairs, hidden, inter, experts, HTR_F32, nullptr};
   TRY_HIP(launch_product(d, type, st));
   const dim3 grid((unsigned)tokens, (hidden + 2047) / 2048);
   TRY_HIP(dtype == HTR_BF16 ? launch(k_weighted_sum<HTR_BF16>, grid, 256, 0, st, out, pos_of, weights, top, hidden, y)
