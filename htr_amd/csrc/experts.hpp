@@ -14,19 +14,26 @@ __global__ __launch_bounds__(ORDER_WAVES * 64) void k_expert_order(const void* _
   __shared__ int s_less[ORDER_WAVES], s_same[ORDER_WAVES];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), e = blockIdx.x;
   const int per = (pairs + ORDER_WAVES * 64 - 1) / (ORDER_WAVES * 64) * 64, p0 = min(pairs, wv * per), p1 = min(pairs, p0 + per);
-  // -1: out of range, or no pair
-  auto id_of = [&](int p) {
-    if (p >= p1) return -1;
-    const long long v = ids64 ? ((const HTR_GLOBAL long long*)ids)[p] : (long long)((const HTR_GLOBAL int*)ids)[p];
-    return v < 0 || v >= experts ? -1 : (int)v;
+  // AHEAD loads on their way at once: -1 for an expert out of range, or no pair
+  constexpr int AHEAD = 8;
+  auto load = [&](int q, int (&v)[AHEAD]) {
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int p = min(q + 64 * k + lane, pairs - 1);
+      const long long id = ids64 ? ((const HTR_GLOBAL long long*)ids)[p] : (long long)((const HTR_GLOBAL int*)ids)[p];
+      v[k] = id < 0 || id >= experts || q + 64 * k + lane >= p1 ? -1 : (int)id;
+    }
   };
   int less = 0, same = 0;
-#pragma unroll 4
-  for (int q = p0; q < p1; q += 64) {
-    const int v = id_of(q + lane);
-    less += (int)__builtin_popcountll(__ballot(v >= 0 && v < e));
-    same += (int)__builtin_popcountll(__ballot(v == e));
-    if (e == 0 && v < 0 && q + lane < p1) pos_of[q + lane] = -1;
+  for (int q = p0; q < p1; q += 64 * AHEAD) {
+    int v[AHEAD];
+    load(q, v);
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      less += (int)__builtin_popcountll(__ballot(v[k] >= 0 && v[k] < e));
+      same += (int)__builtin_popcountll(__ballot(v[k] == e));
+      if (e == 0 && v[k] < 0 && q + 64 * k + lane < p1) pos_of[q + 64 * k + lane] = -1;
+    }
   }
   if (lane == 0) { s_less[wv] = less; s_same[wv] = same; }
   __syncthreads();
@@ -37,16 +44,19 @@ __global__ __launch_bounds__(ORDER_WAVES * 64) void k_expert_order(const void* _
   }
   if (threadIdx.x == 0) ends[e] = total;
   if (same == 0) return;
-#pragma unroll 4
-  for (int q = p0; q < p1; q += 64) {
-    const int p = q + lane;
-    const unsigned long long mine = __ballot(id_of(p) == e);
-    if (mine >> lane & 1ull) {
-      const int pos = at + (int)__builtin_popcountll(mine & ((1ull << lane) - 1ull));
-      token[pos] = p / top;
-      pos_of[p] = pos;
+  for (int q = p0; q < p1; q += 64 * AHEAD) {
+    int v[AHEAD];
+    load(q, v);
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const unsigned long long mine = __ballot(v[k] == e);
+      if (mine >> lane & 1ull) {
+        const int p = q + 64 * k + lane, pos = at + (int)__builtin_popcountll(mine & ((1ull << lane) - 1ull));
+        token[pos] = p / top;
+        pos_of[p] = pos;
+      }
+      at += (int)__builtin_popcountll(mine);
     }
-    at += (int)__builtin_popcountll(mine);
   }
 }
 
