@@ -96,7 +96,9 @@ def fast():
             module.bind(L.htr_abi_version(), str(torch.__version__), address(L.htr_linear), address(L.htr_stream_capture_id),
                         address(L.htr_moe_scratch_bytes), address(L.htr_moe_experts),
                         address(L.htr_linear_route), address(L.htr_dequant_w))
-        except ImportError as e:
+            module.bind_unpacked(address(L.htr_rms_norm), address(L.htr_quantize_e4m3), address(L.htr_product),
+                                 address(L.htr_moe_stacked_scratch_bytes), address(L.htr_moe_stacked))
+        except (ImportError, AttributeError) as e:
             warnings.warn(f"htr_amd/_fast.so cannot be used ({e}): launches are prepared in Python; `python -m htr_amd.build` builds it",
                           RuntimeWarning, stacklevel=2)
             _fast = False

@@ -1,4 +1,4 @@
-// htr_amd._fast: the host side of a packed linear and of a routed-expert layer on torch tensors, in C++.
+// htr_amd._fast: the host side of a packed linear, of a routed-expert layer and of the operators around them on torch tensors, in C++.
 //
 // A decode launch takes the GPU 6 microseconds and took the interpreter 16 (a dozen attribute reads, shape checks, two
 // dictionary look-ups, a 19-argument foreign call), so small calls ran at the interpreter's pace; collecting the 512
@@ -26,6 +26,11 @@ decltype(&htr_moe_scratch_bytes) f_moe_bytes = nullptr;
 decltype(&htr_moe_experts) f_moe = nullptr;
 decltype(&htr_linear_route) f_route = nullptr;
 decltype(&htr_dequant_w) f_dequant = nullptr;
+decltype(&htr_rms_norm) f_norm = nullptr;
+decltype(&htr_quantize_e4m3) f_quantize = nullptr;
+decltype(&htr_product) f_product = nullptr;
+decltype(&htr_moe_stacked_scratch_bytes) f_stacked_bytes = nullptr;
+decltype(&htr_moe_stacked) f_stacked = nullptr;
 
 int dtype_code(at::ScalarType t) {
   switch (t) {
@@ -224,6 +229,185 @@ PyObject* wait_word(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- the operators around the packed linears (htr_amd/unpacked.py): the common case of each, None where the Python path is to handle the call or refuse it
+bool float_of(const at::Tensor& t) { return dtype_code(t.scalar_type()) >= 0; }
+bool half_of(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf; }
+bool aligned16(const at::Tensor& t) { return ((uintptr_t)t.const_data_ptr() & 15) == 0; }
+// consecutive memory on `dev` from a 16-byte boundary on, that torch does not follow
+bool plain(const at::Tensor& t, c10::Device dev) { return t.device() == dev && raw_ok(t) && t.is_contiguous() && aligned16(t) && !differentiable(t); }
+at::ScalarType type_of(long code) { return code == 0 ? at::kBFloat16 : code == 1 ? at::kHalf : at::kFloat; }
+// dims of 8-bit rows' scales (rows = true) or matrices' for values q
+bool scales_ok(const at::Tensor& q, const at::Tensor& s, bool rows) {
+  if (s.scalar_type() != at::kFloat || s.dim() != q.dim() || q.dim() < (rows ? 1 : 2) || q.size(-1) % 128 || s.size(-1) != q.size(-1) / 128) return false;
+  for (int64_t k = 0; k + 1 < q.dim(); ++k) {
+    const bool m = !rows && k + 2 == q.dim();
+    if (s.size(k) != (m ? (q.size(k) + 127) / 128 : q.size(k))) return false;
+  }
+  return true;
+}
+// x as 8-bit rows; a tensor of floats is rounded.  False: not as expected; rc: what the launch returned
+bool rows8(const at::Tensor& x, const at::Tensor* s, c10::Device dev, void* stream, at::Tensor& q, at::Tensor& qs, int& rc) {
+  if (s != nullptr) {
+    if (x.scalar_type() != at::kFloat8_e4m3fn || !scales_ok(x, *s, true) || !plain(*s, dev)) return false;
+    q = x; qs = *s;
+    return true;
+  }
+  const int64_t n = x.size(-1);
+  if (!float_of(x) || n % 128) return false;
+  at::DimVector shape(x.sizes().begin(), x.sizes().end());
+  q = at::empty(shape, x.options().dtype(at::kFloat8_e4m3fn));
+  shape.back() = n / 128;
+  qs = at::empty(shape, x.options().dtype(at::kFloat));
+  rc = f_quantize(x.const_data_ptr(), n, x.numel() / n, (int)n, dtype_code(x.scalar_type()), q.mutable_data_ptr(), qs.mutable_data_ptr(), stream);
+  return rc == HTR_OK;
+}
+// optional tensor argument: false where it is neither None nor a tensor
+bool optional(PyObject* o, const at::Tensor*& t) { t = o == Py_None ? nullptr : tensor_of(o); return o == Py_None || t != nullptr; }
+
+// rms_norm(x, weight, eps, residual or None, quantize, stream)
+PyObject* rms_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  const at::Tensor *x, *w, *r;
+  if (nargs != 6 || f_norm == nullptr || !THPVariable_CheckExact(args[0]) || !optional(args[1], w) || w == nullptr || !optional(args[3], r)) Py_RETURN_NONE;
+  x = tensor_of(args[0]);
+  const double eps = PyFloat_AsDouble(args[2]);
+  const int quantize = PyObject_IsTrue(args[4]);
+  void* stream = PyLong_AsVoidPtr(args[5]);
+  if (PyErr_Occurred()) return nullptr;
+  if (!x->is_cuda() || x->dim() < 1 || !float_of(*x) || x->numel() == 0) Py_RETURN_NONE;
+  const c10::Device dev = x->device();
+  const int64_t n = x->size(-1), rows = x->numel() / n;
+  if (!plain(*x, dev) || !plain(*w, dev) || w->scalar_type() != x->scalar_type() || w->dim() != 1 || w->size(0) != n || (quantize && n % 128) || n > (1 << 30)) Py_RETURN_NONE;
+  if (r != nullptr && (!plain(*r, dev) || r->scalar_type() != x->scalar_type() || r->sizes() != x->sizes())) Py_RETURN_NONE;
+  at::Tensor y, s, t;
+  int rc;
+  {
+    pybind11::gil_scoped_release no_lock;      // as in linear()
+    c10::DeviceGuard guard(dev);
+    y = at::empty(x->sizes(), quantize ? x->options().dtype(at::kFloat8_e4m3fn) : x->options());
+    if (quantize) {
+      at::DimVector shape(x->sizes().begin(), x->sizes().end());
+      shape.back() = n / 128;
+      s = at::empty(shape, x->options().dtype(at::kFloat));
+    }
+    if (r != nullptr) t = at::empty(x->sizes(), x->options());
+    rc = f_norm(x->const_data_ptr(), n, r == nullptr ? nullptr : r->const_data_ptr(), n, w->const_data_ptr(), rows, (int)n, eps, dtype_code(x->scalar_type()),
+                y.mutable_data_ptr(), quantize ? s.mutable_data_ptr() : nullptr, r == nullptr ? nullptr : t.mutable_data_ptr(), stream);
+  }
+  if (rc != HTR_OK) Py_RETURN_NONE;
+  PyObject* out = THPVariable_Wrap(std::move(y));
+  if (quantize) out = PyTuple_Pack(2, Owned{out}.p, Owned{THPVariable_Wrap(std::move(s))}.p);
+  if (r != nullptr) out = PyTuple_Pack(2, Owned{out}.p, Owned{THPVariable_Wrap(std::move(t))}.p);
+  return out;
+  END_HANDLE_TH_ERRORS
+}
+
+// product(x, its scales or None, weight, its scales or None, bias or None, ends or None, the result's type code, stream): linear_fp8 where ends is None,
+// otherwise grouped_mm
+PyObject* product(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  const at::Tensor *x, *xs, *w, *ws, *bias, *ends;
+  if (nargs != 8 || f_product == nullptr || !THPVariable_CheckExact(args[0]) || !optional(args[1], xs) || !optional(args[2], w) || w == nullptr ||
+      !optional(args[3], ws) || !optional(args[4], bias) || !optional(args[5], ends))
+    Py_RETURN_NONE;
+  x = tensor_of(args[0]);
+  const long code = PyLong_AsLong(args[6]);
+  void* stream = PyLong_AsVoidPtr(args[7]);
+  if (PyErr_Occurred()) return nullptr;
+  const int64_t dims = ends == nullptr ? 2 : 3;
+  if (code < 0 || code > 2 || !x->is_cuda() || x->dim() < 1 || x->numel() == 0 || w->dim() != dims || w->numel() == 0) Py_RETURN_NONE;
+  const c10::Device dev = x->device();
+  const int64_t n = w->size(-1), m = w->size(-2), experts = ends == nullptr ? 1 : w->size(0);
+  const bool eight = ws != nullptr;
+  if (x->size(-1) != n || !plain(*x, dev) || !plain(*w, dev) || m > (1 << 30) || n > (1 << 30) || experts > (1 << 30)) Py_RETURN_NONE;
+  if (ends != nullptr && (x->dim() != 2 || ends->scalar_type() != at::kInt || ends->dim() != 1 || ends->size(0) != experts || ends->device() != dev || !ends->is_contiguous()))
+    Py_RETURN_NONE;
+  if (eight ? w->scalar_type() != at::kFloat8_e4m3fn || !scales_ok(*w, *ws, false) || ws->device() != dev || !ws->is_contiguous() || differentiable(*ws)
+            : ends == nullptr || xs != nullptr || !half_of(*w) || x->scalar_type() != w->scalar_type() || n % 8)
+    Py_RETURN_NONE;
+  if (bias != nullptr && (ends != nullptr || bias->scalar_type() != type_of(code) || bias->dim() != 1 || bias->size(0) != m || bias->device() != dev ||
+                          !bias->is_contiguous() || !raw_ok(*bias) || differentiable(*bias)))
+    Py_RETURN_NONE;
+  at::Tensor y, q, qs;
+  int rc = HTR_OK;
+  {
+    pybind11::gil_scoped_release no_lock;      // as in linear()
+    c10::DeviceGuard guard(dev);
+    if (!eight) q = *x;
+    if (eight && !rows8(*x, xs, dev, stream, q, qs, rc)) {
+      rc = HTR_ERR_SIZE;
+    } else {
+      at::DimVector shape(x->sizes().begin(), x->sizes().end());
+      shape.back() = m;
+      y = at::empty(shape, x->options().dtype(type_of(code)));
+      rc = f_product(q.const_data_ptr(), eight ? qs.const_data_ptr() : nullptr, w->const_data_ptr(), eight ? ws->const_data_ptr() : nullptr,
+                     bias == nullptr ? nullptr : bias->const_data_ptr(), ends == nullptr ? nullptr : (const int32_t*)ends->const_data_ptr(), y.mutable_data_ptr(),
+                     x->numel() / n, (int)m, (int)n, (int)experts, eight ? HTR_E4M3 : dtype_code(w->scalar_type()), (int)code, stream);
+    }
+  }
+  if (rc != HTR_OK) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// moe_stacked(x, ids, weights, gate_up, its scales or None, down, its scales or None, stream)
+PyObject* moe_stacked(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  const at::Tensor* t[7];
+  if (nargs != 8 || f_stacked == nullptr || !THPVariable_CheckExact(args[0])) Py_RETURN_NONE;
+  for (int i = 0; i < 7; ++i) if (!optional(args[i], t[i]) || (t[i] == nullptr && i != 4 && i != 6)) Py_RETURN_NONE;
+  void* stream = PyLong_AsVoidPtr(args[7]);
+  if (PyErr_Occurred()) return nullptr;
+  const at::Tensor &x = *t[0], &ids = *t[1], &wt = *t[2], &gu = *t[3], &dn = *t[5];
+  const bool eight = t[4] != nullptr;
+  if (!x.is_cuda() || x.dim() != 2 || !half_of(x) || x.numel() == 0 || ids.dim() != 2 || ids.numel() == 0 || gu.dim() != 3 || dn.dim() != 3 || eight != (t[6] != nullptr))
+    Py_RETURN_NONE;
+  const c10::Device dev = x.device();
+  const int64_t T = x.size(0), H = x.size(1), top = ids.size(1), E = dn.size(0), F = dn.size(2);
+  if (!plain(x, dev) || !plain(gu, dev) || !plain(dn, dev) || dn.size(1) != H || gu.size(0) != E || gu.size(1) != 2 * F || gu.size(2) != H || F < 1 || E < 1) Py_RETURN_NONE;
+  if (E > (1 << 20) || F > (1 << 28) || H > (1 << 28) || top > (1 << 20)) Py_RETURN_NONE;
+  if (eight) {
+    for (int i = 3; i < 7; i += 2)
+      if (t[i]->scalar_type() != at::kFloat8_e4m3fn || !scales_ok(*t[i], *t[i + 1], false) || t[i + 1]->device() != dev || !t[i + 1]->is_contiguous() || differentiable(*t[i + 1]))
+        Py_RETURN_NONE;
+  } else if (gu.scalar_type() != x.scalar_type() || dn.scalar_type() != x.scalar_type()) {
+    Py_RETURN_NONE;
+  }
+  if (ids.size(0) != T || wt.dim() != 2 || wt.size(0) != T || wt.size(1) != top || ids.device() != dev || !ids.is_contiguous() || !raw_ok(ids) ||
+      (ids.scalar_type() != at::kLong && ids.scalar_type() != at::kInt) || wt.device() != dev || wt.scalar_type() != at::kFloat || !wt.is_contiguous() || !raw_ok(wt) ||
+      differentiable(wt))
+    Py_RETURN_NONE;
+  const int dtype = dtype_code(x.scalar_type()), type = eight ? HTR_E4M3 : dtype;
+  const size_t need = f_stacked_bytes(T, (int)top, (int)E, (int)H, (int)F, type);
+  if (need == 0) Py_RETURN_NONE;
+  at::Tensor y;
+  int rc;
+  {
+    pybind11::gil_scoped_release no_lock;      // as in linear()
+    c10::DeviceGuard guard(dev);
+    at::Tensor scratch = at::empty({(int64_t)need}, x.options().dtype(at::kByte));
+    y = at::empty({T, H}, x.options());
+    rc = f_stacked(x.const_data_ptr(), dtype, ids.const_data_ptr(), ids.scalar_type() == at::kLong ? 1 : 0, (const float*)wt.const_data_ptr(), T, (int)top,
+                   gu.const_data_ptr(), eight ? t[4]->const_data_ptr() : nullptr, dn.const_data_ptr(), eight ? t[6]->const_data_ptr() : nullptr, (int)E, (int)H, (int)F, type,
+                   y.mutable_data_ptr(), scratch.mutable_data_ptr(), need, stream);
+  }
+  if (rc == HTR_ERR_LAUNCH) return PyLong_FromLong(rc);      // part of the layer may be queued: an error, not another way to run it
+  if (rc != HTR_OK) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// bind_unpacked(addresses of htr_rms_norm, htr_quantize_e4m3, htr_product, htr_moe_stacked_scratch_bytes, htr_moe_stacked), after bind()
+PyObject* bind_unpacked(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 5) { PyErr_SetString(PyExc_TypeError, "bind_unpacked wants five addresses"); return nullptr; }
+  void* p[5];
+  for (int i = 0; i < 5; ++i) p[i] = PyLong_AsVoidPtr(args[i]);
+  if (PyErr_Occurred()) return nullptr;
+  f_norm = (decltype(f_norm))p[0]; f_quantize = (decltype(f_quantize))p[1]; f_product = (decltype(f_product))p[2];
+  f_stacked_bytes = (decltype(f_stacked_bytes))p[3]; f_stacked = (decltype(f_stacked))p[4];
+  Py_RETURN_NONE;
+}
+
 // bind(version of the library's C ABI, version of the running torch, addresses of htr_linear, htr_stream_capture_id,
 // htr_moe_scratch_bytes, htr_moe_experts and, for linear() beyond 128 rows, htr_linear_route and htr_dequant_w); ImportError where either
 // version is not the one that this file was compiled with
@@ -245,6 +429,10 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 PyMethodDef methods[] = {{"bind", (PyCFunction)(void*)bind, METH_FASTCALL, nullptr},
                          {"linear", (PyCFunction)(void*)linear, METH_FASTCALL, nullptr},
                          {"moe", (PyCFunction)(void*)moe, METH_FASTCALL, nullptr},
+                         {"bind_unpacked", (PyCFunction)(void*)bind_unpacked, METH_FASTCALL, nullptr},
+                         {"rms_norm", (PyCFunction)(void*)rms_norm, METH_FASTCALL, nullptr},
+                         {"product", (PyCFunction)(void*)product, METH_FASTCALL, nullptr},
+                         {"moe_stacked", (PyCFunction)(void*)moe_stacked, METH_FASTCALL, nullptr},
                          {"wait_word", (PyCFunction)(void*)wait_word, METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fast", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -35,6 +35,17 @@ def _refuse_derivatives(what, *tensors):
             raise RuntimeError(f"{what} has no derivative: call it under torch.no_grad(), or on detached tensors")
 
 
+def _fast(x):
+    """(the C++ host path, the current stream of x's device), or None where there is none for it: tracers' tensors, the CPU."""
+    if type(x) is not torch.Tensor or torch.compiler.is_compiling():
+        return None
+    index = x.get_device()
+    if index < 0:
+        return None
+    fast = _native.fast()
+    return None if fast is None else (fast, _raw_stream(index))
+
+
 def _on_one_gpu(what, first, *others):
     if not first.is_cuda:
         raise RuntimeError(f"{what} runs on a ROCm device only; move the tensors to the GPU")
@@ -69,6 +80,11 @@ def rms_norm(x, weight, eps=1e-6, residual=None, quantize=False):
 
     x [..., n] and residual bfloat16, float16 or float32, weight [n] of the same type.  Returns y in x's type, or with quantize=True the pair
     (values, scales) of y in e4m3 (n a multiple of 128); with a residual, (that, t): t is the next block's residual."""
+    path = _fast(x)
+    if path is not None:
+        y = path[0].rms_norm(x, weight, eps, residual, quantize, path[1])
+        if y is not None:
+            return y
     if x.dim() < 1 or x.dtype not in _FLOATS or weight.dtype != x.dtype or weight.shape != x.shape[-1:]:
         raise RuntimeError("rms_norm wants x [..., n] in bfloat16, float16 or float32 and a weight [n] of that type")
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
@@ -166,11 +182,25 @@ def _out_dtype(what, out_dtype, x, bias=None):
     return out_dtype
 
 
+def _product(x, w, ws, bias, ends, out_dtype):
+    """The common case of the products in C++; None where something else is asked for, or is wrong."""
+    q, s = x if type(x) is tuple and len(x) == 2 else (x, None)
+    path = _fast(q)
+    if path is None:
+        return None
+    if out_dtype is None:
+        out_dtype = q.dtype if s is None else torch.bfloat16 if bias is None else bias.dtype
+    return path[0].product(q, s, w, ws, bias, ends, _CODE.get(out_dtype, -1), path[1])
+
+
 def linear_fp8(x, qweight, scales, bias=None, out_dtype=None):
     """y = x @ W^T (+ bias), W [m, n] in e4m3 with a float32 scale for each 128x128 block, any m.
 
     x: [..., n] in bfloat16, float16 or float32, which is rounded to e4m3 for each 128 columns, or 8-bit rows (values, scales) as rms_norm and quantize_fp8
     give them.  y is of x's type; for 8-bit rows of the bias's, or bfloat16, unless out_dtype says."""
+    y = _product(x, qweight, scales, bias, None, out_dtype)
+    if y is not None:
+        return y
     _check_matrix("linear_fp8", qweight, scales, 2)
     m, n = qweight.shape
     dtype = _out_dtype("linear_fp8", out_dtype, x, bias)
@@ -197,6 +227,10 @@ def grouped_mm(x, weight, ends, out_dtype=None):
     8-bit rows or rounded to them.  ends: int32 [E] on the device (the running sum of the experts' row counts); an end below an earlier one counts as
     that one, one beyond R as R; rows from the last end on become zeros.  y [R, m] in x's type (8-bit rows: bfloat16) unless out_dtype says."""
     eight = _pair(weight)
+    if ends is not None:
+        y = _product(x, weight[0], weight[1], None, ends, out_dtype) if eight else _product(x, weight, None, None, ends, out_dtype)
+        if y is not None:
+            return y
     first = x[0] if _pair(x) else x
     if eight:
         _check_matrix("grouped_mm", weight[0], weight[1], 3)
@@ -235,6 +269,14 @@ def moe_experts_stacked(x, expert_ids, expert_weights, gate_up, down):
     Sums are float32; the hidden values are rounded to x's type or e4m3, y [T, H] to x's type.  A token with an expert number out of range
     becomes NaN."""
     eight = _pair(gate_up) and _pair(down)
+    path = _fast(x)
+    if path is not None:
+        (gu, gus), (dn, dns) = (gate_up, down) if eight else ((gate_up, None), (down, None))
+        y = path[0].moe_stacked(x, expert_ids, expert_weights, gu, gus, dn, dns, path[1])
+        if y is not None:
+            if type(y) is int:
+                _native.check(y)
+            return y
     if x.dim() != 2 or x.dtype not in _HALVES:
         raise RuntimeError("moe_experts_stacked wants x [T, H] in bfloat16 or float16")
     if eight:

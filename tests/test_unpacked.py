@@ -482,3 +482,67 @@ def test_status_codes_without_a_gpu():
         L.htr_moe_stacked(x, dt, p, 1, p, T, 2, p, gus, p, gus, 8, 256, 128, t, y, sc, bytes, None)
     assert moe(T=0) == 11 and moe(dt=2) == 5 and moe(dt=1) == 5 and moe(t=3) == 1 and moe(x=None) == 1 and moe(y=odd) == 7
     assert moe(sc=None) == 6 and moe(sc=ctypes.c_void_p(0x1010)) == 6 and moe(bytes=100) == 6
+
+
+# ---- the C++ host path and the Python one
+@pytest.mark.gpu
+def test_both_host_paths_agree(gen, monkeypatch):
+    x, w = randn(gen, 5, 256, dtype=BF16), randn(gen, 256, dtype=BF16)
+    r, b = randn(gen, 5, 256, dtype=BF16), randn(gen, 64, dtype=BF16)
+    q, s = fp8_weight(gen, 64, 256)
+    gu8, dn8 = fp8_weight(gen, 3, 256, 256), fp8_weight(gen, 3, 256, 128)
+    gu, dn = randn(gen, 3, 256, 256, dtype=BF16), randn(gen, 3, 256, 128, dtype=BF16)
+    ends = torch.tensor([2, 2, 4], dtype=torch.int32, device="cuda")
+    ids, wt = torch.tensor([[0, 2], [1, 1], [2, 0], [0, 1], [2, 2]], device="cuda"), torch.rand(5, 2, device="cuda", generator=gen)
+    xq = ops.quantize_fp8(x)
+    calls = [lambda: ops.rms_norm(x, w), lambda: ops.rms_norm(x, w, 1e-5, residual=r), lambda: ops.rms_norm(x, w, residual=r, quantize=True),
+             lambda: ops.rms_norm(x, w, quantize=True), lambda: ops.linear_fp8(x, q, s, b), lambda: ops.linear_fp8(xq, q, s, out_dtype=F32),
+             lambda: ops.linear_fp8(x.float(), q, s), lambda: ops.grouped_mm(x, gu, ends), lambda: ops.grouped_mm(xq, gu8, ends),
+             lambda: ops.grouped_mm(x, gu8, ends, out_dtype=F16), lambda: ops.moe_experts_stacked(x, ids, wt, gu, dn),
+             lambda: ops.moe_experts_stacked(x, ids, wt, gu8, dn8)]
+    flat = lambda o: [o] if isinstance(o, torch.Tensor) else [t for p in o for t in flat(p)]
+    taken = []
+    fast = _native.fast()
+    assert fast is not None
+
+    class Spy:
+        def __getattr__(self, name):
+            def call(*a):
+                y = getattr(fast, name)(*a)
+                taken.append((name, y is not None))
+                return y
+            return call
+
+    for call in calls:
+        monkeypatch.setattr(_native, "fast", Spy)
+        taken.clear()
+        got = flat(call())
+        assert len(taken) == 1 and taken[0][1], taken                  # the C++ path took it
+        monkeypatch.setattr(_native, "fast", lambda: None)
+        want = flat(call())
+        assert len(got) == len(want)
+        for u, v in zip(got, want):
+            assert u.dtype == v.dtype and u.shape == v.shape and torch.equal(u.float(), v.float())
+
+
+@pytest.mark.gpu
+def test_the_cxx_path_leaves_the_rest_to_python(gen):
+    """What it does not take is handled by the other path, or refused there: it queues nothing and raises nothing."""
+    fast, stream = _native.fast(), torch.cuda.current_stream().cuda_stream
+    x, w = randn(gen, 4, 256, dtype=BF16), randn(gen, 256, dtype=BF16)
+    q, s = fp8_weight(gen, 64, 256)
+    for a in ((x[:, ::2], w[:128]), (x[:, 1:129], w[:128]), (x.double(), w.double()), (x, w[:255]), (x, w.float()), (x.cpu(), w), (x, w.cpu()), (x[:0], w), (3, w),
+              (x, None), (x.clone().requires_grad_(), w)):
+        assert fast.rms_norm(*a, 1e-6, None, False, stream) is None
+    assert fast.rms_norm(x, w, 1e-6, x[:2], False, stream) is None and fast.rms_norm(x[:, :200].contiguous(), w[:200], 1e-6, None, True, stream) is None
+    for a in ((x, None, q, s[:, :1], None, None, 0), (x, None, q.float(), s, None, None, 0), (x, None, q, s, w, None, 0), (x, None, q, s, None, None, 3),
+              (x, None, q, s, None, None, -1), (x, s, q, s, None, None, 0), (x.double(), None, q, s, None, None, 0), (x, None, w, None, None, None, 0),
+              (x, None, x[None], None, None, None, 0), (x, None, x[None], None, None, torch.ones(1, device="cuda"), 0), (x[:, 1:], None, q, s, None, None, 0),
+              (x, None, q, s.cpu(), None, None, 0), (x, None, q.T, s, None, None, 0)):
+        assert fast.product(*a, stream) is None
+    ids, wt, gu, dn = torch.zeros(4, 1, dtype=torch.int64, device="cuda"), torch.ones(4, 1, device="cuda"), randn(gen, 1, 16, 256, dtype=BF16), randn(gen, 1, 256, 8, dtype=BF16)
+    for a in ((x, ids.float(), wt, gu, None, dn, None), (x, ids, wt.double(), gu, None, dn, None), (x, ids[:2], wt, gu, None, dn, None), (x, ids, wt, gu, None, dn[:, :8], None),
+              (x, ids, wt, gu, s, dn, None), (x.float(), ids, wt, gu, None, dn, None), (x, ids, wt, gu.half(), None, dn, None), (x, ids, wt, gu[:, :15], None, dn, None)):
+        assert fast.moe_stacked(*a, stream) is None
+    with pytest.raises(TypeError):
+        fast.bind_unpacked(0)
