@@ -55,7 +55,8 @@ SIGNATURES = {
     "htr_dequant_w": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp]),
     "htr_rms_norm": (_i, [_vp, _i64, _vp, _i64, _vp, _i64, _i, ctypes.c_double, _i, _vp, _vp, _vp, _vp]),
     "htr_quantize_e4m3": (_i, [_vp, _i64, _i64, _i, _i, _vp, _vp, _vp]),
-    "htr_product": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _i, _i, _vp]),
+    "htr_product": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _i, _i, _vp]),
+    "htr_product_rounds": (_i, [_i64, _i, _i]),
     "htr_moe_stacked_scratch_bytes": (_sz, [_i64, _i, _i, _i, _i, _i]),
     "htr_moe_stacked": (_i, [_vp, _i, _vp, _i, _vp, _i64, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _sz, _vp]),
 }
@@ -96,7 +97,7 @@ def fast():
             module.bind(L.htr_abi_version(), str(torch.__version__), address(L.htr_linear), address(L.htr_stream_capture_id),
                         address(L.htr_moe_scratch_bytes), address(L.htr_moe_experts),
                         address(L.htr_linear_route), address(L.htr_dequant_w))
-            module.bind_unpacked(address(L.htr_rms_norm), address(L.htr_quantize_e4m3), address(L.htr_product),
+            module.bind_unpacked(address(L.htr_rms_norm), address(L.htr_quantize_e4m3), address(L.htr_product), address(L.htr_product_rounds),
                                  address(L.htr_moe_stacked_scratch_bytes), address(L.htr_moe_stacked))
         except (ImportError, AttributeError) as e:
             warnings.warn(f"htr_amd/_fast.so cannot be used ({e}): launches are prepared in Python; `python -m htr_amd.build` builds it",

@@ -11,15 +11,15 @@ template <int T> constexpr int bytes_of = T == P_F8 ? 1 : 2;
 typedef int i8v __attribute__((ext_vector_type(8)));
 
 struct ProductArgs {
-  const void* x;                         // [.][n]
-  const float* xs;                       // e4m3: [.][n / 128]
+  const void* x;                         // [.][n]; e4m3 matrices: also 16-bit rows, where takes_16bit_rows says so
+  const float* xs;                       // e4m3 rows: [.][n / 128]
   const void* w;                         // [experts][m][n]
   const float* ws;                       // e4m3: [experts][ceil(m / 128)][n / 128]
   const void* bias;                      // [m] in y's type or NULL
   void* y;                               // [rows][m]
   const int* ends;                       // [experts]: expert e has rows ends[e - 1] .. ends[e] - 1; NULL: one expert, all rows
   const int* gather;                     // row r of the product is row gather[r] of x; NULL: r
-  int rows, m, n, experts, y_dtype;
+  int rows, m, n, experts, y_dtype, x_type;
   float* ys;                             // k_product_tile<GATED> with y in e4m3: its scales, [rows][m / 256]
 };
 
@@ -88,9 +88,13 @@ __device__ __forceinline__ float silu(float g) { return g / (1.f + __expf(-g)); 
 // A workgroup owns 16 R rows of a matrix and up to 16 TT rows of x; its waves take the slabs in turn, straight from memory into registers
 // (every byte of the matrix is used by one wave once: LDS would only be a detour), and add up through LDS.
 // Bound: HBM, the matrix read once.
-template <int T, int R, int TT, int STREAM_WAVES>
+// X: the type of x; 16-bit rows with an e4m3 matrix are rounded on the way, by every workgroup for itself: about 110 instructions to a slab, beside
+// its 2 KB or more of the matrix, against a launch ahead of this one.
+template <int T, int X, int R, int TT, int STREAM_WAVES>
 __global__ __launch_bounds__(STREAM_WAVES * 64) void k_product_stream(const ProductArgs a) {
-  constexpr int P = R + TT <= 3 ? 4 : 2;                       // slabs in flight
+  constexpr int P = R + TT <= 3 && !(X != T && STREAM_WAVES > 8) ? 4 : 2;      // slabs in flight
+  constexpr bool ROUNDS = X != T;
+  static_assert(!ROUNDS || T == P_F8, "");
   __shared__ float red[STREAM_WAVES][R * TT * 256];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
   const int m0 = blockIdx.x * 16 * R;
@@ -108,7 +112,7 @@ __global__ __launch_bounds__(STREAM_WAVES * 64) void k_product_stream(const Prod
   for (int t = 0; t < TT; ++t) {
     int r = s.first + min(16 * t + c, s.count - 1);
     if (a.gather != nullptr) r = a.gather[r];
-    xp[t] = (const HTR_GLOBAL uint8_t*)a.x + (size_t)r * row_bytes + 16 * g;
+    xp[t] = (const HTR_GLOBAL uint8_t*)a.x + (size_t)r * (ROUNDS ? 2 * row_bytes : row_bytes) + (ROUNDS ? 32 : 16) * g;
     sp[t] = (const HTR_GLOBAL float*)a.xs + (size_t)r * (a.n >> 7);
   }
   const HTR_GLOBAL float* wsp = (const HTR_GLOBAL float*)a.ws + ((size_t)s.e * ((a.m + 127) >> 7) + (m0 >> 7)) * (a.n >> 7);
@@ -118,6 +122,7 @@ __global__ __launch_bounds__(STREAM_WAVES * 64) void k_product_stream(const Prod
 #pragma unroll
     for (int t = 0; t < TT; ++t) acc[i][t] = f4{0.f, 0.f, 0.f, 0.f};
   u4 A[P][R][2], B[P][TT][2];
+  Eight<X == P_F8 ? HTR_BF16 : X> raw[ROUNDS ? P : 1][TT][4];  // 16 elements of either half of the slab
   float sx[P][TT], sw[P];
   const u4 zero = {0u, 0u, 0u, 0u};
   auto load = [&](int p, int slab) {
@@ -129,13 +134,36 @@ __global__ __launch_bounds__(STREAM_WAVES * 64) void k_product_stream(const Prod
 #pragma unroll
       for (int i = 0; i < R; ++i) { A[p][i][h] = zero; if (in) A[p][i][h] = __builtin_nontemporal_load((const HTR_GLOBAL u4*)(wp[i] + off + 64 * h)); }
 #pragma unroll
-      for (int t = 0; t < TT; ++t) { B[p][t][h] = zero; if (in) B[p][t][h] = *(const HTR_GLOBAL u4*)(xp[t] + off + 64 * h); }
+      for (int t = 0; t < TT; ++t) {
+        if constexpr (ROUNDS) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) raw[p][t][2 * h + k].v = *(const HTR_GLOBAL u4*)(xp[t] + 2 * off + 128 * h + 16 * k);
+        } else {
+          B[p][t][h] = zero;
+          if (in) B[p][t][h] = *(const HTR_GLOBAL u4*)(xp[t] + off + 64 * h);
+        }
+      }
     }
     if constexpr (T == P_F8) {
       sw[p] = wsp[slab];
 #pragma unroll
-      for (int t = 0; t < TT; ++t) sx[p][t] = sp[t][slab];
+      for (int t = 0; t < TT; ++t) if constexpr (!ROUNDS) sx[p][t] = sp[t][slab];
     }
+  };
+  // a row's 128 columns lie in the four lanes c, c + 16, c + 32, c + 48
+  auto round_x = [&](int p, int t) {
+    float f[32], m = 0.f;
+#pragma unroll
+    for (int k = 0; k < 32; ++k) { f[k] = finite_or_nan(raw[p][t][k >> 3].get(k & 7)); m = fmaxf(m, fabsf(f[k])); }
+    u2s r = __builtin_amdgcn_permlane16_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+    m = fmaxf(__uint_as_float(r.x), __uint_as_float(r.y));
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+    m = fmaxf(__uint_as_float(r.x), __uint_as_float(r.y));
+    const int e = e4m3_exponent((double)m);
+    const float inv = exp2i(-e);
+    sx[p][t] = exp2i(e);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) B[p][t][k >> 2][k & 3] = pack_e4m3(f[4 * k] * inv, f[4 * k + 1] * inv, f[4 * k + 2] * inv, f[4 * k + 3] * inv);
   };
 #pragma unroll
   for (int p = 0; p < P; ++p) if (wv + p * STREAM_WAVES < slabs) load(p, wv + p * STREAM_WAVES);
@@ -144,6 +172,10 @@ __global__ __launch_bounds__(STREAM_WAVES * 64) void k_product_stream(const Prod
     for (int p = 0; p < P; ++p) {
       const int slab = s0 + p * STREAM_WAVES;
       if (slab < slabs) {
+        if constexpr (ROUNDS) {
+#pragma unroll
+          for (int t = 0; t < TT; ++t) round_x(p, t);
+        }
 #pragma unroll
         for (int i = 0; i < R; ++i)
 #pragma unroll

@@ -29,6 +29,7 @@ decltype(&htr_dequant_w) f_dequant = nullptr;
 decltype(&htr_rms_norm) f_norm = nullptr;
 decltype(&htr_quantize_e4m3) f_quantize = nullptr;
 decltype(&htr_product) f_product = nullptr;
+decltype(&htr_product_rounds) f_rounds = nullptr;
 decltype(&htr_moe_stacked_scratch_bytes) f_stacked_bytes = nullptr;
 decltype(&htr_moe_stacked) f_stacked = nullptr;
 
@@ -333,14 +334,16 @@ PyObject* product(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   {
     pybind11::gil_scoped_release no_lock;      // as in linear()
     c10::DeviceGuard guard(dev);
-    if (!eight) q = *x;
-    if (eight && !rows8(*x, xs, dev, stream, q, qs, rc)) {
+    // few 16-bit rows are rounded by the product itself
+    const bool as_is = !eight || (xs == nullptr && half_of(*x) && f_rounds(x->numel() / n, (int)experts, ends != nullptr));
+    if (as_is) q = *x;
+    if (!as_is && !rows8(*x, xs, dev, stream, q, qs, rc)) {
       rc = HTR_ERR_SIZE;
     } else {
       at::DimVector shape(x->sizes().begin(), x->sizes().end());
       shape.back() = m;
       y = at::empty(shape, x->options().dtype(type_of(code)));
-      rc = f_product(q.const_data_ptr(), eight ? qs.const_data_ptr() : nullptr, w->const_data_ptr(), eight ? ws->const_data_ptr() : nullptr,
+      rc = f_product(q.const_data_ptr(), as_is ? dtype_code(x->scalar_type()) : HTR_E4M3, as_is ? nullptr : qs.const_data_ptr(), w->const_data_ptr(), eight ? ws->const_data_ptr() : nullptr,
                      bias == nullptr ? nullptr : bias->const_data_ptr(), ends == nullptr ? nullptr : (const int32_t*)ends->const_data_ptr(), y.mutable_data_ptr(),
                      x->numel() / n, (int)m, (int)n, (int)experts, eight ? HTR_E4M3 : dtype_code(w->scalar_type()), (int)code, stream);
     }
@@ -397,14 +400,14 @@ PyObject* moe_stacked(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-// bind_unpacked(addresses of htr_rms_norm, htr_quantize_e4m3, htr_product, htr_moe_stacked_scratch_bytes, htr_moe_stacked), after bind()
+// bind_unpacked(addresses of htr_rms_norm, htr_quantize_e4m3, htr_product, htr_product_rounds, htr_moe_stacked_scratch_bytes, htr_moe_stacked), after bind()
 PyObject* bind_unpacked(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
-  if (nargs != 5) { PyErr_SetString(PyExc_TypeError, "bind_unpacked wants five addresses"); return nullptr; }
-  void* p[5];
-  for (int i = 0; i < 5; ++i) p[i] = PyLong_AsVoidPtr(args[i]);
+  if (nargs != 6) { PyErr_SetString(PyExc_TypeError, "bind_unpacked wants six addresses"); return nullptr; }
+  void* p[6];
+  for (int i = 0; i < 6; ++i) p[i] = PyLong_AsVoidPtr(args[i]);
   if (PyErr_Occurred()) return nullptr;
   f_norm = (decltype(f_norm))p[0]; f_quantize = (decltype(f_quantize))p[1]; f_product = (decltype(f_product))p[2];
-  f_stacked_bytes = (decltype(f_stacked_bytes))p[3]; f_stacked = (decltype(f_stacked))p[4];
+  f_rounds = (decltype(f_rounds))p[3]; f_stacked_bytes = (decltype(f_stacked_bytes))p[4]; f_stacked = (decltype(f_stacked))p[5];
   Py_RETURN_NONE;
 }
 

@@ -77,8 +77,12 @@ hipError_t launch_quantize(const void* x, int dtype, long long rows, int n, long
 
 // ---- products
 template <int T, int R, int TT, int WAVES> hipError_t launch_stream(const ProductArgs& a, hipStream_t st) {
-  const long long tiles = span_bound(a.rows, a.experts, a.ends != nullptr, 16 * TT);
-  return launch(k_product_stream<T, R, TT, WAVES>, dim3((a.m + 16 * R - 1) / (16 * R), (unsigned)tiles), WAVES * 64, 0, st, a);
+  const dim3 grid((a.m + 16 * R - 1) / (16 * R), (unsigned)span_bound(a.rows, a.experts, a.ends != nullptr, 16 * TT));
+  if constexpr (T == P_F8 && TT == 1) {
+    if (a.x_type == HTR_BF16) return launch(k_product_stream<T, HTR_BF16, R, TT, WAVES>, grid, WAVES * 64, 0, st, a);
+    if (a.x_type == HTR_F16) return launch(k_product_stream<T, HTR_F16, R, TT, WAVES>, grid, WAVES * 64, 0, st, a);
+  }
+  return launch(k_product_stream<T, T, R, TT, WAVES>, grid, WAVES * 64, 0, st, a);
 }
 template <int T, int WM, int WN, int AT, int BT, int NS, bool GATED = false> hipError_t launch_tile(const ProductArgs& a, hipStream_t st) {
   constexpr int TM = 16 * AT * WM, TN = 16 * BT * WN;
@@ -122,15 +126,24 @@ template <int N> int best_tile(const TileChoice (&choices)[N], const ProductArgs
 //   one row: 1024x4096 5.0 (16 rows to a workgroup of 8 waves; 4 waves 6.4, tiles of 64x32 10.9), 4096x4096 5.9 (7.4, 12.0), 14336x4096 15.5 (17.2, 16.9),
 //   28672x4096 25.7 (27.2, 29.5); 32 rows: 4096x4096 10.3 (tiles of 64x32 12.4, of 128x32 16.6), 28672x4096 64 (33, 31)
 //   96 rows of 64 experts: 2816x2048 56 (64 rows to a workgroup of 4 waves; 16 rows to one of 8 86; tiles of 128x32 59), 2048x1408 34 (52; 35)
+//   9 rows of 16 experts of 523x7600 in bf16: 52 us with 64 rows to a workgroup
+bool takes_16bit_rows(long long rows, int experts, bool grouped) {
+  return grouped ? rows <= 4ll * experts && span_bound(rows, experts, true, 16) <= 65535 : rows <= 16;
+}
 template <int T> hipError_t launch_product(const ProductArgs& a, hipStream_t st) {
   const int mean = (int)((a.rows + (long long)a.experts - 1) / a.experts);
-  const bool grouped = a.ends != nullptr, narrow = span_bound(a.rows, a.experts, grouped, 16) <= 65535;
+  const bool grouped = a.ends != nullptr, few = takes_16bit_rows(a.rows, a.experts, grouped);
+  if (few) {
+    const long long tiles = grouped ? (a.rows < a.experts ? a.rows : a.experts) : 1, wgs = (a.m + 15) / 16 * tiles;
+    if (grouped && wgs >= 4 * 512) return launch_stream<T, 4, 1, 4>(a, st);
+    // long rows of few workgroups: more waves to share them
+    if (wgs <= 256 && (long long)a.n * bytes_of<T> >= 64 * 128) return launch_stream<T, 1, 1, 16>(a, st);
+    return launch_stream<T, 1, 1, 8>(a, st);
+  }
   if (!grouped) {
-    if (mean <= 16) return launch_stream<T, 1, 1, 8>(a, st);
     if (mean <= 32) return a.m < 8192 ? launch_stream<T, 1, 2, 8>(a, st) : a.m < 16384 ? launch_tile<T, 2, 2, 2, 1, 4>(a, st) : launch_tile<T, 4, 1, 2, 2, 4>(a, st);
-  } else {
-    if (mean <= 4 && narrow) return launch_stream<T, 4, 1, 4>(a, st);
-    if (mean <= 24) return launch_tile<T, 4, 1, 2, 2, 4>(a, st);
+  } else if (mean <= 24) {
+    return launch_tile<T, 4, 1, 2, 2, 4>(a, st);
   }
   switch (best_tile(TILES, a, (size_t)a.n * bytes_of<T>)) {
     case 0: return launch_tile<T, 2, 4, 8, 4, 2>(a, st);
@@ -177,8 +190,9 @@ struct StackedScratch {
     ends = take((size_t)experts * 4);
     token = take(pairs * 4);
     pos_of = take(pairs * 4);
-    xq = take(f8 ? (size_t)tokens * hidden : 0);
-    xs = take(f8 ? (size_t)tokens * (hidden / 128) * 4 : 0);
+    const bool ahead = f8 && !takes_16bit_rows(pairs, experts, true);      // x is rounded by a launch of its own
+    xq = take(ahead ? (size_t)tokens * hidden : 0);
+    xs = take(ahead ? (size_t)tokens * (hidden / 128) * 4 : 0);
     h = take(gates_in_one(pairs, experts) ? 0 : pairs * 2 * inter * 4);
     a = take(pairs * inter * (f8 ? 1 : 2));
     as = take(f8 ? pairs * (inter / 128) * 4 : 0);
@@ -234,18 +248,21 @@ int htr_quantize_e4m3(const void* x, int64_t stride, int64_t rows, int n, int dt
   return HTR_OK;
 }
 
-int htr_product(const void* x, const void* x_scales, const void* w, const void* w_scales, const void* bias, const int32_t* ends, void* y, int64_t rows,
-                int m, int n, int experts, int type, int y_dtype, void* stream) {
+int htr_product_rounds(int64_t rows, int experts, int grouped) { return rows > 0 && experts > 0 && takes_16bit_rows(rows, experts, grouped != 0); }
+
+int htr_product(const void* x, int x_type, const void* x_scales, const void* w, const void* w_scales, const void* bias, const int32_t* ends, void* y,
+                int64_t rows, int m, int n, int experts, int type, int y_dtype, void* stream) {
   const int rc = product_shape(rows, m, n, experts, type, ends != nullptr);
   if (rc != HTR_OK) return rc;
   if (!is_dtype(y_dtype)) return HTR_ERR_DTYPE;
+  if (x_type != type && !(type == HTR_E4M3 && is_16bit(x_type) && takes_16bit_rows(rows, experts, ends != nullptr))) return HTR_ERR_DTYPE;
   if (ends == nullptr && experts != 1) return HTR_ERR_NULL;
   if (rows == 0) return HTR_OK;
-  if (!x || !w || !y || (type == HTR_E4M3 && (!x_scales || !w_scales))) return HTR_ERR_NULL;
+  if (!x || !w || !y || (x_type == HTR_E4M3 && !x_scales) || (type == HTR_E4M3 && !w_scales)) return HTR_ERR_NULL;
   if (!aligned(x, 16) || !aligned(w, 16) || !aligned(y, 16) || !aligned(x_scales, 4) || !aligned(w_scales, 4) || !aligned(ends, 4) ||
       !aligned(bias, element_bytes(y_dtype)))
     return HTR_ERR_ALIGN;
-  const ProductArgs a{x, (const float*)x_scales, w, (const float*)w_scales, bias, y, ends, nullptr, (int)rows, m, n, experts, y_dtype, nullptr};
+  const ProductArgs a{x, (const float*)x_scales, w, (const float*)w_scales, bias, y, ends, nullptr, (int)rows, m, n, experts, y_dtype, x_type, nullptr};
   TRY_HIP(launch_product(a, type, (hipStream_t)stream));
   return HTR_OK;
 }
@@ -273,8 +290,9 @@ int htr_moe_stacked(const void* x, int dtype, const void* ids, int ids_int64, co
   int *ends = (int*)(s + at.ends), *token = (int*)(s + at.token), *pos_of = (int*)(s + at.pos_of);
   float *h = (float*)(s + at.h), *out = (float*)(s + at.out);
   TRY_HIP(launch(k_expert_order, dim3(experts), ORDER_WAVES * 64, 0, st, ids, ids_int64, pairs, top, experts, ends, token, pos_of));
-  ProductArgs a{x, nullptr, gate_up, (const float*)gate_up_scales, nullptr, h, ends, token, pairs, 2 * inter, hidden, experts, HTR_F32, nullptr};
-  if (f8) {
+  ProductArgs a{x, nullptr, gate_up, (const float*)gate_up_scales, nullptr, h, ends, token, pairs, 2 * inter, hidden, experts, HTR_F32, dtype, nullptr};
+  if (f8 && !takes_16bit_rows(pairs, experts, true)) {
+    a.x_type = HTR_E4M3;
     TRY_HIP(launch_quantize(x, dtype, tokens, hidden, hidden, s + at.xq, (float*)(s + at.xs), st));
     a.x = s + at.xq; a.xs = (const float*)(s + at.xs);
   }
@@ -287,7 +305,7 @@ int htr_moe_stacked(const void* x, int dtype, const void* ids, int ids_int64, co
                : dtype == HTR_BF16 ? launch(k_gated<HTR_BF16>, dim3(pairs), 256, 0, st, h, ends, experts, inter, s + at.a, nullptr)
                                    : launch(k_gated<HTR_F16>, dim3(pairs), 256, 0, st, h, ends, experts, inter, s + at.a, nullptr));
   }
-  const ProductArgs d{s + at.a, (const float*)(s + at.as), down, (const float*)down_scales, nullptr, out, ends, nullptr, pairs, hidden, inter, experts, HTR_F32, nullptr};
+  const ProductArgs d{s + at.a, (const float*)(s + at.as), down, (const float*)down_scales, nullptr, out, ends, nullptr, pairs, hidden, inter, experts, HTR_F32, type, nullptr};
   TRY_HIP(launch_product(d, type, st));
   const dim3 grid((unsigned)tokens, (hidden + 2047) / 2048);
   TRY_HIP(dtype == HTR_BF16 ? launch(k_weighted_sum<HTR_BF16>, grid, 256, 0, st, out, pos_of, weights, top, hidden, y)

@@ -156,9 +156,12 @@ def _pair(x):
     return isinstance(x, (tuple, list)) and len(x) == 2
 
 
-def _check_rows(what, x):
-    """x as contiguous 8-bit rows (values, scales); a tensor is rounded to e4m3 first."""
+def _check_rows(what, x, experts, grouped):
+    """x as htr_product takes it with an 8-bit weight: contiguous 8-bit rows (values, scales), to which a tensor is rounded, or few 16-bit rows (x, None)."""
     if not _pair(x):
+        n = x.shape[-1]
+        if x.dtype in _HALVES and n % 128 == 0 and n and _native.lib().htr_product_rounds(x.numel() // n, experts, int(grouped)):
+            return _packed(x), None
         return quantize_fp8(x)
     q, s = x
     if q.dtype != E4M3 or s.dtype != torch.float32 or q.dim() < 1 or s.shape != q.shape[:-1] + (q.shape[-1] // 128,) or q.shape[-1] % 128:
@@ -211,11 +214,11 @@ def linear_fp8(x, qweight, scales, bias=None, out_dtype=None):
         raise RuntimeError("linear_fp8: the bias must be [m] in the result's type")
     _on_one_gpu("linear_fp8", first, qweight, scales, bias, x[1] if _pair(x) else None)
     _refuse_derivatives("linear_fp8", *(x if _pair(x) else (x,)), scales, bias)
-    q, s = _check_rows("linear_fp8", x)
+    q, s = _check_rows("linear_fp8", x, 1, False)
     bias = None if bias is None else bias.contiguous()
     y = torch.empty(first.shape[:-1] + (m,), dtype=dtype, device=q.device)
     if y.numel():
-        _queue(q.device, "htr_product", q.data_ptr(), s.data_ptr(), qweight.data_ptr(), scales.data_ptr(), _ptr(bias), None, y.data_ptr(), y.numel() // m,
+        _queue(q.device, "htr_product", q.data_ptr(), _CODE[q.dtype], _ptr(s), qweight.data_ptr(), scales.data_ptr(), _ptr(bias), None, y.data_ptr(), y.numel() // m,
                m, n, 1, _native.E4M3, _CODE[dtype])
     return y
 
@@ -251,12 +254,12 @@ def grouped_mm(x, weight, ends, out_dtype=None):
         raise RuntimeError("grouped_mm: ends must be int32, one for each expert")
     _on_one_gpu("grouped_mm", first, w, ws, ends, x[1] if _pair(x) else None)
     _refuse_derivatives("grouped_mm", *(x if _pair(x) else (x,)), *((ws,) if eight else (w,)))
-    q, s = _check_rows("grouped_mm", x) if eight else (_packed(x), None)
+    q, s = _check_rows("grouped_mm", x, E, True) if eight else (_packed(x), None)
     ends = ends.contiguous()
     R = first.shape[0]
     y = torch.empty((R, m), dtype=dtype, device=q.device)
     if R:
-        _queue(q.device, "htr_product", q.data_ptr(), _ptr(s), w.data_ptr(), _ptr(ws), None, ends.data_ptr(), y.data_ptr(), R, m, n, E, _CODE[w.dtype],
+        _queue(q.device, "htr_product", q.data_ptr(), _CODE[q.dtype], _ptr(s), w.data_ptr(), _ptr(ws), None, ends.data_ptr(), y.data_ptr(), R, m, n, E, _CODE[w.dtype],
                _CODE[dtype])
     return y
 

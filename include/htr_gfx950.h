@@ -330,15 +330,18 @@ int htr_quantize_e4m3(const void* x, int64_t stride, int64_t rows, int n, int dt
 
 /*
  * y[r] = W_e x[r] (+ bias), e the expert of row r, sums in float32.
- *   type    HTR_E4M3 (x and w with their scales), HTR_BF16 or HTR_F16 (scales NULL)
+ *   type    of w: HTR_E4M3 (with its scales), HTR_BF16 or HTR_F16 (scales NULL)
+ *   x_type  type; with e4m3 matrices also HTR_BF16 or HTR_F16 (x_scales NULL) where htr_product_rounds says so: rounded as by htr_quantize_e4m3
  *   x       [rows][n], w [experts][m][n], 16-byte aligned; n a multiple of 128 (e4m3) or of 8 (16 bits), any m
  *   ends    device int32 [experts]: expert e has rows ends[e - 1] .. ends[e] - 1 (from 0); rows from the last end on become zeros.  An end below
  *           an earlier one, or beyond rows, counts as that one, or as rows.  NULL: one matrix (experts = 1) for all rows
  *   bias    [m] of y_dtype or NULL;  y [rows][m], y_dtype any of the three, 16-byte aligned; it may overlap nothing that is read
  * The result does not depend on which rows come together but for the rounding of sums in another order.
  */
-int htr_product(const void* x, const void* x_scales, const void* w, const void* w_scales, const void* bias, const int32_t* ends, void* y, int64_t rows,
-                int m, int n, int experts, int type, int y_dtype, void* stream);
+int htr_product(const void* x, int x_type, const void* x_scales, const void* w, const void* w_scales, const void* bias, const int32_t* ends, void* y,
+                int64_t rows, int m, int n, int experts, int type, int y_dtype, void* stream);
+/* 1 where htr_product takes 16-bit rows with e4m3 matrices and rounds them on the way (few rows), otherwise 0: htr_quantize_e4m3 first.  grouped: ends is given. */
+int htr_product_rounds(int64_t rows, int experts, int grouped);
 
 /*
  * A routed-expert layer on stacked matrices: y_t = sum_j w[t, j] Down_e( silu(Gate_e x_t) * Up_e x_t ), e = ids[t, j], sums in float32 and in

@@ -199,7 +199,7 @@ def test_linear_fp8(gen, m, n, rows):
         assert y.dtype == dtype
         assert_within(y, want, bound)
         q, s = ops.quantize_fp8(x)
-        assert torch.equal(ops.linear_fp8((q, s), w, ws, b, out_dtype=dtype), y)
+        assert torch.equal(ops.linear_fp8((q, s), w, ws, b, out_dtype=dtype), y)        # rounded ahead or on the way: the same values and sums
     # scales of rows from elsewhere
     s = s * (0.5 + torch.rand(s.shape, device="cuda", generator=gen))
     want, bound = product_bound(value(q, s), value(w, ws), BF16)
@@ -470,10 +470,13 @@ def test_status_codes_without_a_gpu():
     quant = lambda x=p, stride=128, rows=1, n=128, dt=0, q=p, s=p: L.htr_quantize_e4m3(x, stride, rows, n, dt, q, s, None)
     assert quant(rows=0) == 0 and quant(n=64) == 11 and quant(dt=3) == 5 and quant(q=None) == 1 and quant(x=odd) == 7 and quant(stride=129) == 7
     prod = lambda x=p, xs=p, w=p, ws=p, b=None, ends=None, y=p, rows=1, m=128, n=128, E=1, t=3, yt=0: \
-        L.htr_product(x, xs, w, ws, b, ends, y, rows, m, n, E, t, yt, None)
+        L.htr_product(x, t, xs, w, ws, b, ends, y, rows, m, n, E, t, yt, None)
     assert prod(rows=0) == 0 and prod(rows=-1) == 11 and prod(m=0) == 11 and prod(n=64) == 11 and prod(n=4, t=0) == 11 and prod(t=2) == 5 and prod(yt=3) == 5
     assert prod(E=2) == 1 and prod(E=0, ends=p) == 11 and prod(xs=None) == 1 and prod(ws=None) == 1 and prod(w=None) == 1 and prod(x=odd) == 7 and prod(y=odd) == 7
     assert prod(ends=odd) == 7 and prod(b=odd) == 7 and prod(rows=1 << 31) == 11 and prod(E=70000, ends=p) == 11
+    mixed = lambda xt, rows=1, t=3, xs=None: L.htr_product(p, xt, xs, p, None, None, None, p, rows, 128, 128, 1, t, 0, None)
+    assert mixed(2) == 5 and mixed(0, rows=17) == 5 and mixed(1, t=0) == 5 and mixed(3, t=0) == 5 and mixed(0) == 1      # the last one: no scales of w
+    assert L.htr_product_rounds(16, 1, 0) == 1 and L.htr_product_rounds(17, 1, 0) == 0 and L.htr_product_rounds(256, 64, 1) == 1 and L.htr_product_rounds(257, 64, 1) == 0
     need = L.htr_moe_stacked_scratch_bytes
     assert need(4, 2, 8, 256, 128, 3) > 0 and need(0, 2, 8, 256, 128, 3) == 0 and need(4, 2, 8, 256, 72, 3) == 0 and need(4, 2, 8, 256, 72, 0) > 0
     assert need(4, 2, 8, 256, 128, 2) == 0 and need(1 << 24, 4096, 8, 256, 128, 0) == 0
