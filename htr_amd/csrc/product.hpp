@@ -402,14 +402,15 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
     }
 #pragma unroll
     for (int i = 0; i < AT; ++i) {
+      if (i == 0) __builtin_amdgcn_s_setprio(1);                 // a wave with products ahead of one that waits or loads: 1 to 2 %
       if (i == BARRIER) {
+        __builtin_amdgcn_s_setprio(0);
         landed(next, last_lands, std::integral_constant<int, (NS - 2) * (L + (T == P_F8))>());
         issue_scales(from2, ask, stage);
         if constexpr (T == P_F8) read_scales(next);
       }
       if (i < BARRIER) issue_piece(from, asked, prev, i + AT - BARRIER); else issue_piece(from2, ask, stage, i - BARRIER);
       if (i + RA - 1 < AT) read_a(i + RA - 1, stage); else read_a(i + RA - 1 - AT, next);
-      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int t = 0; t < BT; ++t) {
         if constexpr (T == P_F8) {

@@ -135,9 +135,11 @@ template <int T> hipError_t launch_product(const ProductArgs& a, hipStream_t st)
   const bool grouped = a.ends != nullptr, few = takes_16bit_rows(a.rows, a.experts, grouped);
   if (few) {
     const long long tiles = grouped ? (a.rows < a.experts ? a.rows : a.experts) : 1, wgs = (a.m + 15) / 16 * tiles;
+    const long long slabs = ((long long)a.n * bytes_of<T> + 127) / 128;
     if (grouped && wgs >= 4 * 512) return launch_stream<T, 4, 1, 4>(a, st);
-    // long rows of few workgroups: more waves to share them
-    if (wgs <= 256 && (long long)a.n * bytes_of<T> >= 64 * 128) return launch_stream<T, 1, 1, 16>(a, st);
+    // short rows give eight waves too little each; long rows of few workgroups need more waves to share them
+    if (wgs >= 512 && slabs <= 16) return launch_stream<T, 2, 1, 4>(a, st);
+    if (wgs <= 256 && slabs >= 64) return launch_stream<T, 1, 1, 16>(a, st);
     return launch_stream<T, 1, 1, 8>(a, st);
   }
   if (!grouped) {
