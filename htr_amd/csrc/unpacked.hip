@@ -137,7 +137,8 @@ template <int T> hipError_t launch_product(const ProductArgs& a, hipStream_t st)
     const long long tiles = grouped ? (a.rows < a.experts ? a.rows : a.experts) : 1, wgs = (a.m + 15) / 16 * tiles;
     const long long slabs = ((long long)a.n * bytes_of<T> + 127) / 128;
     if (grouped && wgs >= 4 * 512) return launch_stream<T, 4, 1, 4>(a, st);
-    // short rows give eight waves too little each; long rows of few workgroups need more waves to share them
+    // short rows give eight waves too little each (7 rows on 15657x384 in e4m3 5.5 us by 16 rows to a workgroup of 8 waves, 4.7 by 32 to one of 4; 4 tokens over 8
+    // of 16 experts of 1920/384 37 and 31); long rows of few workgroups need more waves to share them
     if (wgs >= 512 && slabs <= 16) return launch_stream<T, 2, 1, 4>(a, st);
     if (wgs <= 256 && slabs >= 64) return launch_stream<T, 1, 1, 16>(a, st);
     return launch_stream<T, 1, 1, 8>(a, st);
@@ -176,9 +177,10 @@ hipError_t launch_product(const ProductArgs& a, int type, hipStream_t st) {
 int product_shape(long long rows, int m, int n, int experts, int type, bool grouped) {
   if (type != HTR_E4M3 && !is_16bit(type)) return HTR_ERR_DTYPE;
   if (rows < 0 || rows > (1ll << 31) - (1 << 20) || m < 1 || n < 1 || experts < 1 || experts > 65535 || n % (type == HTR_E4M3 ? 128 : 8)) return HTR_ERR_SIZE;
-  if (m > (1 << 30) || n > (1 << 28)) return HTR_ERR_SIZE;
+  if (m > (1 << 26) || n > (1 << 22)) return HTR_ERR_SIZE;       // 256 rows of a tile by 32-bit distances; the launch's threads below 2^32
+  // numbers of the smallest tiles, and workgroups where there is one to a tile (rows of fewer slabs than the deepest ring has stages)
   const long long tiles = span_bound(rows, experts, grouped, 32) * ((m + 63) / 64);
-  return tiles > (1ll << 31) - 256 ? HTR_ERR_SIZE : HTR_OK;
+  return tiles > ((long long)n * (type == HTR_E4M3 ? 1 : 2) > 128 * 3 ? (1ll << 31) - (1 << 16) : 1ll << 23) ? HTR_ERR_SIZE : HTR_OK;
 }
 
 // ---- a routed-expert layer: scratch laid out one after the other, every part on a 256-byte boundary
@@ -203,7 +205,7 @@ struct StackedScratch {
   }
 };
 int stacked_shape(long long tokens, int top, int experts, int hidden, int inter, int type) {
-  if (tokens < 1 || top < 1 || experts < 1 || hidden < 1 || inter < 1 || top > 4096 || tokens > (1 << 24) || inter > (1 << 28)) return HTR_ERR_SIZE;
+  if (tokens < 1 || top < 1 || experts < 1 || hidden < 1 || inter < 1 || top > 4096 || tokens >= (1 << 24) || inter > (1 << 28)) return HTR_ERR_SIZE;
   if (type != HTR_E4M3 && !is_16bit(type)) return HTR_ERR_DTYPE;
   if (hidden % 8 || inter % (type == HTR_E4M3 ? 128 : 8)) return HTR_ERR_SIZE;
   // loads go by 32-bit distances from x, from the gathered rows' scales and from an expert's matrices
@@ -227,26 +229,36 @@ int htr_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t 
   if (!aligned(x, size) || !aligned(residual, size) || !aligned(weight, size) || !aligned(sum, size) || !aligned(scales, 4) || (!scales && !aligned(y, size)))
     return HTR_ERR_ALIGN;
   if (scales && n % 128) return HTR_ERR_SIZE;
-  const NormArgs a{x, residual, weight, y, sum, (float*)scales, x_stride, residual_stride, rows, n, eps};
   hipStream_t st = (hipStream_t)stream;
   const bool vector = n % 8 == 0 && n <= 32768 && aligned(x, 16) && aligned(residual, 16) && aligned(weight, 16) && aligned(y, 16) && aligned(sum, 16) &&
                       x_stride % 8 == 0 && residual_stride % 8 == 0;
-  if (!vector) {
-    TRY_HIP(scales ? launch(k_rms_norm_any<true>, dim3((unsigned)rows), 256, 0, st, a, dtype) : launch(k_rms_norm_any<false>, dim3((unsigned)rows), 256, 0, st, a, dtype));
-  } else {
-    TRY_HIP(dtype == HTR_BF16 ? launch_norm<HTR_BF16>(a, scales != nullptr, st) : dtype == HTR_F16 ? launch_norm<HTR_F16>(a, scales != nullptr, st)
-                                                                                               : launch_norm<HTR_F32>(a, scales != nullptr, st));
+  // a launch has fewer than 2^32 threads, up to 1024 of them to a row
+  constexpr int64_t MOST = 1 << 21;
+  for (int64_t r = 0; r < rows; r += MOST) {
+    const int64_t count = rows - r < MOST ? rows - r : MOST;
+    auto at = [&](const void* p, int64_t elements, size_t bytes) { return p ? (void*)((uint8_t*)p + elements * (int64_t)bytes) : nullptr; };
+    const NormArgs a{at(x, r * x_stride, size), at(residual, r * residual_stride, size), weight, at(y, r * n, scales ? 1 : size), at(sum, r * n, size),
+                     (float*)at(scales, r * (n / 128), 4), x_stride, residual_stride, count, n, eps};
+    if (!vector) {
+      TRY_HIP(scales ? launch(k_rms_norm_any<true>, dim3((unsigned)count), 256, 0, st, a, dtype) : launch(k_rms_norm_any<false>, dim3((unsigned)count), 256, 0, st, a, dtype));
+    } else {
+      TRY_HIP(dtype == HTR_BF16 ? launch_norm<HTR_BF16>(a, scales != nullptr, st) : dtype == HTR_F16 ? launch_norm<HTR_F16>(a, scales != nullptr, st)
+                                                                                                 : launch_norm<HTR_F32>(a, scales != nullptr, st));
+    }
   }
   return HTR_OK;
 }
 
 int htr_quantize_e4m3(const void* x, int64_t stride, int64_t rows, int n, int dtype, void* q, void* scales, void* stream) {
-  if (rows < 0 || n < 1 || n % 128 || rows > (1ll << 34) / (n / 128)) return HTR_ERR_SIZE;
+  if (rows < 0 || n < 1 || n % 128 || n > (1 << 30)) return HTR_ERR_SIZE;
   if (!is_dtype(dtype)) return HTR_ERR_DTYPE;
   if (rows == 0) return HTR_OK;
   if (!x || !q || !scales) return HTR_ERR_NULL;
   if (!aligned(x, 16) || stride % 8 || !aligned(q, 8) || !aligned(scales, 4)) return HTR_ERR_ALIGN;
-  TRY_HIP(launch_quantize(x, dtype, rows, n, stride, q, (float*)scales, (hipStream_t)stream));
+  const int64_t most = (1 << 27) / (n / 128);      // rows of 2^31 threads
+  for (int64_t r = 0; r < rows; r += most)
+    TRY_HIP(launch_quantize((const uint8_t*)x + r * stride * (int64_t)element_bytes(dtype), dtype, rows - r < most ? rows - r : most, n, stride, (uint8_t*)q + r * n,
+                            (float*)scales + r * (n / 128), (hipStream_t)stream));
   return HTR_OK;
 }
 

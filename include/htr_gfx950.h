@@ -332,7 +332,7 @@ int htr_quantize_e4m3(const void* x, int64_t stride, int64_t rows, int n, int dt
  * y[r] = W_e x[r] (+ bias), e the expert of row r, sums in float32.
  *   type    of w: HTR_E4M3 (with its scales), HTR_BF16 or HTR_F16 (scales NULL)
  *   x_type  type; with e4m3 matrices also HTR_BF16 or HTR_F16 (x_scales NULL) where htr_product_rounds says so: rounded as by htr_quantize_e4m3
- *   x       [rows][n], w [experts][m][n], 16-byte aligned; n a multiple of 128 (e4m3) or of 8 (16 bits), any m
+ *   x       [rows][n], w [experts][m][n], 16-byte aligned; n a multiple of 128 (e4m3) or of 8 (16 bits), up to 2^22; m up to 2^26; experts up to 65535
  *   ends    device int32 [experts]: expert e has rows ends[e - 1] .. ends[e] - 1 (from 0); rows from the last end on become zeros.  An end below
  *           an earlier one, or beyond rows, counts as that one, or as rows.  NULL: one matrix (experts = 1) for all rows
  *   bias    [m] of y_dtype or NULL;  y [rows][m], y_dtype any of the three, 16-byte aligned; it may overlap nothing that is read
@@ -350,7 +350,7 @@ int htr_product_rounds(int64_t rows, int experts, int grouped);
  *   gate_up  [experts][2 inter][hidden], gate rows first;  down [experts][hidden][inter];  scales as in htr_product, or NULL
  *   ids      [tokens][top] int32 or int64 and weights [tokens][top] float32, on the device; an expert out of range makes its token NaN
  *   scratch  htr_moe_stacked_scratch_bytes() bytes (0: sizes that are not taken), 256-byte aligned, of any content, used until the launches are done
- * hidden a multiple of 8 (e4m3: 128), inter too.  htr_moe_experts is this layer on HTR-W1 matrices.
+ * hidden a multiple of 8 (e4m3: 128), inter too; x, and gate_up of one expert, of fewer than 2^32 bytes.  htr_moe_experts is this layer on HTR-W1 matrices.
  */
 size_t htr_moe_stacked_scratch_bytes(int64_t tokens, int top, int experts, int hidden, int inter, int type);
 int htr_moe_stacked(const void* x, int dtype, const void* ids, int ids_int64, const float* weights, int64_t tokens, int top, const void* gate_up,

@@ -413,6 +413,51 @@ def test_a_block_of_them_eager_on_streams_and_captured(gen):
         assert torch.equal(out[0], want[k][0]) and torch.equal(out[1], want[k][1])
 
 
+@pytest.mark.gpu
+def test_beyond_32_bits(gen):
+    """Matrices, rows and results whose places in memory pass 2^32 bytes."""
+    E, m, n = 40, 8192, 16384
+    w = torch.zeros(E, m, n, dtype=torch.uint8, device="cuda").view(E4M3)              # 5.4 GB
+    ws = torch.zeros(E, m // 128, n // 128, device="cuda")
+    q, s = fp8_weight(gen, 256, n)
+    w[E - 1, m - 256:], ws[E - 1, m // 128 - 2:] = q, s
+    ends = torch.zeros(E, dtype=torch.int32, device="cuda")
+    for rows in (3, 200):
+        ends[E - 1] = rows
+        x = ops.quantize_fp8(randn(gen, rows, n))
+        want, bound = product_bound(value(*x), value(q, s), BF16)
+        y = ops.grouped_mm(x, (w, ws), ends)
+        assert_within(y[:, m - 256:], want, bound)
+        assert (y[:, :m - 256] == 0).all()
+    del w, ws
+    rows, n = 1_200_000, 128
+    x, q, s = randn(gen, rows, n, dtype=BF16), *fp8_weight(gen, 2048, n)
+    y = ops.linear_fp8(x, q, s)                                                        # 4.9 GB
+    last = slice(rows - 5, rows)
+    assert torch.equal(y[last], ops.linear_fp8(x[last].clone(), q, s))
+    y = ops.rms_norm(y, torch.ones(2048, dtype=BF16, device="cuda"), residual=y)[0]
+    tail = ops.linear_fp8(x[last].clone(), q, s)
+    assert torch.equal(y[last], ops.rms_norm(tail, torch.ones(2048, dtype=BF16, device="cuda"), residual=tail)[0])
+
+
+@pytest.mark.gpu
+def test_more_rows_than_a_launch_takes(gen):
+    rows = (1 << 21) + 3
+    x, w = randn(gen, rows, 128, dtype=BF16), randn(gen, 128, dtype=BF16)
+    for a, b in zip(ops.rms_norm(x, w, quantize=True), ops.rms_norm(x[rows - 7:].clone(), w, quantize=True)):
+        assert torch.equal(a[rows - 7:].float(), b.float())
+    assert torch.equal(ops.rms_norm(x[:, 1:], w[1:], residual=x[:, 1:])[0][rows - 7:], ops.rms_norm(x[rows - 7:, 1:].clone(), w[1:].clone(), residual=x[rows - 7:, 1:].clone())[0])
+
+
+@pytest.mark.gpu
+def test_under_torch_compile(gen):
+    run = _block(gen)
+    x, h = randn(gen, 9, 256, dtype=BF16), randn(gen, 9, 256, dtype=BF16)
+    got = torch.compile(run, backend="eager")(x, h)
+    for a, b in zip(got, run(x, h)):
+        assert torch.equal(a, b)
+
+
 # ---- refusals
 def test_refusals_without_a_gpu():
     x, w = torch.zeros(2, 128, dtype=BF16), torch.zeros(128, dtype=BF16)
@@ -474,6 +519,7 @@ def test_status_codes_without_a_gpu():
     assert prod(rows=0) == 0 and prod(rows=-1) == 11 and prod(m=0) == 11 and prod(n=64) == 11 and prod(n=4, t=0) == 11 and prod(t=2) == 5 and prod(yt=3) == 5
     assert prod(E=2) == 1 and prod(E=0, ends=p) == 11 and prod(xs=None) == 1 and prod(ws=None) == 1 and prod(w=None) == 1 and prod(x=odd) == 7 and prod(y=odd) == 7
     assert prod(ends=odd) == 7 and prod(b=odd) == 7 and prod(rows=1 << 31) == 11 and prod(E=70000, ends=p) == 11
+    assert prod(n=(1 << 22) + 128) == 11 and prod(m=(1 << 26) + 1) == 11 and quant(n=(1 << 30) + 128) == 11         # places in a tile, and a launch, in 32 bits
     mixed = lambda xt, rows=1, t=3, xs=None: L.htr_product(p, xt, xs, p, None, None, None, p, rows, 128, 128, 1, t, 0, None)
     assert mixed(2) == 5 and mixed(0, rows=17) == 5 and mixed(1, t=0) == 5 and mixed(3, t=0) == 5 and mixed(0) == 1      # the last one: no scales of w
     assert L.htr_product_rounds(16, 1, 0) == 1 and L.htr_product_rounds(17, 1, 0) == 0 and L.htr_product_rounds(256, 64, 1) == 1 and L.htr_product_rounds(257, 64, 1) == 0
