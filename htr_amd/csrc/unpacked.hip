@@ -48,7 +48,7 @@ size_t element_bytes(int dtype) { return dtype == HTR_F32 ? 4 : dtype == HTR_E4M
 bool aligned(const void* p, size_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
 
 // ---- norm
-template <int T, bool RES, bool QUANT>
+template <int T, bool RES, bool QUANT, bool ANY>
 hipError_t launch_norm(const NormArgs& a, hipStream_t st) {
   const int eights = (a.n + 7) / 8;
   const dim3 grid((unsigned)a.rows);
@@ -56,14 +56,21 @@ hipError_t launch_norm(const NormArgs& a, hipStream_t st) {
   const int nv = eights <= 1024 ? 1 : eights <= 2048 ? 2 : 4;
   const unsigned threads = ((eights + nv - 1) / nv + 63) / 64 * 64;
   switch (nv) {
-    case 1: return launch(k_rms_norm<T, 1, RES, QUANT>, grid, threads, 0, st, a);
-    case 2: return launch(k_rms_norm<T, 2, RES, QUANT>, grid, threads, 0, st, a);
-    default: return launch(k_rms_norm<T, 4, RES, QUANT>, grid, threads, 0, st, a);
+    case 1: return launch(k_rms_norm<T, 1, RES, QUANT, ANY>, grid, threads, 0, st, a);
+    case 2: return launch(k_rms_norm<T, 2, RES, QUANT, ANY>, grid, threads, 0, st, a);
+    default: return launch(k_rms_norm<T, 4, RES, QUANT, ANY>, grid, threads, 0, st, a);
   }
 }
-template <int T> hipError_t launch_norm(const NormArgs& a, bool quant, hipStream_t st) {
-  if (a.residual) return quant ? launch_norm<T, true, true>(a, st) : launch_norm<T, true, false>(a, st);
-  return quant ? launch_norm<T, false, true>(a, st) : launch_norm<T, false, false>(a, st);
+template <int T, bool ANY> hipError_t launch_norm(const NormArgs& a, hipStream_t st) {
+  const bool quant = a.scales != nullptr;
+  if (a.residual) return quant ? launch_norm<T, true, true, ANY>(a, st) : launch_norm<T, true, false, ANY>(a, st);
+  return quant ? launch_norm<T, false, true, ANY>(a, st) : launch_norm<T, false, false, ANY>(a, st);
+}
+template <int T> hipError_t launch_norm(const NormArgs& a, hipStream_t st) {
+  if (a.n > 32768) return launch(a.scales ? k_rms_norm_long<true> : k_rms_norm_long<false>, dim3((unsigned)a.rows), 1024, 0, st, a, T);
+  const bool vector = a.n % 8 == 0 && aligned(a.x, 16) && aligned(a.residual, 16) && aligned(a.weight, 16) && aligned(a.y, 16) && aligned(a.sum, 16) &&
+                      a.x_stride % 8 == 0 && a.residual_stride % 8 == 0;
+  return vector ? launch_norm<T, false>(a, st) : launch_norm<T, true>(a, st);
 }
 
 hipError_t launch_quantize(const void* x, int dtype, long long rows, int n, long long stride, void* q, float* scales, hipStream_t st) {
@@ -230,8 +237,6 @@ int htr_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t 
     return HTR_ERR_ALIGN;
   if (scales && n % 128) return HTR_ERR_SIZE;
   hipStream_t st = (hipStream_t)stream;
-  const bool vector = n % 8 == 0 && n <= 32768 && aligned(x, 16) && aligned(residual, 16) && aligned(weight, 16) && aligned(y, 16) && aligned(sum, 16) &&
-                      x_stride % 8 == 0 && residual_stride % 8 == 0;
   // a launch has fewer than 2^32 threads, up to 1024 of them to a row
   constexpr int64_t MOST = 1 << 21;
   for (int64_t r = 0; r < rows; r += MOST) {
@@ -239,12 +244,7 @@ int htr_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t 
     auto at = [&](const void* p, int64_t elements, size_t bytes) { return p ? (void*)((uint8_t*)p + elements * (int64_t)bytes) : nullptr; };
     const NormArgs a{at(x, r * x_stride, size), at(residual, r * residual_stride, size), weight, at(y, r * n, scales ? 1 : size), at(sum, r * n, size),
                      (float*)at(scales, r * (n / 128), 4), x_stride, residual_stride, count, n, eps};
-    if (!vector) {
-      TRY_HIP(scales ? launch(k_rms_norm_any<true>, dim3((unsigned)count), 256, 0, st, a, dtype) : launch(k_rms_norm_any<false>, dim3((unsigned)count), 256, 0, st, a, dtype));
-    } else {
-      TRY_HIP(dtype == HTR_BF16 ? launch_norm<HTR_BF16>(a, scales != nullptr, st) : dtype == HTR_F16 ? launch_norm<HTR_F16>(a, scales != nullptr, st)
-                                                                                                 : launch_norm<HTR_F32>(a, scales != nullptr, st));
-    }
+    TRY_HIP(dtype == HTR_BF16 ? launch_norm<HTR_BF16>(a, st) : dtype == HTR_F16 ? launch_norm<HTR_F16>(a, st) : launch_norm<HTR_F32>(a, st));
   }
   return HTR_OK;
 }

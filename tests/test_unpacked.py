@@ -154,6 +154,25 @@ def test_norm_takes_strides_and_any_alignment(gen, quantize):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("n", [5, 9, 513, 1001, 8191, 8193, 16391, 32767, 32769])
+def test_norm_of_rows_that_end_inside_a_run(gen, dtype, n):
+    """Odd widths, odd distances from row to row, nothing on a 16-byte boundary; what lies around the rows is not read into them."""
+    big = torch.full((4, n + 4), float("nan"), dtype=dtype, device="cuda")
+    x, w = big[:, 3:n + 3], torch.full((n + 2,), float("nan"), dtype=dtype, device="cuda")
+    x.copy_(randn(gen, 4, n))
+    w[1:-1] = randn(gen, n)
+    r = randn(gen, 4, n, dtype=dtype, scale=3)
+    for residual in (None, r):
+        y = ops.rms_norm(x, w[1:-1], 1e-5, residual=residual)
+        want, t = norm64(x, w[1:-1], 1e-5, residual)
+        if residual is not None:
+            y, total = y
+            assert torch.equal(total, t)
+        assert_within(y, want, want.abs() * 3.01 * 2.0 ** -24 + half_step(want * (1 + 2.0 ** -22), dtype))     # as in test_norm
+
+
+@pytest.mark.gpu
 def test_norm_of_nothing():
     x, w = torch.empty(0, 128, device="cuda", dtype=BF16), torch.ones(128, device="cuda", dtype=BF16)
     assert ops.rms_norm(x, w).shape == (0, 128)
