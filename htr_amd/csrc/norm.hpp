@@ -121,15 +121,28 @@ template <> struct Eight<HTR_F32> {
   }
 };
 
-// Eight finite products (t w) r of a row, 16 neighbouring lanes holding a block of 128: their e4m3 values and the block's scale.
-// p = t w is exact in float32 for 16-bit types (22 bits); the factor r of the row is kept in 64 bits, so that the scale is the right one also
-// where the block's largest value lies next to 448 times a power of two.  For float32 rows p is a 64-bit product.
+// Eight products (t w) r of a row, 16 neighbouring lanes holding a block of 128: their e4m3 values and the block's scale.
+// p = t w is exact in float32 for 16-bit types (22 bits at most) where the block's largest stays inside: below 2^-80 parts that count may fall off its lower end.
+// The factor r of the row is kept in 64 bits, so that the scale is the right one also where the block's largest value lies next to 448 times a power of two.
+// Other blocks, and float32 rows, have 64-bit products.
 template <int T>
 __device__ __forceinline__ u2 quantize8(const Eight<T>& t, const Eight<T>& w, double r, float& scale) {
   double y[8];
-  double amax;
-  if constexpr (T == HTR_F32) {
-    amax = 0.0;
+  double amax = 0.0;
+  bool exact = false;
+  if constexpr (T != HTR_F32) {
+    float p[8], m = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) { p[k] = t.get(k) * w.get(k); m = fmaxf(m, fabsf(p[k])); }
+    m = max16(m);
+    exact = m >= 0x1p-80f && m < INFINITY;      // the same in all 16 lanes
+    if (exact) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) y[k] = (double)p[k] * r;
+      amax = (double)m * r;
+    }
+  }
+  if (!exact) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       y[k] = (double)finite_or_nan(t.get(k)) * (double)w.get(k) * r;
@@ -137,15 +150,6 @@ __device__ __forceinline__ u2 quantize8(const Eight<T>& t, const Eight<T>& w, do
       amax = fmax(amax, fabs(y[k]));
     }
     amax = max16(amax);
-  } else {
-    float m = 0.f;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float p = finite_or_nan(t.get(k) * w.get(k));
-      m = fmaxf(m, fabsf(p));
-      y[k] = (double)p * r;
-    }
-    amax = (double)max16(m) * r;
   }
   const int e = min(e4m3_exponent(amax), 120);      // beyond: larger than float32 can hold
   const double inv = __builtin_bit_cast(double, (unsigned long long)(1023 - e) << 52);
@@ -259,9 +263,14 @@ __global__ __launch_bounds__(1024) void k_rms_norm(const NormArgs a) {
     } else {
       if (c >= n) continue;
       float f[8];
-      const float rf = (float)r;
+      if (r > 0x1p-100 && r < 0x1p100) {
+        const float rf = (float)r;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] = t[i].get(k) * rf * w[i].get(k);
+        for (int k = 0; k < 8; ++k) f[k] = t[i].get(k) * rf * w[i].get(k);
+      } else {      // the factor may have no float32, t r has
+#pragma unroll
+        for (int k = 0; k < 8; ++k) f[k] = (float)(t[i].get(k) * r) * w[i].get(k);
+      }
       Eight<T> y;
       y.set(f);
       store(y, a.y, c);
@@ -308,8 +317,7 @@ __global__ __launch_bounds__(1024) void k_rms_norm_long(const NormArgs a, int dt
       if (lane == 0) ((HTR_GLOBAL float*)a.scales)[(size_t)row * (n >> 7) + b] = exp2i(e);
     }
   } else {
-    const float rf = (float)r;
-    for (int c = threadIdx.x; c < n; c += 1024) store_elem_g(a.y, dtype, (size_t)(row * n) + c, at(c) * rf * load_elem_g(a.weight, dtype, c));
+    for (int c = threadIdx.x; c < n; c += 1024) store_elem_g(a.y, dtype, (size_t)(row * n) + c, (float)(at(c) * r) * load_elem_g(a.weight, dtype, c));
   }
 }
 

@@ -140,6 +140,26 @@ def test_norm_of_zeros_infinities_and_nan(gen):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [256, 40960])
+@pytest.mark.parametrize("dtype,size,weight", [(F32, 1e38, 1.0), (F32, 1e-39, 1.0), (F32, 1e30, 1e20), (BF16, 2.0 ** 125, 1.0), (BF16, 2.0 ** 124, 2.0 ** 20),
+                                               (BF16, 2.0 ** -100, 2.0 ** -40), (F16, 2.0 ** -12, 2.0 ** -12)])
+def test_norm_of_rows_of_any_size(gen, dtype, n, size, weight):
+    """Factors, or products with the weight, that float32 cannot hold, of results that it can."""
+    sign = lambda: torch.randint(0, 2, (3, n), device="cuda", generator=gen) * 2 - 1
+    x = (sign() * size * (1 + torch.rand(3, n, device="cuda", generator=gen))).to(dtype)
+    w = (weight * (1 + torch.rand(n, device="cuda", generator=gen))).to(dtype)
+    assert x.isfinite().all()
+    want, _ = norm64(x, w, 0.0, None)
+    # as in test_norm; below the smallest normal value a rounding in float32 is off by half of 2^-149
+    assert_within(ops.rms_norm(x, w, 0.0), want, want.abs() * 3.01 * 2.0 ** -24 + 2.0 ** -149 + half_step(want * (1 + 2.0 ** -22), dtype))
+    q, s = ops.rms_norm(x, w, 0.0, quantize=True)
+    assert torch.equal(s.double(), quantized(want)[1])
+    v = (want / s.double().repeat_interleave(128, -1)).abs()                               # as in test_norm_in_eight_bits
+    step = torch.exp2(torch.floor(torch.log2(v.clamp(min=2.0 ** -6))) - 3)
+    assert_within(q, want / s.double().repeat_interleave(128, -1), step / 2 + v * 2.0 ** -23)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("quantize", [False, True])
 def test_norm_takes_strides_and_any_alignment(gen, quantize):
     big, w = randn(gen, 6, 3, 400, dtype=BF16), randn(gen, 257, dtype=BF16)
