@@ -213,7 +213,7 @@ def linear_fp8(x, qweight, scales, bias=None, out_dtype=None):
     if bias is not None and (bias.dtype != dtype or bias.shape != (m,)):
         raise RuntimeError("linear_fp8: the bias must be [m] in the result's type")
     _on_one_gpu("linear_fp8", first, qweight, scales, bias, x[1] if _pair(x) else None)
-    _refuse_derivatives("linear_fp8", *(x if _pair(x) else (x,)), scales, bias)
+    _refuse_derivatives("linear_fp8", *(x if _pair(x) else (x,)), qweight, scales, bias)
     q, s = _check_rows("linear_fp8", x, 1, False)
     bias = None if bias is None else bias.contiguous()
     y = torch.empty(first.shape[:-1] + (m,), dtype=dtype, device=q.device)
@@ -250,10 +250,10 @@ def grouped_mm(x, weight, ends, out_dtype=None):
     dtype = _out_dtype("grouped_mm", out_dtype, x)
     if first.dim() != 2 or first.shape[1] != n:
         raise RuntimeError(f"grouped_mm wants rows [R, {n}]")
-    if ends.dtype != torch.int32 or ends.shape != (E,):
+    if ends is None or ends.dtype != torch.int32 or ends.shape != (E,):
         raise RuntimeError("grouped_mm: ends must be int32, one for each expert")
     _on_one_gpu("grouped_mm", first, w, ws, ends, x[1] if _pair(x) else None)
-    _refuse_derivatives("grouped_mm", *(x if _pair(x) else (x,)), *((ws,) if eight else (w,)))
+    _refuse_derivatives("grouped_mm", *(x if _pair(x) else (x,)), w, ws)
     q, s = _check_rows("grouped_mm", x, E, True) if eight else (_packed(x), None)
     ends = ends.contiguous()
     R = first.shape[0]
@@ -300,7 +300,7 @@ def moe_experts_stacked(x, expert_ids, expert_weights, gate_up, down):
     if expert_ids.dim() != 2 or expert_ids.shape[0] != T or expert_ids.shape != expert_weights.shape or expert_ids.dtype not in (torch.int32, torch.int64):
         raise RuntimeError("moe_experts_stacked: expert_ids int32 or int64 [T, top], expert_weights [T, top]")
     _on_one_gpu("moe_experts_stacked", x, gu, gus, dn, dns, expert_ids, expert_weights)
-    _refuse_derivatives("moe_experts_stacked", x, expert_weights, *((gus, dns) if eight else (gu, dn)))
+    _refuse_derivatives("moe_experts_stacked", x, expert_weights, gu, gus, dn, dns)
     top = expert_ids.shape[1]
     if T == 0 or top == 0:
         return torch.zeros((T, H), dtype=x.dtype, device=x.device)

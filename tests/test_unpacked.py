@@ -543,6 +543,14 @@ def test_refusals_on_a_gpu(gen):
             call()
         with torch.no_grad():
             call()
+    gu8, dn8 = fp8_weight(gen, 1, 256, 128), fp8_weight(gen, 1, 128, 128)
+    asks = lambda p: (p[0].clone().requires_grad_(), p[1])
+    for call in (lambda: ops.linear_fp8(x, *asks((q, s))), lambda: ops.linear_fp8(asks(ops.quantize_fp8(x)), q, s), lambda: ops.grouped_mm(x, asks(gu8), ends),
+                 lambda: ops.moe_experts_stacked(x, ids, wt, asks(gu8), dn8), lambda: ops.moe_experts_stacked(x, ids, wt, gu8, asks(dn8))):
+        with pytest.raises(RuntimeError, match="no derivative"):
+            call()
+    with pytest.raises(RuntimeError, match="ends must be int32"):
+        ops.grouped_mm(x, x[None], None)
 
 
 def test_status_codes_without_a_gpu():
