@@ -121,48 +121,47 @@ template <> struct Eight<HTR_F32> {
   }
 };
 
-// Eight products (t w) r of a row, 16 neighbouring lanes holding a block of 128: their e4m3 values and the block's scale.
-// p = t w is exact in float32 for 16-bit types (22 bits at most) where the block's largest stays inside: below 2^-80 parts that count may fall off its lower end.
-// The factor r of the row is kept in 64 bits, so that the scale is the right one also where the block's largest value lies next to 448 times a power of two.
-// Other blocks, and float32 rows, have 64-bit products.
+// Eight products (t w) r of a row, 16 neighbouring lanes holding a block of 128: their e4m3 values and the block's scale, in float32 to one rounding.
+// t w = p + l without an error (l = 0 for 16-bit types, whose products have 22 bits at most); the factor r of the row, 64 bits, over the scale is u + v;
+// then p u + (p v + l u).  The scale is the right one also where the block's largest value lies next to 448 times a power of two: there, and where
+// parts that count may fall off either end of float32, the block is formed in 64 bits.
 template <int T>
 __device__ __forceinline__ u2 quantize8(const Eight<T>& t, const Eight<T>& w, double r, float& scale) {
-  double y[8];
-  double amax = 0.0;
-  bool exact = false;
-  if constexpr (T != HTR_F32) {
-    float p[8], m = 0.f;
+  float p[8], l[8], m = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) { p[k] = t.get(k) * w.get(k); m = fmaxf(m, fabsf(p[k])); }
-    m = max16(m);
-    exact = m >= 0x1p-80f && m < INFINITY;      // the same in all 16 lanes
-    if (exact) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) y[k] = (double)p[k] * r;
-      amax = (double)m * r;
-    }
+  for (int k = 0; k < 8; ++k) {
+    p[k] = t.get(k) * w.get(k);
+    if constexpr (T == HTR_F32) l[k] = __builtin_fmaf(t.get(k), w.get(k), -p[k]);
+    m = fmaxf(m, fabsf(p[k]));
   }
-  if (!exact) {
+  m = max16(m);                                     // the same in all 16 lanes, and what follows from it
+  int e = e4m3_exponent((double)m * r);
+  bool exact = m >= 0x1p-80f && m < INFINITY && e > -100 && e < 100;
+  if constexpr (T == HTR_F32) exact = exact && e == e4m3_exponent((double)m * r * (1.0 + 0x1p-22)) && e == e4m3_exponent((double)m * r * (1.0 - 0x1p-22));
+  float y[8];
+  if (exact) {
+    const double f = r * __builtin_bit_cast(double, (unsigned long long)(1023 - e) << 52);
+    const float u = (float)f, v = (float)(f - u);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      y[k] = (double)finite_or_nan(t.get(k)) * (double)w.get(k) * r;
-      if (fabs(y[k]) > (double)__FLT_MAX__) y[k] = __builtin_nan("");
-      amax = fmax(amax, fabs(y[k]));
+      if constexpr (T == HTR_F32) y[k] = __builtin_fmaf(p[k], u, __builtin_fmaf(l[k], u, p[k] * v));
+      else y[k] = __builtin_fmaf(p[k], u, p[k] * v);
     }
-    amax = max16(amax);
+  } else {
+    double d[8], amax = 0.0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      d[k] = (double)finite_or_nan(t.get(k)) * (double)w.get(k) * r;
+      if (fabs(d[k]) > (double)__FLT_MAX__) d[k] = __builtin_nan("");
+      amax = fmax(amax, fabs(d[k]));
+    }
+    e = min(e4m3_exponent(max16(amax)), 120);       // beyond: larger than float32 can hold
+    const double inv = __builtin_bit_cast(double, (unsigned long long)(1023 - e) << 52);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) y[k] = (float)(d[k] * inv);
   }
-  const int e = min(e4m3_exponent(amax), 120);      // beyond: larger than float32 can hold
-  const double inv = __builtin_bit_cast(double, (unsigned long long)(1023 - e) << 52);
   scale = exp2i(e);
-  u2 q;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float f[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) f[k] = (float)(y[4 * h + k] * inv);
-    q[h] = pack_e4m3(f[0], f[1], f[2], f[3]);
-  }
-  return q;
+  return u2{pack_e4m3(y[0], y[1], y[2], y[3]), pack_e4m3(y[4], y[5], y[6], y[7])};
 }
 // The same for eight values in float32 as they are
 __device__ __forceinline__ u2 quantize8(const float (&v)[8], float& scale) {
@@ -188,10 +187,25 @@ struct NormArgs {
   double eps;
 };
 
+// sum of a wave, the same in every lane: within 16 lanes by DPP, across them by swaps of rows of lanes (a shuffle through LDS takes several times as long)
+template <int CTRL> __device__ __forceinline__ double dpp_mov64(double v) {
+  const unsigned long long u = __builtin_bit_cast(unsigned long long, v);
+  const uint32_t lo = __float_as_uint(dpp_mov<CTRL>(__uint_as_float((uint32_t)u))), hi = __float_as_uint(dpp_mov<CTRL>(__uint_as_float((uint32_t)(u >> 32))));
+  return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+}
+__device__ __forceinline__ double wave_sum(double v) {
+  v += dpp_mov64<0xB1>(v); v += dpp_mov64<0x4E>(v); v += dpp_mov64<0x141>(v); v += dpp_mov64<0x140>(v);
+  auto both = [](double v, auto swap) {
+    const unsigned long long u = __builtin_bit_cast(unsigned long long, v);
+    const u2s lo = swap((uint32_t)u), hi = swap((uint32_t)(u >> 32));
+    return __builtin_bit_cast(double, (unsigned long long)hi.x << 32 | lo.x) + __builtin_bit_cast(double, (unsigned long long)hi.y << 32 | lo.y);
+  };
+  v = both(v, [](uint32_t x) { return __builtin_amdgcn_permlane16_swap(x, x, false, false); });
+  return both(v, [](uint32_t x) { return __builtin_amdgcn_permlane32_swap(x, x, false, false); });
+}
 // sum over the workgroup, the same in every thread
 __device__ __forceinline__ double block_sum(double v, double* lds) {
-#pragma unroll
-  for (int off = 32; off; off >>= 1) v += __shfl_xor(v, off);
+  v = wave_sum(v);
   const int waves = (blockDim.x + 63) >> 6;
   if (waves == 1) return v;
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
