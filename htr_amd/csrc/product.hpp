@@ -26,38 +26,58 @@ struct ProductArgs {
 // Rows first .. first + count - 1 of expert e are tile number t of tiles of `height` rows, expert by expert; e = experts: rows behind the last
 // expert's; e = -1: no such tile.  Ends are taken as what they may be: at least the one before, at least 0, at most `rows`.
 struct Span { int e, first, count; };
+// running maximum and sum of a wave's values, none below 0, by DPP: four steps within 16 lanes, then the last lane of 16 and of 32 to those behind
+template <int CTRL, int ROWS = 0xF> __device__ __forceinline__ int dpp_or(int old, int v) { return __builtin_amdgcn_update_dpp(old, v, CTRL, ROWS, 0xF, false); }
+__device__ __forceinline__ int scan_max(int v) {
+  v = max(v, dpp_or<0x111>(0, v)); v = max(v, dpp_or<0x112>(0, v)); v = max(v, dpp_or<0x114>(0, v)); v = max(v, dpp_or<0x118>(0, v));
+  v = max(v, dpp_or<0x142, 0xA>(0, v)); return max(v, dpp_or<0x143, 0xC>(0, v));
+}
+__device__ __forceinline__ int scan_sum(int v) {
+  v += dpp_or<0x111>(0, v); v += dpp_or<0x112>(0, v); v += dpp_or<0x114>(0, v); v += dpp_or<0x118>(0, v);
+  v += dpp_or<0x142, 0xA>(0, v); return v + dpp_or<0x143, 0xC>(0, v);
+}
+// 64 experts from `base` on, one to a lane: where its rows begin and end, its tiles, and those up to its last; end0, tiles0: of the experts before
+struct Experts { int start, end, tiles, sum; };
+__device__ __forceinline__ Experts experts_from(const ProductArgs& a, int height, int base, int end0, int tiles0) {
+  const int e = base + (int)(threadIdx.x & 63);
+  Experts x;
+  x.end = max(scan_max(e < a.experts ? max(0, min(a.ends[e], a.rows)) : 0), end0);
+  x.start = dpp_or<0x138>(end0, x.end);      // the lane before
+  x.tiles = (x.end - x.start + height - 1) / height;
+  x.sum = scan_sum(x.tiles) + tiles0;
+  return x;
+}
 __device__ __forceinline__ Span find_span(const ProductArgs& a, int height, int t) {
   if (a.ends == nullptr) {
     const int first = t * height;
     return first < a.rows ? Span{0, first, min(height, a.rows - first)} : Span{-1, 0, 0};
   }
-  const int lane = threadIdx.x & 63;
   int end0 = 0, tiles0 = 0;
   for (int base = 0; base < a.experts; base += 64) {
-    int end = base + lane < a.experts ? min(a.ends[base + lane], a.rows) : 0;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) { const int u = __shfl_up(end, off); if (lane >= off) end = max(end, u); }
-    end = max(end, end0);
-    int start = __shfl_up(end, 1);
-    if (lane == 0) start = end0;
-    const int tiles = (end - start + height - 1) / height;
-    int sum = tiles;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) { const int u = __shfl_up(sum, off); if (lane >= off) sum += u; }
-    sum += tiles0;
-    const unsigned long long in = __ballot(sum > t);
+    const Experts x = experts_from(a, height, base, end0, tiles0);
+    const unsigned long long in = __ballot(x.sum > t);
     if (in) {
       const int l = __builtin_ctzll(in);
-      const int skip = (t - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(tiles, l))) * height;
-      const int first = __builtin_amdgcn_readlane(start, l) + skip;
-      return Span{base + l, first, min(height, __builtin_amdgcn_readlane(end, l) - first)};
+      const int skip = (t - (__builtin_amdgcn_readlane(x.sum, l) - __builtin_amdgcn_readlane(x.tiles, l))) * height;
+      const int first = __builtin_amdgcn_readlane(x.start, l) + skip;
+      return Span{base + l, first, min(height, __builtin_amdgcn_readlane(x.end, l) - first)};
     }
-    end0 = __builtin_amdgcn_readlane(end, 63);
-    tiles0 = __builtin_amdgcn_readlane(sum, 63);
+    end0 = __builtin_amdgcn_readlane(x.end, 63);
+    tiles0 = __builtin_amdgcn_readlane(x.sum, 63);
   }
   // t - tiles0 tiles behind the last expert's; the grid is a bound, so this may lie beyond 32 bits of rows
   const long long first = end0 + (long long)(t - tiles0) * height;
   return first < a.rows ? Span{a.experts, (int)first, min(height, a.rows - (int)first)} : Span{-1, 0, 0};
+}
+// tiles that find_span knows, those of rows behind the last expert's among them
+__device__ __forceinline__ int count_spans(const ProductArgs& a, int height) {
+  int end0 = 0, tiles0 = 0;
+  for (int base = 0; a.ends != nullptr && base < a.experts; base += 64) {
+    const Experts x = experts_from(a, height, base, end0, tiles0);
+    end0 = __builtin_amdgcn_readlane(x.end, 63);
+    tiles0 = __builtin_amdgcn_readlane(x.sum, 63);
+  }
+  return tiles0 + (a.rows - end0 + height - 1) / height;
 }
 // tiles that find_span knows at most: experts with rows leave one short tile each, and so do the rows behind them
 inline long long span_bound(long long rows, int experts, bool grouped, int height) {
@@ -222,7 +242,7 @@ __global__ __launch_bounds__(STREAM_WAVES * 64) void k_product_stream(const Prod
 // hidden columns; y [rows][m / 2] is silu(gate) up, in 16 bits or in e4m3 (then TM / 2 = 128 columns share a scale; rows behind the last expert's are left).
 __device__ __forceinline__ int swizzle_w(int r) { return ((r >> 1) & 1) | ((r >> 3 & 3) << 1); }
 __device__ __forceinline__ int swizzle_x(int r) { return (r >> 1) & 7; }
-constexpr int TILE_XCDS = 8;
+constexpr int TILE_XCDS = 8, TOGETHER = 8;
 
 // eight consecutive outputs of a row, from i on, as far as the row goes
 template <int Y> __device__ __forceinline__ void store8(const ProductArgs& a, float (&f)[8], size_t at, int i) {
@@ -241,7 +261,7 @@ template <int Y> __device__ __forceinline__ void store8(const ProductArgs& a, fl
 }
 
 template <int T, int WM, int WN, int AT, int BT, int NS, bool GATED>
-__global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductArgs a, int mtiles, int ttiles, int together) {
+__global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductArgs a, int mtiles) {
   constexpr int WAVES = WM * WN, TM = 16 * AT * WM, TN = 16 * BT * WN;
   constexpr int XW = (TN + 63) / 64;                             // waves that load rows' scales
   constexpr int SCALES = T == P_F8 ? XW * 256 + 256 : 0, STAGE = (TM + TN) * 128 + SCALES;    // e4m3: the rows' scales, then the matrix's
@@ -256,18 +276,21 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
   const int wm = wv / WN, wn = wv % WN;
   const size_t row_bytes = (size_t)a.n * bytes_of<T>;
   const int slabs = (int)((row_bytes + 127) >> 7);
-  // Workgroups go to the eight XCDs in turn: neighbouring tiles to one XCD, one for each of its workgroups, `together` tiles of x by a few of the matrix, whose
-  // rows its L2 serves to several of them; the next run to the next XCD.  Tiles without rows, which are the last, fall on all alike.
-  const int run = gridDim.x / TILE_XCDS;
-  int id = (int)(blockIdx.x % TILE_XCDS) * run + (int)(blockIdx.x / TILE_XCDS);
+  // Workgroups go to the eight XCDs in turn, and 256 of them are one to a compute unit: of each 256 tiles one XCD takes 32 neighbours, TOGETHER tiles of x by a
+  // few of the matrix, whose rows its L2 serves to several of them.
+  const int all = blockIdx.x & ~255, run = min(256, (int)gridDim.x - all) / TILE_XCDS;
+  int id = all + (int)(blockIdx.x % TILE_XCDS) * run + (int)(blockIdx.x & 255) / TILE_XCDS;
+
+  // the launch knows a bound of the tiles only, and workgroups that come to nothing are to be the last
+  const int ttiles = count_spans(a, TN);
 
   // The tile in hand, and the next one that has products, if there is one; rows behind the last expert's become zeros on the way
   struct Tile { Span s; int m0; };
   Tile mine, then;
   auto find = [&](Tile& t) {
     for (; id < mtiles * ttiles; id += gridDim.x) {
-      const int strip = id / (mtiles * together), t0 = strip * together, high = min(together, ttiles - t0);
-      const int rest = id - strip * mtiles * together;
+      const int strip = id / (mtiles * TOGETHER), t0 = strip * TOGETHER, high = min(TOGETHER, ttiles - t0);
+      const int rest = id - strip * mtiles * TOGETHER;
       t.m0 = rest / high * TM;
       t.s = find_span(a, TN, t0 + rest % high);
       if (t.s.e == a.experts) { if constexpr (!GATED) zero_rows(a, t.s, t.m0, TM); }

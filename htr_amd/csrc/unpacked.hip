@@ -106,7 +106,7 @@ template <int T, int WM, int WN, int AT, int BT, int NS, bool GATED = false> hip
   // tile to tile
   const bool stream = (long long)a.n * bytes_of<T> > 128 * (NS - 1);
   const long long wgs = 256 * (160 * 1024 / LDS), up = (tiles + TILE_XCDS - 1) / TILE_XCDS * TILE_XCDS;
-  return launch(k_product_tile<T, WM, WN, AT, BT, NS, GATED>, dim3((unsigned)(stream && wgs < up ? wgs : up)), WM * WN * 64, LDS, st, a, (int)mtiles, (int)ttiles, 8);
+  return launch(k_product_tile<T, WM, WN, AT, BT, NS, GATED>, dim3((unsigned)(stream && wgs < up ? wgs : up)), WM * WN * 64, LDS, st, a, (int)mtiles);
 }
 // Which tiles for many rows: the ones whose rounds take the least time by what a slab of a tile takes where the compute units have little else to do
 // and where all are at work (measured on 64 .. 8192 rows of 4096 .. 14336 columns, ns; both types: their slabs have the same bytes).  A larger tile multiplies
