@@ -276,19 +276,18 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
   const int wm = wv / WN, wn = wv % WN;
   const size_t row_bytes = (size_t)a.n * bytes_of<T>;
   const int slabs = (int)((row_bytes + 127) >> 7);
-  // Workgroups go to the eight XCDs in turn, and 256 of them are one to a compute unit: of each 256 tiles one XCD takes 32 neighbours, TOGETHER tiles of x by a
-  // few of the matrix, whose rows its L2 serves to several of them.
-  const int all = blockIdx.x & ~255, run = min(256, (int)gridDim.x - all) / TILE_XCDS;
-  int id = all + (int)(blockIdx.x % TILE_XCDS) * run + (int)(blockIdx.x & 255) / TILE_XCDS;
-
-  // the launch knows a bound of the tiles only, and workgroups that come to nothing are to be the last
-  const int ttiles = count_spans(a, TN);
+  // Workgroups go to the eight XCDs in turn: neighbouring tiles to one XCD, one for each of its workgroups as far as there are tiles, TOGETHER tiles of x by a few
+  // of the matrix, whose rows its L2 serves to several of them; the next run to the next XCD.  The launch knows a bound of the tiles only: without
+  // counting them whole XCDs would come to nothing.
+  const int ttiles = count_spans(a, TN), total = mtiles * ttiles;
+  const int run = min((int)gridDim.x, (total + TILE_XCDS - 1) / TILE_XCDS * TILE_XCDS) / TILE_XCDS, nth = blockIdx.x / TILE_XCDS;
+  int id = nth < run ? (int)(blockIdx.x % TILE_XCDS) * run + nth : total;
 
   // The tile in hand, and the next one that has products, if there is one; rows behind the last expert's become zeros on the way
   struct Tile { Span s; int m0; };
   Tile mine, then;
   auto find = [&](Tile& t) {
-    for (; id < mtiles * ttiles; id += gridDim.x) {
+    for (; id < total; id += gridDim.x) {
       const int strip = id / (mtiles * TOGETHER), t0 = strip * TOGETHER, high = min(TOGETHER, ttiles - t0);
       const int rest = id - strip * mtiles * TOGETHER;
       t.m0 = rest / high * TM;

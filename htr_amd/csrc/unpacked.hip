@@ -108,13 +108,15 @@ template <int T, int WM, int WN, int AT, int BT, int NS, bool GATED = false> hip
   const long long wgs = 256 * (160 * 1024 / LDS), up = (tiles + TILE_XCDS - 1) / TILE_XCDS * TILE_XCDS;
   return launch(k_product_tile<T, WM, WN, AT, BT, NS, GATED>, dim3((unsigned)(stream && wgs < up ? wgs : up)), WM * WN * 64, LDS, st, a, (int)mtiles);
 }
-// Which tiles for many rows: the ones whose rounds take the least time by what a slab of a tile takes where the compute units have little else to do
-// and where all are at work (measured on 64 .. 8192 rows of 4096 .. 14336 columns, ns; both types: their slabs have the same bytes).  A larger tile multiplies
-// more for what it loads, a smaller one leaves fewer compute units idle: 333 rows on 6144x4096 in e4m3 52 us by 256x256, 27 by 128x128, 25 by 128x64;
-// 1000 on 14336x4096 68, 99, 109; 100 on 6144x4096 51, 28, 22 and 15 by 64x64.
+// Which tiles for many rows: the ones whose rounds take the least time by what a slab of a tile takes (ns) with a tile to a few compute units, and with all
+// at work, as many to each as fit.  Measured on 48 .. 8192 rows of 4096 .. 8192 columns, matrices from HBM.  A larger tile multiplies more for what it loads, a
+// smaller one leaves fewer compute units idle: 256 rows on 4096x8192 in e4m3 99 us by 256x256, 50 by 128x128, 40 by 128x64, 29 by 64x64, 35 by 64x32; 512 rows
+// 97, 50, 41, 47, 61; 4096 rows 126, 183, 200, 283, 385.
 struct TileChoice { int tm, tn, at_once; float light, full; };
-constexpr TileChoice TILES[] = {{256, 256, 1, 1450.f, 1950.f}, {256, 128, 1, 950.f, 1300.f}, {128, 128, 1, 700.f, 800.f},
-                                {128, 64, 2, 550.f, 850.f},    {64, 64, 2, 420.f, 600.f},    {64, 32, 3, 290.f, 450.f}};
+constexpr TileChoice TILES_8[] = {{256, 256, 1, 1440.f, 1900.f}, {256, 128, 1, 1050.f, 1100.f}, {128, 128, 1, 710.f, 760.f},
+                                  {128, 64, 2, 570.f, 870.f},    {64, 64, 2, 395.f, 685.f},     {64, 32, 3, 285.f, 695.f}};
+constexpr TileChoice TILES_16[] = {{256, 256, 1, 1380.f, 1700.f}, {256, 128, 1, 810.f, 1000.f}, {128, 128, 1, 580.f, 640.f},
+                                   {128, 64, 2, 480.f, 735.f},    {64, 64, 2, 315.f, 510.f},    {64, 32, 3, 290.f, 450.f}};
 // gate and up in one: 128 hidden columns to a tile
 constexpr TileChoice GATED_TILES[] = {{256, 256, 1, 1450.f, 1950.f}, {256, 128, 1, 950.f, 1300.f}, {256, 64, 1, 750.f, 950.f}, {256, 32, 1, 600.f, 700.f}};
 template <int N> int best_tile(const TileChoice (&choices)[N], const ProductArgs& a, size_t row_bytes) {
@@ -125,9 +127,12 @@ template <int N> int best_tile(const TileChoice (&choices)[N], const ProductArgs
     const float mtiles = (float)((a.m + c.tm - 1) / c.tm), full = (float)a.rows / c.tn;
     const float experts = (float)(a.rows < a.experts ? a.rows : a.experts);
     // an expert's last tile is half full on average
-    const float tiles = mtiles * (a.ends == nullptr ? ceilf(full) : fmaxf(experts, full + 0.5f * experts));
-    const float rounds = tiles / (256.f * c.at_once), whole = floorf(rounds), part = rounds - whole;
-    const float ns = (4000.f + (float)((row_bytes + 127) >> 7) * (whole * c.full + (part > 0.f ? c.light + part * (c.full - c.light) : 0.f)));
+    const float tiles = mtiles * (a.experts == 1 ? ceilf(full) : fmaxf(experts, full + 0.5f * experts));
+    const float whole = floorf(tiles / (256.f * c.at_once)), rest = tiles - whole * 256.f * c.at_once;
+    // the last round: the share of compute units at work, or where several tiles fit, tiles to one beyond the first; with half of them at one more, all wait
+    const float beyond = fmaxf(rest / 256.f - 1.f, 0.f), some = beyond - floorf(beyond);
+    const float share = c.at_once == 1 ? rest / 256.f : (floorf(beyond) + (some > 0.f ? fminf(1.f, (1.f + 4.f * some) / 3.f) : 0.f)) / (c.at_once - 1.f);
+    const float ns = 4000.f + (float)((row_bytes + 127) >> 7) * (whole * c.full + (rest > 0.f ? c.light + share * (c.full - c.light) : 0.f));
     if (k == 0 || ns < least) { least = ns; best = k; }
   }
   return best;
@@ -159,7 +164,7 @@ template <int T> hipError_t launch_product(const ProductArgs& a, hipStream_t st)
   } else if (mean <= 24) {
     return launch_tile<T, 4, 1, 2, 2, 4>(a, st);
   }
-  switch (best_tile(TILES, a, (size_t)a.n * bytes_of<T>)) {
+  switch (T == P_F8 ? best_tile(TILES_8, a, (size_t)a.n) : best_tile(TILES_16, a, (size_t)a.n * 2)) {
     case 0: return launch_tile<T, 2, 4, 8, 4, 2>(a, st);
     case 1: return launch_tile<T, 4, 2, 4, 4, 3>(a, st);
     case 2: return launch_tile<T, 2, 2, 4, 4, 3>(a, st);
