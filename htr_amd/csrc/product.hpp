@@ -107,7 +107,7 @@ __device__ __forceinline__ float silu(float g) { return g / (1.f + __expf(-g)); 
 // ------------------------------------------------------------------------------------------------ few rows
 // A workgroup owns 16 R rows of a matrix and up to 16 TT rows of x; its waves take the slabs in turn, straight from memory into registers
 // (every byte of the matrix is used by one wave once: LDS would only be a detour), and add up through LDS.
-// Bound: HBM, the matrix read once.
+// Bound: HBM, the matrix read once: 96 rows of 64 experts of 2816x2048 in e4m3 52 us, 5.2 TB/s; one row on 1024x4096 5.0 us, the latency of two loads and the sum.
 // X: the type of x; 16-bit rows with an e4m3 matrix are rounded on the way, by every workgroup for itself: about 110 instructions to a slab, beside
 // its 2 KB or more of the matrix, against a launch ahead of this one.
 template <int T, int X, int R, int TT, int STREAM_WAVES>
@@ -230,6 +230,8 @@ __global__ __launch_bounds__(STREAM_WAVES * 64) void k_product_stream(const Prod
 }
 
 // ------------------------------------------------------------------------------------------------ many rows
+// Bound: the matrix unit (its power) for thousands of rows, LDS loads' latency below, HBM where every expert has few.  8192 rows on 14336x4096 in e4m3 418 us, 2.3 PFLOP/s
+// (the library with one scale 2.9); 24576 rows of 64 experts of 2048x1408 in 16 bits 187 us.  A slab of a 256x256 tile takes 1.6 us in 16 bits and 1.8 in e4m3.
 // A workgroup of WM x WN waves takes tiles of TM = 16 AT WM rows of a matrix by TN = 16 BT WN rows of x, one after the other, their slabs one stream: slabs go
 // from memory straight to LDS, a ring of NS stages.  While one slab is multiplied from registers, the next one is read, and the one NS behind is asked for;
 // a tile's last products run while the next tile's first slabs arrive, and its results go out during the next one's products.
