@@ -322,6 +322,35 @@ def test_grouped_mm(gen, counts, kind, m, n, behind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", [BF16, E4M3], ids=str)
+@pytest.mark.parametrize("counts,m", [([e * 7 % 37 for e in range(130)], 512), ([2000, 0, 3100], 4096), ([0] * 63 + [1900, 0, 2500] + [1] * 70, 1000),
+                                      ([300 - 4 * e for e in range(75)], 1024), ([0] * 64 + [700], 2900)], ids=lambda c: str(len(c) if isinstance(c, list) else c))
+def test_grouped_mm_of_more_tiles_than_run_at_once(gen, kind, counts, m):
+    """More than 64 experts, several tiles to a workgroup, every height of tile."""
+    n, behind = 256, 45
+    R, E = sum(counts) + behind, len(counts)
+    if kind == E4M3:
+        x, w = ops.quantize_fp8(randn(gen, R, n)), fp8_weight(gen, E, m, n)
+        xd, wd = value(*x), w
+    else:
+        x, w = randn(gen, R, n, dtype=kind), randn(gen, E, m, n, dtype=kind, scale=n ** -0.5)
+        xd, wd = x.double(), w
+    ends = _ends(counts)
+    y = ops.grouped_mm(x, w, ends)
+    first = 0
+    for e, c in enumerate(counts):
+        if c:
+            want, bound = product_bound(xd[first:first + c], value(wd[0][e], wd[1][e]) if kind == E4M3 else wd[e].double(), BF16)
+            assert_within(y[first:first + c], want, bound)
+        first += c
+    assert (y[first:] == 0).all()
+    wild = ends.clone()
+    wild[0::3] -= 2 ** 30                      # each counts as the one before it
+    meant = wild.clamp(0, R).cummax(0).values.int()
+    assert torch.equal(ops.grouped_mm(x, w, wild), ops.grouped_mm(x, w, meant))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("n", [8, 24, 56, 64, 72, 120, 136, 1000])
 @pytest.mark.parametrize("counts", [[3, 1], [100, 90], [300, 400]])
 def test_grouped_mm_on_short_rows(gen, n, counts):
@@ -404,6 +433,19 @@ def test_moe_experts_stacked(gen, eight, dtype, T, E, top, H, F):
     assert_within(y, want, bound)
     assert torch.equal(ops.moe_experts_stacked(x, ids.int(), wt.double(), gate_up, down), y)
     assert torch.equal(ops.moe_experts_stacked(x, ids, wt, gate_up, down), y)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("eight", [False, True], ids=["16", "8"])
+def test_moe_of_more_experts_than_a_wave_has_lanes(gen, eight):
+    T, E, top, H, F, dtype = 60, 70, 7, 256, 128, BF16
+    x, wt = randn(gen, T, H, dtype=dtype), torch.rand(T, top, device="cuda", generator=gen)
+    ids = torch.argsort(torch.rand(T, E, device="cuda", generator=gen))[:, :top]
+    if eight:
+        gate_up, down = fp8_weight(gen, E, 2 * F, H), fp8_weight(gen, E, H, F)
+    else:
+        gate_up, down = randn(gen, E, 2 * F, H, dtype=dtype, scale=H ** -0.5), randn(gen, E, H, F, dtype=dtype, scale=F ** -0.5)
+    assert_within(ops.moe_experts_stacked(x, ids, wt, gate_up, down), *moe64(x, ids, wt, gate_up, down, eight, dtype))
 
 
 @pytest.mark.gpu
