@@ -71,7 +71,11 @@ template <int T, bool ANY> hipError_t launch_norm(const NormArgs& a, hipStream_t
   return quant ? launch_norm<T, false, true, ANY>(a, st) : launch_norm<T, false, false, ANY>(a, st);
 }
 template <int T> hipError_t launch_norm(const NormArgs& a, hipStream_t st) {
-  if (a.n > 32768) return launch(a.scales ? k_rms_norm_long<true> : k_rms_norm_long<false>, dim3((unsigned)a.rows), 1024, 0, st, a, T);
+  if (a.n > 32768) {
+    const dim3 grid((unsigned)a.rows);
+    if (a.residual) return a.scales ? launch(k_rms_norm_long<T, true, true>, grid, 1024, 0, st, a) : launch(k_rms_norm_long<T, true, false>, grid, 1024, 0, st, a);
+    return a.scales ? launch(k_rms_norm_long<T, false, true>, grid, 1024, 0, st, a) : launch(k_rms_norm_long<T, false, false>, grid, 1024, 0, st, a);
+  }
   const bool vector = a.n % 8 == 0 && aligned(a.x, 16) && aligned(a.residual, 16) && aligned(a.weight, 16) && aligned(a.y, 16) && aligned(a.sum, 16) &&
                       a.x_stride % 8 == 0 && a.residual_stride % 8 == 0;
   return vector ? launch_norm<T, false>(a, st) : launch_norm<T, true>(a, st);
@@ -237,7 +241,7 @@ extern "C" {
 
 int htr_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, const void* weight, int64_t rows, int n, double eps,
                  int dtype, void* y, void* scales, void* sum, void* stream) {
-  if (rows < 0 || rows > 0x7FFFFFFF || n < 1) return HTR_ERR_SIZE;
+  if (rows < 0 || rows > 0x7FFFFFFF || n < 1 || n > (1 << 30)) return HTR_ERR_SIZE;
   if (!is_dtype(dtype)) return HTR_ERR_DTYPE;
   if (rows == 0) return HTR_OK;
   if (!x || !weight || !y || (residual != nullptr) != (sum != nullptr)) return HTR_ERR_NULL;

@@ -319,7 +319,7 @@ int htr_dequant_w(const void* qweight, const void* scales, const void* su, const
  *   weight       [n] of dtype
  *   y            [rows][n]: of dtype where scales is NULL, otherwise e4m3 with scales [rows][n / 128], n a multiple of 128
  *   sum          [rows][n] of dtype: t.  Nothing written may overlap anything read.
- * 0 <= rows < 2^31.  Any alignment of the elements; multiples of 16 bytes (and of 8 columns) are faster, rows of more than 32768 columns slower.
+ * 0 <= rows < 2^31, 1 <= n <= 2^30.  Any alignment of the elements; multiples of 16 bytes (and of 8 columns) are faster.
  */
 int htr_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, const void* weight, int64_t rows, int n, double eps,
                  int dtype, void* y, void* scales, void* sum, void* stream);

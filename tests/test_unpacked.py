@@ -629,7 +629,7 @@ def test_status_codes_without_a_gpu():
     assert prod(rows=0) == 0 and prod(rows=-1) == 11 and prod(m=0) == 11 and prod(n=64) == 11 and prod(n=4, t=0) == 11 and prod(t=2) == 5 and prod(yt=3) == 5
     assert prod(E=2) == 1 and prod(E=0, ends=p) == 11 and prod(xs=None) == 1 and prod(ws=None) == 1 and prod(w=None) == 1 and prod(x=odd) == 7 and prod(y=odd) == 7
     assert prod(ends=odd) == 7 and prod(b=odd) == 7 and prod(rows=1 << 31) == 11 and prod(E=70000, ends=p) == 11
-    assert prod(n=(1 << 22) + 128) == 11 and prod(m=(1 << 26) + 1) == 11 and quant(n=(1 << 30) + 128) == 11         # places in a tile, and a launch, in 32 bits
+    assert prod(n=(1 << 22) + 128) == 11 and prod(m=(1 << 26) + 1) == 11 and quant(n=(1 << 30) + 128) == 11 and norm(n=(1 << 30) + 8) == 11         # places in a tile, and a launch, in 32 bits
     mixed = lambda xt, rows=1, t=3, xs=None: L.htr_product(p, xt, xs, p, None, None, None, p, rows, 128, 128, 1, t, 0, None)
     assert mixed(2) == 5 and mixed(0, rows=17) == 5 and mixed(1, t=0) == 5 and mixed(3, t=0) == 5 and mixed(0) == 1      # the last one: no scales of w
     assert L.htr_product_rounds(16, 1, 0) == 1 and L.htr_product_rounds(17, 1, 0) == 0 and L.htr_product_rounds(256, 64, 1) == 1 and L.htr_product_rounds(257, 64, 1) == 0
