@@ -157,12 +157,21 @@ template <int T> hipError_t launch_product(const ProductArgs& a, hipStream_t st)
     const long long tiles = grouped ? (a.rows < a.experts ? a.rows : a.experts) : 1, wgs = (a.m + 15) / 16 * tiles;
     const long long slabs = ((long long)a.n * bytes_of<T> + 127) / 128;
     if (grouped && wgs >= 4 * 512) return launch_stream<T, 4, 1, 4>(a, st);
-    // short rows give eight waves too little each (7 rows on 15657x384 in e4m3 5.5 us by 16 rows to a workgroup of 8 waves, 4.7 by 32 to one of 4; 4 tokens over 8
-    // of 16 experts of 1920/384 37 and 31); long rows of few workgroups need more waves to share them
-    if (wgs >= 512 && slabs <= 16) return launch_stream<T, 2, 1, 4>(a, st);
+    // Rows of fewer slabs than waves leave some idle (7 rows on 15657x384 in e4m3 5.5 us by 16 rows to a workgroup of 8 waves, 4.7 by 32 to one of 4), and rows
+    // to be rounded are rounded by half as many (4 tokens over 8 of 16 experts of 1920/384 37 and 31); long rows of few workgroups need more waves to share them
+    if (wgs >= 512 && (slabs < 8 || (slabs <= 16 && T == P_F8 && a.x_type != HTR_E4M3))) return launch_stream<T, 2, 1, 4>(a, st);
     if (wgs <= 256 && slabs >= 64) return launch_stream<T, 1, 1, 16>(a, st);
     return launch_stream<T, 1, 1, 8>(a, st);
   }
+  // Matrices so small that each compute unit has a workgroup of 16 of their rows by 16 or 32 of x at most: many waves for each are faster than a ring for few (us,
+  // 16 bits: 64 rows on 1024x4096 11.0, by 32 rows 15.0, by tiles of 64x32 20.1; on 2048x4096 19.6, 15.4, 20.4; on 4096x4096 38, 29, 21.3)
+  auto workgroups = [&](int height) {
+    const float full = (float)a.rows / height, experts = (float)(a.rows < a.experts ? a.rows : a.experts);
+    return (float)((a.m + 15) / 16) * (a.experts == 1 ? ceilf(full) : fmaxf(experts, full + 0.5f * experts));
+  };
+  const bool y_fits = span_bound(a.rows, a.experts, grouped, 16) <= 65535;      // the grid's second dimension
+  if (y_fits && workgroups(16) <= 256.f) return launch_stream<T, 1, 1, 8>(a, st);
+  if (y_fits && workgroups(32) <= 256.f) return launch_stream<T, 1, 2, 8>(a, st);
   if (!grouped) {
     if (mean <= 32) return a.m < 8192 ? launch_stream<T, 1, 2, 8>(a, st) : a.m < 16384 ? launch_tile<T, 2, 2, 2, 1, 4>(a, st) : launch_tile<T, 4, 1, 2, 2, 4>(a, st);
   } else if (mean <= 24) {
