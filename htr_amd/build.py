@@ -7,6 +7,7 @@ compiles anything.  Run `python -m htr_amd.build`.
 import os
 import subprocess
 import sys
+import tempfile
 
 CSRC = os.path.join(os.path.dirname(os.path.abspath(__file__)), "csrc")
 LIB = os.path.join(CSRC, "libhtr_gfx950.so")
@@ -43,10 +44,12 @@ def binding_command():
 
 
 def build(verbose=False, extra=()):
-    objects = [source[:-4] + ".o" for source in SOURCES]
+    """Compiles the sources side by side and links them; `extra` goes to both steps.  The objects lie in a folder of this build alone."""
     flags = [f for f in HIPCC_FLAGS if f != "-shared"]
-    _run([[hipcc()] + flags + list(extra) + ["-c", source, "-o", obj] for source, obj in zip(SOURCES, objects)] + [binding_command()], verbose)
-    _run([[hipcc(), "--offload-arch=gfx950", "-shared", "-o", LIB] + objects], verbose)
+    with tempfile.TemporaryDirectory() as folder:
+        objects = [os.path.join(folder, os.path.basename(source)[:-4] + ".o") for source in SOURCES]
+        _run([[hipcc()] + flags + list(extra) + ["-c", source, "-o", obj] for source, obj in zip(SOURCES, objects)] + [binding_command()], verbose)
+        _run([[hipcc(), "--offload-arch=gfx950", "-shared"] + list(extra) + ["-o", LIB] + objects], verbose)
     return LIB
 
 
