@@ -57,6 +57,7 @@ SIGNATURES = {
     "htr_quantize_e4m3": (_i, [_vp, _i64, _i64, _i, _i, _vp, _vp, _vp]),
     "htr_product": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _i, _i, _vp]),
     "htr_product_rounds": (_i, [_i64, _i, _i]),
+    "htr_product_plan": (_i, [_i64, _i, _i, _i, _i, _i, _i, _i, ctypes.POINTER(ctypes.c_int)]),
     "htr_moe_stacked_scratch_bytes": (_sz, [_i64, _i, _i, _i, _i, _i]),
     "htr_moe_stacked": (_i, [_vp, _i, _vp, _i, _vp, _i64, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _sz, _vp]),
 }

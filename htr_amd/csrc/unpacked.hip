@@ -91,7 +91,28 @@ hipError_t launch_quantize(const void* x, int dtype, long long rows, int n, long
 }
 
 // ---- products
-template <int T, int R, int TT, int WAVES> hipError_t launch_stream(const ProductArgs& a, hipStream_t st) {
+// The kernels by their template arguments, for who launches them and for who asks which one is launched
+template <int R_, int TT_, int WAVES_> struct Stream { static constexpr int R = R_, TT = TT_, WAVES = WAVES_; };
+template <int WM_, int WN_, int AT_, int BT_, int NS_, bool GATED_ = false> struct Tiles {
+  static constexpr int WM = WM_, WN = WN_, AT = AT_, BT = BT_, NS = NS_, TM = 16 * AT_ * WM_, TN = 16 * BT_ * WN_;
+  static constexpr bool GATED = GATED_;
+  template <int T> static constexpr size_t LDS = NS * ((TM + TN) * 128 + (T == P_F8 ? (TN + 63) / 64 * 256 + 256 : 0)) + (GATED && T == P_F8 ? WM * TN * 4 : 0);
+};
+struct TileGrid { long long mtiles, tiles; unsigned workgroups; };      // tiles: a bound where rows are grouped
+template <int T, typename K> TileGrid tile_grid(const ProductArgs& a) {
+  constexpr size_t LDS = K::template LDS<T>;
+  static_assert(LDS <= 160 * 1024, "a compute unit's LDS");
+  TileGrid g;
+  g.mtiles = (a.m + K::TM - 1) / K::TM;
+  g.tiles = g.mtiles * span_bound(a.rows, a.experts, a.ends != nullptr, K::TN);
+  // as many workgroups as run at once (an MI355X has 256 compute units), a multiple of the XCDs; rows of fewer slabs than stages have no stream to run on from
+  // tile to tile
+  const bool stream = (long long)a.n * bytes_of<T> > 128 * (K::NS - 1);
+  const long long wgs = 256 * (160 * 1024 / LDS), up = (g.tiles + TILE_XCDS - 1) / TILE_XCDS * TILE_XCDS;
+  g.workgroups = (unsigned)(stream && wgs < up ? wgs : up);
+  return g;
+}
+template <int T, int R, int TT, int WAVES> hipError_t launch_kernel(Stream<R, TT, WAVES>, const ProductArgs& a, hipStream_t st) {
   const dim3 grid((a.m + 16 * R - 1) / (16 * R), (unsigned)span_bound(a.rows, a.experts, a.ends != nullptr, 16 * TT));
   if constexpr (T == P_F8 && TT == 1) {
     if (a.x_type == HTR_BF16) return launch(k_product_stream<T, HTR_BF16, R, TT, WAVES>, grid, WAVES * 64, 0, st, a);
@@ -99,18 +120,23 @@ template <int T, int R, int TT, int WAVES> hipError_t launch_stream(const Produc
   }
   return launch(k_product_stream<T, T, R, TT, WAVES>, grid, WAVES * 64, 0, st, a);
 }
-template <int T, int WM, int WN, int AT, int BT, int NS, bool GATED = false> hipError_t launch_tile(const ProductArgs& a, hipStream_t st) {
-  constexpr int TM = 16 * AT * WM, TN = 16 * BT * WN;
-  constexpr size_t LDS = NS * ((TM + TN) * 128 + (T == P_F8 ? (TN + 63) / 64 * 256 + 256 : 0)) + (GATED && T == P_F8 ? WM * TN * 4 : 0);
-  static_assert(LDS <= 160 * 1024, "a compute unit's LDS");
-  const long long mtiles = (a.m + TM - 1) / TM, ttiles = span_bound(a.rows, a.experts, a.ends != nullptr, TN), tiles = mtiles * ttiles;
+template <int T, int WM, int WN, int AT, int BT, int NS, bool GATED> hipError_t launch_kernel(Tiles<WM, WN, AT, BT, NS, GATED> k, const ProductArgs& a, hipStream_t st) {
+  constexpr size_t LDS = decltype(k)::template LDS<T>;
+  const TileGrid g = tile_grid<T, decltype(k)>(a);
   const hipError_t e = allow_lds<k_product_tile<T, WM, WN, AT, BT, NS, GATED>>(LDS);
   if (e != hipSuccess) return e;
-  // as many workgroups as run at once (an MI355X has 256 compute units), a multiple of the XCDs; rows of fewer slabs than stages have no stream to run on from
-  // tile to tile
-  const bool stream = (long long)a.n * bytes_of<T> > 128 * (NS - 1);
-  const long long wgs = 256 * (160 * 1024 / LDS), up = (tiles + TILE_XCDS - 1) / TILE_XCDS * TILE_XCDS;
-  return launch(k_product_tile<T, WM, WN, AT, BT, NS, GATED>, dim3((unsigned)(stream && wgs < up ? wgs : up)), WM * WN * 64, LDS, st, a, (int)mtiles);
+  return launch(k_product_tile<T, WM, WN, AT, BT, NS, GATED>, dim3(g.workgroups), WM * WN * 64, LDS, st, a, (int)g.mtiles);
+}
+// what htr_product_plan says of a kernel: matrix rows and rows of x to a tile, waves and ring stages (0: no ring), workgroups, tiles
+template <int T, int R, int TT, int WAVES> void describe_kernel(Stream<R, TT, WAVES>, const ProductArgs& a, int* out) {
+  const long long tiles = (a.m + 16 * R - 1) / (16 * R) * span_bound(a.rows, a.experts, a.ends != nullptr, 16 * TT);
+  const int v[6] = {16 * R, 16 * TT, WAVES, 0, (int)tiles, (int)tiles};
+  memcpy(out, v, sizeof(v));
+}
+template <int T, int WM, int WN, int AT, int BT, int NS, bool GATED> void describe_kernel(Tiles<WM, WN, AT, BT, NS, GATED> k, const ProductArgs& a, int* out) {
+  const TileGrid g = tile_grid<T, decltype(k)>(a);
+  const int v[6] = {k.TM, k.TN, WM * WN, NS, (int)g.workgroups, (int)g.tiles};
+  memcpy(out, v, sizeof(v));
 }
 // Which tiles for many rows: the ones whose rounds take the least time by what a slab of a tile takes (ns) with a tile to a few compute units, and with all
 // at work, as many to each as fit.  Measured on 48 .. 8192 rows of 4096 .. 8192 columns, matrices from HBM.  A larger tile multiplies more for what it loads, a
@@ -150,18 +176,19 @@ template <int N> int best_tile(const TileChoice (&choices)[N], const ProductArgs
 bool takes_16bit_rows(long long rows, int experts, bool grouped) {
   return grouped ? rows <= 4ll * experts && span_bound(rows, experts, true, 16) <= 65535 : rows <= 16;
 }
-template <int T> hipError_t launch_product(const ProductArgs& a, hipStream_t st) {
+// The kernel for a product, handed to `take`
+template <int T, typename F> auto product_kernel(const ProductArgs& a, F take) {
   const int mean = (int)((a.rows + (long long)a.experts - 1) / a.experts);
   const bool grouped = a.ends != nullptr, few = takes_16bit_rows(a.rows, a.experts, grouped);
   if (few) {
     const long long tiles = grouped ? (a.rows < a.experts ? a.rows : a.experts) : 1, wgs = (a.m + 15) / 16 * tiles;
     const long long slabs = ((long long)a.n * bytes_of<T> + 127) / 128;
-    if (grouped && wgs >= 4 * 512) return launch_stream<T, 4, 1, 4>(a, st);
+    if (grouped && wgs >= 4 * 512) return take(Stream<4, 1, 4>{});
     // Rows of fewer slabs than waves leave some idle (7 rows on 15657x384 in e4m3 5.5 us by 16 rows to a workgroup of 8 waves, 4.7 by 32 to one of 4), and rows
     // to be rounded are rounded by half as many (4 tokens over 8 of 16 experts of 1920/384 37 and 31); long rows of few workgroups need more waves to share them
-    if (wgs >= 512 && (slabs < 8 || (slabs <= 16 && T == P_F8 && a.x_type != HTR_E4M3))) return launch_stream<T, 2, 1, 4>(a, st);
-    if (wgs <= 256 && slabs >= 64) return launch_stream<T, 1, 1, 16>(a, st);
-    return launch_stream<T, 1, 1, 8>(a, st);
+    if (wgs >= 512 && (slabs < 8 || (slabs <= 16 && T == P_F8 && a.x_type != HTR_E4M3))) return take(Stream<2, 1, 4>{});
+    if (wgs <= 256 && slabs >= 64) return take(Stream<1, 1, 16>{});
+    return take(Stream<1, 1, 8>{});
   }
   // Matrices so small that each compute unit has a workgroup of 16 of their rows by 16 or 32 of x at most: many waves for each are faster than a ring for few (us,
   // 16 bits: 64 rows on 1024x4096 11.0, by 32 rows 15.0, by tiles of 64x32 20.1; on 2048x4096 19.6, 15.4, 20.4; on 4096x4096 38, 29, 21.3)
@@ -170,39 +197,44 @@ template <int T> hipError_t launch_product(const ProductArgs& a, hipStream_t st)
     return (float)((a.m + 15) / 16) * (a.experts == 1 ? ceilf(full) : fmaxf(experts, full + 0.5f * experts));
   };
   const bool y_fits = span_bound(a.rows, a.experts, grouped, 16) <= 65535;      // the grid's second dimension
-  if (y_fits && workgroups(16) <= 256.f) return launch_stream<T, 1, 1, 8>(a, st);
-  if (y_fits && workgroups(32) <= 256.f) return launch_stream<T, 1, 2, 8>(a, st);
+  if (y_fits && workgroups(16) <= 256.f) return take(Stream<1, 1, 8>{});
+  if (y_fits && workgroups(32) <= 256.f) return take(Stream<1, 2, 8>{});
   if (!grouped) {
-    if (mean <= 32) return a.m < 8192 ? launch_stream<T, 1, 2, 8>(a, st) : a.m < 16384 ? launch_tile<T, 2, 2, 2, 1, 4>(a, st) : launch_tile<T, 4, 1, 2, 2, 4>(a, st);
+    if (mean <= 32) return a.m < 8192 ? take(Stream<1, 2, 8>{}) : a.m < 16384 ? take(Tiles<2, 2, 2, 1, 4>{}) : take(Tiles<4, 1, 2, 2, 4>{});
   } else if (mean <= 24) {
-    return launch_tile<T, 4, 1, 2, 2, 4>(a, st);
+    return take(Tiles<4, 1, 2, 2, 4>{});
   }
   switch (T == P_F8 ? best_tile(TILES_8, a, (size_t)a.n) : best_tile(TILES_16, a, (size_t)a.n * 2)) {
-    case 0: return launch_tile<T, 2, 4, 8, 4, 2>(a, st);
-    case 1: return launch_tile<T, 4, 2, 4, 4, 3>(a, st);
-    case 2: return launch_tile<T, 2, 2, 4, 4, 3>(a, st);
-    case 3: return launch_tile<T, 2, 2, 4, 2, 3>(a, st);
-    case 4: return launch_tile<T, 2, 2, 2, 2, 4>(a, st);
-    default: return launch_tile<T, 2, 2, 2, 1, 4>(a, st);
+    case 0: return take(Tiles<2, 4, 8, 4, 2>{});
+    case 1: return take(Tiles<4, 2, 4, 4, 3>{});
+    case 2: return take(Tiles<2, 2, 4, 4, 3>{});
+    case 3: return take(Tiles<2, 2, 4, 2, 3>{});
+    case 4: return take(Tiles<2, 2, 2, 2, 4>{});
+    default: return take(Tiles<2, 2, 2, 1, 4>{});
   }
 }
 // silu(gate) up of rows by expert, where one launch is the better way (few rows to an expert: the matrices are read by k_product_stream, k_gated follows)
 bool gates_in_one(long long rows, int experts) { return rows > 4ll * experts; }
-template <int T> hipError_t launch_gated_product(const ProductArgs& a, hipStream_t st) {
+template <int T, typename F> auto gated_kernel(const ProductArgs& a, F take) {
   switch (best_tile(GATED_TILES, a, (size_t)a.n * bytes_of<T>)) {
-    case 0: return launch_tile<T, 2, 4, 8, 4, 2, true>(a, st);
-    case 1: return launch_tile<T, 4, 2, 4, 4, 3, true>(a, st);
-    case 2: return launch_tile<T, 2, 2, 8, 2, 3, true>(a, st);
-    default: return launch_tile<T, 4, 1, 4, 2, 4, true>(a, st);
+    case 0: return take(Tiles<2, 4, 8, 4, 2, true>{});
+    case 1: return take(Tiles<4, 2, 4, 4, 3, true>{});
+    case 2: return take(Tiles<2, 2, 8, 2, 3, true>{});
+    default: return take(Tiles<4, 1, 4, 2, 4, true>{});
   }
 }
-hipError_t launch_gated_product(const ProductArgs& a, int type, hipStream_t st) {
-  return type == HTR_E4M3 ? launch_gated_product<P_F8>(a, st) : type == HTR_BF16 ? launch_gated_product<HTR_BF16>(a, st) : launch_gated_product<HTR_F16>(a, st);
+template <int T> hipError_t launch_product(const ProductArgs& a, bool gated, hipStream_t st) {
+  auto take = [&](auto kernel) { return launch_kernel<T>(kernel, a, st); };
+  return gated ? gated_kernel<T>(a, take) : product_kernel<T>(a, take);
 }
-hipError_t launch_product(const ProductArgs& a, int type, hipStream_t st) {
-  return type == HTR_E4M3 ? launch_product<P_F8>(a, st) : type == HTR_BF16 ? launch_product<HTR_BF16>(a, st) : launch_product<HTR_F16>(a, st);
+hipError_t launch_product(const ProductArgs& a, int type, bool gated, hipStream_t st) {
+  return type == HTR_E4M3 ? launch_product<P_F8>(a, gated, st) : type == HTR_BF16 ? launch_product<HTR_BF16>(a, gated, st) : launch_product<HTR_F16>(a, gated, st);
 }
-// what launch_product takes: HTR_OK or the status to refuse with
+template <int T> void describe_product(const ProductArgs& a, bool gated, int* out) {
+  auto take = [&](auto kernel) { describe_kernel<T>(kernel, a, out); };
+  if (gated) gated_kernel<T>(a, take); else product_kernel<T>(a, take);
+}
+// what product_kernel takes: HTR_OK or the status to refuse with
 int product_shape(long long rows, int m, int n, int experts, int type, bool grouped) {
   if (type != HTR_E4M3 && !is_16bit(type)) return HTR_ERR_DTYPE;
   if (rows < 0 || rows > (1ll << 31) - (1 << 20) || m < 1 || n < 1 || experts < 1 || experts > 65535 || n % (type == HTR_E4M3 ? 128 : 8)) return HTR_ERR_SIZE;
@@ -286,6 +318,22 @@ int htr_quantize_e4m3(const void* x, int64_t stride, int64_t rows, int n, int dt
 
 int htr_product_rounds(int64_t rows, int experts, int grouped) { return rows > 0 && experts > 0 && takes_16bit_rows(rows, experts, grouped != 0); }
 
+int htr_product_plan(int64_t rows, int m, int n, int experts, int grouped, int gated, int type, int x_type, int* out6) {
+  if (!out6) return HTR_ERR_NULL;
+  const int rc = product_shape(rows, m, n, experts, type, grouped != 0);
+  if (rc != HTR_OK) return rc;
+  if (x_type != type && !(type == HTR_E4M3 && is_16bit(x_type) && !gated && takes_16bit_rows(rows, experts, grouped != 0))) return HTR_ERR_DTYPE;
+  if (rows == 0 || (gated && (!grouped || m % (type == HTR_E4M3 ? 256 : 16) || !gates_in_one(rows, experts))) || (!grouped && experts != 1)) return HTR_ERR_SIZE;
+  const int some = 0;      // the choice asks whether there are ends, not what they hold
+  ProductArgs a{};
+  a.rows = (int)rows; a.m = m; a.n = n; a.experts = experts; a.x_type = x_type;
+  a.ends = grouped ? &some : nullptr;
+  if (type == HTR_E4M3) describe_product<P_F8>(a, gated != 0, out6);
+  else if (type == HTR_BF16) describe_product<HTR_BF16>(a, gated != 0, out6);
+  else describe_product<HTR_F16>(a, gated != 0, out6);
+  return HTR_OK;
+}
+
 int htr_product(const void* x, int x_type, const void* x_scales, const void* w, const void* w_scales, const void* bias, const int32_t* ends, void* y,
                 int64_t rows, int m, int n, int experts, int type, int y_dtype, void* stream) {
   const int rc = product_shape(rows, m, n, experts, type, ends != nullptr);
@@ -299,7 +347,7 @@ int htr_product(const void* x, int x_type, const void* x_scales, const void* w, 
       !aligned(bias, element_bytes(y_dtype)))
     return HTR_ERR_ALIGN;
   const ProductArgs a{x, (const float*)x_scales, w, (const float*)w_scales, bias, y, ends, nullptr, (int)rows, m, n, experts, y_dtype, x_type, nullptr};
-  TRY_HIP(launch_product(a, type, (hipStream_t)stream));
+  TRY_HIP(launch_product(a, type, false, (hipStream_t)stream));
   return HTR_OK;
 }
 
@@ -334,15 +382,15 @@ int htr_moe_stacked(const void* x, int dtype, const void* ids, int ids_int64, co
   }
   if (gates_in_one(pairs, experts)) {
     a.y = s + at.a; a.ys = (float*)(s + at.as); a.y_dtype = type;
-    TRY_HIP(launch_gated_product(a, type, st));
+    TRY_HIP(launch_product(a, type, true, st));
   } else {
-    TRY_HIP(launch_product(a, type, st));
+    TRY_HIP(launch_product(a, type, false, st));
     TRY_HIP(f8 ? launch(k_gated<P_F8>, dim3(pairs), 256, 0, st, h, ends, experts, inter, s + at.a, (float*)(s + at.as))
                : dtype == HTR_BF16 ? launch(k_gated<HTR_BF16>, dim3(pairs), 256, 0, st, h, ends, experts, inter, s + at.a, nullptr)
                                    : launch(k_gated<HTR_F16>, dim3(pairs), 256, 0, st, h, ends, experts, inter, s + at.a, nullptr));
   }
   const ProductArgs d{s + at.a, (const float*)(s + at.as), down, (const float*)down_scales, nullptr, out, ends, nullptr, pairs, hidden, inter, experts, HTR_F32, type, nullptr};
-  TRY_HIP(launch_product(d, type, st));
+  TRY_HIP(launch_product(d, type, false, st));
   const dim3 grid((unsigned)tokens, (hidden + 2047) / 2048);
   TRY_HIP(dtype == HTR_BF16 ? launch(k_weighted_sum<HTR_BF16>, grid, 256, 0, st, out, pos_of, weights, top, hidden, y)
                             : launch(k_weighted_sum<HTR_F16>, grid, 256, 0, st, out, pos_of, weights, top, hidden, y));

@@ -1,0 +1,249 @@
+"""Every kernel behind ops.linear_fp8 and ops.grouped_mm, by the plan that the library says it takes, against 64 bits.
+
+Each case names the kernel that it is for, and a test without a GPU holds it to that: a change of the rules that choose a kernel cannot move a case to
+another one unnoticed.  Rows have more slabs of 128 bytes than the ring has stages wherever a kernel has a ring, so that it turns; cases marked `several` have
+more tiles than workgroups.
+
+Tolerances are bounds by arithmetic.  A float32 sum of n products is off by at most n 2^-23 times the sum of their magnitudes, in any order, rounded or cut
+off.  An e4m3 matrix instruction adds the products of eight consecutive columns first, to 2^-13 of the largest by its operands' exponents (an exponent is
+never below that of 2^-6): eight of them are off by at most 2^-10 of that, and it is at most the product of the largest magnitudes, or 2^-6, of either side."""
+import ctypes
+
+import pytest
+import torch
+
+from htr_amd import _native, ops
+from test_unpacked import BF16, E4M3, F16, F32, assert_within, fp8_weight, gen, half_step, randn, value  # noqa: F401
+
+CODE = {BF16: 0, F16: 1, F32: 2, E4M3: 3}
+
+
+def plan(rows, m, n, experts=1, grouped=False, gated=False, kind=E4M3, x_kind=None):
+    """(matrix rows of a tile, rows of x, waves, stages, workgroups, tiles) or the status."""
+    out = (ctypes.c_int * 6)()
+    rc = _native.lib().htr_product_plan(rows, m, n, experts, int(grouped), int(gated), CODE[kind], CODE[x_kind or kind], out)
+    return tuple(out) if rc == 0 else rc
+
+
+def uneven(experts, rows):
+    """Rows of each expert: popular and unpopular ones, the second without any; one more than 64 for each of as many as that comes to."""
+    if experts == 1 or rows == 65 * experts:
+        return [rows // experts] * experts
+    share = [0 if e == 1 else 1 + e * 7 % 5 for e in range(experts)]
+    counts = [rows * s // sum(share) for s in share]
+    counts[-1] += rows - sum(counts)
+    return counts
+
+
+# ---- the cases: sizes, then {matrix rows, rows of x, waves, stages} of the kernel they are for, and whether it has several tiles to a workgroup
+DENSE = [      # e4m3; rows, m, n
+    (3, 900, 640, (16, 16, 8, 0), False),
+    (3, 900, 8192, (16, 16, 16, 0), False),
+    (5, 9001, 640, (32, 16, 4, 0), False),
+    (20, 5003, 1152, (16, 32, 8, 0), False),
+    (60, 1541, 1152, (16, 32, 8, 0), False),
+    (24, 9000, 640, (64, 32, 4, 4), False),
+    (50, 2051, 640, (64, 32, 4, 4), False),
+    (33, 12296, 640, (64, 64, 4, 4), False),
+    (17, 16392, 640, (128, 32, 4, 4), False),
+    (33, 20003, 640, (128, 64, 4, 3), False),
+    (96, 20008, 640, (128, 128, 4, 3), False),
+    (800, 16392, 640, (256, 128, 8, 3), True),
+    (800, 28677, 384, (256, 256, 8, 2), True),
+]
+GROUPED_16 = [      # experts, rows, m, n
+    (4, 9, 200, 328, (16, 16, 8, 0), False),
+    (3, 5, 300, 5000, (16, 16, 16, 0), False),
+    (2, 4, 9001, 72, (32, 16, 4, 0), False),
+    (2, 6, 16390, 136, (64, 16, 4, 0), False),
+    (2, 40, 1542, 1000, (16, 32, 8, 0), False),
+    (3, 96, 1000, 264, (64, 32, 4, 4), False),
+    (66, 1600, 520, 328, (64, 32, 4, 4), True),
+    (3, 130, 3000, 264, (64, 64, 4, 4), False),
+    (10, 650, 2080, 264, (64, 64, 4, 4), True),
+    (66, 300, 1003, 264, (128, 32, 4, 4), True),
+    (16, 500, 2056, 200, (128, 64, 4, 3), False),
+    (66, 2600, 1000, 200, (128, 64, 4, 3), True),
+    (3, 800, 4104, 200, (128, 128, 4, 3), True),
+    (3, 200, 28683, 200, (256, 128, 8, 3), True),
+    (5, 1200, 6152, 1000, (256, 256, 8, 2), False),
+    (3, 1600, 8200, 136, (256, 256, 8, 2), True),
+]
+GROUPED_8 = [
+    (4, 9, 200, 640, (16, 16, 8, 0), False),
+    (2, 6, 16390, 256, (64, 16, 4, 0), False),
+    (2, 40, 1542, 1152, (16, 32, 8, 0), False),
+    (3, 96, 1000, 640, (64, 32, 4, 4), False),
+    (66, 1600, 520, 640, (64, 32, 4, 4), True),
+    (5, 130, 3000, 640, (64, 64, 4, 4), False),
+    (22, 1430, 960, 640, (64, 64, 4, 4), True),
+    (66, 300, 523, 640, (128, 32, 4, 4), True),
+    (66, 2000, 1032, 640, (128, 64, 4, 3), True),
+    (3, 800, 4104, 640, (128, 128, 4, 3), True),
+    (3, 200, 28683, 640, (256, 128, 8, 3), True),
+    (3, 1600, 8200, 384, (256, 256, 8, 2), True),
+]
+RING = {(256, 256, 8, 2), (256, 128, 8, 3), (128, 128, 4, 3), (128, 64, 4, 3), (64, 64, 4, 4), (64, 32, 4, 4), (128, 32, 4, 4)}
+STREAM = {(16, 16, 8, 0), (16, 16, 16, 0), (32, 16, 4, 0), (64, 16, 4, 0), (16, 32, 8, 0)}
+
+
+def held_to(rows, m, n, experts, grouped, gated, kind, kernel, several, counts):
+    p = plan(rows, m, n, experts, grouped, gated, kind)
+    assert p[:4] == kernel, p
+    slabs = -(-n * (1 if kind == E4M3 else 2) // 128)
+    assert kernel[3] == 0 or slabs > kernel[3]
+    tiles = -(-m // kernel[0]) * sum(-(-c // kernel[1]) for c in counts)
+    assert tiles <= p[5]
+    if several:
+        assert tiles > p[4], (tiles, p)
+
+
+@pytest.mark.parametrize("kind", [BF16, F16, E4M3], ids=str)
+def test_every_kernel_has_a_case(kind):
+    eight = kind == E4M3
+    grouped = GROUPED_8 if eight else GROUPED_16
+    for experts, rows, m, n, kernel, several in grouped:
+        held_to(rows, m, n, experts, True, False, kind, kernel, several, uneven(experts, rows))
+    if eight:
+        for rows, m, n, kernel, several in DENSE:
+            held_to(rows, m, n, 1, False, False, kind, kernel, several, [rows])
+    assert {c[4] for c in (GROUPED_8 + [(1,) + c for c in DENSE] if eight else GROUPED_16)} == RING | STREAM
+    # every ring goes on from tile to tile somewhere
+    assert RING <= {c[4] for c in grouped if c[5]}
+
+
+def test_plans_are_of_these_kernels_only():
+    """No sizes lead to a kernel that no case is for."""
+    for kind in (BF16, E4M3):
+        unit = 128 if kind == E4M3 else 8
+        for experts in (1, 3, 16, 130):
+            for rows in (1, 2, 5, 17, 33, 60, 128, 300, 700, 2000, 9000, 60000):
+                for m in (1, 64, 257, 1024, 4096, 9000, 16384, 70000):
+                    for n in (unit, 1024, 16384):
+                        assert plan(rows, m, n, experts, True, False, kind)[:4] in RING | STREAM
+                        if experts == 1 and kind == E4M3:
+                            assert plan(rows, m, n)[:4] in RING | STREAM
+
+
+def test_status_codes_of_plans():
+    assert plan(0, 128, 128) == 11 and plan(-1, 128, 128) == 11 and plan(1, 0, 128) == 11 and plan(1, 128, 64) == 11 and plan(1, 128, 128, 2) == 11
+    assert plan(1, 128, 128, kind=F32) == 5 and plan(16, 128, 128, x_kind=BF16)[:2] == (16, 16) and plan(17, 128, 128, x_kind=BF16) == 5
+    assert plan(4, 256, 128, 1, True, True) == 11 and plan(5, 256, 128, 1, True, True)[:2] == (256, 32) and plan(5, 256, 128, 1, False, True) == 11
+    assert plan(5, 128, 128, 1, True, True) == 11 and plan(5, 24, 8, 1, True, True, BF16) == 11 and plan(5, 256, 128, 1, True, True, x_kind=F16) == 5
+    assert _native.lib().htr_product_plan(1, 128, 128, 1, 0, 0, 3, 3, None) == 1
+
+
+# ---- against 64 bits
+def within_8(a):
+    """For each eight columns the largest magnitude, or the least normal value of e4m3 at the block's scale, of 8-bit rows or matrices (values, scales)."""
+    q, s = a
+    s = s.double().repeat_interleave(16, -1)
+    if s.shape[:-1] != q.shape[:-1]:
+        s = s.repeat_interleave(128, -2)[..., :q.shape[-2], :]
+    return q.double().abs().nan_to_num(0.0).unflatten(-1, (-1, 8)).amax(-1).clamp(min=2.0 ** -6) * s
+
+
+def sums(x, w):
+    """(x @ w^T, what the sums may be off) for rows and a matrix in 16 bits, or both in pairs."""
+    eight = isinstance(x, tuple)
+    xd, wd = (value(*x), value(*w)) if eight else (x.double(), w.double())
+    off = (xd.abs() @ wd.abs().T) * (xd.shape[1] * 2.0 ** -23 + 4 * 2.0 ** -24)
+    if eight:
+        off = off + (within_8(x) @ within_8(w).T) * 2.0 ** -10
+    return xd @ wd.T, off
+
+
+def product_bound(x, w, dtype, bias=None):
+    y, off = sums(x, w)
+    if bias is not None:
+        y = y + bias.double()
+        off = off + y.abs() * 2.0 ** -24
+    return y, off * 1.01 + half_step(y.abs() + off, dtype)
+
+
+def fenced(t):
+    """t in memory with NaN (0xFF) right in front of it and right behind it."""
+    raw = t.contiguous().view(torch.uint8).reshape(-1)
+    room = torch.full((raw.numel() + 512,), 0xFF, dtype=torch.uint8, device=t.device)
+    room[256:256 + raw.numel()] = raw
+    return room[256:256 + raw.numel()].view(t.dtype).view(t.shape)
+
+
+def raw_product(x, w, ends, bias, dtype):
+    """htr_product into the middle of a marked buffer, whose marks stay."""
+    (q, s), (wq, ws) = x if isinstance(x, tuple) else (x, None), w if isinstance(w, tuple) else (w, None)
+    rows, m, n, experts = q.shape[0], wq.shape[-2], q.shape[1], wq.shape[0] if wq.dim() == 3 else 1
+    room = torch.full((rows * m + 128,), 77.0, dtype=dtype, device=q.device)
+    p = lambda t: None if t is None else t.data_ptr()
+    _native.check(_native.lib().htr_product(p(q), CODE[q.dtype], p(s), p(wq), p(ws), p(bias), p(ends), p(room[64:]), rows, m, n, experts, CODE[wq.dtype], CODE[dtype],
+                                            torch.cuda.current_stream().cuda_stream))
+    assert (room[:64] == 77).all() and (room[64 + rows * m:] == 77).all()
+    return room[64:64 + rows * m].view(rows, m)
+
+
+ids = lambda cases: [f"{'x'.join(map(str, c[:-2]))}-{c[-2][0]}x{c[-2][1]}" for c in cases]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,m,n,kernel,several", DENSE, ids=ids(DENSE))
+def test_dense(gen, rows, m, n, kernel, several):
+    w = tuple(map(fenced, fp8_weight(gen, m, n)))
+    x = tuple(map(fenced, ops.quantize_fp8(randn(gen, rows, n))))
+    for dtype, biased in ((BF16, True), (F32, False), (F16, True)):
+        bias = fenced(randn(gen, m, dtype=dtype)) if biased else None
+        y = raw_product(x, w, None, bias, dtype)
+        assert_within(y, *product_bound(x, w, dtype, bias))
+        assert torch.equal(ops.linear_fp8(x, *w, bias, out_dtype=dtype), y)
+    clean = ops.linear_fp8(x, *w)
+    x[0].view(torch.uint8)[rows // 2, n - 3] = 0x7F            # NaN: of its row alone
+    y = ops.linear_fp8(x, *w)
+    assert y[rows // 2].isnan().all()
+    y[rows // 2] = clean[rows // 2]
+    assert torch.equal(y, clean)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,m,n", [(5, 203, 328), (20, 5003, 200), (24, 9000, 72), (70, 1000, 392), (300, 4104, 1000), (800, 16390, 136)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_dense_in_16_bits(gen, rows, m, n, dtype):
+    """One 16-bit matrix for all rows, which the C ABI takes."""
+    x, w, bias = fenced(randn(gen, rows, n, dtype=dtype)), fenced(randn(gen, m, n, dtype=dtype)), fenced(randn(gen, m, dtype=dtype))
+    assert_within(raw_product(x, w, None, bias, dtype), *product_bound(x, w, dtype, bias))
+
+
+def by_kind(wide, narrow):
+    """Parameters (kind, case): those of 16 bits in both types, those of e4m3."""
+    every = [(k, c) for k in (BF16, F16) for c in wide] + [(E4M3, c) for c in narrow]
+    return pytest.mark.parametrize("kind,case", every, ids=[f"{str(k)[6:]}-{i}" for (k, c), i in zip(every, ids(wide) * 2 + ids(narrow))])
+
+
+@pytest.mark.gpu
+@by_kind(GROUPED_16, GROUPED_8)
+def test_grouped(gen, kind, case):
+    experts, rows, m, n, kernel, several = case
+    counts, behind = uneven(experts, rows), 37
+    if plan(rows + behind, m, n, experts, True, False, kind)[:4] != kernel:      # rows behind the last expert's are for the cases whose kernel stays
+        behind = 0
+    ends = torch.tensor(counts, dtype=torch.int32).cumsum(0).to(torch.int32).cuda()
+    if kind == E4M3:
+        w = tuple(map(fenced, fp8_weight(gen, experts, m, n)))
+        x = tuple(map(fenced, ops.quantize_fp8(randn(gen, rows + behind, n))))
+        part, matrix = lambda a, b: (x[0][a:b], x[1][a:b]), lambda e: (w[0][e], w[1][e])
+    else:
+        w, x = fenced(randn(gen, experts, m, n, dtype=kind, scale=n ** -0.5)), fenced(randn(gen, rows + behind, n, dtype=kind))
+        part, matrix = lambda a, b: x[a:b], lambda e: w[e]
+    for dtype in (F32, BF16):
+        y = raw_product(x, w, ends, None, dtype)
+        first = 0
+        for e, c in enumerate(counts):
+            if c:
+                assert_within(y[first:first + c], *product_bound(part(first, first + c), matrix(e), dtype))
+            first += c
+        assert (y[first:] == 0).all()
+    assert torch.equal(ops.grouped_mm(x, w, ends, out_dtype=BF16), y)
+    at = rows // 3
+    (x[0].view(torch.uint8) if kind == E4M3 else x)[at, n - 1] = 0x7F if kind == E4M3 else float("nan")
+    z = ops.grouped_mm(x, w, ends, out_dtype=BF16)
+    assert z[at].isnan().all()
+    z[at] = y[at]
+    assert torch.equal(z, y)
