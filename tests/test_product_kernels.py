@@ -1,4 +1,4 @@
-"""Every kernel behind ops.linear_fp8 and ops.grouped_mm, by the plan that the library says it takes, against 64 bits.
+"""Every kernel behind ops.linear_fp8, ops.grouped_mm and ops.moe_experts_stacked, by the plan that the library says it takes, against 64 bits.
 
 Each case names the kernel that it is for, and a test without a GPU holds it to that: a change of the rules that choose a kernel cannot move a case to
 another one unnoticed.  Rows have more slabs of 128 bytes than the ring has stages wherever a kernel has a ring, so that it turns; cases marked `several` have
@@ -13,7 +13,7 @@ import pytest
 import torch
 
 from htr_amd import _native, ops
-from test_unpacked import BF16, E4M3, F16, F32, assert_within, fp8_weight, gen, half_step, randn, value  # noqa: F401
+from test_unpacked import BF16, E4M3, F16, F32, assert_within, fp8_weight, gen, half_step, quantized, randn, to_e4m3, value  # noqa: F401
 
 CODE = {BF16: 0, F16: 1, F32: 2, E4M3: 3}
 
@@ -83,8 +83,22 @@ GROUPED_8 = [
     (3, 200, 28683, 640, (256, 128, 8, 3), True),
     (3, 1600, 8200, 384, (256, 256, 8, 2), True),
 ]
+GATED_16 = [      # experts, rows, 2 F, H
+    (16, 96, 6160, 264, (256, 32, 4, 4), True),
+    (16, 400, 6160, 200, (256, 64, 4, 3), True),
+    (16, 800, 6160, 200, (256, 128, 8, 3), True),
+    (3, 1600, 8208, 136, (256, 256, 8, 2), True),
+    (5, 1600, 6160, 1000, (256, 256, 8, 2), False),
+]
+GATED_8 = [
+    (66, 300, 1024, 640, (256, 32, 4, 4), True),
+    (16, 300, 8192, 640, (256, 64, 4, 3), True),
+    (16, 600, 7936, 640, (256, 128, 8, 3), True),
+    (8, 1600, 8192, 384, (256, 256, 8, 2), True),
+]
 RING = {(256, 256, 8, 2), (256, 128, 8, 3), (128, 128, 4, 3), (128, 64, 4, 3), (64, 64, 4, 4), (64, 32, 4, 4), (128, 32, 4, 4)}
 STREAM = {(16, 16, 8, 0), (16, 16, 16, 0), (32, 16, 4, 0), (64, 16, 4, 0), (16, 32, 8, 0)}
+GATED = {(256, 256, 8, 2), (256, 128, 8, 3), (256, 64, 4, 3), (256, 32, 4, 4)}
 
 
 def held_to(rows, m, n, experts, grouped, gated, kind, kernel, several, counts):
@@ -101,15 +115,18 @@ def held_to(rows, m, n, experts, grouped, gated, kind, kernel, several, counts):
 @pytest.mark.parametrize("kind", [BF16, F16, E4M3], ids=str)
 def test_every_kernel_has_a_case(kind):
     eight = kind == E4M3
-    grouped = GROUPED_8 if eight else GROUPED_16
+    grouped, gated = (GROUPED_8, GATED_8) if eight else (GROUPED_16, GATED_16)
     for experts, rows, m, n, kernel, several in grouped:
         held_to(rows, m, n, experts, True, False, kind, kernel, several, uneven(experts, rows))
+    for experts, rows, m, n, kernel, several in gated:
+        held_to(rows, m, n, experts, True, True, kind, kernel, several, uneven(experts, rows))
     if eight:
         for rows, m, n, kernel, several in DENSE:
             held_to(rows, m, n, 1, False, False, kind, kernel, several, [rows])
     assert {c[4] for c in (GROUPED_8 + [(1,) + c for c in DENSE] if eight else GROUPED_16)} == RING | STREAM
+    assert {c[4] for c in gated} == GATED
     # every ring goes on from tile to tile somewhere
-    assert RING <= {c[4] for c in grouped if c[5]}
+    assert RING <= {c[4] for c in grouped if c[5]} and GATED <= {c[4] for c in gated if c[5]}
 
 
 def test_plans_are_of_these_kernels_only():
@@ -123,6 +140,8 @@ def test_plans_are_of_these_kernels_only():
                         assert plan(rows, m, n, experts, True, False, kind)[:4] in RING | STREAM
                         if experts == 1 and kind == E4M3:
                             assert plan(rows, m, n)[:4] in RING | STREAM
+                        if m % 256 == 0 and rows > 4 * experts:
+                            assert plan(rows, m, n, experts, True, True, kind)[:4] in GATED
 
 
 def test_status_codes_of_plans():
@@ -247,3 +266,84 @@ def test_grouped(gen, kind, case):
     assert z[at].isnan().all()
     z[at] = y[at]
     assert torch.equal(z, y)
+
+
+# ---- routed experts
+def layer64(x, ids, wt, gate_up, down, dtype):
+    """(y, bound) of the layer with its roundings: what the sums may make of each hidden value before it is rounded, and of the second product."""
+    eight = isinstance(gate_up, tuple)
+    T, top = ids.shape
+    xs = quantized(x.double()) if eight else x
+    experts = (gate_up[0] if eight else gate_up).shape[0]
+    y = torch.zeros(T, (down[0] if eight else down).shape[1], dtype=torch.float64, device=x.device)
+    bound = torch.zeros_like(y)
+    silu = lambda g: g / (1 + torch.exp(-g))
+    flat, wflat = ids.reshape(-1), wt.reshape(-1).double()
+    for e in range(experts):
+        pairs = torch.nonzero(flat == e)[:, 0]
+        if not len(pairs):
+            continue
+        tok = pairs // top
+        pick = lambda a: tuple(t[e] for t in a) if eight else a[e]
+        g, off = sums(tuple(t[tok] for t in xs) if eight else xs[tok], pick(gate_up))
+        F = g.shape[1] // 2
+        up, h = g[:, F:], silu(g[:, :F]) * g[:, F:]
+        # silu's slope is 1.1 at most; exp, whose argument is rounded, and three float32 operations
+        slack = 1.1 * off[:, :F] * (up.abs() + off[:, F:]) + silu(g[:, :F]).abs() * off[:, F:] + h.abs() * (g[:, :F].abs() + 8) * 2.0 ** -23
+        lo, hi = h - slack, h + slack
+        wd = value(*pick(down)) if eight else down[e].double()
+        if eight:
+            q, s = quantized(h)
+            rows = (q, s)
+            wide = s.repeat_interleave(128, -1)
+            h, lo, hi = q * wide, to_e4m3(lo / wide) * wide, to_e4m3(hi / wide) * wide
+            room = torch.maximum(hi - h, h - lo) + wide * 2.0 ** -9            # another scale: another subnormal step
+            inner = (within_8(rows) * 2 + room.unflatten(-1, (-1, 8)).amax(-1)) @ within_8(pick(down)).T * 2.0 ** -10
+        else:
+            lo, hi = lo - half_step(lo, dtype), hi + half_step(hi, dtype)
+            room = torch.maximum(hi - h, h - lo)
+            inner = 0.0
+        out, away = h @ wd.T, room @ wd.abs().T
+        away = away + ((h.abs() + room) @ wd.abs().T) * (F * 2.0 ** -23 + 2.0 ** -21) + inner
+        w = wflat[pairs][:, None]
+        y.index_add_(0, tok, w * out)
+        bound.index_add_(0, tok, w.abs() * away + (w * out).abs() * (2.0 ** -22 + top * 2.0 ** -23))
+    return y, bound * 1.01 + half_step(y.abs() + bound, dtype)
+
+
+def layer(gen, T, top, experts, H, F, kind, dtype, counts):
+    """Inputs of a layer whose experts have exactly these rows."""
+    flat = torch.repeat_interleave(torch.arange(experts), torch.tensor(counts))
+    flat = flat[torch.randperm(T * top, generator=torch.Generator().manual_seed(7))]
+    x, wt = fenced(randn(gen, T, H, dtype=dtype)), torch.rand(T, top, device="cuda", generator=gen)
+    if kind == E4M3:
+        gate_up, down = tuple(map(fenced, fp8_weight(gen, experts, 2 * F, H))), tuple(map(fenced, fp8_weight(gen, experts, H, F)))
+    else:
+        gate_up, down = (fenced(randn(gen, experts, *s, dtype=dtype, scale=s[1] ** -0.5)) for s in ((2 * F, H), (H, F)))
+    return x, flat.view(T, top).cuda(), wt, gate_up, down
+
+
+@pytest.mark.gpu
+@by_kind(GATED_16, GATED_8)
+def test_gated(gen, kind, case):
+    experts, rows, m, n, kernel, several = case
+    top, dtype = 2, BF16 if kind == E4M3 else kind
+    call = layer(gen, rows // top, top, experts, n, m // 2, kind, dtype, uneven(experts, rows))
+    y = ops.moe_experts_stacked(*call)
+    assert_within(y, *layer64(*call, dtype))
+    assert torch.equal(ops.moe_experts_stacked(*call), y)
+    call[0][3, n // 2] = float("nan")
+    z = ops.moe_experts_stacked(*call)
+    assert z[3].isnan().all()
+    z[3] = y[3]
+    assert torch.equal(z, y)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,F", [(8, 8), (72, 136), (136, 72), (1000, 328), (328, 1000)])
+@pytest.mark.parametrize("T,top,experts", [(1, 1, 1), (3, 2, 4), (60, 2, 5), (700, 1, 3)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_layers_on_odd_sizes(gen, dtype, H, F, T, top, experts):
+    """Multiples of 8 that are none of 128, in one launch for gate and up and in two."""
+    call = layer(gen, T, top, experts, H, F, dtype, dtype, uneven(experts, T * top))
+    assert_within(ops.moe_experts_stacked(*call), *layer64(*call, dtype))
