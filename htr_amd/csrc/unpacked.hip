@@ -190,8 +190,10 @@ template <int T, typename F> auto product_kernel(const ProductArgs& a, F take) {
     if (wgs <= 256 && slabs >= 64) return take(Stream<1, 1, 16>{});
     return take(Stream<1, 1, 8>{});
   }
-  // Matrices so small that each compute unit has a workgroup of 16 of their rows by 16 or 32 of x at most: many waves for each are faster than a ring for few (us,
-  // 16 bits: 64 rows on 1024x4096 11.0, by 32 rows 15.0, by tiles of 64x32 20.1; on 2048x4096 19.6, 15.4, 20.4; on 4096x4096 38, 29, 21.3)
+  // Matrices so small that each compute unit has a workgroup of 16 of their rows by 16 or 32 of x at most: many waves for each are faster than a ring for few.
+  // Measured from HBM on 17 .. 384 rows of 256 .. 4096 matrix rows of 1024, 4096 and 8192 columns, 108 sizes in each type: the way taken was the fastest in all.
+  // us by 16 rows, by 32, by tiles of 64x32: 64 rows on 1024x4096 in 16 bits 10.6, 14.7, 20.8, in e4m3 7.2, 9.8, 11.9; 48 rows on 2048x4096 19.5, 15.0, 21.0 and
+  // 11.8, 9.9, 11.9; beyond the limits 192 rows on 1024x4096 26.1, 26.2, 20.7 and 16.1, 18.6, 11.8, 64 rows on 4096x4096 38, 30, 22 and 21.6, 19.4, 12.6.
   auto workgroups = [&](int height) {
     const float full = (float)a.rows / height, experts = (float)(a.rows < a.experts ? a.rows : a.experts);
     return (float)((a.m + 15) / 16) * (a.experts == 1 ? ceilf(full) : fmaxf(experts, full + 0.5f * experts));
@@ -202,7 +204,9 @@ template <int T, typename F> auto product_kernel(const ProductArgs& a, F take) {
   if (!grouped) {
     if (mean <= 32) return a.m < 8192 ? take(Stream<1, 2, 8>{}) : a.m < 16384 ? take(Tiles<2, 2, 2, 1, 4>{}) : take(Tiles<4, 1, 2, 2, 4>{});
   } else if (mean <= 24) {
-    return take(Tiles<4, 1, 2, 2, 4>{});
+    // experts' rows are uneven: where 16 rows to a workgroup leave two to a compute unit they are still ahead of tiles of 128x32 (us, 192 rows of 8 experts of
+    // 512x4096 in e4m3 12.1 and 16.8, in 16 bits 19.6 and 26.7; of 512x768 4.4 and 6.1, 5.9 and 8.4; 1056 rows of 48 of 72x3200 in 16 bits 20.1 and 19.4)
+    return y_fits && workgroups(16) <= 512.f ? take(Stream<1, 1, 8>{}) : take(Tiles<4, 1, 2, 2, 4>{});
   }
   switch (T == P_F8 ? best_tile(TILES_8, a, (size_t)a.n) : best_tile(TILES_16, a, (size_t)a.n * 2)) {
     case 0: return take(Tiles<2, 4, 8, 4, 2>{});

@@ -152,6 +152,14 @@ def test_status_codes_of_plans():
     assert _native.lib().htr_product_plan(1, 128, 128, 1, 0, 0, 3, 3, None) == 1
 
 
+@pytest.mark.parametrize("kind", [BF16, E4M3], ids=str)
+def test_uneven_experts_of_small_matrices(kind):
+    """Up to two workgroups of 16x16 to a compute unit and 24 rows to an expert stay with the streaming kernel, as measured; beyond is the ring."""
+    for rows, m, experts in ((192, 512, 8), (384, 256, 16), (768, 128, 32), (1536, 64, 64)):
+        assert plan(rows, m, 768, experts, True, False, kind)[:4] == (16, 16, 8, 0)
+        assert plan(rows, 2 * m, 768, experts, True, False, kind)[3] > 0 and plan(2 * rows, m, 768, experts, True, False, kind)[3] > 0
+
+
 # ---- against 64 bits
 def within_8(a):
     """For each eight columns the largest magnitude, or the least normal value of e4m3 at the block's scale, of 8-bit rows or matrices (values, scales)."""
