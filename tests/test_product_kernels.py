@@ -94,7 +94,7 @@ GATED_8 = [
     (66, 300, 1024, 640, (256, 32, 4, 4), True),
     (16, 300, 8192, 640, (256, 64, 4, 3), True),
     (16, 600, 7936, 640, (256, 128, 8, 3), True),
-    (8, 1600, 8192, 384, (256, 256, 8, 2), True),
+    (3, 1600, 8448, 384, (256, 256, 8, 2), True),
 ]
 RING = {(256, 256, 8, 2), (256, 128, 8, 3), (128, 128, 4, 3), (128, 64, 4, 3), (64, 64, 4, 4), (64, 32, 4, 4), (128, 32, 4, 4)}
 STREAM = {(16, 16, 8, 0), (16, 16, 16, 0), (32, 16, 4, 0), (64, 16, 4, 0), (16, 32, 8, 0)}
@@ -158,6 +158,14 @@ def test_uneven_experts_of_small_matrices(kind):
     for rows, m, experts in ((192, 512, 8), (384, 256, 16), (768, 128, 32), (1536, 64, 64)):
         assert plan(rows, m, 768, experts, True, False, kind)[:4] == (16, 16, 8, 0)
         assert plan(rows, 2 * m, 768, experts, True, False, kind)[3] > 0 and plan(2 * rows, m, 768, experts, True, False, kind)[3] > 0
+
+
+@pytest.mark.parametrize("kind", [BF16, E4M3], ids=str)
+def test_tiles_of_gate_and_up(kind):
+    """As measured: an expert's rows in tiles of 128 where half a tile of 256 would be empty, and of 256 where they fill it."""
+    for rows, m, n, experts, kernel in ((9000, 2816, 2048, 64, (256, 128)), (6000, 1536, 2048, 32, (256, 256)), (1024, 1536, 2048, 32, (256, 64)),
+                                        (192, 4096, 4096, 8, (256, 32)), (32768, 1536, 2048, 128, (256, 128))):
+        assert plan(rows, m, n, experts, True, True, kind)[:2] == kernel
 
 
 # ---- against 64 bits
