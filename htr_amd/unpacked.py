@@ -10,9 +10,12 @@ The reference leaves these modules to its caller (its plugin returns Unquantized
 
 8-bit rows are a pair (values float8_e4m3fn [..., n], scales float32 [..., n / 128]), 8-bit matrices a pair (values [.., m, n], scales
 [.., ceil(m / 128), n / 128]); a value stands for itself times its block's scale.  The scales made here are powers of two, the least that brings
-the block to 448 or below; scales from elsewhere may be any.  Infinities and NaN become NaN.
+the block to 448 or below; scales from elsewhere need not be.  Infinities and NaN become NaN.
 
-Sums, norms and products are float32 or wider, results are rounded once.  Nothing here has a derivative, as no packed linear has one in its
+Norms sum in 64 bits, products of 16-bit values in float32.  Products of e4m3 values are first added eight consecutive
+columns at a time, as the matrix instructions do: each eight is off by at most 2^-10 of the largest magnitude in x times that in the matrix (one below 2^-6 of its
+scale counts as that).  Everything beyond is float32, the product of a row's scale and a block's as well, which has to be in its normal range.  Results are
+rounded once.  Nothing here has a derivative, as no packed linear has one in its
 activations: a call that torch would differentiate is refused.  Calls only queue kernels on the current stream of x's device, allocate with torch and
 may be captured into a graph.
 """
@@ -269,7 +272,7 @@ def moe_experts_stacked(x, expert_ids, expert_weights, gate_up, down):
 
     x [T, H] in bfloat16 or float16; expert_ids [T, top] int32 or int64; expert_weights [T, top]; gate_up [E, 2F, H] (gate rows first) and down
     [E, H, F] of x's type, H and F multiples of 8, or 8-bit pairs (multiples of 128), with which x and the hidden values are rounded to e4m3 as well.
-    Sums are float32; the hidden values are rounded to x's type or e4m3, y [T, H] to x's type.  A token with an expert number out of range
+    Sums are as in the products; the hidden values are rounded to x's type or e4m3 in between, y [T, H] to x's type.  A token with an expert number out of range
     becomes NaN."""
     eight = _pair(gate_up) and _pair(down)
     path = _fast(x)

@@ -312,7 +312,7 @@ int htr_dequant_w(const void* qweight, const void* scales, const void* su, const
  *
  * e4m3 rows carry a float32 scale for each 128 columns, [rows][n / 128]; e4m3 matrices one for each 128x128 block, [ceil(m / 128)][n / 128].
  * The scales that these calls make are powers of two, the least from amax / 448 up (amax: the block's largest finite magnitude, at least
- * 2^-100); scales they are given may be any float32.  Infinities and NaN become NaN.
+ * 2^-100); scales they are given need not be.  Infinities and NaN become NaN.
  *
  * htr_rms_norm: t = round(x + residual), y = t weight / sqrt(mean(t^2) + eps), the mean in 64 bits.
  *   x, residual  [rows][n] of dtype with that many elements from row to row; residual may be NULL (then sum is, too: t = x)
@@ -329,7 +329,9 @@ int htr_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t 
 int htr_quantize_e4m3(const void* x, int64_t stride, int64_t rows, int n, int dtype, void* q, void* scales, void* stream);
 
 /*
- * y[r] = W_e x[r] (+ bias), e the expert of row r, sums in float32.
+ * y[r] = W_e x[r] (+ bias), e the expert of row r.  Sums are float32, except that products of e4m3 values are first added eight consecutive columns at
+ * a time: each eight is off by at most 2^-10 of the largest magnitude in x times that in w (a magnitude below 2^-6 of its scale counts as that).  The
+ * product of a row's scale and a block's is float32 as well: it has to be in its normal range.
  *   type    of w: HTR_E4M3 (with its scales), HTR_BF16 or HTR_F16 (scales NULL)
  *   x_type  type; with e4m3 matrices also HTR_BF16 or HTR_F16 (x_scales NULL) where htr_product_rounds says so: rounded as by htr_quantize_e4m3
  *   x       [rows][n], w [experts][m][n], 16-byte aligned; n a multiple of 128 (e4m3) or of 8 (16 bits), up to 2^22; m up to 2^26; experts up to 65535
@@ -349,8 +351,8 @@ int htr_product_rounds(int64_t rows, int experts, int grouped);
 int htr_product_plan(int64_t rows, int m, int n, int experts, int grouped, int gated, int type, int x_type, int* out6);
 
 /*
- * A routed-expert layer on stacked matrices: y_t = sum_j w[t, j] Down_e( silu(Gate_e x_t) * Up_e x_t ), e = ids[t, j], sums in float32 and in
- * ascending j, y of dtype (bf16 or f16).  The hidden values between the products are rounded to dtype, or to e4m3 with scales.
+ * A routed-expert layer on stacked matrices: y_t = sum_j w[t, j] Down_e( silu(Gate_e x_t) * Up_e x_t ), e = ids[t, j], sums as in htr_product, over j in
+ * float32 and ascending, y of dtype (bf16 or f16).  The hidden values between the products are rounded to dtype, or to e4m3 with scales.
  *   type     dtype, or HTR_E4M3 (x is then rounded to e4m3 as well)
  *   gate_up  [experts][2 inter][hidden], gate rows first;  down [experts][hidden][inter];  scales as in htr_product, or NULL
  *   ids      [tokens][top] int32 or int64 and weights [tokens][top] float32, on the device; an expert out of range makes its token NaN

@@ -284,6 +284,35 @@ def test_grouped(gen, kind, case):
     assert torch.equal(z, y)
 
 
+def wide_range(gen, rows, n):
+    """8-bit rows whose eight consecutive columns hold one large value among small ones, all magnitudes of e4m3 and its subnormals among them."""
+    size = torch.exp2(-9 + 9 * torch.rand(rows, n, device="cuda", generator=gen))
+    at = torch.randint(0, 8, (rows, n // 8, 1), device="cuda", generator=gen)
+    size.view(rows, n // 8, 8).scatter_(2, at, torch.exp2(4 + 4.8 * torch.rand(rows, n // 8, 1, device="cuda", generator=gen)))
+    return (size * (torch.randint(0, 2, (rows, n), device="cuda", generator=gen) * 2 - 1)).to(E4M3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,m", [(2, 900), (40, 1030), (300, 5000)])
+def test_sums_of_e4m3_products_of_a_wide_range(gen, rows, m):
+    """What the operators say of their sums, on values for which it differs from float32."""
+    n = 384
+    x = wide_range(gen, rows, n), 1 + torch.rand(rows, n // 128, device="cuda", generator=gen)
+    w = wide_range(gen, m, n), 1 + torch.rand(-(-m // 128), n // 128, device="cuda", generator=gen)
+    assert_within(ops.linear_fp8(x, *w, out_dtype=F32), *product_bound(x, w, F32))
+    assert_within(ops.grouped_mm(x, (w[0][None], w[1][None]), torch.tensor([rows], dtype=torch.int32, device="cuda"), out_dtype=F32), *product_bound(x, w, F32))
+    # a large product and its negative in one eight: what is left of the others is what the bound allows, in another eight all of it
+    q = torch.zeros(rows, n, device="cuda")
+    q[:, 0], q[:, 1], q[:, 2], q[:, 9] = 256, -256, 2.0 ** -8, 2.0 ** -8
+    ones = torch.ones(m, n, device="cuda").to(E4M3), torch.ones(-(-m // 128), n // 128, device="cuda")
+    y = ops.linear_fp8((q.to(E4M3), torch.ones(rows, n // 128, device="cuda")), *ones, out_dtype=F32)
+    assert ((y - 2 * 2.0 ** -8).abs() <= 256 * 2.0 ** -10).all()
+    q[:, 1] = 0
+    q[:, 8] = -256
+    y = ops.linear_fp8((q.to(E4M3), torch.ones(rows, n // 128, device="cuda")), *ones, out_dtype=F32)
+    assert ((y - 2 * 2.0 ** -8).abs() <= 2 * 256 * 2.0 ** -10).all()
+
+
 # ---- routed experts
 def layer64(x, ids, wt, gate_up, down, dtype):
     """(y, bound) of the layer with its roundings: what the sums may make of each hidden value before it is rounded, and of the second product."""
