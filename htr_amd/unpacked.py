@@ -156,7 +156,12 @@ def dequantize_fp8(q, scales):
 
 
 def _pair(x):
-    return isinstance(x, (tuple, list)) and len(x) == 2
+    """Whether x is a pair (values, scales); half a pair is refused."""
+    if not isinstance(x, (tuple, list)):
+        return False
+    if len(x) != 2 or not isinstance(x[0], torch.Tensor) or not isinstance(x[1], torch.Tensor):
+        raise RuntimeError("8-bit rows and matrices are pairs (values, scales) of tensors")
+    return True
 
 
 def _check_rows(what, x, experts, grouped):
@@ -173,7 +178,7 @@ def _check_rows(what, x, experts, grouped):
 
 
 def _check_matrix(what, q, s, dims):
-    if q.dtype != E4M3 or s.dtype != torch.float32 or q.dim() != dims or q.shape[-1] % 128 or 0 in q.shape \
+    if not isinstance(q, torch.Tensor) or not isinstance(s, torch.Tensor) or q.dtype != E4M3 or s.dtype != torch.float32 or q.dim() != dims or q.shape[-1] % 128 or 0 in q.shape \
             or s.shape != q.shape[:-2] + (-(-q.shape[-2] // 128), q.shape[-1] // 128):
         raise RuntimeError(f"{what}: an 8-bit weight is (float8_e4m3fn [.., m, n], float32 [.., ceil(m / 128), n / 128]), n a multiple of 128")
     if not q.is_contiguous() or not s.is_contiguous() or q.data_ptr() % 16:
@@ -190,7 +195,7 @@ def _out_dtype(what, out_dtype, x, bias=None):
 
 def _product(x, w, ws, bias, ends, out_dtype):
     """The common case of the products in C++; None where something else is asked for, or is wrong."""
-    q, s = x if type(x) is tuple and len(x) == 2 else (x, None)
+    q, s = x if type(x) is tuple and len(x) == 2 and x[1] is not None else (x, None)
     path = _fast(q)
     if path is None:
         return None
