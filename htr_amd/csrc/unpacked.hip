@@ -115,10 +115,11 @@ template <int T, typename K> TileGrid tile_grid(const ProductArgs& a) {
 template <int T, int R, int TT, int WAVES> hipError_t launch_kernel(Stream<R, TT, WAVES>, const ProductArgs& a, hipStream_t st) {
   const dim3 grid((a.m + 16 * R - 1) / (16 * R), (unsigned)span_bound(a.rows, a.experts, a.ends != nullptr, 16 * TT));
   if constexpr (T == P_F8 && TT == 1) {
-    if (a.x_type == HTR_BF16) return launch(k_product_stream<T, HTR_BF16, R, TT, WAVES>, grid, WAVES * 64, 0, st, a);
-    if (a.x_type == HTR_F16) return launch(k_product_stream<T, HTR_F16, R, TT, WAVES>, grid, WAVES * 64, 0, st, a);
+    if (a.wide) return launch(a.x_type == HTR_BF16 ? k_product_stream<T, HTR_BF16, R, TT, WAVES, true> : k_product_stream<T, HTR_F16, R, TT, WAVES, true>, grid, WAVES * 64, 0, st, a);
+    if (a.x_type == HTR_BF16) return launch(k_product_stream<T, HTR_BF16, R, TT, WAVES, false>, grid, WAVES * 64, 0, st, a);
+    if (a.x_type == HTR_F16) return launch(k_product_stream<T, HTR_F16, R, TT, WAVES, false>, grid, WAVES * 64, 0, st, a);
   }
-  return launch(k_product_stream<T, T, R, TT, WAVES>, grid, WAVES * 64, 0, st, a);
+  return launch(k_product_stream<T, T, R, TT, WAVES, false>, grid, WAVES * 64, 0, st, a);
 }
 template <int T, int WM, int WN, int AT, int BT, int NS, bool GATED> hipError_t launch_kernel(Tiles<WM, WN, AT, BT, NS, GATED> k, const ProductArgs& a, hipStream_t st) {
   constexpr size_t LDS = decltype(k)::template LDS<T>;
@@ -149,8 +150,8 @@ constexpr TileChoice TILES_16[] = {{256, 256, 1, 1380.f, 1700.f}, {256, 128, 1, 
                                    {128, 64, 2, 480.f, 735.f},    {64, 64, 2, 315.f, 510.f},    {64, 32, 3, 290.f, 450.f}};
 // gate and up in one: 128 hidden columns to a tile.  Fitted to whole layers of 32 .. 4096 tokens, matrices from HBM, in 16 bits and e4m3: 8 experts (top 2) of 4096/2048,
 // 64 (6) of 2048/1408, 16 (4) of 1024/512, 32 (4) and 128 (8) of 2048/768.  The way taken is within 5 % of the fastest in these 54, within 17 % on sizes apart from
-// them (us by 256x256, x128, x64, x32: 1500 tokens of 64 experts in e4m3 263, 224, 236, 275, in 16 bits 403, 351, 374, 439; 256 tokens of 8 in 16 bits 161, 131,
-// 128, 149; 1500 tokens of 32 in e4m3 95.5, 101, 101, 116).
+// them (us by 256x256, x128, x64, x32: 1500 tokens of 64 experts in e4m3 263, 222, 289, 312, in 16 bits 403, 351, 374, 439; 256 tokens of 8 in 16 bits 161, 131,
+// 128, 149; 1500 tokens of 32 in e4m3 95, 100, 123, 130).
 constexpr TileChoice GATED_TILES[] = {{256, 256, 1, 1450.f, 2250.f}, {256, 128, 1, 950.f, 1250.f}, {256, 64, 1, 750.f, 950.f}, {256, 32, 1, 600.f, 700.f}};
 template <int N> int best_tile(const TileChoice (&choices)[N], const ProductArgs& a, size_t row_bytes) {
   int best = 0;
@@ -221,7 +222,7 @@ template <int T, typename F> auto product_kernel(const ProductArgs& a, F take) {
   }
 }
 // silu(gate) up of rows by expert, where one launch is the better way (few rows to an expert: the matrices are read by k_product_stream, k_gated follows)
-bool gates_in_one(long long rows, int experts) { return rows > 4ll * experts; }
+bool gates_in_one(long long rows, int experts) { return !takes_16bit_rows(rows, experts, true); }
 template <int T, typename F> auto gated_kernel(const ProductArgs& a, F take) {
   switch (best_tile(GATED_TILES, a, (size_t)a.n * bytes_of<T>)) {
     case 0: return take(Tiles<2, 4, 8, 4, 2, true>{});
@@ -262,7 +263,7 @@ struct StackedScratch {
     ends = take((size_t)experts * 4);
     token = take(pairs * 4);
     pos_of = take(pairs * 4);
-    const bool ahead = f8 && !takes_16bit_rows(pairs, experts, true);      // x is rounded by a launch of its own
+    const bool ahead = f8 && gates_in_one(pairs, experts);      // x is rounded by a launch of its own
     xq = take(ahead ? (size_t)tokens * hidden : 0);
     xs = take(ahead ? (size_t)tokens * (hidden / 128) * 4 : 0);
     h = take(gates_in_one(pairs, experts) ? 0 : pairs * 2 * inter * 4);
@@ -353,7 +354,7 @@ int htr_product(const void* x, int x_type, const void* x_scales, const void* w, 
   if (!aligned(x, 16) || !aligned(w, 16) || !aligned(y, 16) || !aligned(x_scales, 4) || !aligned(w_scales, 4) || !aligned(ends, 4) ||
       !aligned(bias, element_bytes(y_dtype)))
     return HTR_ERR_ALIGN;
-  const ProductArgs a{x, (const float*)x_scales, w, (const float*)w_scales, bias, y, ends, nullptr, (int)rows, m, n, experts, y_dtype, x_type, nullptr};
+  const ProductArgs a{x, (const float*)x_scales, w, (const float*)w_scales, bias, y, ends, nullptr, (int)rows, m, n, experts, y_dtype, x_type, nullptr, false};
   TRY_HIP(launch_product(a, type, false, (hipStream_t)stream));
   return HTR_OK;
 }
@@ -381,8 +382,8 @@ int htr_moe_stacked(const void* x, int dtype, const void* ids, int ids_int64, co
   int *ends = (int*)(s + at.ends), *token = (int*)(s + at.token), *pos_of = (int*)(s + at.pos_of);
   float *h = (float*)(s + at.h), *out = (float*)(s + at.out);
   TRY_HIP(launch(k_expert_order, dim3(experts), ORDER_WAVES * 64, 0, st, ids, ids_int64, pairs, top, experts, ends, token, pos_of));
-  ProductArgs a{x, nullptr, gate_up, (const float*)gate_up_scales, nullptr, h, ends, token, pairs, 2 * inter, hidden, experts, HTR_F32, dtype, nullptr};
-  if (f8 && !takes_16bit_rows(pairs, experts, true)) {
+  ProductArgs a{x, nullptr, gate_up, (const float*)gate_up_scales, nullptr, h, ends, token, pairs, 2 * inter, hidden, experts, HTR_F32, dtype, nullptr, f8};
+  if (f8 && gates_in_one(pairs, experts)) {
     a.x_type = HTR_E4M3;
     TRY_HIP(launch_quantize(x, dtype, tokens, hidden, hidden, s + at.xq, (float*)(s + at.xs), st));
     a.x = s + at.xq; a.xs = (const float*)(s + at.xs);
@@ -396,7 +397,7 @@ int htr_moe_stacked(const void* x, int dtype, const void* ids, int ids_int64, co
                : dtype == HTR_BF16 ? launch(k_gated<HTR_BF16>, dim3(pairs), 256, 0, st, h, ends, experts, inter, s + at.a, nullptr)
                                    : launch(k_gated<HTR_F16>, dim3(pairs), 256, 0, st, h, ends, experts, inter, s + at.a, nullptr));
   }
-  const ProductArgs d{s + at.a, (const float*)(s + at.as), down, (const float*)down_scales, nullptr, out, ends, nullptr, pairs, hidden, inter, experts, HTR_F32, type, nullptr};
+  const ProductArgs d{s + at.a, (const float*)(s + at.as), down, (const float*)down_scales, nullptr, out, ends, nullptr, pairs, hidden, inter, experts, HTR_F32, type, nullptr, false};
   TRY_HIP(launch_product(d, type, false, st));
   const dim3 grid((unsigned)tokens, (hidden + 2047) / 2048);
   TRY_HIP(dtype == HTR_BF16 ? launch(k_weighted_sum<HTR_BF16>, grid, 256, 0, st, out, pos_of, weights, top, hidden, y)

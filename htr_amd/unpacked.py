@@ -277,7 +277,8 @@ def moe_experts_stacked(x, expert_ids, expert_weights, gate_up, down):
 
     x [T, H] in bfloat16 or float16; expert_ids [T, top] int32 or int64; expert_weights [T, top]; gate_up [E, 2F, H] (gate rows first) and down
     [E, H, F] of x's type, H and F multiples of 8, or 8-bit pairs (multiples of 128), with which x and the hidden values are rounded to e4m3 as well.
-    Sums are as in the products; the hidden values are rounded to x's type or e4m3 in between, y [T, H] to x's type.  A token with an expert number out of range
+    Sums are as in the products, those of gate and up in 8 bits float32 throughout with up to some tens of rows to an expert (an e4m3 rounding follows them);
+    the hidden values are rounded to x's type or e4m3 in between, y [T, H] to x's type.  A token with an expert number out of range
     becomes NaN."""
     eight = _pair(gate_up) and _pair(down)
     path = _fast(x)

@@ -345,14 +345,15 @@ int htr_product(const void* x, int x_type, const void* x_scales, const void* w, 
 /* 1 where htr_product takes 16-bit rows with e4m3 matrices and rounds them on the way (few rows), otherwise 0: htr_quantize_e4m3 first.  grouped: ends is given. */
 int htr_product_rounds(int64_t rows, int experts, int grouped);
 /* The kernel behind htr_product for these sizes, or (gated = 1, with grouped = 1) behind the first product of htr_moe_stacked, where gate and up are
- * one launch: m = 2 inter, more than 4 rows to an expert, HTR_ERR_SIZE otherwise.  out6 = {matrix rows of a tile, rows of x of a tile, waves of a workgroup,
+ * one launch: m = 2 inter, more than 4 rows to an expert on average, HTR_ERR_SIZE otherwise.  out6 = {matrix rows of a tile, rows of x of a tile, waves of a workgroup,
  * stages of its ring in LDS (0: each workgroup has one tile, straight from memory), workgroups, tiles (grouped: at most)}.  Workgroups of the ring
  * kernel go on from tile to tile.  For tests and tuning. */
 int htr_product_plan(int64_t rows, int m, int n, int experts, int grouped, int gated, int type, int x_type, int* out6);
 
 /*
  * A routed-expert layer on stacked matrices: y_t = sum_j w[t, j] Down_e( silu(Gate_e x_t) * Up_e x_t ), e = ids[t, j], sums as in htr_product, over j in
- * float32 and ascending, y of dtype (bf16 or f16).  The hidden values between the products are rounded to dtype, or to e4m3 with scales.
+ * float32 and ascending, y of dtype (bf16 or f16).  Gate and up in e4m3 have float32 sums throughout, since they are rounded to e4m3 next, with up to 4 rows
+ * to an expert on average and where htr_product_plan says tiles of up to 64 rows of x.  The hidden values between the products are rounded to dtype, or to e4m3 with scales.
  *   type     dtype, or HTR_E4M3 (x is then rounded to e4m3 as well)
  *   gate_up  [experts][2 inter][hidden], gate rows first;  down [experts][hidden][inter];  scales as in htr_product, or NULL
  *   ids      [tokens][top] int32 or int64 and weights [tokens][top] float32, on the device; an expert out of range makes its token NaN
