@@ -187,7 +187,14 @@ template <int T, typename F> auto product_kernel(const ProductArgs& a, F take) {
   if (few) {
     const long long tiles = grouped ? (a.rows < a.experts ? a.rows : a.experts) : 1, wgs = (a.m + 15) / 16 * tiles;
     const long long slabs = ((long long)a.n * bytes_of<T> + 127) / 128;
-    if (grouped && wgs >= 4 * 512) return take(Stream<4, 1, 4>{});
+    // In 16 bits a ring is ahead where there are that many (92 sizes of 4 to 160 experts, up to 4 rows to one: 0.81 to 0.87 of the time on average, 1.03 at worst; us by
+    // 64 rows to a workgroup of 4 waves, by tiles of 64x64: 96 rows of 64 experts of 2816x2048 146 and 127, 12 of 8 of 14336x4096 242 and 178, 72 of 48 of
+    // 1536x2560 85 and 63, 48 of 24 of 3000x3000 122 and 80, 160 of 160 of 1024x1024 51 and 48).  Rows that all have one expert take less either way (256 rows of
+    // 64 experts of 2816x2048 in e4m3 22 us, evenly 69).
+    if (grouped && wgs >= 4 * 512) {
+      if constexpr (T == P_F8) return take(Stream<4, 1, 4>{});
+      return take(Tiles<2, 2, 2, 2, 4>{});
+    }
     // Rows of fewer slabs than waves leave some idle (7 rows on 15657x384 in e4m3 5.5 us by 16 rows to a workgroup of 8 waves, 4.7 by 32 to one of 4), and rows
     // to be rounded are rounded by half as many (4 tokens over 8 of 16 experts of 1920/384 37 and 31); long rows of few workgroups need more waves to share them
     if (wgs >= 512 && (slabs < 8 || (slabs <= 16 && T == P_F8 && a.x_type != HTR_E4M3))) return take(Stream<2, 1, 4>{});

@@ -55,7 +55,7 @@ GROUPED_16 = [      # experts, rows, m, n
     (4, 9, 200, 328, (16, 16, 8, 0), False),
     (3, 5, 300, 5000, (16, 16, 16, 0), False),
     (2, 4, 9001, 72, (32, 16, 4, 0), False),
-    (2, 6, 16390, 136, (64, 16, 4, 0), False),
+    (2, 6, 16390, 264, (64, 64, 4, 4), False),
     (2, 40, 1542, 1000, (16, 32, 8, 0), False),
     (3, 96, 1000, 264, (64, 32, 4, 4), False),
     (66, 1600, 520, 328, (64, 32, 4, 4), True),
@@ -123,7 +123,8 @@ def test_every_kernel_has_a_case(kind):
     if eight:
         for rows, m, n, kernel, several in DENSE:
             held_to(rows, m, n, 1, False, False, kind, kernel, several, [rows])
-    assert {c[4] for c in (GROUPED_8 + [(1,) + c for c in DENSE] if eight else GROUPED_16)} == RING | STREAM
+    # 64 matrix rows to a streaming workgroup are for e4m3
+    assert {c[4] for c in (GROUPED_8 + [(1,) + c for c in DENSE] if eight else GROUPED_16)} == RING | STREAM - (set() if eight else {(64, 16, 4, 0)})
     assert {c[4] for c in gated} == GATED
     # every ring goes on from tile to tile somewhere
     assert RING <= {c[4] for c in grouped if c[5]} and GATED <= {c[4] for c in gated if c[5]}
@@ -158,6 +159,13 @@ def test_uneven_experts_of_small_matrices(kind):
     for rows, m, experts in ((192, 512, 8), (384, 256, 16), (768, 128, 32), (1536, 64, 64)):
         assert plan(rows, m, 768, experts, True, False, kind)[:4] == (16, 16, 8, 0)
         assert plan(rows, 2 * m, 768, experts, True, False, kind)[3] > 0 and plan(2 * rows, m, 768, experts, True, False, kind)[3] > 0
+
+
+def test_few_rows_by_type():
+    """As measured for either: where experts with few rows make workgroups enough, e4m3 streams and 16 bits take a ring."""
+    for rows, m, n, experts in ((96, 2816, 2048, 64), (12, 14336, 4096, 8), (72, 1536, 2560, 48), (160, 1024, 1024, 160)):
+        assert plan(rows, m, n, experts, True, False, BF16)[:4] == plan(rows, m, n, experts, True, False, F16)[:4] == (64, 64, 4, 4)
+        assert plan(rows, m, n // 128 * 128, experts, True, False, E4M3)[:4] == (64, 16, 4, 0)
 
 
 @pytest.mark.parametrize("kind", [BF16, E4M3], ids=str)
