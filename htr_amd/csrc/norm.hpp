@@ -9,7 +9,7 @@
 // several thousandths between machines, and by 2 % behind a second quantization.  A power of two costs no precision but at the lower
 // end, where values below 2^-15 of the block's largest lose a bit more.
 // Bound: HBM (x, r and w read once, t and y or q and s written once).  A workgroup takes one row and keeps it in registers between the two passes.
-// 8192 rows of 4096 in bf16 to e4m3: 24 us (4.1 TB/s), with a residual 41 us (5.7 TB/s; a copy of large arrays reaches 5.2); one row 3.3 us.
+// 8192 rows of 4096 in bf16 to e4m3: 25 us (4.0 TB/s), with a residual 40 us (5.9 TB/s; a copy of large arrays reaches 5.1, a read alone 7.3); one row 3.3 us.
 
 // ---- e4m3
 // the scale of a block whose largest finite magnitude is `amax`: amax = f 2^e with f in [1/2, 1), 448 = 0.875 2^9.  A block of zeros (or of
@@ -218,7 +218,7 @@ __device__ __forceinline__ double block_sum(double v, double* lds) {
 
 // NV runs of eight columns to a thread; n <= 8 NV threads.  Every row on a 16-byte boundary and n a multiple of 8, or (ANY) neither: the last run of a
 // row may then be a part of one.  Runs from any address cost little next to loads of single elements: 8000 rows of 1001 bf16 columns with their
-// residual 18 us (element by element 54; 12 at the rate of a copy).
+// residual 19 us (element by element 54; 13 at the rate of a copy).
 // The squares are summed in 64 bits: a row's mean of many of them keeps what float32 holds, for two instructions to an element
 // that the memory hides.
 template <int T, int NV, bool RES, bool QUANT, bool ANY>
@@ -294,7 +294,7 @@ __global__ __launch_bounds__(1024) void k_rms_norm(const NormArgs a) {
 }
 
 // Rows of more than 32768 columns: read twice, the second time from the cache; with a residual the sums as they were written.  2000 rows of 40960 in bf16 to e4m3
-// 133 us, 4.3 TB/s (loads of single elements 530).
+// with a residual 125 us, 4.6 TB/s of bytes read or written once (loads of single elements 530); without one 75 us, 3.3 TB/s, the second reading apart.
 template <int T, bool RES, bool QUANT>
 __global__ __launch_bounds__(1024) void k_rms_norm_long(const NormArgs a) {
   __shared__ double s_sum[16];

@@ -127,7 +127,8 @@ __device__ __forceinline__ float silu(float g) { return g / (1.f + __expf(-g)); 
 // ------------------------------------------------------------------------------------------------ few rows
 // A workgroup owns 16 R rows of a matrix and up to 16 TT rows of x; its waves take the slabs in turn, straight from memory into registers
 // (every byte of the matrix is used by one wave once: LDS would only be a detour), and add up through LDS.
-// Bound: HBM, the matrix read once: 96 rows of 64 experts of 2816x2048 in e4m3 52 us, 5.2 TB/s; one row on 1024x4096 5.0 us, the latency of two loads and the sum.
+// Bound: HBM, the matrix read once: 96 rows of 64 experts of 2816x2048 in e4m3 52 us, 5.4 TB/s (a kernel that only reads reaches 7.3); one row on 1024x4096 5.0 us, the
+// latency of two loads and the sum.
 // X: the type of x; 16-bit rows with an e4m3 matrix are rounded on the way, by every workgroup for itself: about 110 instructions to a slab, beside
 // its 2 KB or more of the matrix, against a launch ahead of this one.  WIDE: e4m3 products in float32 sums.
 template <int T, int X, int R, int TT, int STREAM_WAVES, bool WIDE>
