@@ -414,6 +414,12 @@ def test_layers_in_8_bits_round_the_hidden_values_as_defined(gen, dtype, T, top,
     # in linear_fp8, 1.5e-5 off, one value in some thousand fell there: 1.3e-3 to 5e-3 of the result.
     rounding = (want.to(dtype).double() - want).norm()
     assert (y.double() - want).norm() <= 1.05 * rounding + 3e-4 * want.norm(), ((y.double() - want).norm() / want.norm(), rounding / want.norm())
+    if T > 1:
+        call[0][1, H // 2] = float("nan")
+        z = ops.moe_experts_stacked(*call)
+        assert z[1].isnan().all()
+        z[1] = y[1]
+        assert torch.equal(z, y)
 
 
 @pytest.mark.gpu
