@@ -176,7 +176,7 @@ template <int N> int best_tile(const TileChoice (&choices)[N], const ProductArgs
 //   one row: 1024x4096 5.0 (16 rows to a workgroup of 8 waves; 4 waves 6.4, tiles of 64x32 10.9), 4096x4096 5.9 (7.4, 12.0), 14336x4096 15.5 (17.2, 16.9),
 //   28672x4096 25.7 (27.2, 29.5); 32 rows: 4096x4096 10.3 (tiles of 64x32 12.4, of 128x32 16.6), 28672x4096 64 (33, 31)
 //   96 rows of 64 experts: 2816x2048 56 (64 rows to a workgroup of 4 waves; 16 rows to one of 8 86; tiles of 128x32 59), 2048x1408 34 (52; 35)
-//   9 rows of 16 experts of 523x7600 in bf16: 52 us with 64 rows to a workgroup
+//   9 rows of 16 experts of 523x7600 in bf16: 28 us (64 rows to a workgroup of 4 waves 54, tiles of 64x32 37)
 bool takes_16bit_rows(long long rows, int experts, bool grouped) {
   return grouped ? rows <= 4ll * experts && span_bound(rows, experts, true, 16) <= 65535 : rows <= 16;
 }
