@@ -14,8 +14,8 @@ the block to 448 or below; scales from elsewhere need not be.  Infinities and Na
 
 Norms sum in 64 bits, products of 16-bit values in float32.  Products of e4m3 values are first added eight consecutive
 columns at a time, as the matrix instructions do: each eight is off by at most 2^-10 of the largest magnitude in x times that in the matrix (one below 2^-6 of its
-scale counts as that).  Everything beyond is float32, the product of a row's scale and a block's as well, which has to be in its normal range.  Results are
-rounded once.  Nothing here has a derivative, as no packed linear has one in its
+scale counts as that).  Everything beyond is float32, the product of a row's scale and a block's as well (below 2^-126 it has fewer bits, beyond float32 it is
+infinite).  Results are rounded once.  Nothing here has a derivative, as no packed linear has one in its
 activations: a call that torch would differentiate is refused.  Calls only queue kernels on the current stream of x's device, allocate with torch and
 may be captured into a graph.
 """

@@ -331,7 +331,7 @@ int htr_quantize_e4m3(const void* x, int64_t stride, int64_t rows, int n, int dt
 /*
  * y[r] = W_e x[r] (+ bias), e the expert of row r.  Sums are float32, except that products of e4m3 values are first added eight consecutive columns at
  * a time: each eight is off by at most 2^-10 of the largest magnitude in x times that in w (a magnitude below 2^-6 of its scale counts as that).  The
- * product of a row's scale and a block's is float32 as well: it has to be in its normal range.
+ * product of a row's scale and a block's is float32 as well: one below 2^-126 has fewer bits, one beyond float32 is infinite, and NaN times a zero.
  *   type    of w: HTR_E4M3 (with its scales), HTR_BF16 or HTR_F16 (scales NULL)
  *   x_type  type; with e4m3 matrices also HTR_BF16 or HTR_F16 (x_scales NULL) where htr_product_rounds says so: rounded as by htr_quantize_e4m3
  *   x       [rows][n], w [experts][m][n], 16-byte aligned; n a multiple of 128 (e4m3) or of 8 (16 bits), up to 2^22; m up to 2^26; experts up to 65535

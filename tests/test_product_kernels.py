@@ -322,6 +322,20 @@ def test_sums_of_e4m3_products_of_a_wide_range(gen, rows, m):
     assert ((y - 2 * 2.0 ** -8).abs() <= 2 * 256 * 2.0 ** -10).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,m", [(2, 900), (40, 1030), (300, 5000)])
+def test_products_of_scales_at_the_ends_of_float32(gen, rows, m):
+    """Zeros have the scale 2^-108: with any block's they stay zeros; values whose scales' product is just normal, or just finite, are products like others."""
+    w, ws = fp8_weight(gen, m, 256)
+    y = ops.linear_fp8(torch.zeros(rows, 256, dtype=BF16, device="cuda"), w, ws * 2.0 ** -30)
+    assert (y == 0).all()
+    q, s = ops.quantize_fp8(randn(gen, rows, 256))
+    for at in (-125, 90):
+        x = q, torch.full_like(s, 2.0 ** (at // 2))
+        block = torch.full_like(ws, 2.0 ** (at - at // 2))
+        assert_within(ops.linear_fp8(x, w, block, out_dtype=F32), *product_bound(x, (w, block), F32))
+
+
 # ---- routed experts
 def float32_sums(pairs, experts, H, F):
     """Whether gate and up of an 8-bit layer have float32 sums: few rows, and tiles of up to 64."""
