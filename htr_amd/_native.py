@@ -15,6 +15,7 @@ LIB_PATH = os.environ.get("HTR_GFX950_LIB") or os.path.join(_CSRC, "libhtr_gfx95
 
 BF16, F16, F32 = 0, 1, 2
 E4M3 = 3
+I8 = 4
 MAX_BATCH = 2048
 MAX_ROWS_PER_TILE = 128
 MAX_GROUP_ROWS = 32
@@ -55,6 +56,9 @@ SIGNATURES = {
     "htr_dequant_w": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp]),
     "htr_rms_norm": (_i, [_vp, _i64, _vp, _i64, _vp, _i64, _i, ctypes.c_double, _i, _vp, _vp, _vp, _vp]),
     "htr_quantize_e4m3": (_i, [_vp, _i64, _i64, _i, _i, _vp, _vp, _vp]),
+    "htr_rms_norm_int8": (_i, [_vp, _i64, _vp, _i64, _vp, _i64, _i, ctypes.c_double, _i, _vp, _vp, _vp, _vp]),
+    "htr_quantize_int8": (_i, [_vp, _i64, _i64, _i, _i, _vp, _vp, _vp]),
+    "htr_route": (_i, [_vp, _i64, _i, _i64, _i, _i, _i, _vp, _i, _i, _i, _i, ctypes.c_double, _vp, _vp, _vp]),
     "htr_product": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _i, _i, _vp]),
     "htr_product_rounds": (_i, [_i64, _i, _i]),
     "htr_product_plan": (_i, [_i64, _i, _i, _i, _i, _i, _i, _i, ctypes.POINTER(ctypes.c_int)]),
@@ -99,7 +103,8 @@ def fast():
                         address(L.htr_moe_scratch_bytes), address(L.htr_moe_experts),
                         address(L.htr_linear_route), address(L.htr_dequant_w))
             module.bind_unpacked(address(L.htr_rms_norm), address(L.htr_quantize_e4m3), address(L.htr_product), address(L.htr_product_rounds),
-                                 address(L.htr_moe_stacked_scratch_bytes), address(L.htr_moe_stacked))
+                                 address(L.htr_moe_stacked_scratch_bytes), address(L.htr_moe_stacked), address(L.htr_rms_norm_int8), address(L.htr_quantize_int8),
+                                 address(L.htr_route))
         except (ImportError, AttributeError) as e:
             warnings.warn(f"htr_amd/_fast.so cannot be used ({e}): launches are prepared in Python; `python -m htr_amd.build` builds it",
                           RuntimeWarning, stacklevel=2)

@@ -1,20 +1,24 @@
 // Part of unpacked.hip, included inside its anonymous namespace: products of rows with matrices that are not HTR-W1, one matrix or one for each expert.
 //
-//   y[r][i] = sum_k x[r][k] w_e[i][k],  e the expert of row r;  e4m3: the sum over each block of 128 columns times xs[r][k / 128] ws_e[i / 128][k / 128]
+//   y[r][i] = sum_k x[r][k] w_e[i][k],  e the expert of row r;  e4m3: the sum over each block of 128 columns times xs[r][k / 128] ws_e[i / 128][k / 128];
+//   int8: the sum, exact in 32 bits, times xs[r] ws_e[i]
 //
-// Everything is cut into slabs of 128 bytes of a row: 128 e4m3 values, one v_mfma_f32_16x16x128_f8f6f4 whose result is scaled into the sum, or
-// 64 16-bit ones, two v_mfma_f32_16x16x32.  A lane feeds bytes 16 g .. and 64 + 16 g .. of its row (g = lane / 16): another order of the
+// Everything is cut into slabs of 128 bytes of a row: 128 e4m3 values, one v_mfma_f32_16x16x128_f8f6f4 whose result is scaled into the sum, 128
+// integers, two v_mfma_i32_16x16x64_i8, or 64 16-bit values, two v_mfma_f32_16x16x32.  A lane feeds bytes 16 g .. and 64 + 16 g .. of its row (g = lane / 16): another order of the
 // columns than the instructions' own, the same for both operands.  Matrix rows are MFMA rows (D: rows 4 g + i, four to a lane), activation
 // rows are MFMA columns (lane % 16), so that a lane holds consecutive outputs of one row.
-enum { P_F8 = 3 };                       // beside HTR_BF16, HTR_F16: the operands' type
-template <int T> constexpr int bytes_of = T == P_F8 ? 1 : 2;
+enum { P_F8 = 3, P_I8 = 4 };             // beside HTR_BF16, HTR_F16: the operands' type
+template <int T> constexpr int bytes_of = T == P_F8 || T == P_I8 ? 1 : 2;
+typedef int i4 __attribute__((ext_vector_type(4)));
+template <int T> struct SumOf { typedef f4 type; typedef float one; };      // what products are summed in
+template <> struct SumOf<P_I8> { typedef i4 type; typedef int one; };
 typedef int i8v __attribute__((ext_vector_type(8)));
 
 struct ProductArgs {
   const void* x;                         // [.][n]; e4m3 matrices: also 16-bit rows, where takes_16bit_rows says so
-  const float* xs;                       // e4m3 rows: [.][n / 128]
+  const float* xs;                       // e4m3 rows: [.][n / 128]; int8: [.]
   const void* w;                         // [experts][m][n]
-  const float* ws;                       // e4m3: [experts][ceil(m / 128)][n / 128]
+  const float* ws;                       // e4m3: [experts][ceil(m / 128)][n / 128]; int8: [experts][m]
   const void* bias;                      // [m] in y's type or NULL
   void* y;                               // [rows][m]
   const int* ends;                       // [experts]: expert e has rows ends[e - 1] .. ends[e] - 1; NULL: one expert, all rows
@@ -117,8 +121,9 @@ __device__ __forceinline__ h8 widen(uint32_t lo, uint32_t hi) {
   return h8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
 __device__ __forceinline__ Wide widen(const u4 (&q)[2]) { return Wide{{widen(q[0].x, q[0].y), widen(q[0].z, q[0].w), widen(q[1].x, q[1].y), widen(q[1].z, q[1].w)}}; }
-template <int T> __device__ __forceinline__ f4 mfma_16(const u4& a, const u4& b, const f4& c) {
-  if constexpr (T == HTR_BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+template <int T> __device__ __forceinline__ typename SumOf<T>::type mfma_16(const u4& a, const u4& b, const typename SumOf<T>::type& c) {
+  if constexpr (T == P_I8) return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i4, a), __builtin_bit_cast(i4, b), c, 0, 0, 0);
+  else if constexpr (T == HTR_BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
   else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
 }
 
@@ -136,7 +141,9 @@ __global__ __launch_bounds__(STREAM_WAVES * 64) void k_product_stream(const Prod
   constexpr int P = R + TT <= 3 && !(X != T && STREAM_WAVES > 8) ? 4 : 2;      // slabs in flight
   constexpr bool ROUNDS = X != T;
   static_assert((!ROUNDS && !WIDE) || T == P_F8, "");
-  __shared__ float red[STREAM_WAVES][R * TT * 256];
+  typedef typename SumOf<T>::type Sum;
+  typedef typename SumOf<T>::one One;
+  __shared__ One red[STREAM_WAVES][R * TT * 256];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
   const int m0 = blockIdx.x * 16 * R;
   const Span s = find_span(a, 16 * TT, blockIdx.y);
@@ -157,20 +164,20 @@ __global__ __launch_bounds__(STREAM_WAVES * 64) void k_product_stream(const Prod
     sp[t] = (const HTR_GLOBAL float*)a.xs + (size_t)r * (a.n >> 7);
   }
   const HTR_GLOBAL float* wsp = (const HTR_GLOBAL float*)a.ws + ((size_t)s.e * ((a.m + 127) >> 7) + (m0 >> 7)) * (a.n >> 7);
-  f4 acc[R][TT];
+  Sum acc[R][TT];
 #pragma unroll
   for (int i = 0; i < R; ++i)
 #pragma unroll
-    for (int t = 0; t < TT; ++t) acc[i][t] = f4{0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < TT; ++t) acc[i][t] = Sum{0, 0, 0, 0};
   u4 A[P][R][2], B[P][TT][2];
-  Eight<X == P_F8 ? HTR_BF16 : X> raw[ROUNDS ? P : 1][TT][4];  // 16 elements of either half of the slab
+  Eight<X == P_F8 || X == P_I8 ? HTR_BF16 : X> raw[ROUNDS ? P : 1][TT][4];  // 16 elements of either half of the slab
   float sx[P][TT], sw[P];
   const u4 zero = {0u, 0u, 0u, 0u};
   auto load = [&](int p, int slab) {
     const size_t off = (size_t)slab << 7;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      // 16-bit rows may end inside the slab, at a multiple of 16 bytes
+      // other than e4m3 rows may end inside the slab, at a multiple of 16 bytes
       const bool in = T == P_F8 || off + 64 * h + 16 * g < row_bytes;
 #pragma unroll
       for (int i = 0; i < R; ++i) { A[p][i][h] = zero; if (in) A[p][i][h] = __builtin_nontemporal_load((const HTR_GLOBAL u4*)(wp[i] + off + 64 * h)); }
@@ -241,15 +248,20 @@ __global__ __launch_bounds__(STREAM_WAVES * 64) void k_product_stream(const Prod
 #pragma unroll
   for (int i = 0; i < R; ++i)
 #pragma unroll
-    for (int t = 0; t < TT; ++t) *(f4*)&red[wv][(i * TT + t) * 256 + lane * 4] = acc[i][t];
+    for (int t = 0; t < TT; ++t) *(Sum*)&red[wv][(i * TT + t) * 256 + lane * 4] = acc[i][t];
   __syncthreads();
   for (int idx = threadIdx.x; idx < R * TT * 256; idx += STREAM_WAVES * 64) {
     const int i = idx % (16 * R), t = idx / (16 * R);            // matrix row, row of x
     const int at = ((i >> 4) * TT + (t >> 4)) * 256 + (((i & 15) >> 2) * 16 + (t & 15)) * 4 + (i & 3);
-    float v = 0.f;
+    One sum = 0;
 #pragma unroll
-    for (int k = 0; k < STREAM_WAVES; ++k) v += red[k][at];
+    for (int k = 0; k < STREAM_WAVES; ++k) sum += red[k][at];
     if (t < s.count && m0 + i < a.m) {
+      float v = (float)sum;
+      if constexpr (T == P_I8) {
+        const int r = a.gather != nullptr ? a.gather[s.first + t] : s.first + t;
+        v = v * ((const HTR_GLOBAL float*)a.xs)[r] * ((const HTR_GLOBAL float*)a.ws)[(size_t)s.e * a.m + m0 + i];
+      }
       if (a.bias != nullptr) v += load_elem_g(a.bias, a.y_dtype, m0 + i);
       store_elem_g(a.y, a.y_dtype, (size_t)(s.first + t) * a.m + m0 + i, v);
     }
@@ -268,7 +280,8 @@ __global__ __launch_bounds__(STREAM_WAVES * 64) void k_product_stream(const Prod
 // Row number 4 q + j of a wave's MFMA tiles 2 h and 2 h + 1 are its rows 32 h + 8 q + j and + 4: a lane then holds eight consecutive outputs, and four
 // lanes 64 bytes of a row in 16 bits.
 // GATED: the matrix is gate over up, m / 2 rows each; a tile takes TM / 2 of either, 32 by 32 in turn, so that a lane holds gate and up of eight consecutive
-// hidden columns; y [rows][m / 2] is silu(gate) up, in 16 bits or in e4m3 (then TM / 2 = 128 columns share a scale; rows behind the last expert's are left).
+// hidden columns; y [rows][m / 2] is silu(gate) up, in 16 bits, in float32 (int8: a row's scale is not known before its last column) or in e4m3 (then TM / 2 = 128 columns share a
+// scale); rows behind the last expert's are left.
 __device__ __forceinline__ int swizzle_w(int r) { return ((r >> 1) & 1) | ((r >> 3 & 3) << 1); }
 __device__ __forceinline__ int swizzle_x(int r) { return (r >> 1) & 7; }
 constexpr int TILE_XCDS = 8, TOGETHER = 8;
@@ -371,7 +384,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
   };
   Source src, src2;
   source(mine, src);
-  // 16-bit rows may end inside the last slab, at a multiple of 16 bytes: chunks from there on are loaded as the slab's first, and zeroed in LDS
+  // Other than e4m3 rows may end inside the last slab, at a multiple of 16 bytes: chunks from there on are loaded as the slab's first, and zeroed in LDS
   const int tail = (int)(row_bytes & 127) >> 4;
   auto place = [&](int j, int stage) { return stage * STAGE + (j < LW ? (j * WAVES + wv) * 1024 : TM * 128 + ((j - LW) * WAVES + wv) * 1024); };
   auto issue = [&](Source& src, int slab, int stage, int from, int to) {
@@ -427,11 +440,12 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
     for (int t = 0; t < BT; ++t) sx[t] = base[wn * 16 * BT + 16 * t + c];
     if constexpr (GATED) { sw[0] = base[XW * 64]; sw[1] = base[XW * 64 + 1]; } else sw[0] = base[XW * 64 + ((wm * 16 * AT) >> 7)];
   };
-  f4 acc[AT][BT];
+  typedef typename SumOf<T>::type Sum;
+  Sum acc[AT][BT];
 #pragma unroll
   for (int i = 0; i < AT; ++i)
 #pragma unroll
-    for (int t = 0; t < BT; ++t) acc[i][t] = f4{0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < BT; ++t) acc[i][t] = Sum{0, 0, 0, 0};
   int stage = 0;                                                 // of the slab in registers
   auto after = [](int st, int by) { const int to = st + by; return to >= NS ? to - NS : to; };
   constexpr int PIECES = AT < 4 ? AT : 4;                        // MFMA tiles over which the loads of a slab are spread
@@ -459,8 +473,10 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
     }
     f4 sums[2][WIDE ? BT : 1];
     auto add_sums = [&](int i) {
+      if constexpr (WIDE) {
 #pragma unroll
-      for (int t = 0; t < BT; ++t) acc[i][t] += sums[i & 1][t] * sc[GATED ? i >> 1 & 1 : 0][t];
+        for (int t = 0; t < BT; ++t) acc[i][t] += sums[i & 1][t] * sc[GATED ? i >> 1 & 1 : 0][t];
+      }
     };
 #pragma unroll
     for (int i = 0; i < AT; ++i) {
@@ -545,7 +561,44 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
     src = src2;
     if (++slab < slabs) continue;
     slab = 0;
-    if constexpr (GATED) {
+    // int8: the scales of the lane's rows of x, and of eight consecutive rows of the matrix, as far as it goes
+    auto row_scale = [&](int t) {
+      int r = mine.s.first + min(wn * 16 * BT + 16 * t + c, mine.s.count - 1);
+      if (a.gather != nullptr) r = a.gather[r];
+      return ((const HTR_GLOBAL float*)a.xs)[r];
+    };
+    auto matrix_scales = [&](int i, int end, float (&w)[8]) {
+      const HTR_GLOBAL float* p = (const HTR_GLOBAL float*)a.ws + (size_t)mine.s.e * a.m;
+      if (i + 8 <= end) {
+        const f4 lo = *(const HTR_GLOBAL f4_any*)(p + i), hi = *(const HTR_GLOBAL f4_any*)(p + i + 4);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) { w[k] = lo[k]; w[4 + k] = hi[k]; }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) w[k] = p[min(i + k, end - 1)];
+      }
+    };
+    if constexpr (GATED && T == P_I8) {
+      const int F = a.m >> 1, i0 = (mine.m0 >> 1) + wm * 8 * AT + 8 * g;      // hidden columns; first of the lane's
+      float rs[BT];
+#pragma unroll
+      for (int t = 0; t < BT; ++t) rs[t] = row_scale(t);
+#pragma unroll
+      for (int h = 0; h < AT / 4; ++h) {
+        float gate[8], up[8];
+        matrix_scales(i0 + 32 * h, F, gate);
+        matrix_scales(F + i0 + 32 * h, a.m, up);
+#pragma unroll
+        for (int t = 0; t < BT; ++t) {
+          float f[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            f[k] = silu((float)acc[4 * h + (k >> 2)][t][k & 3] * rs[t] * gate[k]) * ((float)acc[4 * h + 2 + (k >> 2)][t][k & 3] * rs[t] * up[k]);
+          const int r = wn * 16 * BT + 16 * t + c;
+          if (r < mine.s.count && i0 + 32 * h < F) { Eight<HTR_F32> v; v.set(f); v.store(a.y, (size_t)(mine.s.first + r) * F + i0 + 32 * h); }
+        }
+      }
+    } else if constexpr (GATED) {
       const int F = a.m >> 1, i0 = (mine.m0 >> 1) + wm * 8 * AT + 8 * g;      // hidden columns; first of the lane's
       float amax[BT];
 #pragma unroll
@@ -604,6 +657,13 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
       const int i0 = mine.m0 + wm * 16 * AT + 8 * g;               // first of the lane's outputs
       auto put = [&](auto type) {
         constexpr int Y = decltype(type)::value;
+        float ws[T == P_I8 ? AT / 2 : 1][8], rs[T == P_I8 ? BT : 1];
+        if constexpr (T == P_I8) {
+#pragma unroll
+          for (int h = 0; h < AT / 2; ++h) matrix_scales(i0 + 32 * h, a.m, ws[h]);
+#pragma unroll
+          for (int t = 0; t < BT; ++t) rs[t] = row_scale(t);
+        }
 #pragma unroll
         for (int t = 0; t < BT; ++t) {
           const int r = wn * 16 * BT + 16 * t + c;
@@ -611,7 +671,10 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
           for (int h = 0; h < AT / 2; ++h) {
             float f[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) f[k] = acc[2 * h + (k >> 2)][t][k & 3];
+            for (int k = 0; k < 8; ++k) {
+              f[k] = (float)acc[2 * h + (k >> 2)][t][k & 3];
+              if constexpr (T == P_I8) f[k] = f[k] * rs[t] * ws[h][k];
+            }
             if (r < mine.s.count && i0 + 32 * h < a.m) store8<Y>(a, f, (size_t)(mine.s.first + r) * a.m + i0 + 32 * h, i0 + 32 * h);
           }
         }
@@ -623,7 +686,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
 #pragma unroll
     for (int i = 0; i < AT; ++i)
 #pragma unroll
-      for (int t = 0; t < BT; ++t) acc[i][t] = f4{0.f, 0.f, 0.f, 0.f};
+      for (int t = 0; t < BT; ++t) acc[i][t] = Sum{0, 0, 0, 0};
     if (!more) break;
     mine = then;
   }

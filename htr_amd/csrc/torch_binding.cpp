@@ -28,6 +28,9 @@ decltype(&htr_linear_route) f_route = nullptr;
 decltype(&htr_dequant_w) f_dequant = nullptr;
 decltype(&htr_rms_norm) f_norm = nullptr;
 decltype(&htr_quantize_e4m3) f_quantize = nullptr;
+decltype(&htr_rms_norm_int8) f_norm_int8 = nullptr;
+decltype(&htr_quantize_int8) f_quantize_int8 = nullptr;
+decltype(&htr_route) f_experts = nullptr;
 decltype(&htr_product) f_product = nullptr;
 decltype(&htr_product_rounds) f_rounds = nullptr;
 decltype(&htr_moe_stacked_scratch_bytes) f_stacked_bytes = nullptr;
@@ -239,6 +242,8 @@ bool plain(const at::Tensor& t, c10::Device dev) { return t.device() == dev && r
 at::ScalarType type_of(long code) { return code == 0 ? at::kBFloat16 : code == 1 ? at::kHalf : at::kFloat; }
 // dims of 8-bit rows' scales (rows = true) or matrices' for values q
 bool scales_ok(const at::Tensor& q, const at::Tensor& s, bool rows) {
+  if (q.scalar_type() == at::kChar)
+    return s.scalar_type() == at::kFloat && q.dim() >= 1 && q.size(-1) % 16 == 0 && q.size(-1) < (1 << 17) && s.sizes() == q.sizes().slice(0, q.dim() - 1);
   if (s.scalar_type() != at::kFloat || s.dim() != q.dim() || q.dim() < (rows ? 1 : 2) || q.size(-1) % 128 || s.size(-1) != q.size(-1) / 128) return false;
   for (int64_t k = 0; k + 1 < q.dim(); ++k) {
     const bool m = !rows && k + 2 == q.dim();
@@ -246,17 +251,24 @@ bool scales_ok(const at::Tensor& q, const at::Tensor& s, bool rows) {
   }
   return true;
 }
-// x as 8-bit rows; a tensor of floats is rounded.  False: not as expected; rc: what the launch returned
-bool rows8(const at::Tensor& x, const at::Tensor* s, c10::Device dev, void* stream, at::Tensor& q, at::Tensor& qs, int& rc) {
+int type_code(at::ScalarType t) { return t == at::kFloat8_e4m3fn ? HTR_E4M3 : t == at::kChar ? HTR_I8 : dtype_code(t); }
+// x as 8-bit rows of `kind`; a tensor of floats is rounded.  False: not as expected; rc: what the launch returned
+bool rows8(const at::Tensor& x, const at::Tensor* s, at::ScalarType kind, c10::Device dev, void* stream, at::Tensor& q, at::Tensor& qs, int& rc) {
   if (s != nullptr) {
-    if (x.scalar_type() != at::kFloat8_e4m3fn || !scales_ok(x, *s, true) || !plain(*s, dev)) return false;
+    if (x.scalar_type() != kind || !scales_ok(x, *s, true) || !plain(*s, dev)) return false;
     q = x; qs = *s;
     return true;
   }
   const int64_t n = x.size(-1);
-  if (!float_of(x) || n % 128) return false;
+  if (!float_of(x) || n % (kind == at::kChar ? 16 : 128)) return false;
   at::DimVector shape(x.sizes().begin(), x.sizes().end());
-  q = at::empty(shape, x.options().dtype(at::kFloat8_e4m3fn));
+  q = at::empty(shape, x.options().dtype(kind));
+  if (kind == at::kChar) {
+    shape.pop_back();
+    qs = at::empty(shape, x.options().dtype(at::kFloat));
+    rc = f_quantize_int8(x.const_data_ptr(), n, x.numel() / n, (int)n, dtype_code(x.scalar_type()), q.mutable_data_ptr(), qs.mutable_data_ptr(), stream);
+    return rc == HTR_OK;
+  }
   shape.back() = n / 128;
   qs = at::empty(shape, x.options().dtype(at::kFloat));
   rc = f_quantize(x.const_data_ptr(), n, x.numel() / n, (int)n, dtype_code(x.scalar_type()), q.mutable_data_ptr(), qs.mutable_data_ptr(), stream);
@@ -265,34 +277,34 @@ bool rows8(const at::Tensor& x, const at::Tensor* s, c10::Device dev, void* stre
 // optional tensor argument: false where it is neither None nor a tensor
 bool optional(PyObject* o, const at::Tensor*& t) { t = o == Py_None ? nullptr : tensor_of(o); return o == Py_None || t != nullptr; }
 
-// rms_norm(x, weight, eps, residual or None, quantize, stream)
+// rms_norm(x, weight, eps, residual or None, quantize (0: no, 1: to e4m3, 2: to int8), stream)
 PyObject* rms_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   const at::Tensor *x, *w, *r;
   if (nargs != 6 || f_norm == nullptr || !THPVariable_CheckExact(args[0]) || !optional(args[1], w) || w == nullptr || !optional(args[3], r)) Py_RETURN_NONE;
   x = tensor_of(args[0]);
   const double eps = PyFloat_AsDouble(args[2]);
-  const int quantize = PyObject_IsTrue(args[4]);
+  const long quantize = PyLong_AsLong(args[4]);
   void* stream = PyLong_AsVoidPtr(args[5]);
   if (PyErr_Occurred()) return nullptr;
-  if (!x->is_cuda() || x->dim() < 1 || !float_of(*x) || x->numel() == 0) Py_RETURN_NONE;
+  if (!x->is_cuda() || x->dim() < 1 || !float_of(*x) || x->numel() == 0 || quantize < 0 || quantize > 2) Py_RETURN_NONE;
   const c10::Device dev = x->device();
   const int64_t n = x->size(-1), rows = x->numel() / n;
-  if (!plain(*x, dev) || !plain(*w, dev) || w->scalar_type() != x->scalar_type() || w->dim() != 1 || w->size(0) != n || (quantize && n % 128) || n > (1 << 30)) Py_RETURN_NONE;
+  if (!plain(*x, dev) || !plain(*w, dev) || w->scalar_type() != x->scalar_type() || w->dim() != 1 || w->size(0) != n || (quantize && n % (quantize == 2 ? 16 : 128)) || n > (1 << 30)) Py_RETURN_NONE;
   if (r != nullptr && (!plain(*r, dev) || r->scalar_type() != x->scalar_type() || r->sizes() != x->sizes())) Py_RETURN_NONE;
   at::Tensor y, s, t;
   int rc;
   {
     pybind11::gil_scoped_release no_lock;      // as in linear()
     c10::DeviceGuard guard(dev);
-    y = at::empty(x->sizes(), quantize ? x->options().dtype(at::kFloat8_e4m3fn) : x->options());
+    y = at::empty(x->sizes(), quantize ? x->options().dtype(quantize == 2 ? at::kChar : at::kFloat8_e4m3fn) : x->options());
     if (quantize) {
       at::DimVector shape(x->sizes().begin(), x->sizes().end());
-      shape.back() = n / 128;
+      if (quantize == 2) shape.pop_back(); else shape.back() = n / 128;
       s = at::empty(shape, x->options().dtype(at::kFloat));
     }
     if (r != nullptr) t = at::empty(x->sizes(), x->options());
-    rc = f_norm(x->const_data_ptr(), n, r == nullptr ? nullptr : r->const_data_ptr(), n, w->const_data_ptr(), rows, (int)n, eps, dtype_code(x->scalar_type()),
+    rc = (quantize == 2 ? f_norm_int8 : f_norm)(x->const_data_ptr(), n, r == nullptr ? nullptr : r->const_data_ptr(), n, w->const_data_ptr(), rows, (int)n, eps, dtype_code(x->scalar_type()),
                 y.mutable_data_ptr(), quantize ? s.mutable_data_ptr() : nullptr, r == nullptr ? nullptr : t.mutable_data_ptr(), stream);
   }
   if (rc != HTR_OK) Py_RETURN_NONE;
@@ -303,7 +315,7 @@ PyObject* rms_norm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-// product(x, its scales or None, weight, its scales or None, bias or None, ends or None, the result's type code, stream): linear_fp8 where ends is None,
+// product(x, its scales or None, weight, its scales or None, bias or None, ends or None, the result's type code, stream): linear_fp8 or linear_int8 where ends is None,
 // otherwise grouped_mm
 PyObject* product(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
@@ -323,7 +335,7 @@ PyObject* product(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (x->size(-1) != n || !plain(*x, dev) || !plain(*w, dev) || m > (1 << 30) || n > (1 << 30) || experts > (1 << 30)) Py_RETURN_NONE;
   if (ends != nullptr && (x->dim() != 2 || ends->scalar_type() != at::kInt || ends->dim() != 1 || ends->size(0) != experts || ends->device() != dev || !ends->is_contiguous()))
     Py_RETURN_NONE;
-  if (eight ? w->scalar_type() != at::kFloat8_e4m3fn || !scales_ok(*w, *ws, false) || ws->device() != dev || !ws->is_contiguous() || differentiable(*ws)
+  if (eight ? (w->scalar_type() != at::kFloat8_e4m3fn && w->scalar_type() != at::kChar) || !scales_ok(*w, *ws, false) || ws->device() != dev || !ws->is_contiguous() || differentiable(*ws)
             : ends == nullptr || xs != nullptr || !half_of(*w) || x->scalar_type() != w->scalar_type() || n % 8)
     Py_RETURN_NONE;
   if (bias != nullptr && (ends != nullptr || bias->scalar_type() != type_of(code) || bias->dim() != 1 || bias->size(0) != m || bias->device() != dev ||
@@ -335,17 +347,17 @@ PyObject* product(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     pybind11::gil_scoped_release no_lock;      // as in linear()
     c10::DeviceGuard guard(dev);
     // few 16-bit rows are rounded by the product itself
-    const bool as_is = !eight || (xs == nullptr && half_of(*x) && f_rounds(x->numel() / n, (int)experts, ends != nullptr));
+    const bool as_is = !eight || (xs == nullptr && w->scalar_type() == at::kFloat8_e4m3fn && half_of(*x) && f_rounds(x->numel() / n, (int)experts, ends != nullptr));
     if (as_is) q = *x;
-    if (!as_is && !rows8(*x, xs, dev, stream, q, qs, rc)) {
+    if (!as_is && !rows8(*x, xs, w->scalar_type(), dev, stream, q, qs, rc)) {
       rc = HTR_ERR_SIZE;
     } else {
       at::DimVector shape(x->sizes().begin(), x->sizes().end());
       shape.back() = m;
       y = at::empty(shape, x->options().dtype(type_of(code)));
-      rc = f_product(q.const_data_ptr(), as_is ? dtype_code(x->scalar_type()) : HTR_E4M3, as_is ? nullptr : qs.const_data_ptr(), w->const_data_ptr(), eight ? ws->const_data_ptr() : nullptr,
+      rc = f_product(q.const_data_ptr(), type_code(q.scalar_type()), as_is ? nullptr : qs.const_data_ptr(), w->const_data_ptr(), eight ? ws->const_data_ptr() : nullptr,
                      bias == nullptr ? nullptr : bias->const_data_ptr(), ends == nullptr ? nullptr : (const int32_t*)ends->const_data_ptr(), y.mutable_data_ptr(),
-                     x->numel() / n, (int)m, (int)n, (int)experts, eight ? HTR_E4M3 : dtype_code(w->scalar_type()), (int)code, stream);
+                     x->numel() / n, (int)m, (int)n, (int)experts, type_code(w->scalar_type()), (int)code, stream);
     }
   }
   if (rc != HTR_OK) Py_RETURN_NONE;
@@ -370,8 +382,9 @@ PyObject* moe_stacked(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (!plain(x, dev) || !plain(gu, dev) || !plain(dn, dev) || dn.size(1) != H || gu.size(0) != E || gu.size(1) != 2 * F || gu.size(2) != H || F < 1 || E < 1) Py_RETURN_NONE;
   if (E > (1 << 20) || F > (1 << 28) || H > (1 << 28) || top > (1 << 20)) Py_RETURN_NONE;
   if (eight) {
+    if (gu.scalar_type() != at::kFloat8_e4m3fn && gu.scalar_type() != at::kChar) Py_RETURN_NONE;
     for (int i = 3; i < 7; i += 2)
-      if (t[i]->scalar_type() != at::kFloat8_e4m3fn || !scales_ok(*t[i], *t[i + 1], false) || t[i + 1]->device() != dev || !t[i + 1]->is_contiguous() || differentiable(*t[i + 1]))
+      if (t[i]->scalar_type() != gu.scalar_type() || !scales_ok(*t[i], *t[i + 1], false) || t[i + 1]->device() != dev || !t[i + 1]->is_contiguous() || differentiable(*t[i + 1]))
         Py_RETURN_NONE;
   } else if (gu.scalar_type() != x.scalar_type() || dn.scalar_type() != x.scalar_type()) {
     Py_RETURN_NONE;
@@ -380,7 +393,7 @@ PyObject* moe_stacked(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       (ids.scalar_type() != at::kLong && ids.scalar_type() != at::kInt) || wt.device() != dev || wt.scalar_type() != at::kFloat || !wt.is_contiguous() || !raw_ok(wt) ||
       differentiable(wt))
     Py_RETURN_NONE;
-  const int dtype = dtype_code(x.scalar_type()), type = eight ? HTR_E4M3 : dtype;
+  const int dtype = dtype_code(x.scalar_type()), type = type_code(gu.scalar_type());
   const size_t need = f_stacked_bytes(T, (int)top, (int)E, (int)H, (int)F, type);
   if (need == 0) Py_RETURN_NONE;
   at::Tensor y;
@@ -400,14 +413,55 @@ PyObject* moe_stacked(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-// bind_unpacked(addresses of htr_rms_norm, htr_quantize_e4m3, htr_product, htr_product_rounds, htr_moe_stacked_scratch_bytes, htr_moe_stacked), after bind()
+// route(logits, top, "softmax" or "sigmoid", bias or None, groups, top_groups, group_best, renormalize, scale, stream)
+PyObject* route(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  const at::Tensor* bias;
+  if (nargs != 10 || f_experts == nullptr || !THPVariable_CheckExact(args[0]) || !PyUnicode_Check(args[2]) || !optional(args[3], bias)) Py_RETURN_NONE;
+  for (int i : {1, 4, 5, 6}) if (!PyLong_Check(args[i])) Py_RETURN_NONE;
+  const at::Tensor& x = *tensor_of(args[0]);
+  const bool sigmoid = PyUnicode_CompareWithASCIIString(args[2], "sigmoid") == 0;
+  if (!sigmoid && PyUnicode_CompareWithASCIIString(args[2], "softmax") != 0) Py_RETURN_NONE;
+  const long top = PyLong_AsLong(args[1]), groups = PyLong_AsLong(args[4]), top_groups = PyLong_AsLong(args[5]), best = PyLong_AsLong(args[6]);
+  const int renormalize = PyObject_IsTrue(args[7]);
+  const double scale = PyFloat_AsDouble(args[8]);
+  void* stream = PyLong_AsVoidPtr(args[9]);
+  if (PyErr_Occurred()) return nullptr;
+  if (!x.is_cuda() || x.dim() < 1 || !float_of(x) || x.numel() == 0 || !raw_ok(x) || !x.is_contiguous() || differentiable(x)) Py_RETURN_NONE;
+  const c10::Device dev = x.device();
+  const int64_t E = x.size(-1);
+  if (E > (1 << 20) || top < 1 || top > E || groups < 1 || groups > E || top_groups < 1 || top_groups > groups || best < 1 || best > 2) Py_RETURN_NONE;
+  if (bias != nullptr && (bias->device() != dev || bias->scalar_type() != at::kFloat || bias->dim() != 1 || bias->size(0) != E || !bias->is_contiguous() || !raw_ok(*bias) ||
+                          differentiable(*bias)))
+    Py_RETURN_NONE;
+  at::Tensor ids, weights;
+  int rc;
+  {
+    pybind11::gil_scoped_release no_lock;      // as in linear()
+    c10::DeviceGuard guard(dev);
+    at::DimVector shape(x.sizes().begin(), x.sizes().end());
+    shape.back() = top;
+    ids = at::empty(shape, x.options().dtype(at::kInt));
+    weights = at::empty(shape, x.options().dtype(at::kFloat));
+    rc = f_experts(x.const_data_ptr(), E, dtype_code(x.scalar_type()), x.numel() / E, (int)E, (int)top, sigmoid, bias == nullptr ? nullptr : (const float*)bias->const_data_ptr(),
+                   (int)groups, (int)top_groups, (int)best, renormalize, scale, (int32_t*)ids.mutable_data_ptr(), (float*)weights.mutable_data_ptr(), stream);
+  }
+  if (rc != HTR_OK) Py_RETURN_NONE;
+  PyObject* first = THPVariable_Wrap(std::move(ids));
+  return PyTuple_Pack(2, Owned{first}.p, Owned{THPVariable_Wrap(std::move(weights))}.p);
+  END_HANDLE_TH_ERRORS
+}
+
+// bind_unpacked(addresses of htr_rms_norm, htr_quantize_e4m3, htr_product, htr_product_rounds, htr_moe_stacked_scratch_bytes, htr_moe_stacked, htr_rms_norm_int8,
+// htr_quantize_int8, htr_route), after bind()
 PyObject* bind_unpacked(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
-  if (nargs != 6) { PyErr_SetString(PyExc_TypeError, "bind_unpacked wants six addresses"); return nullptr; }
-  void* p[6];
-  for (int i = 0; i < 6; ++i) p[i] = PyLong_AsVoidPtr(args[i]);
+  if (nargs != 9) { PyErr_SetString(PyExc_TypeError, "bind_unpacked wants nine addresses"); return nullptr; }
+  void* p[9];
+  for (int i = 0; i < 9; ++i) p[i] = PyLong_AsVoidPtr(args[i]);
   if (PyErr_Occurred()) return nullptr;
   f_norm = (decltype(f_norm))p[0]; f_quantize = (decltype(f_quantize))p[1]; f_product = (decltype(f_product))p[2];
   f_rounds = (decltype(f_rounds))p[3]; f_stacked_bytes = (decltype(f_stacked_bytes))p[4]; f_stacked = (decltype(f_stacked))p[5];
+  f_norm_int8 = (decltype(f_norm_int8))p[6]; f_quantize_int8 = (decltype(f_quantize_int8))p[7]; f_experts = (decltype(f_experts))p[8];
   Py_RETURN_NONE;
 }
 
@@ -435,6 +489,7 @@ PyMethodDef methods[] = {{"bind", (PyCFunction)(void*)bind, METH_FASTCALL, nullp
                          {"bind_unpacked", (PyCFunction)(void*)bind_unpacked, METH_FASTCALL, nullptr},
                          {"rms_norm", (PyCFunction)(void*)rms_norm, METH_FASTCALL, nullptr},
                          {"product", (PyCFunction)(void*)product, METH_FASTCALL, nullptr},
+                         {"route", (PyCFunction)(void*)route, METH_FASTCALL, nullptr},
                          {"moe_stacked", (PyCFunction)(void*)moe_stacked, METH_FASTCALL, nullptr},
                          {"wait_word", (PyCFunction)(void*)wait_word, METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};

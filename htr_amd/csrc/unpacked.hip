@@ -1,5 +1,5 @@
 // Kernels for MI355X (gfx950) around the packed linears, behind the same C ABI: the norm in front of them, and products with matrices that a
-// checkpoint keeps in 16 bits or in e4m3 with block scales, whole or by expert.  Own translation unit: the packed kernels take two minutes to
+// checkpoint keeps in 16 bits, in e4m3 with block scales or in int8 with a scale for each channel, whole or by expert, and the router of experts.  Own translation unit: the packed kernels take two minutes to
 // compile, these a few seconds.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -19,6 +19,8 @@ namespace {
 #include "norm.hpp"
 #include "product.hpp"
 #include "experts.hpp"
+#include "int8.hpp"
+#include "route.hpp"
 
 #define TRY_HIP(EXPR) do { const hipError_t e_ = (EXPR); if (e_ != hipSuccess) return htr_note_hip_error((int)e_); } while (0)
 
@@ -44,7 +46,8 @@ template <auto Kernel> hipError_t allow_lds(size_t bytes) {
 
 bool is_16bit(int dtype) { return dtype == HTR_BF16 || dtype == HTR_F16; }
 bool is_dtype(int dtype) { return is_16bit(dtype) || dtype == HTR_F32; }
-size_t element_bytes(int dtype) { return dtype == HTR_F32 ? 4 : dtype == HTR_E4M3 ? 1 : 2; }
+bool is_8bit(int type) { return type == HTR_E4M3 || type == HTR_I8; }
+size_t element_bytes(int dtype) { return dtype == HTR_F32 ? 4 : is_8bit(dtype) ? 1 : 2; }
 bool aligned(const void* p, size_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
 
 // ---- norm
@@ -88,6 +91,29 @@ hipError_t launch_quantize(const void* x, int dtype, long long rows, int n, long
   if (dtype == HTR_BF16) return launch(k_quantize<HTR_BF16>, grid, 256, 0, st, x, stride, blocks, per_row, (uint8_t*)q, scales);
   if (dtype == HTR_F16) return launch(k_quantize<HTR_F16>, grid, 256, 0, st, x, stride, blocks, per_row, (uint8_t*)q, scales);
   return launch(k_quantize<HTR_F32>, grid, 256, 0, st, x, stride, blocks, per_row, (uint8_t*)q, scales);
+}
+
+// ---- rows to int8: one workgroup to a row, one, two or four runs of eight columns to a thread
+template <typename F> hipError_t by_runs(int n, F take) {
+  const int eights = n / 8, nv = eights <= 1024 ? 1 : eights <= 2048 ? 2 : 4;
+  if (n > I8_MOST) return take(std::integral_constant<int, 0>(), 1024u);
+  const unsigned threads = ((eights + nv - 1) / nv + 63) / 64 * 64;
+  return nv == 1 ? take(std::integral_constant<int, 1>(), threads) : nv == 2 ? take(std::integral_constant<int, 2>(), threads) : take(std::integral_constant<int, 4>(), threads);
+}
+template <int T, bool G> hipError_t launch_round(const void* x, long long stride, long long rows, int n, const int* last, void* q, void* scales, hipStream_t st) {
+  return by_runs(n, [&](auto nv, unsigned threads) {
+    return launch(k_round_rows<T, decltype(nv)::value, G>, dim3((unsigned)rows), threads, 0, st, x, stride, n, last, (uint8_t*)q, (float*)scales);
+  });
+}
+hipError_t launch_round(const void* x, int dtype, long long stride, long long rows, int n, void* q, void* scales, hipStream_t st) {
+  return dtype == HTR_BF16 ? launch_round<HTR_BF16, false>(x, stride, rows, n, nullptr, q, scales, st)
+         : dtype == HTR_F16 ? launch_round<HTR_F16, false>(x, stride, rows, n, nullptr, q, scales, st)
+                            : launch_round<HTR_F32, false>(x, stride, rows, n, nullptr, q, scales, st);
+}
+template <int T> hipError_t launch_norm_int8(const NormArgs& a, hipStream_t st) {
+  return by_runs(a.n, [&](auto nv, unsigned threads) {
+    return launch(a.residual ? k_rms_norm_int8<T, decltype(nv)::value, true> : k_rms_norm_int8<T, decltype(nv)::value, false>, dim3((unsigned)a.rows), threads, 0, st, a);
+  });
 }
 
 // ---- products
@@ -192,7 +218,7 @@ template <int T, typename F> auto product_kernel(const ProductArgs& a, F take) {
     // 1536x2560 85 and 63, 48 of 24 of 3000x3000 122 and 80, 160 of 160 of 1024x1024 51 and 48).  Rows that all have one expert take less either way (256 rows of
     // 64 experts of 2816x2048 in e4m3 22 us, evenly 69).
     if (grouped && wgs >= 4 * 512) {
-      if constexpr (T == P_F8) return take(Stream<4, 1, 4>{});
+      if constexpr (T == P_F8 || T == P_I8) return take(Stream<4, 1, 4>{});
       return take(Tiles<2, 2, 2, 2, 4>{});
     }
     // Rows of fewer slabs than waves leave some idle (7 rows on 15657x384 in e4m3 5.5 us by 16 rows to a workgroup of 8 waves, 4.7 by 32 to one of 4), and rows
@@ -219,7 +245,7 @@ template <int T, typename F> auto product_kernel(const ProductArgs& a, F take) {
     // 512x4096 in e4m3 12.1 and 16.8, in 16 bits 19.6 and 26.7; of 512x768 4.4 and 6.1, 5.9 and 8.4; 1056 rows of 48 of 72x3200 in 16 bits 20.1 and 19.4)
     return y_fits && workgroups(16) <= 512.f ? take(Stream<1, 1, 8>{}) : take(Tiles<4, 1, 2, 2, 4>{});
   }
-  switch (T == P_F8 ? best_tile(TILES_8, a, (size_t)a.n) : best_tile(TILES_16, a, (size_t)a.n * 2)) {
+  switch (T == P_F8 || T == P_I8 ? best_tile(TILES_8, a, (size_t)a.n) : best_tile(TILES_16, a, (size_t)a.n * 2)) {
     case 0: return take(Tiles<2, 4, 8, 4, 2>{});
     case 1: return take(Tiles<4, 2, 4, 4, 3>{});
     case 2: return take(Tiles<2, 2, 4, 4, 3>{});
@@ -243,20 +269,23 @@ template <int T> hipError_t launch_product(const ProductArgs& a, bool gated, hip
   return gated ? gated_kernel<T>(a, take) : product_kernel<T>(a, take);
 }
 hipError_t launch_product(const ProductArgs& a, int type, bool gated, hipStream_t st) {
-  return type == HTR_E4M3 ? launch_product<P_F8>(a, gated, st) : type == HTR_BF16 ? launch_product<HTR_BF16>(a, gated, st) : launch_product<HTR_F16>(a, gated, st);
+  return type == HTR_E4M3 ? launch_product<P_F8>(a, gated, st) : type == HTR_I8 ? launch_product<P_I8>(a, gated, st) : type == HTR_BF16 ? launch_product<HTR_BF16>(a, gated, st) : launch_product<HTR_F16>(a, gated, st);
 }
 template <int T> void describe_product(const ProductArgs& a, bool gated, int* out) {
   auto take = [&](auto kernel) { describe_kernel<T>(kernel, a, out); };
   if (gated) gated_kernel<T>(a, take); else product_kernel<T>(a, take);
 }
+// columns: whole blocks of e4m3, rows on 16-byte boundaries
+int unit_of(int type) { return type == HTR_E4M3 ? 128 : type == HTR_I8 ? 16 : 8; }
 // what product_kernel takes: HTR_OK or the status to refuse with
 int product_shape(long long rows, int m, int n, int experts, int type, bool grouped) {
-  if (type != HTR_E4M3 && !is_16bit(type)) return HTR_ERR_DTYPE;
-  if (rows < 0 || rows > (1ll << 31) - (1 << 20) || m < 1 || n < 1 || experts < 1 || experts > 65535 || n % (type == HTR_E4M3 ? 128 : 8)) return HTR_ERR_SIZE;
+  if (!is_8bit(type) && !is_16bit(type)) return HTR_ERR_DTYPE;
+  if (rows < 0 || rows > (1ll << 31) - (1 << 20) || m < 1 || n < 1 || experts < 1 || experts > 65535 || n % unit_of(type)) return HTR_ERR_SIZE;
+  if (type == HTR_I8 && n >= 1 << 17) return HTR_ERR_SIZE;        // 2^14 a product, sums below 2^31
   if (m > (1 << 26) || n > (1 << 22)) return HTR_ERR_SIZE;       // 256 rows of a tile by 32-bit distances; the launch's threads below 2^32
   // numbers of the smallest tiles, and workgroups where there is one to a tile (rows of fewer slabs than the deepest ring has stages)
   const long long tiles = span_bound(rows, experts, grouped, 32) * ((m + 63) / 64);
-  return tiles > ((long long)n * (type == HTR_E4M3 ? 1 : 2) > 128 * 3 ? (1ll << 31) - (1 << 16) : 1ll << 23) ? HTR_ERR_SIZE : HTR_OK;
+  return tiles > ((long long)n * (is_8bit(type) ? 1 : 2) > 128 * 3 ? (1ll << 31) - (1 << 16) : 1ll << 23) ? HTR_ERR_SIZE : HTR_OK;
 }
 
 // ---- a routed-expert layer: scratch laid out one after the other, every part on a 256-byte boundary
@@ -266,26 +295,33 @@ struct StackedScratch {
     size_t at = 0;
     auto take = [&](size_t n) { const size_t here = at; at += (n + 255) / 256 * 256; return here; };
     const size_t pairs = (size_t)tokens * top;
-    const bool f8 = type == HTR_E4M3;
+    const bool f8 = type == HTR_E4M3, i8 = type == HTR_I8, in_one = gates_in_one(pairs, experts);
     ends = take((size_t)experts * 4);
     token = take(pairs * 4);
     pos_of = take(pairs * 4);
-    const bool ahead = f8 && gates_in_one(pairs, experts);      // x is rounded by a launch of its own
+    const bool ahead = i8 || (f8 && in_one);      // x is rounded by a launch of its own
     xq = take(ahead ? (size_t)tokens * hidden : 0);
-    xs = take(ahead ? (size_t)tokens * (hidden / 128) * 4 : 0);
-    h = take(gates_in_one(pairs, experts) ? 0 : pairs * 2 * inter * 4);
-    a = take(pairs * inter * (f8 ? 1 : 2));
-    as = take(f8 ? pairs * (inter / 128) * 4 : 0);
+    xs = take(i8 ? (size_t)tokens * 4 : ahead ? (size_t)tokens * (hidden / 128) * 4 : 0);
+    h = take(!in_one ? pairs * 2 * inter * 4 : i8 ? pairs * inter * 4 : 0);
+    a = take(pairs * inter * (f8 || i8 ? 1 : 2));
+    as = take(i8 ? pairs * 4 : f8 ? pairs * (inter / 128) * 4 : 0);
     out = take(pairs * hidden * 4);
     bytes = at;
   }
 };
+hipError_t launch_route(const RouteArgs& a, hipStream_t st) {
+  const dim3 grid((unsigned)((a.tokens + ROUTE_WAVES - 1) / ROUTE_WAVES));
+  const int per = (a.experts + 63) / 64;
+  return per <= 1 ? launch(k_route<1>, grid, ROUTE_WAVES * 64, 0, st, a) : per <= 2 ? launch(k_route<2>, grid, ROUTE_WAVES * 64, 0, st, a)
+         : per <= 4 ? launch(k_route<4>, grid, ROUTE_WAVES * 64, 0, st, a) : per <= 8 ? launch(k_route<8>, grid, ROUTE_WAVES * 64, 0, st, a)
+                    : launch(k_route<16>, grid, ROUTE_WAVES * 64, 0, st, a);
+}
 int stacked_shape(long long tokens, int top, int experts, int hidden, int inter, int type) {
   if (tokens < 1 || top < 1 || experts < 1 || hidden < 1 || inter < 1 || top > 4096 || tokens >= (1 << 24) || inter > (1 << 28)) return HTR_ERR_SIZE;
-  if (type != HTR_E4M3 && !is_16bit(type)) return HTR_ERR_DTYPE;
-  if (hidden % 8 || inter % (type == HTR_E4M3 ? 128 : 8)) return HTR_ERR_SIZE;
+  if (!is_8bit(type) && !is_16bit(type)) return HTR_ERR_DTYPE;
+  if (hidden % 8 || inter % unit_of(type)) return HTR_ERR_SIZE;
   // loads go by 32-bit distances from x, from the gathered rows' scales and from an expert's matrices
-  const unsigned long long size = type == HTR_E4M3 ? 1 : 2, most = 1ull << 32;
+  const unsigned long long size = is_8bit(type) ? 1 : 2, most = 1ull << 32;
   if (tokens * top > (1 << 30) || (unsigned long long)tokens * hidden * size >= most || 2ull * inter * hidden * size >= most) return HTR_ERR_SIZE;
   const int rc = product_shape(tokens * top, 2 * inter, hidden, experts, type, true);
   return rc != HTR_OK ? rc : product_shape(tokens * top, hidden, inter, experts, type, true);
@@ -318,6 +354,39 @@ int htr_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t 
   return HTR_OK;
 }
 
+int htr_rms_norm_int8(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, const void* weight, int64_t rows, int n, double eps,
+                      int dtype, void* y, void* scales, void* sum, void* stream) {
+  if (rows < 0 || rows > 0x7FFFFFFF || n < 1 || n > (1 << 30) || n % 16) return HTR_ERR_SIZE;
+  if (!is_dtype(dtype)) return HTR_ERR_DTYPE;
+  if (rows == 0) return HTR_OK;
+  if (!x || !weight || !y || !scales || (residual != nullptr) != (sum != nullptr)) return HTR_ERR_NULL;
+  const size_t size = element_bytes(dtype);
+  if (!aligned(x, size) || !aligned(residual, size) || !aligned(weight, size) || !aligned(sum, size) || !aligned(scales, 4)) return HTR_ERR_ALIGN;
+  hipStream_t st = (hipStream_t)stream;
+  constexpr int64_t MOST = 1 << 21;      // as in htr_rms_norm
+  for (int64_t r = 0; r < rows; r += MOST) {
+    const int64_t count = rows - r < MOST ? rows - r : MOST;
+    auto at = [&](const void* p, int64_t elements, size_t bytes) { return p ? (void*)((uint8_t*)p + elements * (int64_t)bytes) : nullptr; };
+    const NormArgs a{at(x, r * x_stride, size), at(residual, r * residual_stride, size), weight, at(y, r * n, 1), at(sum, r * n, size), (float*)scales + r,
+                     x_stride, residual_stride, count, n, eps};
+    TRY_HIP(dtype == HTR_BF16 ? launch_norm_int8<HTR_BF16>(a, st) : dtype == HTR_F16 ? launch_norm_int8<HTR_F16>(a, st) : launch_norm_int8<HTR_F32>(a, st));
+  }
+  return HTR_OK;
+}
+
+int htr_quantize_int8(const void* x, int64_t stride, int64_t rows, int n, int dtype, void* q, void* scales, void* stream) {
+  if (rows < 0 || n < 1 || n % 16 || n > (1 << 30)) return HTR_ERR_SIZE;
+  if (!is_dtype(dtype)) return HTR_ERR_DTYPE;
+  if (rows == 0) return HTR_OK;
+  if (!x || !q || !scales) return HTR_ERR_NULL;
+  if (!aligned(x, element_bytes(dtype)) || !aligned(q, 8) || !aligned(scales, 4)) return HTR_ERR_ALIGN;
+  constexpr int64_t MOST = 1 << 21;
+  for (int64_t r = 0; r < rows; r += MOST)
+    TRY_HIP(launch_round((const uint8_t*)x + r * stride * (int64_t)element_bytes(dtype), dtype, stride, rows - r < MOST ? rows - r : MOST, n, (uint8_t*)q + r * n,
+                         (float*)scales + r, (hipStream_t)stream));
+  return HTR_OK;
+}
+
 int htr_quantize_e4m3(const void* x, int64_t stride, int64_t rows, int n, int dtype, void* q, void* scales, void* stream) {
   if (rows < 0 || n < 1 || n % 128 || n > (1 << 30)) return HTR_ERR_SIZE;
   if (!is_dtype(dtype)) return HTR_ERR_DTYPE;
@@ -338,12 +407,13 @@ int htr_product_plan(int64_t rows, int m, int n, int experts, int grouped, int g
   const int rc = product_shape(rows, m, n, experts, type, grouped != 0);
   if (rc != HTR_OK) return rc;
   if (x_type != type && !(type == HTR_E4M3 && is_16bit(x_type) && !gated && takes_16bit_rows(rows, experts, grouped != 0))) return HTR_ERR_DTYPE;
-  if (rows == 0 || (gated && (!grouped || m % (type == HTR_E4M3 ? 256 : 16) || !gates_in_one(rows, experts))) || (!grouped && experts != 1)) return HTR_ERR_SIZE;
+  if (rows == 0 || (gated && (!grouped || m % (2 * unit_of(type)) || !gates_in_one(rows, experts))) || (!grouped && experts != 1)) return HTR_ERR_SIZE;
   const int some = 0;      // the choice asks whether there are ends, not what they hold
   ProductArgs a{};
   a.rows = (int)rows; a.m = m; a.n = n; a.experts = experts; a.x_type = x_type;
   a.ends = grouped ? &some : nullptr;
   if (type == HTR_E4M3) describe_product<P_F8>(a, gated != 0, out6);
+  else if (type == HTR_I8) describe_product<P_I8>(a, gated != 0, out6);
   else if (type == HTR_BF16) describe_product<HTR_BF16>(a, gated != 0, out6);
   else describe_product<HTR_F16>(a, gated != 0, out6);
   return HTR_OK;
@@ -357,7 +427,7 @@ int htr_product(const void* x, int x_type, const void* x_scales, const void* w, 
   if (x_type != type && !(type == HTR_E4M3 && is_16bit(x_type) && takes_16bit_rows(rows, experts, ends != nullptr))) return HTR_ERR_DTYPE;
   if (ends == nullptr && experts != 1) return HTR_ERR_NULL;
   if (rows == 0) return HTR_OK;
-  if (!x || !w || !y || (x_type == HTR_E4M3 && !x_scales) || (type == HTR_E4M3 && !w_scales)) return HTR_ERR_NULL;
+  if (!x || !w || !y || (is_8bit(x_type) && !x_scales) || (is_8bit(type) && !w_scales)) return HTR_ERR_NULL;
   if (!aligned(x, 16) || !aligned(w, 16) || !aligned(y, 16) || !aligned(x_scales, 4) || !aligned(w_scales, 4) || !aligned(ends, 4) ||
       !aligned(bias, element_bytes(y_dtype)))
     return HTR_ERR_ALIGN;
@@ -375,9 +445,9 @@ int htr_moe_stacked(const void* x, int dtype, const void* ids, int ids_int64, co
                     void* scratch, size_t scratch_bytes, void* stream) {
   const int rc = stacked_shape(tokens, top, experts, hidden, inter, type);
   if (rc != HTR_OK) return rc;
-  if (!is_16bit(dtype) || (type != HTR_E4M3 && type != dtype)) return HTR_ERR_DTYPE;
-  const bool f8 = type == HTR_E4M3;
-  if (!x || !ids || !weights || !gate_up || !down || !y || (f8 && (!gate_up_scales || !down_scales))) return HTR_ERR_NULL;
+  if (!is_16bit(dtype) || (!is_8bit(type) && type != dtype)) return HTR_ERR_DTYPE;
+  const bool f8 = type == HTR_E4M3, i8 = type == HTR_I8;
+  if (!x || !ids || !weights || !gate_up || !down || !y || ((f8 || i8) && (!gate_up_scales || !down_scales))) return HTR_ERR_NULL;
   if (!aligned(x, 16) || !aligned(gate_up, 16) || !aligned(down, 16) || !aligned(y, 16) || !aligned(ids, ids_int64 ? 8 : 4) || !aligned(weights, 4) ||
       !aligned(gate_up_scales, 4) || !aligned(down_scales, 4))
     return HTR_ERR_ALIGN;
@@ -390,12 +460,23 @@ int htr_moe_stacked(const void* x, int dtype, const void* ids, int ids_int64, co
   float *h = (float*)(s + at.h), *out = (float*)(s + at.out);
   TRY_HIP(launch(k_expert_order, dim3(experts), ORDER_WAVES * 64, 0, st, ids, ids_int64, pairs, top, experts, ends, token, pos_of));
   ProductArgs a{x, nullptr, gate_up, (const float*)gate_up_scales, nullptr, h, ends, token, pairs, 2 * inter, hidden, experts, HTR_F32, dtype, nullptr, f8};
-  if (f8 && gates_in_one(pairs, experts)) {
+  if (i8) {
+    a.x_type = HTR_I8;
+    TRY_HIP(launch_round(x, dtype, hidden, tokens, hidden, s + at.xq, s + at.xs, st));
+    a.x = s + at.xq; a.xs = (const float*)(s + at.xs);
+  } else if (f8 && gates_in_one(pairs, experts)) {
     a.x_type = HTR_E4M3;
     TRY_HIP(launch_quantize(x, dtype, tokens, hidden, hidden, s + at.xq, (float*)(s + at.xs), st));
     a.x = s + at.xq; a.xs = (const float*)(s + at.xs);
   }
-  if (gates_in_one(pairs, experts)) {
+  if (i8) {
+    // silu(gate) up stays float32 until a row's largest is known
+    const bool in_one = gates_in_one(pairs, experts);
+    TRY_HIP(launch_product(a, type, in_one, st));
+    const int* last = ends + experts - 1;
+    TRY_HIP((in_one ? launch_round<HTR_F32, false>(h, inter, pairs, inter, last, s + at.a, s + at.as, st)
+                    : launch_round<HTR_F32, true>(h, 2 * inter, pairs, inter, last, s + at.a, s + at.as, st)));
+  } else if (gates_in_one(pairs, experts)) {
     a.y = s + at.a; a.ys = (float*)(s + at.as); a.y_dtype = type;
     TRY_HIP(launch_product(a, type, true, st));
   } else {
@@ -409,6 +490,23 @@ int htr_moe_stacked(const void* x, int dtype, const void* ids, int ids_int64, co
   const dim3 grid((unsigned)tokens, (hidden + 2047) / 2048);
   TRY_HIP(dtype == HTR_BF16 ? launch(k_weighted_sum<HTR_BF16>, grid, 256, 0, st, out, pos_of, weights, top, hidden, y)
                             : launch(k_weighted_sum<HTR_F16>, grid, 256, 0, st, out, pos_of, weights, top, hidden, y));
+  return HTR_OK;
+}
+
+int htr_route(const void* logits, int64_t stride, int dtype, int64_t tokens, int experts, int top, int sigmoid, const float* bias, int groups, int top_groups,
+              int group_best, int renormalize, double scale, int32_t* ids, float* weights, void* stream) {
+  if (tokens < 0 || tokens > 0x7FFFFFFF || experts < 1 || experts > ROUTE_MOST || top < 1 || top > experts || top > 64) return HTR_ERR_SIZE;
+  if (groups < 1 || groups > 64 || experts % groups || top_groups < 1 || top_groups > groups || group_best < 1 || group_best > 2 || top > experts / groups * top_groups) return HTR_ERR_SIZE;
+  if (!is_dtype(dtype)) return HTR_ERR_DTYPE;
+  if (tokens == 0) return HTR_OK;
+  if (!logits || !ids || !weights) return HTR_ERR_NULL;
+  if (!aligned(logits, element_bytes(dtype)) || !aligned(bias, 4) || !aligned(ids, 4) || !aligned(weights, 4)) return HTR_ERR_ALIGN;
+  constexpr int64_t MOST = 1 << 22;      // a launch has fewer than 2^32 threads, 64 of them to a token
+  for (int64_t t = 0; t < tokens; t += MOST) {
+    const RouteArgs a{(const uint8_t*)logits + t * stride * (int64_t)element_bytes(dtype), bias, ids + t * top, weights + t * top, stride, tokens - t < MOST ? tokens - t : MOST,
+                      dtype, experts, top, sigmoid, groups, top_groups, group_best, renormalize, scale};
+    TRY_HIP(launch_route(a, (hipStream_t)stream));
+  }
   return HTR_OK;
 }
 }  // extern "C"

@@ -45,6 +45,8 @@ typedef enum {
 enum { HTR_BF16 = 0, HTR_F16 = 1, HTR_F32 = 2 };
 /* operands of the products outside HTR-W1: OCP e4m3 (one byte, no infinities) */
 enum { HTR_E4M3 = 3 };
+/* or 8-bit integers with one scale for each row */
+enum { HTR_I8 = 4 };
 
 #define HTR_ABI_VERSION 2      /* what htr_abi_version returns */
 #define HTR_MAX_BATCH 2048      /* activation rows one htr_linear launch accepts */
@@ -314,6 +316,10 @@ int htr_dequant_w(const void* qweight, const void* scales, const void* su, const
  * The scales that these calls make are powers of two, the least from amax / 448 up (amax: the block's largest finite magnitude, at least
  * 2^-100); scales they are given need not be.  Infinities and NaN become NaN.
  *
+ * int8 rows carry one float32 scale each, [rows]; int8 matrices one for each of their rows (channels), [experts][m].  The scales that these calls make are
+ * amax / 127 in float32 (amax: the row's largest magnitude, at least 2^-100), the values the quotients by them to the nearest integer, halves away from
+ * zero.  A row with an infinity or NaN, or whose scale float32 cannot hold, gets the scale NaN and the values 0.
+ *
  * htr_rms_norm: t = round(x + residual), y = t weight / sqrt(mean(t^2) + eps), the mean in 64 bits.
  *   x, residual  [rows][n] of dtype with that many elements from row to row; residual may be NULL (then sum is, too: t = x)
  *   weight       [n] of dtype
@@ -324,6 +330,13 @@ int htr_dequant_w(const void* qweight, const void* scales, const void* su, const
 int htr_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, const void* weight, int64_t rows, int n, double eps,
                  int dtype, void* y, void* scales, void* sum, void* stream);
 
+/* The same to int8: y int8 [rows][n], scales [rows] (never NULL), n a multiple of 16. */
+int htr_rms_norm_int8(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, const void* weight, int64_t rows, int n, double eps,
+                      int dtype, void* y, void* scales, void* sum, void* stream);
+
+/* Rows [rows][n] of dtype, `stride` elements apart, to int8 [rows][n] (8-byte aligned) with scales [rows].  n a multiple of 16. */
+int htr_quantize_int8(const void* x, int64_t stride, int64_t rows, int n, int dtype, void* q, void* scales, void* stream);
+
 /* Rows [rows][n] of dtype, `stride` elements apart, to e4m3 [rows][n] with scales [rows][n / 128].  n a multiple of 128, x on a 16-byte boundary,
  * stride a multiple of 8. */
 int htr_quantize_e4m3(const void* x, int64_t stride, int64_t rows, int n, int dtype, void* q, void* scales, void* stream);
@@ -332,9 +345,10 @@ int htr_quantize_e4m3(const void* x, int64_t stride, int64_t rows, int n, int dt
  * y[r] = W_e x[r] (+ bias), e the expert of row r.  Sums are float32, except that products of e4m3 values are first added eight consecutive columns at
  * a time: each eight is off by at most 2^-10 of the largest magnitude in x times that in w (a magnitude below 2^-6 of its scale counts as that).  The
  * product of a row's scale and a block's is float32 as well: one below 2^-126 has fewer bits, one beyond float32 is infinite, and NaN times a zero.
- *   type    of w: HTR_E4M3 (with its scales), HTR_BF16 or HTR_F16 (scales NULL)
+ * Sums of int8 products are exact; they are converted to float32, then multiplied with the row's and with the channel's scale.
+ *   type    of w: HTR_E4M3 or HTR_I8 (with its scales), HTR_BF16 or HTR_F16 (scales NULL)
  *   x_type  type; with e4m3 matrices also HTR_BF16 or HTR_F16 (x_scales NULL) where htr_product_rounds says so: rounded as by htr_quantize_e4m3
- *   x       [rows][n], w [experts][m][n], 16-byte aligned; n a multiple of 128 (e4m3) or of 8 (16 bits), up to 2^22; m up to 2^26; experts up to 65535
+ *   x       [rows][n], w [experts][m][n], 16-byte aligned; n a multiple of 128 (e4m3), of 16 (int8, below 2^17) or of 8 (16 bits), up to 2^22; m up to 2^26; experts up to 65535
  *   ends    device int32 [experts]: expert e has rows ends[e - 1] .. ends[e] - 1 (from 0); rows from the last end on become zeros.  An end below
  *           an earlier one, or beyond rows, counts as that one, or as rows.  NULL: one matrix (experts = 1) for all rows
  *   bias    [m] of y_dtype or NULL;  y [rows][m], y_dtype any of the three, 16-byte aligned; it may overlap nothing that is read
@@ -353,17 +367,29 @@ int htr_product_plan(int64_t rows, int m, int n, int experts, int grouped, int g
 /*
  * A routed-expert layer on stacked matrices: y_t = sum_j w[t, j] Down_e( silu(Gate_e x_t) * Up_e x_t ), e = ids[t, j], sums as in htr_product, over j in
  * float32 and ascending, y of dtype (bf16 or f16).  Gate and up in e4m3 have float32 sums throughout, since they are rounded to e4m3 next, with up to 4 rows
- * to an expert on average and where htr_product_plan says tiles of up to 64 rows of x.  The hidden values between the products are rounded to dtype, or to e4m3 with scales.
- *   type     dtype, or HTR_E4M3 (x is then rounded to e4m3 as well)
+ * to an expert on average and where htr_product_plan says tiles of up to 64 rows of x.  The hidden values between the products are rounded to dtype, to e4m3 with scales, or by row to int8 (float32 until then).
+ *   type     dtype, or HTR_E4M3 or HTR_I8 (x is then rounded to it as well)
  *   gate_up  [experts][2 inter][hidden], gate rows first;  down [experts][hidden][inter];  scales as in htr_product, or NULL
  *   ids      [tokens][top] int32 or int64 and weights [tokens][top] float32, on the device; an expert out of range makes its token NaN
  *   scratch  htr_moe_stacked_scratch_bytes() bytes (0: sizes that are not taken), 256-byte aligned, of any content, used until the launches are done
- * hidden a multiple of 8 (e4m3: 128), inter too; x, and gate_up of one expert, of fewer than 2^32 bytes.  htr_moe_experts is this layer on HTR-W1 matrices.
+ * hidden a multiple of 8 (e4m3: 128, int8: 16), inter too; x, and gate_up of one expert, of fewer than 2^32 bytes.  htr_moe_experts is this layer on HTR-W1 matrices.
  */
 size_t htr_moe_stacked_scratch_bytes(int64_t tokens, int top, int experts, int hidden, int inter, int type);
 int htr_moe_stacked(const void* x, int dtype, const void* ids, int ids_int64, const float* weights, int64_t tokens, int top, const void* gate_up,
                     const void* gate_up_scales, const void* down, const void* down_scales, int experts, int hidden, int inter, int type, void* y,
                     void* scratch, size_t scratch_bytes, void* stream);
+
+/*
+ * Routing: ids [tokens][top] and weights [tokens][top] of each token's experts from a router's logits [tokens][experts] of dtype, `stride` elements from
+ * token to token, as htr_moe_stacked and htr_moe_experts take them.  Scores s_e = softmax_e(l), or 1 / (1 + exp(-l_e)) where sigmoid; experts in descending
+ * order of s_e + bias_e, without a bias (NULL) of l_e; ties go to the lowest number.  With groups > 1 (consecutive experts) only those of the best top_groups groups
+ * compete, a group being as good as the sum of its group_best (1 or 2) largest s_e + bias_e (one, without a bias: its largest l_e).  Weights are the scores,
+ * divided by their sum if renormalize, times scale.  Scores and sums in 64 bits.  A logit, or bias, of -inf masks an expert: behind all others, weight 0, also in a
+ * group's sum; a token without any other expert has weights 0.  NaN ranks first, and its weight is NaN.
+ * experts up to 1024, top up to 64 and to the experts of top_groups groups, groups up to 64 and a divisor of experts.
+ */
+int htr_route(const void* logits, int64_t stride, int dtype, int64_t tokens, int experts, int top, int sigmoid, const float* bias, int groups, int top_groups,
+              int group_best, int renormalize, double scale, int32_t* ids, float* weights, void* stream);
 
 /*
  * Timing anchors: measurement only, the results they leave in y are meaningless.  No reference counterpart (the
