@@ -6,7 +6,10 @@
 //
 // A logit or bias of -inf masks its expert: it comes behind every other, with weight 0; a token of which every expert is masked has weights 0.  NaN ranks first.
 // Scores and ranks are 64 bits: experts' ranks lie within 2^-24 of each other in one token of some thousand, and an expert taken for its neighbour is another result.
-constexpr int ROUTE_MOST = 1024, ROUTE_WAVES = 4;
+// One wave to a token.  Ranks that are logits are float32 as they are; others are first formed in float32, and only those that lie within what float32 may be off of each
+// other, or of what decides, are compared in 64 bits (Route); what that does not cover is done in 64 bits throughout (route_exact).  The weights of the chosen are
+// 64 bits either way.
+constexpr int ROUTE_MOST = 1024, ROUTE_WAVES = 4, ROUTE_TOGETHER = 4096;
 
 struct RouteArgs {
   const void* logits;                 // [tokens][experts], `stride` elements from token to token
@@ -16,6 +19,7 @@ struct RouteArgs {
   long long stride, tokens;
   int dtype, experts, top, sigmoid, groups, top_groups, group_best, renormalize;
   double scale;
+  int size, parts_log2;               // experts of a group, lanes to a group
 };
 
 // ranks as integers of the same order: -0 as 0, NaN (of either sign) above all
@@ -26,18 +30,23 @@ __device__ __forceinline__ long long order_of(double v) {
 }
 constexpr long long ORDER_MASKED = (long long)0x800FFFFFFFFFFFFFull;      // order_of(-inf)
 constexpr long long ORDER_NONE = (long long)0x8000000000000000ull;        // no expert, or one that is taken
+// the same of float32 that is not NaN, in unsigned numbers from 1 on (0: no expert)
+__device__ __forceinline__ uint32_t key_of(float v) {
+  const uint32_t u = __float_as_uint(v + 0.f);
+  return u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float value_of_key(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); }
+constexpr uint32_t KEY_MASKED = 0x007FFFFFu;                             // of -inf
+
 template <typename V> __device__ __forceinline__ V wave_largest(V v) {
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) { const V w = __shfl_xor(v, off); v = w > v ? w : v; }
   return v;
 }
+__device__ __forceinline__ double sigmoid64(float l) { return 1.0 / (1.0 + exp(-(double)l)); }
 
-// One wave to a token, PER consecutive experts to a lane
-template <int PER>
-__global__ __launch_bounds__(ROUTE_WAVES * 64) void k_route(const RouteArgs a) {
-  const int lane = threadIdx.x & 63;
-  const long long token = (long long)blockIdx.x * ROUTE_WAVES + (threadIdx.x >> 6);
-  if (token >= a.tokens) return;
+// ---- in 64 bits: PER consecutive experts to a lane, the largest taken one after the other
+template <int PER> __device__ __forceinline__ void route_exact(const RouteArgs& a, long long token, int lane) {
   double l[PER], score[PER], most = -INFINITY;
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
@@ -66,7 +75,7 @@ __global__ __launch_bounds__(ROUTE_WAVES * 64) void k_route(const RouteArgs a) {
     rank[j] = e >= a.experts ? ORDER_NONE : l[j] == -INFINITY ? ORDER_MASKED : order_of(a.bias != nullptr ? score[j] + (double)b : l[j]);
   }
   if (a.groups > 1) {
-    const int size = a.experts / a.groups;
+    const int size = a.size;
     long long mine = ORDER_NONE;                    // lane g: what ranks group g
     for (int g = 0; g < a.groups; ++g) {
       double sum = 0.0;
@@ -137,4 +146,275 @@ __global__ __launch_bounds__(ROUTE_WAVES * 64) void k_route(const RouteArgs a) {
     ((HTR_GLOBAL int*)a.ids)[token * a.top + lane] = id;
     ((HTR_GLOBAL float*)a.weights)[token * a.top + lane] = (float)(weight * a.scale);
   }
+}
+
+// ---- with float32 ranks.  Lanes in runs of `parts` = 2^parts_log2 to a group (without groups: all 64); element i of lane p of group g is expert g size + p + i parts.
+// The threshold between the chosen and the others is found by halving the span of ranks (as integers): a comparison and a count of lanes to each element, until exactly
+// `top` lie above it, which takes about ten steps; the largest one by one takes a wave's maximum for each.  Whatever lies next to the threshold is a candidate, too, and
+// candidates too close to each other are ordered by their ranks in 64 bits, groups likewise.
+struct Candidate { uint32_t key; int e; float l, b; };
+template <int H> __device__ __forceinline__ void two_largest(float& first, float& second) {      // with lane ^ H
+  const float f = lane_xor_dpp<H>(first), s = lane_xor_dpp<H>(second);
+  second = fmaxf(fmaxf(second, s), fminf(first, f));
+  first = fmaxf(first, f);
+}
+template <int PER> struct Route {
+  const RouteArgs& a;
+  const int lane, parts_log2, parts, g, p, e0;
+  const bool biased, scored;      // scored: some ranks are no logits
+  float l[PER], b[PER], most;     // a token's; most: the largest logit (softmax)
+  __device__ __forceinline__ Route(const RouteArgs& a, int lane)
+      : a(a), lane(lane), parts_log2(a.parts_log2), parts(1 << a.parts_log2), g(lane >> a.parts_log2), p(lane & ((1 << a.parts_log2) - 1)), e0(g * a.size + p),
+        biased(a.bias != nullptr), scored(a.bias != nullptr || (a.groups > 1 && a.group_best > 1)) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) b[i] = biased && in(i) ? ((const HTR_GLOBAL float*)a.bias)[e0 + i * parts] : 0.f;
+  }
+  __device__ __forceinline__ bool in(int i) const { return g < a.groups && p + i * parts < a.size; }
+  __device__ __forceinline__ void load(long long token, float (&to)[PER]) const {
+    const size_t row = (size_t)(token * a.stride) + e0;
+    auto from = [&](auto type) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) to[i] = in(i) ? load_elem_g(a.logits, decltype(type)::value, row + i * parts) : -INFINITY;
+    };
+    if (a.dtype == HTR_F32) from(std::integral_constant<int, HTR_F32>());
+    else if (a.dtype == HTR_BF16) from(std::integral_constant<int, HTR_BF16>());
+    else from(std::integral_constant<int, HTR_F16>());
+  }
+  __device__ __forceinline__ double all64() const {      // the softmax's sum
+    double total = 0.0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) total += l[i] == -INFINITY ? 0.0 : exp((double)l[i] - (double)most);
+    return wave_sum(total);
+  }
+
+  // The token's candidates: their number, at least `top`; 0 where ranks are no finite numbers, or there are more than 64.  `to`(n): where they go.
+  template <typename F> __device__ __forceinline__ int select(F to) {
+    const int top = a.top;
+    bool odd = false;
+    most = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) { odd |= !(l[i] < INFINITY); most = fmaxf(most, l[i]); }
+    if (!a.sigmoid) most = value_of_key(wave_max(key_of(most)));
+    float rank[PER], score[PER];
+    if (scored) {
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const float e = __expf(a.sigmoid ? -l[i] : l[i] - most);
+        score[i] = a.sigmoid ? __builtin_amdgcn_rcpf(1.f + e) : e;
+        sum += e;
+      }
+      if (!a.sigmoid) {
+        sum = 1.f / wave_sum(sum);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) score[i] *= sum;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      rank[i] = l[i];
+      if (biased) {
+        rank[i] = l[i] == -INFINITY || b[i] == -INFINITY ? -INFINITY : score[i] + b[i];
+        odd |= !(rank[i] < 0x1p60f) || (rank[i] < -0x1p60f && rank[i] != -INFINITY);
+      }
+    }
+    if (__ballot(odd)) return 0;
+    // float32 ranks, and differences of two, are off by less: a score by 2 PER + 32 steps of 2^-24 at most (the exponential and its argument 6, the sum PER + 5, its
+    // inverse and the product 3), the sum with the bias by one more of its own
+    const float slack = (2 * PER + 32) * 0x1p-24f;
+    bool out = g >= a.groups;
+    if (a.groups > 1) {
+      // a lane's two largest, then those of the group's lanes
+      float first = -INFINITY, second = -INFINITY;
+      const bool by_rank = biased || a.group_best == 1, two = a.group_best > 1 && a.size > 1;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const float v = by_rank || rank[i] == -INFINITY ? rank[i] : score[i];
+        second = fmaxf(second, fminf(first, v));
+        first = fmaxf(first, v);
+      }
+      if (parts > 1) two_largest<1>(first, second);
+      if (parts > 2) two_largest<2>(first, second);
+      if (parts > 4) two_largest<4>(first, second);
+      if (parts > 8) two_largest<8>(first, second);
+      if (parts > 16) {
+        float f0, f1, s0, s1;
+        halves16(first, f0, f1);
+        halves16(second, s0, s1);
+        second = fmaxf(fmaxf(s0, s1), fminf(f0, f1));
+        first = fmaxf(f0, f1);
+      }
+      // each group's lanes compare it with as many others at once
+      const unsigned long long own = ((1ull << parts) - 1) << (g << parts_log2);
+      auto count_better = [&](auto mine, auto near, bool& close) {
+        int better = 0;
+        for (int k = 0; k < a.groups; k += parts) {
+          const auto other = __shfl(mine, (k + p) << parts_log2);
+          const bool there = k + p < a.groups;
+          better += (int)__builtin_popcountll(__ballot(there && (other > mine || (other == mine && k + p < g))) & own);
+          close |= there && k + p != g && !(other > mine + near) && !(other < mine - near);
+        }
+        return better;
+      };
+      const float mine = two ? first + second : first;
+      bool close = false, none = false;
+      int better = count_better(mine, 2.f * slack * (1.f + fabsf(mine)), close);
+      // groups so close that float32 does not tell which is better count where one of them may be in and another out
+      if (scored && __ballot(close && g < a.groups && mine > -INFINITY && better <= a.top_groups && better >= a.top_groups - 1)) {
+        const double total = a.sigmoid ? 1.0 : all64();
+        double first = -INFINITY, second = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const double v = rank[i] == -INFINITY ? -INFINITY : (a.sigmoid ? sigmoid64(l[i]) : exp((double)l[i] - (double)most) / total) + (double)b[i];
+          second = fmax(second, fmin(first, v));
+          first = fmax(first, v);
+        }
+        for (int off = 1; off < parts; off <<= 1) {
+          const double f = __shfl_xor(first, off), s = __shfl_xor(second, off);
+          second = fmax(fmax(second, s), fmin(first, f));
+          first = fmax(first, f);
+        }
+        better = count_better(two ? first + second : first, 0.0, none);
+      }
+      out |= better >= a.top_groups;
+    }
+    uint32_t key[PER], largest = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      key[i] = !in(i) ? 0u : out ? KEY_MASKED : key_of(rank[i]);
+      largest = max(largest, key[i]);
+    }
+    largest = __builtin_amdgcn_readfirstlane(wave_max(largest));
+    auto count = [&](uint32_t from) {
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) n += (int)__builtin_popcountll(__ballot(key[i] >= from));
+      return n;
+    };
+    // at least `top` from lo on, fewer from hi on
+    uint32_t hi = largest + 1, lo, step = 1u << 20;
+    int n;
+    for (;;) {
+      lo = hi > step ? hi - step : 1u;
+      n = count(lo);
+      if (n >= top) break;
+      hi = lo;
+      step = min(step * 4, 1u << 28);
+    }
+    while (n != top && hi - lo > 1) {
+      const uint32_t mid = lo + ((hi - lo) >> 1);
+      const int m = count(mid);
+      if (m >= top) { lo = mid; n = m; } else hi = mid;
+    }
+    unsigned long long taken[PER];
+    if ((biased && lo > KEY_MASKED) || n == top) {
+      if (biased && lo > KEY_MASKED) {
+        const float t = value_of_key(lo);
+        lo = __builtin_amdgcn_readfirstlane(key_of(t - slack * (1.f + fabsf(t))));
+        n = count(lo);
+        if (n > 64) return 0;
+      }
+#pragma unroll
+      for (int i = 0; i < PER; ++i) taken[i] = __ballot(key[i] >= lo);
+    } else {
+      // lo itself is the rank of several, of which the first by number are taken
+      int ahead = 0;
+      unsigned long long at[PER];
+      const unsigned long long mine = (parts == 64 ? ~0ull : (1ull << parts) - 1) << (g << parts_log2), before = (1ull << (g << parts_log2)) - 1, lower = (1ull << lane) - 1;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        at[i] = __ballot(key[i] == lo);
+        ahead += (int)__builtin_popcountll(__ballot(key[i] > lo)) + (int)__builtin_popcountll(at[i] & before);
+      }
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int here = ahead + (int)__builtin_popcountll(at[i] & mine & lower);
+        ahead += (int)__builtin_popcountll(at[i] & mine);
+        taken[i] = __ballot(key[i] > lo || (key[i] == lo && here < top));
+      }
+      n = top;
+    }
+    Candidate* place = to(n);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (taken[i] >> lane & 1ull)
+        place[__builtin_amdgcn_mbcnt_hi((uint32_t)(taken[i] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)taken[i], 0))] = Candidate{key[i], e0 + i * parts, l[i], b[i]};
+      place += (int)__builtin_popcountll(taken[i]);
+    }
+    return n;
+  }
+
+  // Of tokens' candidates, LANES places and lanes to each, the chosen in order with their weights.  n, most, total: of the lane's token
+  template <int LANES> __device__ __forceinline__ void finish(const Candidate* place, long long token, int n, float most, double total) const {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const int k = lane & (LANES - 1), top = a.top;
+    place += lane - k;
+    const Candidate c = k < n ? place[k] : Candidate{KEY_MASKED, 0, -INFINITY, 0.f};
+    const bool none = c.key == KEY_MASKED;
+    const float v = value_of_key(c.key), near = (2 * PER + 32) * 0x1p-24f * (1.f + fabsf(v));
+    int order = 0;
+    bool close = false;
+    for (int j = 0; j < (LANES == 64 ? n : LANES); ++j) {
+      const uint32_t key = place[j].key;
+      const int e = place[j].e;
+      order += j < n && (key > c.key || (key == c.key && e < c.e));
+      close |= j < n && j != k && fabsf(value_of_key(key) - v) <= near;
+    }
+    // scores of the candidates; of the softmax over the sum of all only where that does not cancel
+    double w = none ? 0.0 : a.sigmoid ? sigmoid64(c.l) : exp((double)c.l - (double)most) / total;
+    if (biased && __ballot(close && !none)) {
+      const long long mine = none ? ORDER_MASKED : order_of(w + (double)c.b);
+      order = 0;
+      for (int j = 0; j < LANES; ++j) {
+        const long long other = __shfl(mine, lane - k + j);
+        order += j < n && (other > mine || (other == mine && place[j].e < c.e));
+      }
+    }
+    const bool chosen = k < n && order < top;
+    if (a.renormalize) {
+      double all = chosen ? w : 0.0;
+      if constexpr (LANES == 64) all = wave_sum(all);
+      else { all += dpp_mov64<0xB1>(all); all += dpp_mov64<0x4E>(all); all += dpp_mov64<0x141>(all); all += dpp_mov64<0x140>(all); }
+      w = all == 0.0 ? 0.0 : w / all;
+    }
+    if (chosen) {
+      ((HTR_GLOBAL int*)a.ids)[token * top + order] = c.e;
+      ((HTR_GLOBAL float*)a.weights)[token * top + order] = (float)(w * a.scale);
+    }
+  }
+};
+
+// TOKENS = 1, or 4 tokens to a wave, of which those with up to 16 candidates are finished together: what comes behind the selection has few lanes to a token at work
+template <int PER, int TOKENS>
+__global__ __launch_bounds__(ROUTE_WAVES * 64) void k_route(const RouteArgs a) {
+  __shared__ Candidate candidates[ROUTE_WAVES][TOKENS == 1 ? 64 : 128];
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const long long first = ((long long)blockIdx.x * ROUTE_WAVES + wv) * TOKENS;
+  if (first >= a.tokens) return;
+  Candidate *together = candidates[wv], *alone = candidates[wv] + (TOKENS == 1 ? 0 : 64);
+  Route<PER> r(a, lane);
+  float logits[TOKENS][PER];
+#pragma unroll
+  for (int q = 0; q < TOKENS; ++q) r.load(min(first + q, a.tokens - 1), logits[q]);
+  int n = 0;
+  float most = 0.f;
+  double total = 1.0;
+#pragma unroll
+  for (int q = 0; q < TOKENS; ++q) {
+    if (first + q >= a.tokens) break;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) r.l[i] = logits[q][i];
+    const int found = r.select([&](int n) { return TOKENS > 1 && n <= 16 ? together + 16 * q : alone; });
+    if (found == 0) { route_exact<(PER < 16 ? PER : 16)>(a, first + q, lane); continue; }
+    const double sum = !a.sigmoid && r.most > -INFINITY && (!a.renormalize || r.biased) ? r.all64() : 1.0;
+    if (TOKENS == 1 || found > 16) {
+      r.template finish<64>(alone, first + q, found, r.most, sum);
+    } else if (lane >> 4 == q) {
+      n = found;
+      most = r.most;
+      total = sum;
+    }
+  }
+  if constexpr (TOKENS > 1) r.template finish<16>(together, first + (lane >> 4), n, most, total);
 }

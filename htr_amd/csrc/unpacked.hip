@@ -309,12 +309,19 @@ struct StackedScratch {
     bytes = at;
   }
 };
-hipError_t launch_route(const RouteArgs& a, hipStream_t st) {
-  const dim3 grid((unsigned)((a.tokens + ROUTE_WAVES - 1) / ROUTE_WAVES));
-  const int per = (a.experts + 63) / 64;
-  return per <= 1 ? launch(k_route<1>, grid, ROUTE_WAVES * 64, 0, st, a) : per <= 2 ? launch(k_route<2>, grid, ROUTE_WAVES * 64, 0, st, a)
-         : per <= 4 ? launch(k_route<4>, grid, ROUTE_WAVES * 64, 0, st, a) : per <= 8 ? launch(k_route<8>, grid, ROUTE_WAVES * 64, 0, st, a)
-                    : launch(k_route<16>, grid, ROUTE_WAVES * 64, 0, st, a);
+template <int PER> hipError_t launch_route(const RouteArgs& a, hipStream_t st) {
+  auto grid = [&](int tokens) { return dim3((unsigned)((a.tokens + ROUTE_WAVES * tokens - 1) / (ROUTE_WAVES * tokens))); };
+  if constexpr (PER <= 8)
+    if (a.top <= 16 && a.tokens >= ROUTE_TOGETHER) return launch(k_route<PER, 4>, grid(4), ROUTE_WAVES * 64, 0, st, a);
+  return launch(k_route<PER, 1>, grid(1), ROUTE_WAVES * 64, 0, st, a);
+}
+hipError_t launch_route(RouteArgs a, hipStream_t st) {
+  a.size = a.experts / a.groups;
+  a.parts_log2 = 6;
+  while ((64 >> a.parts_log2) < a.groups) --a.parts_log2;
+  const int per = (a.size + (1 << a.parts_log2) - 1) >> a.parts_log2;      // below 2 ROUTE_MOST / 64
+  return per <= 1 ? launch_route<1>(a, st) : per <= 2 ? launch_route<2>(a, st) : per <= 4 ? launch_route<4>(a, st) : per <= 8 ? launch_route<8>(a, st)
+         : per <= 16 ? launch_route<16>(a, st) : launch_route<32>(a, st);
 }
 int stacked_shape(long long tokens, int top, int experts, int hidden, int inter, int type) {
   if (tokens < 1 || top < 1 || experts < 1 || hidden < 1 || inter < 1 || top > 4096 || tokens >= (1 << 24) || inter > (1 << 28)) return HTR_ERR_SIZE;
@@ -504,7 +511,7 @@ int htr_route(const void* logits, int64_t stride, int dtype, int64_t tokens, int
   constexpr int64_t MOST = 1 << 22;      // a launch has fewer than 2^32 threads, 64 of them to a token
   for (int64_t t = 0; t < tokens; t += MOST) {
     const RouteArgs a{(const uint8_t*)logits + t * stride * (int64_t)element_bytes(dtype), bias, ids + t * top, weights + t * top, stride, tokens - t < MOST ? tokens - t : MOST,
-                      dtype, experts, top, sigmoid, groups, top_groups, group_best, renormalize, scale};
+                      dtype, experts, top, sigmoid, groups, top_groups, group_best, renormalize, scale, 0, 0};
     TRY_HIP(launch_route(a, (hipStream_t)stream));
   }
   return HTR_OK;
