@@ -164,6 +164,19 @@ __global__ __launch_bounds__(STREAM_WAVES * 64) void k_product_stream(const Prod
     sp[t] = (const HTR_GLOBAL float*)a.xs + (size_t)r * (a.n >> 7);
   }
   const HTR_GLOBAL float* wsp = (const HTR_GLOBAL float*)a.ws + ((size_t)s.e * ((a.m + 127) >> 7) + (m0 >> 7)) * (a.n >> 7);
+  // int8: the scales of what this thread stores, asked for ahead of everything else
+  constexpr int STORES = (R * TT * 256 + STREAM_WAVES * 64 - 1) / (STREAM_WAVES * 64);
+  float row_scale[T == P_I8 ? STORES : 1], matrix_scale[T == P_I8 ? STORES : 1];
+  if constexpr (T == P_I8) {
+#pragma unroll
+    for (int k = 0; k < STORES; ++k) {
+      const int idx = min((int)threadIdx.x + k * STREAM_WAVES * 64, R * TT * 256 - 1);
+      int r = s.first + min(idx / (16 * R), s.count - 1);
+      if (a.gather != nullptr) r = a.gather[r];
+      row_scale[k] = ((const HTR_GLOBAL float*)a.xs)[r];
+      matrix_scale[k] = ((const HTR_GLOBAL float*)a.ws)[(size_t)s.e * a.m + min(m0 + idx % (16 * R), a.m - 1)];
+    }
+  }
   Sum acc[R][TT];
 #pragma unroll
   for (int i = 0; i < R; ++i)
@@ -173,12 +186,11 @@ __global__ __launch_bounds__(STREAM_WAVES * 64) void k_product_stream(const Prod
   Eight<X == P_F8 || X == P_I8 ? HTR_BF16 : X> raw[ROUNDS ? P : 1][TT][4];  // 16 elements of either half of the slab
   float sx[P][TT], sw[P];
   const u4 zero = {0u, 0u, 0u, 0u};
-  auto load = [&](int p, int slab) {
+  auto load_slab = [&](int p, int slab, auto whole) {
     const size_t off = (size_t)slab << 7;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      // other than e4m3 rows may end inside the slab, at a multiple of 16 bytes
-      const bool in = T == P_F8 || off + 64 * h + 16 * g < row_bytes;
+      const bool in = decltype(whole)::value || off + 64 * h + 16 * g < row_bytes;
 #pragma unroll
       for (int i = 0; i < R; ++i) { A[p][i][h] = zero; if (in) A[p][i][h] = __builtin_nontemporal_load((const HTR_GLOBAL u4*)(wp[i] + off + 64 * h)); }
 #pragma unroll
@@ -197,6 +209,12 @@ __global__ __launch_bounds__(STREAM_WAVES * 64) void k_product_stream(const Prod
 #pragma unroll
       for (int t = 0; t < TT; ++t) if constexpr (!ROUNDS) sx[p][t] = sp[t][slab];
     }
+  };
+  // other than e4m3 rows may end inside the last slab, at a multiple of 16 bytes
+  const int whole_slabs = (int)(row_bytes >> 7);
+  auto load = [&](int p, int slab) {
+    if (T == P_F8 || slab < whole_slabs) load_slab(p, slab, std::true_type());
+    else load_slab(p, slab, std::false_type());
   };
   // a row's 128 columns lie in the four lanes c, c + 16, c + 32, c + 48
   auto round_x = [&](int p, int t) {
@@ -250,18 +268,18 @@ __global__ __launch_bounds__(STREAM_WAVES * 64) void k_product_stream(const Prod
 #pragma unroll
     for (int t = 0; t < TT; ++t) *(Sum*)&red[wv][(i * TT + t) * 256 + lane * 4] = acc[i][t];
   __syncthreads();
-  for (int idx = threadIdx.x; idx < R * TT * 256; idx += STREAM_WAVES * 64) {
+#pragma unroll
+  for (int k = 0; k < STORES; ++k) {
+    const int idx = threadIdx.x + k * STREAM_WAVES * 64;
+    if (R * TT * 256 % (STREAM_WAVES * 64) != 0 && idx >= R * TT * 256) break;
     const int i = idx % (16 * R), t = idx / (16 * R);            // matrix row, row of x
     const int at = ((i >> 4) * TT + (t >> 4)) * 256 + (((i & 15) >> 2) * 16 + (t & 15)) * 4 + (i & 3);
     One sum = 0;
 #pragma unroll
-    for (int k = 0; k < STREAM_WAVES; ++k) sum += red[k][at];
+    for (int w = 0; w < STREAM_WAVES; ++w) sum += red[w][at];
     if (t < s.count && m0 + i < a.m) {
       float v = (float)sum;
-      if constexpr (T == P_I8) {
-        const int r = a.gather != nullptr ? a.gather[s.first + t] : s.first + t;
-        v = v * ((const HTR_GLOBAL float*)a.xs)[r] * ((const HTR_GLOBAL float*)a.ws)[(size_t)s.e * a.m + m0 + i];
-      }
+      if constexpr (T == P_I8) v = v * row_scale[k] * matrix_scale[k];
       if (a.bias != nullptr) v += load_elem_g(a.bias, a.y_dtype, m0 + i);
       store_elem_g(a.y, a.y_dtype, (size_t)(s.first + t) * a.m + m0 + i, v);
     }
@@ -302,18 +320,22 @@ template <int Y> __device__ __forceinline__ void store8(const ProductArgs& a, fl
   }
 }
 
+// floats of a tile's scales in int8, whole loads of a wave
+constexpr int scales_of_tile(int tm, int tn) { return (tm + tn + 63) / 64 * 64; }
+
 template <int T, int WM, int WN, int AT, int BT, int NS, bool GATED>
 __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductArgs a, int mtiles) {
   constexpr int WAVES = WM * WN, TM = 16 * AT * WM, TN = 16 * BT * WN;
   constexpr int XW = (TN + 63) / 64;                             // waves that load rows' scales
   constexpr int SCALES = T == P_F8 ? XW * 256 + 256 : 0, STAGE = (TM + TN) * 128 + SCALES;    // e4m3: the rows' scales, then the matrix's
   constexpr int LW = TM / 8 / WAVES, LX = TN / 8 / WAVES, L = LW + LX;        // 1 KB loads of a wave to a stage
-  constexpr int RA = T == P_F8 || AT < 4 ? 2 : 4;                // MFMA tiles of the matrix in registers
+  constexpr int RA = T == P_F8 || AT < 4 || (T == P_I8 && AT > 4) ? 2 : 4;      // MFMA tiles of the matrix in registers
   constexpr int BARRIER = AT - RA + 1;                           // the tile of products before which the next slab has landed
   constexpr bool WIDE = GATED && T == P_F8 && BT <= 2;           // float32 sums of what is rounded to e4m3 next
   static_assert(T != P_F8 || XW < WAVES, "a wave for the matrix's scales");
   static_assert(AT % 2 == 0 && TM % (8 * WAVES) == 0 && TN % (8 * WAVES) == 0 && AT % RA == 0, "whole loads, registers in turn");
   static_assert(!GATED || (AT % 4 == 0 && (T != P_F8 || TM == 256)), "32 gates and 32 ups to a wave; whole blocks of 128");
+  constexpr int TILE_SCALES = T == P_I8 ? scales_of_tile(TM, TN) : 0;      // int8: two tiles' scales behind the ring, the matrix's, then the rows'
   extern __shared__ __align__(16) uint8_t lds[];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
   const int wm = wv / WN, wn = wv % WN;
@@ -401,6 +423,28 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
     if constexpr (T == P_F8)
       __builtin_amdgcn_global_load_lds((const HTR_GLOBAL void*)(src.scales + slab + src.scale),
                                        (__attribute__((address_space(3))) void*)(lds + stage * STAGE + (TM + TN) * 128 + min(wv, XW) * 256), 4, 0, 0);
+  };
+  // int8: a tile's scales, asked for ahead of its first slab and so there with it.  One load more than `landed` counts makes it wait longer, never shorter.
+  auto issue_tile_scales = [&](const Tile& t, int which) {
+    if constexpr (T == P_I8) {
+#pragma unroll
+      for (int k = 0; k < TILE_SCALES; k += WAVES * 64) {
+        if (k + wv * 64 >= TILE_SCALES) break;
+        const int j = k + wv * 64 + lane;
+        const HTR_GLOBAL float* p = (const HTR_GLOBAL float*)a.ws + (size_t)t.s.e * a.m;
+        if (j >= TM) {
+          int r = t.s.first + min(j - TM, t.s.count - 1);
+          if (a.gather != nullptr) r = a.gather[r];
+          p = (const HTR_GLOBAL float*)a.xs + r;
+        } else if (GATED) {
+          const int half = TM / 2, F = a.m >> 1;
+          p += min((t.m0 >> 1) + (j < half ? j : j - half), F - 1) + (j < half ? 0 : F);
+        } else {
+          p += min(t.m0 + j, a.m - 1);
+        }
+        __builtin_amdgcn_global_load_lds((const HTR_GLOBAL void*)p, (__attribute__((address_space(3))) void*)(lds + NS * STAGE + (which * TILE_SCALES + k + wv * 64) * 4), 4, 0, 0);
+      }
+    }
   };
   // The stage is there for every wave, and every wave has read all of the one before.  `behind`: later loads of this wave, which may still be on their way (they
   // arrive in order; results being stored in between only make the wait longer); `last`: the stage holds its tile's last slab
@@ -530,6 +574,8 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
     }
     stage = next;
   };
+  issue_tile_scales(mine, 0);
+  int which = 0;                                                 // int8: the half of the scales' place that the tile in hand has
   // slabs behind the last one: the last one again, for nothing
 #pragma unroll
   for (int st = 0; st < NS - 1; ++st) {
@@ -553,7 +599,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
     if (slab + NS == slabs) {
       id += gridDim.x;
       more = find(then);
-      if (more) source(then, src2);
+      if (more) { source(then, src2); issue_tile_scales(then, which ^ 1); }
     }
     const int ask = slab + NS < slabs ? slab + NS : slabs >= NS ? slab + NS - slabs : slabs - 1;
     multiply(asked, src, ask, src2, slab + 2 == slabs);
@@ -561,22 +607,13 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
     src = src2;
     if (++slab < slabs) continue;
     slab = 0;
-    // int8: the scales of the lane's rows of x, and of eight consecutive rows of the matrix, as far as it goes
-    auto row_scale = [&](int t) {
-      int r = mine.s.first + min(wn * 16 * BT + 16 * t + c, mine.s.count - 1);
-      if (a.gather != nullptr) r = a.gather[r];
-      return ((const HTR_GLOBAL float*)a.xs)[r];
-    };
-    auto matrix_scales = [&](int i, int end, float (&w)[8]) {
-      const HTR_GLOBAL float* p = (const HTR_GLOBAL float*)a.ws + (size_t)mine.s.e * a.m;
-      if (i + 8 <= end) {
-        const f4 lo = *(const HTR_GLOBAL f4_any*)(p + i), hi = *(const HTR_GLOBAL f4_any*)(p + i + 4);
+    // int8: the scales of the lane's rows of x, and of eight consecutive rows of the matrix
+    const float* tile_scales = (const float*)(lds + NS * STAGE) + which * TILE_SCALES;
+    auto row_scale = [&](int t) { return tile_scales[TM + wn * 16 * BT + 16 * t + c]; };
+    auto matrix_scales = [&](int i, float (&w)[8]) {
+      const f4 lo = *(const f4*)(tile_scales + i), hi = *(const f4*)(tile_scales + i + 4);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) { w[k] = lo[k]; w[4 + k] = hi[k]; }
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) w[k] = p[min(i + k, end - 1)];
-      }
+      for (int k = 0; k < 4; ++k) { w[k] = lo[k]; w[4 + k] = hi[k]; }
     };
     if constexpr (GATED && T == P_I8) {
       const int F = a.m >> 1, i0 = (mine.m0 >> 1) + wm * 8 * AT + 8 * g;      // hidden columns; first of the lane's
@@ -586,8 +623,8 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
 #pragma unroll
       for (int h = 0; h < AT / 4; ++h) {
         float gate[8], up[8];
-        matrix_scales(i0 + 32 * h, F, gate);
-        matrix_scales(F + i0 + 32 * h, a.m, up);
+        matrix_scales(wm * 8 * AT + 8 * g + 32 * h, gate);
+        matrix_scales(TM / 2 + wm * 8 * AT + 8 * g + 32 * h, up);
 #pragma unroll
         for (int t = 0; t < BT; ++t) {
           float f[8];
@@ -657,26 +694,28 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
       const int i0 = mine.m0 + wm * 16 * AT + 8 * g;               // first of the lane's outputs
       auto put = [&](auto type) {
         constexpr int Y = decltype(type)::value;
-        float ws[T == P_I8 ? AT / 2 : 1][8], rs[T == P_I8 ? BT : 1];
-        if constexpr (T == P_I8) {
+        auto each = [&](int t, int h, auto scaled) {
+          const int r = wn * 16 * BT + 16 * t + c;
+          float f[8];
 #pragma unroll
-          for (int h = 0; h < AT / 2; ++h) matrix_scales(i0 + 32 * h, a.m, ws[h]);
+          for (int k = 0; k < 8; ++k) f[k] = scaled((float)acc[2 * h + (k >> 2)][t][k & 3], k);
+          if (r < mine.s.count && i0 + 32 * h < a.m) store8<Y>(a, f, (size_t)(mine.s.first + r) * a.m + i0 + 32 * h, i0 + 32 * h);
+        };
+        if constexpr (T == P_I8) {
+          float ws[8], rs[BT];
 #pragma unroll
           for (int t = 0; t < BT; ++t) rs[t] = row_scale(t);
-        }
-#pragma unroll
-        for (int t = 0; t < BT; ++t) {
-          const int r = wn * 16 * BT + 16 * t + c;
 #pragma unroll
           for (int h = 0; h < AT / 2; ++h) {
-            float f[8];
+            matrix_scales(wm * 16 * AT + 8 * g + 32 * h, ws);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              f[k] = (float)acc[2 * h + (k >> 2)][t][k & 3];
-              if constexpr (T == P_I8) f[k] = f[k] * rs[t] * ws[h][k];
-            }
-            if (r < mine.s.count && i0 + 32 * h < a.m) store8<Y>(a, f, (size_t)(mine.s.first + r) * a.m + i0 + 32 * h, i0 + 32 * h);
+            for (int t = 0; t < BT; ++t) each(t, h, [&](float v, int k) { return v * rs[t] * ws[k]; });
           }
+        } else {
+#pragma unroll
+          for (int t = 0; t < BT; ++t)
+#pragma unroll
+            for (int h = 0; h < AT / 2; ++h) each(t, h, [](float v, int) { return v; });
         }
       };
       if (a.y_dtype == HTR_BF16) put(std::integral_constant<int, HTR_BF16>());
@@ -689,6 +728,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
       for (int t = 0; t < BT; ++t) acc[i][t] = Sum{0, 0, 0, 0};
     if (!more) break;
     mine = then;
+    which ^= 1;
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // loads for nothing: they write to LDS
 }

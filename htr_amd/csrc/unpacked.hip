@@ -122,7 +122,7 @@ template <int R_, int TT_, int WAVES_> struct Stream { static constexpr int R = 
 template <int WM_, int WN_, int AT_, int BT_, int NS_, bool GATED_ = false> struct Tiles {
   static constexpr int WM = WM_, WN = WN_, AT = AT_, BT = BT_, NS = NS_, TM = 16 * AT_ * WM_, TN = 16 * BT_ * WN_;
   static constexpr bool GATED = GATED_;
-  template <int T> static constexpr size_t LDS = NS * ((TM + TN) * 128 + (T == P_F8 ? (TN + 63) / 64 * 256 + 256 : 0)) + (GATED && T == P_F8 ? WM * TN * 4 : 0);
+  template <int T> static constexpr size_t LDS = NS * ((TM + TN) * 128 + (T == P_F8 ? (TN + 63) / 64 * 256 + 256 : 0)) + (GATED && T == P_F8 ? WM * TN * 4 : 0) + (T == P_I8 ? 2 * 4 * scales_of_tile(TM, TN) : 0);
 };
 struct TileGrid { long long mtiles, tiles; unsigned workgroups; };      // tiles: a bound where rows are grouped
 template <int T, typename K> TileGrid tile_grid(const ProductArgs& a) {
