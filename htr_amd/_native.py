@@ -61,6 +61,7 @@ SIGNATURES = {
     "htr_route": (_i, [_vp, _i64, _i, _i64, _i, _i, _i, _vp, _i, _i, _i, _i, ctypes.c_double, _vp, _vp, _vp]),
     "htr_product": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i, _i, _i, _i, _i, _vp]),
     "htr_product_rounds": (_i, [_i64, _i, _i]),
+    "htr_product_rounds_int8": (_i, [_i64, _i]),
     "htr_product_plan": (_i, [_i64, _i, _i, _i, _i, _i, _i, _i, ctypes.POINTER(ctypes.c_int)]),
     "htr_moe_stacked_scratch_bytes": (_sz, [_i64, _i, _i, _i, _i, _i]),
     "htr_moe_stacked": (_i, [_vp, _i, _vp, _i, _vp, _i64, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _sz, _vp]),
@@ -104,7 +105,7 @@ def fast():
                         address(L.htr_linear_route), address(L.htr_dequant_w))
             module.bind_unpacked(address(L.htr_rms_norm), address(L.htr_quantize_e4m3), address(L.htr_product), address(L.htr_product_rounds),
                                  address(L.htr_moe_stacked_scratch_bytes), address(L.htr_moe_stacked), address(L.htr_rms_norm_int8), address(L.htr_quantize_int8),
-                                 address(L.htr_route))
+                                 address(L.htr_route), address(L.htr_product_rounds_int8))
         except (ImportError, AttributeError) as e:
             warnings.warn(f"htr_amd/_fast.so cannot be used ({e}): launches are prepared in Python; `python -m htr_amd.build` builds it",
                           RuntimeWarning, stacklevel=2)

@@ -14,7 +14,8 @@ LIB = os.path.join(CSRC, "libhtr_gfx950.so")
 # two translation units, compiled side by side; the kernels live in the parts they include
 SOURCES = [os.path.join(CSRC, "htr_gfx950.hip"), os.path.join(CSRC, "unpacked.hip")]
 PARTS = [os.path.join(CSRC, f) for f in ("decode.hpp", "linear.hpp", "linear_batch.hpp", "linear_tile.hpp", "linear_gemm.hpp", "linear_wide.hpp", "moe.hpp", "dequant.hpp",
-                                         "viterbi.hpp", "anchors.hpp", "plan.hpp", "norm.hpp", "product.hpp", "experts.hpp", "int8.hpp", "route.hpp")]
+                                         "viterbi.hpp", "anchors.hpp", "plan.hpp", "norm.hpp", "product.hpp", "experts.hpp", "int8.hpp", "int8_rows.hpp",
+                                         "route.hpp")]
 BINDING_SOURCE = os.path.join(CSRC, "torch_binding.cpp")
 BINDING = os.path.join(os.path.dirname(CSRC), "_fast.so")
 HEADER = os.path.join(os.path.dirname(CSRC), os.pardir, "include", "htr_gfx950.h")

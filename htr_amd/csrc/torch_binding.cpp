@@ -31,6 +31,7 @@ decltype(&htr_quantize_e4m3) f_quantize = nullptr;
 decltype(&htr_rms_norm_int8) f_norm_int8 = nullptr;
 decltype(&htr_quantize_int8) f_quantize_int8 = nullptr;
 decltype(&htr_route) f_experts = nullptr;
+decltype(&htr_product_rounds_int8) f_rounds_int8 = nullptr;
 decltype(&htr_product) f_product = nullptr;
 decltype(&htr_product_rounds) f_rounds = nullptr;
 decltype(&htr_moe_stacked_scratch_bytes) f_stacked_bytes = nullptr;
@@ -346,8 +347,10 @@ PyObject* product(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   {
     pybind11::gil_scoped_release no_lock;      // as in linear()
     c10::DeviceGuard guard(dev);
-    // few 16-bit rows are rounded by the product itself
-    const bool as_is = !eight || (xs == nullptr && w->scalar_type() == at::kFloat8_e4m3fn && half_of(*x) && f_rounds(x->numel() / n, (int)experts, ends != nullptr));
+    // few floating rows are rounded by the product itself
+    const int64_t rows = x->numel() / n;
+    const bool as_is = !eight || (xs == nullptr && (w->scalar_type() == at::kChar ? ends == nullptr && float_of(*x) && n % 16 == 0 && f_rounds_int8(rows, (int)n)
+                                                                                  : half_of(*x) && f_rounds(rows, (int)experts, ends != nullptr)));
     if (as_is) q = *x;
     if (!as_is && !rows8(*x, xs, w->scalar_type(), dev, stream, q, qs, rc)) {
       rc = HTR_ERR_SIZE;
@@ -453,15 +456,16 @@ PyObject* route(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 }
 
 // bind_unpacked(addresses of htr_rms_norm, htr_quantize_e4m3, htr_product, htr_product_rounds, htr_moe_stacked_scratch_bytes, htr_moe_stacked, htr_rms_norm_int8,
-// htr_quantize_int8, htr_route), after bind()
+// htr_quantize_int8, htr_route, htr_product_rounds_int8), after bind()
 PyObject* bind_unpacked(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
-  if (nargs != 9) { PyErr_SetString(PyExc_TypeError, "bind_unpacked wants nine addresses"); return nullptr; }
-  void* p[9];
-  for (int i = 0; i < 9; ++i) p[i] = PyLong_AsVoidPtr(args[i]);
+  if (nargs != 10) { PyErr_SetString(PyExc_TypeError, "bind_unpacked wants ten addresses"); return nullptr; }
+  void* p[10];
+  for (int i = 0; i < 10; ++i) p[i] = PyLong_AsVoidPtr(args[i]);
   if (PyErr_Occurred()) return nullptr;
   f_norm = (decltype(f_norm))p[0]; f_quantize = (decltype(f_quantize))p[1]; f_product = (decltype(f_product))p[2];
   f_rounds = (decltype(f_rounds))p[3]; f_stacked_bytes = (decltype(f_stacked_bytes))p[4]; f_stacked = (decltype(f_stacked))p[5];
   f_norm_int8 = (decltype(f_norm_int8))p[6]; f_quantize_int8 = (decltype(f_quantize_int8))p[7]; f_experts = (decltype(f_experts))p[8];
+  f_rounds_int8 = (decltype(f_rounds_int8))p[9];
   Py_RETURN_NONE;
 }
 

@@ -20,6 +20,7 @@ namespace {
 #include "product.hpp"
 #include "experts.hpp"
 #include "int8.hpp"
+#include "int8_rows.hpp"
 #include "route.hpp"
 
 #define TRY_HIP(EXPR) do { const hipError_t e_ = (EXPR); if (e_ != hipSuccess) return htr_note_hip_error((int)e_); } while (0)
@@ -277,6 +278,36 @@ template <int T> void describe_product(const ProductArgs& a, bool gated, int* ou
 }
 // columns: whole blocks of e4m3, rows on 16-byte boundaries
 int unit_of(int type) { return type == HTR_E4M3 ? 128 : type == HTR_I8 ? 16 : 8; }
+// ---- few rows in int8
+struct RowsGrid { int columns, tiles, workgroups; size_t lds; };
+RowsGrid rows_grid(int rows, int m, int n) {
+  RowsGrid g;
+  g.columns = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
+  g.tiles = (m + ROWS_TILE - 1) / ROWS_TILE;
+  g.lds = rows_lds(rows, g.columns, n);
+  // two workgroups to a compute unit where the rows of x are few to prepare (us by two and by one: 1 row on 6144x4096 7.7 and 8.0, 4 on 14336x4096 12.0 and 12.7,
+  // 8 on 152064x4096 102 and 101, 32 on 28672x4096 30 and 25)
+  const int most = rows <= 4 && g.lds <= 80 * 1024 ? 512 : 256;
+  g.workgroups = g.tiles < most ? g.tiles : most;
+  return g;
+}
+template <int X, int CT> hipError_t launch_rows(const RowsArgs& a, const RowsGrid& g, hipStream_t st) {
+  const hipError_t e = allow_lds<k_product_rows<X, CT>>(160 * 1024);
+  return e != hipSuccess ? e : launch(k_product_rows<X, CT>, dim3(g.workgroups), ROWS_WAVES * 64, g.lds, st, a, g.tiles);
+}
+hipError_t launch_rows(const RowsArgs& a, hipStream_t st) {
+  const RowsGrid g = rows_grid(a.rows, a.m, a.n);
+  if (a.x_type == HTR_BF16) return launch_rows<HTR_BF16, 1>(a, g, st);
+  if (a.x_type == HTR_F16) return launch_rows<HTR_F16, 1>(a, g, st);
+  if (a.x_type == HTR_F32) return launch_rows<HTR_F32, 1>(a, g, st);
+  return g.columns == 8 ? launch_rows<P_I8, 1>(a, g, st) : g.columns == 16 ? launch_rows<P_I8, 2>(a, g, st) : launch_rows<P_I8, 4>(a, g, st);
+}
+// Up to 32 rows that LDS holds.  us by k_product_rows and by the faster of the kernels for more rows: 1 row on 1024x4096 4.9 and 5.3, on 6144x4096 7.7 and 10.1, 8 on
+// 152064x4096 101 and 125, 16 on 14336x4096 14.0 and 15.8, 32 on 28672x4096 25 and 29, on 4096x4096 9.6 and 8.8
+bool takes_rows(int64_t rows, int n) { return rows >= 1 && rows <= 32 && rows_lds((int)rows, 32, n) <= 160 * 1024; }
+// Up to 8 of them rounded on the way, by every workgroup for itself: 1 row on 6144x4096 9.5 us, 8 rows 11.3 (rounded ahead 7.7 and 8.5, and 4.5 for that launch), 16 rows
+// on 14336x4096 19.2 (14.0 and 4.6)
+bool rounds_rows(int64_t rows, int n) { return rows <= 8 && takes_rows(rows, n); }
 // what product_kernel takes: HTR_OK or the status to refuse with
 int product_shape(long long rows, int m, int n, int experts, int type, bool grouped) {
   if (!is_8bit(type) && !is_16bit(type)) return HTR_ERR_DTYPE;
@@ -407,14 +438,24 @@ int htr_quantize_e4m3(const void* x, int64_t stride, int64_t rows, int n, int dt
   return HTR_OK;
 }
 
+int htr_product_rounds_int8(int64_t rows, int n) { return rounds_rows(rows, n); }
+
 int htr_product_rounds(int64_t rows, int experts, int grouped) { return rows > 0 && experts > 0 && takes_16bit_rows(rows, experts, grouped != 0); }
 
 int htr_product_plan(int64_t rows, int m, int n, int experts, int grouped, int gated, int type, int x_type, int* out6) {
   if (!out6) return HTR_ERR_NULL;
   const int rc = product_shape(rows, m, n, experts, type, grouped != 0);
   if (rc != HTR_OK) return rc;
-  if (x_type != type && !(type == HTR_E4M3 && is_16bit(x_type) && !gated && takes_16bit_rows(rows, experts, grouped != 0))) return HTR_ERR_DTYPE;
+  if (x_type != type && !(type == HTR_E4M3 && is_16bit(x_type) && !gated && takes_16bit_rows(rows, experts, grouped != 0)) &&
+      !(type == HTR_I8 && is_dtype(x_type) && !grouped && rounds_rows(rows, n)))
+    return HTR_ERR_DTYPE;
   if (rows == 0 || (gated && (!grouped || m % (2 * unit_of(type)) || !gates_in_one(rows, experts))) || (!grouped && experts != 1)) return HTR_ERR_SIZE;
+  if (type == HTR_I8 && !grouped && takes_rows(rows, n)) {
+    const RowsGrid g = rows_grid((int)rows, m, n);
+    const int v[6] = {ROWS_TILE, g.columns, ROWS_WAVES, 0, g.workgroups, g.tiles};
+    memcpy(out6, v, sizeof(v));
+    return HTR_OK;
+  }
   const int some = 0;      // the choice asks whether there are ends, not what they hold
   ProductArgs a{};
   a.rows = (int)rows; a.m = m; a.n = n; a.experts = experts; a.x_type = x_type;
@@ -431,13 +472,20 @@ int htr_product(const void* x, int x_type, const void* x_scales, const void* w, 
   const int rc = product_shape(rows, m, n, experts, type, ends != nullptr);
   if (rc != HTR_OK) return rc;
   if (!is_dtype(y_dtype)) return HTR_ERR_DTYPE;
-  if (x_type != type && !(type == HTR_E4M3 && is_16bit(x_type) && takes_16bit_rows(rows, experts, ends != nullptr))) return HTR_ERR_DTYPE;
+  if (x_type != type && !(type == HTR_E4M3 && is_16bit(x_type) && takes_16bit_rows(rows, experts, ends != nullptr)) &&
+      !(type == HTR_I8 && is_dtype(x_type) && ends == nullptr && rounds_rows(rows, n)))
+    return HTR_ERR_DTYPE;
   if (ends == nullptr && experts != 1) return HTR_ERR_NULL;
   if (rows == 0) return HTR_OK;
   if (!x || !w || !y || (is_8bit(x_type) && !x_scales) || (is_8bit(type) && !w_scales)) return HTR_ERR_NULL;
   if (!aligned(x, 16) || !aligned(w, 16) || !aligned(y, 16) || !aligned(x_scales, 4) || !aligned(w_scales, 4) || !aligned(ends, 4) ||
       !aligned(bias, element_bytes(y_dtype)))
     return HTR_ERR_ALIGN;
+  if (type == HTR_I8 && ends == nullptr && takes_rows(rows, n)) {
+    const RowsArgs r{x, (const float*)x_scales, (const uint8_t*)w, (const float*)w_scales, bias, y, (int)rows, m, n, x_type, y_dtype};
+    TRY_HIP(launch_rows(r, (hipStream_t)stream));
+    return HTR_OK;
+  }
   const ProductArgs a{x, (const float*)x_scales, w, (const float*)w_scales, bias, y, ends, nullptr, (int)rows, m, n, experts, y_dtype, x_type, nullptr, false};
   TRY_HIP(launch_product(a, type, false, (hipStream_t)stream));
   return HTR_OK;

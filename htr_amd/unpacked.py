@@ -214,8 +214,11 @@ def _pair(x):
 
 
 def _check_rows(what, x, experts, grouped, kind=E4M3):
-    """x as htr_product takes it with an 8-bit weight: contiguous 8-bit rows (values, scales), to which a tensor is rounded, or few 16-bit rows (x, None)."""
+    """x as htr_product takes it with an 8-bit weight: contiguous 8-bit rows (values, scales), to which a tensor is rounded, or few floating rows (x, None)."""
     if kind is I8:
+        n = x.shape[-1] if isinstance(x, torch.Tensor) else 0
+        if n and not grouped and x.dtype in _FLOATS and n % 16 == 0 and _native.lib().htr_product_rounds_int8(x.numel() // n, n):
+            return _packed(x), None
         q, s = x if _pair(x) else quantize_int8(x)
         if q.dtype != I8 or s.dtype != torch.float32 or q.dim() < 1 or s.shape != q.shape[:-1] or q.shape[-1] % 16:
             raise RuntimeError(f"{what}: 8-bit rows for an int8 weight are (int8 [..., n], float32 [...]), n a multiple of 16")

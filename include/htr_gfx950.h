@@ -347,7 +347,8 @@ int htr_quantize_e4m3(const void* x, int64_t stride, int64_t rows, int n, int dt
  * product of a row's scale and a block's is float32 as well: one below 2^-126 has fewer bits, one beyond float32 is infinite, and NaN times a zero.
  * Sums of int8 products are exact; they are converted to float32, then multiplied with the row's and with the channel's scale.
  *   type    of w: HTR_E4M3 or HTR_I8 (with its scales), HTR_BF16 or HTR_F16 (scales NULL)
- *   x_type  type; with e4m3 matrices also HTR_BF16 or HTR_F16 (x_scales NULL) where htr_product_rounds says so: rounded as by htr_quantize_e4m3
+ *   x_type  type; with e4m3 matrices also HTR_BF16 or HTR_F16 (x_scales NULL) where htr_product_rounds says so: rounded as by htr_quantize_e4m3;
+ *           with one int8 matrix also HTR_BF16, HTR_F16 or HTR_F32 where htr_product_rounds_int8 says so: rounded as by htr_quantize_int8
  *   x       [rows][n], w [experts][m][n], 16-byte aligned; n a multiple of 128 (e4m3), of 16 (int8, below 2^17) or of 8 (16 bits), up to 2^22; m up to 2^26; experts up to 65535
  *   ends    device int32 [experts]: expert e has rows ends[e - 1] .. ends[e] - 1 (from 0); rows from the last end on become zeros.  An end below
  *           an earlier one, or beyond rows, counts as that one, or as rows.  NULL: one matrix (experts = 1) for all rows
@@ -358,10 +359,12 @@ int htr_product(const void* x, int x_type, const void* x_scales, const void* w, 
                 int64_t rows, int m, int n, int experts, int type, int y_dtype, void* stream);
 /* 1 where htr_product takes 16-bit rows with e4m3 matrices and rounds them on the way (few rows), otherwise 0: htr_quantize_e4m3 first.  grouped: ends is given. */
 int htr_product_rounds(int64_t rows, int experts, int grouped);
+/* 1 where htr_product takes floating rows with one int8 matrix (ends NULL) and rounds them on the way (few rows, n up to some thousand), otherwise 0. */
+int htr_product_rounds_int8(int64_t rows, int n);
 /* The kernel behind htr_product for these sizes, or (gated = 1, with grouped = 1) behind the first product of htr_moe_stacked, where gate and up are
  * one launch: m = 2 inter, more than 4 rows to an expert on average, HTR_ERR_SIZE otherwise.  out6 = {matrix rows of a tile, rows of x of a tile, waves of a workgroup,
- * stages of its ring in LDS (0: each workgroup has one tile, straight from memory), workgroups, tiles (grouped: at most)}.  Workgroups of the ring
- * kernel go on from tile to tile.  For tests and tuning. */
+ * stages of its ring in LDS (0: straight from memory), workgroups, tiles (grouped: at most)}.  Where there are fewer workgroups than tiles they go on from
+ * tile to tile.  For tests and tuning. */
 int htr_product_plan(int64_t rows, int m, int n, int experts, int grouped, int gated, int type, int x_type, int* out6);
 
 /*

@@ -222,7 +222,7 @@ def test_more_rows_than_a_launch_takes(gen):
 # ---- products
 @pytest.mark.gpu
 @pytest.mark.parametrize("m,n", [(1, 16), (100, 256), (128, 656), (384, 4096), (1030, 1168)])
-@pytest.mark.parametrize("rows", [1, 2, 5, 16, 17, 33, 64, 65, 100, 193, 300])
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 5, 7, 8, 9, 16, 17, 32, 33, 64, 65, 100, 193, 300])
 def test_linear_int8(gen, m, n, rows):
     w, ws = weight(gen, m, n)
     for dtype, bias in ((BF16, False), (F16, True), (F32, True)):
@@ -235,6 +235,27 @@ def test_linear_int8(gen, m, n, rows):
         assert_within(y, want, bound)
         assert torch.equal(ops.linear_int8(pair, w, ws, b, out_dtype=dtype), y)        # rounded ahead or on the way
     assert ops.linear_int8(pair, w, ws).dtype == BF16 and ops.linear_int8(pair, w, ws, b.half()).dtype == F16
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n", [(5, 32), (7, 2048), (2047, 2064), (2600, 272), (70000, 48), (300, 20480), (9, 131056)])
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 6, 8, 11, 16, 23, 32])
+def test_few_rows(gen, m, n, rows):
+    """Rows that lie in LDS: matrices of more and of fewer tiles than workgroups, more than 32 tiles to one, rows of less than a step, and sizes that LDS does not hold."""
+    w, ws = weight(gen, m, n)
+    x, b = randn(gen, rows, n), randn(gen, m)
+    pair = ops.quantize_int8(x)
+    want, bound = product_bound(pair, (w, ws), F32, b)
+    y = ops.linear_int8(x, w, ws, b)
+    assert_within(y, want, bound)
+    assert torch.equal(ops.linear_int8(pair, w, ws, b), y)
+    around = torch.full((rows + 2, m), 7.0, device="cuda")            # what lies around the result is left
+    L, p = _native.lib(), lambda t: t.data_ptr()
+    if (m * 4) % 16 == 0:
+        y = around[1:rows + 1]
+        assert L.htr_product(p(pair[0]), 4, p(pair[1]), p(w), p(ws), p(b), None, p(y), rows, m, n, 1, 4, 2, torch.cuda.current_stream().cuda_stream) == 0
+        assert_within(y, want, bound)
+        assert (around[0] == 7).all() and (around[-1] == 7).all()
 
 
 @pytest.mark.gpu
@@ -567,8 +588,12 @@ def test_status_codes_without_a_gpu():
     assert quant(rows=0) == 0 and quant(n=24) == 11 and quant(dt=4) == 5 and quant(q=None) == 1 and quant(x=odd) == 7 and quant(q=odd) == 7 and quant(n=(1 << 30) + 16) == 11
     prod = lambda x=p, xs=p, w=p, ws=p, b=None, ends=None, y=p, rows=1, m=128, n=128, E=1, xt=4, yt=0: \
         L.htr_product(x, xt, xs, w, ws, b, ends, y, rows, m, n, E, 4, yt, None)
-    assert prod(rows=0) == 0 and prod(n=24) == 11 and prod(n=1 << 17) == 11 and prod(m=0) == 11 and prod(yt=4) == 5 and prod(xt=3) == 5 and prod(xt=2) == 5 and prod(E=2) == 1
+    assert prod(rows=0) == 0 and prod(n=24) == 11 and prod(n=1 << 17) == 11 and prod(m=0) == 11 and prod(yt=4) == 5 and prod(xt=3) == 5 and prod(xt=2, ws=None) == 1 and prod(xt=2, rows=9) == 5 and prod(E=2) == 1
     assert prod(xs=None) == 1 and prod(ws=None) == 1 and prod(x=odd) == 7 and prod(w=odd) == 7 and prod(ws=odd) == 7 and prod(xs=odd) == 7
+    # floating rows with an int8 matrix: few, that the product rounds itself, and one matrix
+    floating = lambda xt, rows=1, n=128, ends=None, x=p: L.htr_product(x, xt, None, p, None, None, ends, p, rows, 64, n, 1, 4, 0, None)
+    assert [L.htr_product_rounds_int8(*a) for a in ((1, 4096), (8, 4096), (9, 4096), (0, 4096), (1, 131056), (8, 14336), (8, 24576))] == [1, 1, 0, 0, 1, 1, 0]
+    assert floating(0) == 1 and floating(2) == 1 and floating(3) == 5 and floating(0, rows=9) == 5 and floating(0, ends=p) == 5 and floating(1, rows=8, n=24576) == 5
     need = L.htr_moe_stacked_scratch_bytes
     assert need(4, 2, 8, 256, 128, 4) > 0 and need(4, 2, 8, 256, 72, 4) == 0 and need(4, 2, 8, 72, 128, 4) == 0 and need(4, 2, 8, 256, 80, 4) > 0 and need(4, 2, 8, 1 << 17, 128, 4) == 0
     a256 = ctypes.c_void_p(0x100000)
