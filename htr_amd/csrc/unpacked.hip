@@ -255,8 +255,60 @@ template <int T, typename F> auto product_kernel(const ProductArgs& a, F take) {
     default: return take(Tiles<2, 2, 2, 1, 4>{});
   }
 }
+// ---- few rows in int8
+struct RowsGrid { int columns, kw, most, mtiles, workgroups; long long tiles; size_t lds; bool fits; };      // most: rows of a span; tiles: a bound where rows are grouped
+RowsGrid rows_grid(const ProductArgs& a) {
+  const bool grouped = a.ends != nullptr;
+  RowsGrid g;
+  // Experts' rows are uneven: spans of 16 or 32 read a matrix once that spans of 8 would read twice (us by 8, 16 and 32: 96 rows of 64 experts of 2816x2048 45.8, 46.0
+  // and 60 by whole teams, 256 62.5, 57.5 and 63, 500 -, 67.9 and 65.4; 80 of 8 of 14336x4096 -, 93 and 77)
+  g.columns = grouped ? (a.rows <= 6ll * a.experts ? 16 : 32) : a.rows <= 8 ? 8 : a.rows <= 16 ? 16 : 32;
+  g.most = a.rows < g.columns ? a.rows : g.columns;
+  // Waves to a team.  One matrix: all, so that few tiles come to as many workgroups (us by 8, 4 and 2: 1 row on 28672x4096 20.5, 21.7 and 22.3, 8 on 152064x4096 99.5, 100.3
+  // and 98.4).  Experts have tiles enough; fewer waves to one mean fewer ends of tiles, more leave long rows to few (96 rows of 64 experts of 2816x2048 51.7, 47.1 and
+  // 46.0, of 2048x1408 31.4, 28.9 and 26.9; 32 of 8 of 14336x4096 74.0, 73.3 and 76.3)
+  g.kw = !grouped ? 8 : a.n > 2048 ? 4 : 2;
+  g.mtiles = (a.m + rows_tile(g.kw) - 1) / rows_tile(g.kw);
+  const long long spans = span_bound(a.rows, a.experts, grouped, g.columns);
+  g.tiles = g.mtiles * spans;
+  g.lds = rows_lds(g.most, g.columns, a.n, g.kw, grouped);
+  // two workgroups to a compute unit where the rows of x are few to prepare (us by two and by one: 1 row on 6144x4096 7.7 and 8.0, 4 on 14336x4096 12.0 and 12.7,
+  // 8 on 152064x4096 102 and 101, 32 on 28672x4096 30 and 25)
+  int most = (a.rows <= 4 || grouped) && g.lds <= 80 * 1024 ? 512 : 256;
+  g.workgroups = (int)(g.tiles < most ? g.tiles : most);
+  g.fits = g.lds <= 160 * 1024 && spans / g.workgroups + 4 <= ROWS_SPANS;
+  return g;
+}
+template <int X, int CT, int KW, bool GROUPED> hipError_t launch_rows(const ProductArgs& a, const RowsGrid& g, hipStream_t st) {
+  const hipError_t e = allow_lds<k_product_rows<X, CT, KW, GROUPED>>(160 * 1024);
+  return e != hipSuccess ? e : launch(k_product_rows<X, CT, KW, GROUPED>, dim3(g.workgroups), ROWS_WAVES * 64, g.lds, st, a, g.mtiles, g.most);
+}
+hipError_t launch_rows(const ProductArgs& a, hipStream_t st) {
+  const RowsGrid g = rows_grid(a);
+  if (a.ends != nullptr) {
+    if (g.kw == 4) return g.columns == 16 ? launch_rows<P_I8, 2, 4, true>(a, g, st) : launch_rows<P_I8, 4, 4, true>(a, g, st);
+    return g.columns == 16 ? launch_rows<P_I8, 2, 2, true>(a, g, st) : launch_rows<P_I8, 4, 2, true>(a, g, st);
+  }
+  if (a.x_type == HTR_BF16) return launch_rows<HTR_BF16, 1, 8, false>(a, g, st);
+  if (a.x_type == HTR_F16) return launch_rows<HTR_F16, 1, 8, false>(a, g, st);
+  if (a.x_type == HTR_F32) return launch_rows<HTR_F32, 1, 8, false>(a, g, st);
+  return g.columns == 8    ? launch_rows<P_I8, 1, 8, false>(a, g, st)
+         : g.columns == 16 ? launch_rows<P_I8, 2, 8, false>(a, g, st)
+                           : launch_rows<P_I8, 4, 8, false>(a, g, st);
+}
+// Up to 32 rows of one matrix that LDS holds.  us by k_product_rows and by the faster of the kernels for more rows: 1 row on 1024x4096 4.9 and 5.3, on 6144x4096 7.7 and
+// 10.1, 8 on 152064x4096 101 and 125, 16 on 14336x4096 14.0 and 15.8, 32 on 28672x4096 25 and 29, on 4096x4096 9.6 and 8.8
+bool takes_rows(int64_t rows, int n) { return rows >= 1 && rows <= 32 && rows_lds((int)rows, 32, n, 8, false) <= 160 * 1024; }
+// Up to 8 of them rounded on the way, by every workgroup for itself: 1 row on 6144x4096 9.5 us, 8 rows 11.3 (rounded ahead 7.7 and 8.5, and 4.5 for that launch), 16 rows
+// on 14336x4096 19.2 (14.0 and 4.6)
+bool rounds_rows(int64_t rows, int n) { return rows <= 8 && takes_rows(rows, n); }
+// Up to 8 rows to an expert on average (us by k_product_rows and by the fastest of the others, 64 experts of 2816x2048: 96 rows 46 and 53, 256 57 and 69, 500 65 and 70,
+// 800 73 and 69; 8 of 14336x4096: 48 rows 74 and 88; 64 of 2048x1408: 400 rows 36 and 37, 800 43 and 39)
+bool few_int8(long long rows, int experts) { return rows <= 8ll * experts; }
+// the kernel for few rows, for a product in int8
+bool takes_rows(const ProductArgs& a) { return a.ends == nullptr ? takes_rows(a.rows, a.n) : few_int8(a.rows, a.experts) && rows_grid(a).fits; }
 // silu(gate) up of rows by expert, where one launch is the better way (few rows to an expert: the matrices are read by k_product_stream, k_gated follows)
-bool gates_in_one(long long rows, int experts) { return !takes_16bit_rows(rows, experts, true); }
+bool gates_in_one(long long rows, int experts, int type) { return type == HTR_I8 ? !few_int8(rows, experts) : !takes_16bit_rows(rows, experts, true); }
 template <int T, typename F> auto gated_kernel(const ProductArgs& a, F take) {
   switch (best_tile(GATED_TILES, a, (size_t)a.n * bytes_of<T>)) {
     case 0: return take(Tiles<2, 4, 8, 4, 2, true>{});
@@ -270,6 +322,7 @@ template <int T> hipError_t launch_product(const ProductArgs& a, bool gated, hip
   return gated ? gated_kernel<T>(a, take) : product_kernel<T>(a, take);
 }
 hipError_t launch_product(const ProductArgs& a, int type, bool gated, hipStream_t st) {
+  if (type == HTR_I8 && !gated && takes_rows(a)) return launch_rows(a, st);
   return type == HTR_E4M3 ? launch_product<P_F8>(a, gated, st) : type == HTR_I8 ? launch_product<P_I8>(a, gated, st) : type == HTR_BF16 ? launch_product<HTR_BF16>(a, gated, st) : launch_product<HTR_F16>(a, gated, st);
 }
 template <int T> void describe_product(const ProductArgs& a, bool gated, int* out) {
@@ -278,36 +331,6 @@ template <int T> void describe_product(const ProductArgs& a, bool gated, int* ou
 }
 // columns: whole blocks of e4m3, rows on 16-byte boundaries
 int unit_of(int type) { return type == HTR_E4M3 ? 128 : type == HTR_I8 ? 16 : 8; }
-// ---- few rows in int8
-struct RowsGrid { int columns, tiles, workgroups; size_t lds; };
-RowsGrid rows_grid(int rows, int m, int n) {
-  RowsGrid g;
-  g.columns = rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
-  g.tiles = (m + ROWS_TILE - 1) / ROWS_TILE;
-  g.lds = rows_lds(rows, g.columns, n);
-  // two workgroups to a compute unit where the rows of x are few to prepare (us by two and by one: 1 row on 6144x4096 7.7 and 8.0, 4 on 14336x4096 12.0 and 12.7,
-  // 8 on 152064x4096 102 and 101, 32 on 28672x4096 30 and 25)
-  const int most = rows <= 4 && g.lds <= 80 * 1024 ? 512 : 256;
-  g.workgroups = g.tiles < most ? g.tiles : most;
-  return g;
-}
-template <int X, int CT> hipError_t launch_rows(const RowsArgs& a, const RowsGrid& g, hipStream_t st) {
-  const hipError_t e = allow_lds<k_product_rows<X, CT>>(160 * 1024);
-  return e != hipSuccess ? e : launch(k_product_rows<X, CT>, dim3(g.workgroups), ROWS_WAVES * 64, g.lds, st, a, g.tiles);
-}
-hipError_t launch_rows(const RowsArgs& a, hipStream_t st) {
-  const RowsGrid g = rows_grid(a.rows, a.m, a.n);
-  if (a.x_type == HTR_BF16) return launch_rows<HTR_BF16, 1>(a, g, st);
-  if (a.x_type == HTR_F16) return launch_rows<HTR_F16, 1>(a, g, st);
-  if (a.x_type == HTR_F32) return launch_rows<HTR_F32, 1>(a, g, st);
-  return g.columns == 8 ? launch_rows<P_I8, 1>(a, g, st) : g.columns == 16 ? launch_rows<P_I8, 2>(a, g, st) : launch_rows<P_I8, 4>(a, g, st);
-}
-// Up to 32 rows that LDS holds.  us by k_product_rows and by the faster of the kernels for more rows: 1 row on 1024x4096 4.9 and 5.3, on 6144x4096 7.7 and 10.1, 8 on
-// 152064x4096 101 and 125, 16 on 14336x4096 14.0 and 15.8, 32 on 28672x4096 25 and 29, on 4096x4096 9.6 and 8.8
-bool takes_rows(int64_t rows, int n) { return rows >= 1 && rows <= 32 && rows_lds((int)rows, 32, n) <= 160 * 1024; }
-// Up to 8 of them rounded on the way, by every workgroup for itself: 1 row on 6144x4096 9.5 us, 8 rows 11.3 (rounded ahead 7.7 and 8.5, and 4.5 for that launch), 16 rows
-// on 14336x4096 19.2 (14.0 and 4.6)
-bool rounds_rows(int64_t rows, int n) { return rows <= 8 && takes_rows(rows, n); }
 // what product_kernel takes: HTR_OK or the status to refuse with
 int product_shape(long long rows, int m, int n, int experts, int type, bool grouped) {
   if (!is_8bit(type) && !is_16bit(type)) return HTR_ERR_DTYPE;
@@ -326,7 +349,7 @@ struct StackedScratch {
     size_t at = 0;
     auto take = [&](size_t n) { const size_t here = at; at += (n + 255) / 256 * 256; return here; };
     const size_t pairs = (size_t)tokens * top;
-    const bool f8 = type == HTR_E4M3, i8 = type == HTR_I8, in_one = gates_in_one(pairs, experts);
+    const bool f8 = type == HTR_E4M3, i8 = type == HTR_I8, in_one = gates_in_one(pairs, experts, type);
     ends = take((size_t)experts * 4);
     token = take(pairs * 4);
     pos_of = take(pairs * 4);
@@ -449,17 +472,17 @@ int htr_product_plan(int64_t rows, int m, int n, int experts, int grouped, int g
   if (x_type != type && !(type == HTR_E4M3 && is_16bit(x_type) && !gated && takes_16bit_rows(rows, experts, grouped != 0)) &&
       !(type == HTR_I8 && is_dtype(x_type) && !grouped && rounds_rows(rows, n)))
     return HTR_ERR_DTYPE;
-  if (rows == 0 || (gated && (!grouped || m % (2 * unit_of(type)) || !gates_in_one(rows, experts))) || (!grouped && experts != 1)) return HTR_ERR_SIZE;
-  if (type == HTR_I8 && !grouped && takes_rows(rows, n)) {
-    const RowsGrid g = rows_grid((int)rows, m, n);
-    const int v[6] = {ROWS_TILE, g.columns, ROWS_WAVES, 0, g.workgroups, g.tiles};
-    memcpy(out6, v, sizeof(v));
-    return HTR_OK;
-  }
+  if (rows == 0 || (gated && (!grouped || m % (2 * unit_of(type)) || !gates_in_one(rows, experts, type))) || (!grouped && experts != 1)) return HTR_ERR_SIZE;
   const int some = 0;      // the choice asks whether there are ends, not what they hold
   ProductArgs a{};
   a.rows = (int)rows; a.m = m; a.n = n; a.experts = experts; a.x_type = x_type;
   a.ends = grouped ? &some : nullptr;
+  if (type == HTR_I8 && !gated && takes_rows(a)) {
+    const RowsGrid g = rows_grid(a);
+    const int v[6] = {rows_tile(g.kw), g.columns, ROWS_WAVES, 0, g.workgroups, (int)g.tiles};
+    memcpy(out6, v, sizeof(v));
+    return HTR_OK;
+  }
   if (type == HTR_E4M3) describe_product<P_F8>(a, gated != 0, out6);
   else if (type == HTR_I8) describe_product<P_I8>(a, gated != 0, out6);
   else if (type == HTR_BF16) describe_product<HTR_BF16>(a, gated != 0, out6);
@@ -481,11 +504,6 @@ int htr_product(const void* x, int x_type, const void* x_scales, const void* w, 
   if (!aligned(x, 16) || !aligned(w, 16) || !aligned(y, 16) || !aligned(x_scales, 4) || !aligned(w_scales, 4) || !aligned(ends, 4) ||
       !aligned(bias, element_bytes(y_dtype)))
     return HTR_ERR_ALIGN;
-  if (type == HTR_I8 && ends == nullptr && takes_rows(rows, n)) {
-    const RowsArgs r{x, (const float*)x_scales, (const uint8_t*)w, (const float*)w_scales, bias, y, (int)rows, m, n, x_type, y_dtype};
-    TRY_HIP(launch_rows(r, (hipStream_t)stream));
-    return HTR_OK;
-  }
   const ProductArgs a{x, (const float*)x_scales, w, (const float*)w_scales, bias, y, ends, nullptr, (int)rows, m, n, experts, y_dtype, x_type, nullptr, false};
   TRY_HIP(launch_product(a, type, false, (hipStream_t)stream));
   return HTR_OK;
@@ -519,19 +537,19 @@ int htr_moe_stacked(const void* x, int dtype, const void* ids, int ids_int64, co
     a.x_type = HTR_I8;
     TRY_HIP(launch_round(x, dtype, hidden, tokens, hidden, s + at.xq, s + at.xs, st));
     a.x = s + at.xq; a.xs = (const float*)(s + at.xs);
-  } else if (f8 && gates_in_one(pairs, experts)) {
+  } else if (f8 && gates_in_one(pairs, experts, type)) {
     a.x_type = HTR_E4M3;
     TRY_HIP(launch_quantize(x, dtype, tokens, hidden, hidden, s + at.xq, (float*)(s + at.xs), st));
     a.x = s + at.xq; a.xs = (const float*)(s + at.xs);
   }
   if (i8) {
     // silu(gate) up stays float32 until a row's largest is known
-    const bool in_one = gates_in_one(pairs, experts);
+    const bool in_one = gates_in_one(pairs, experts, type);
     TRY_HIP(launch_product(a, type, in_one, st));
     const int* last = ends + experts - 1;
     TRY_HIP((in_one ? launch_round<HTR_F32, false>(h, inter, pairs, inter, last, s + at.a, s + at.as, st)
                     : launch_round<HTR_F32, true>(h, 2 * inter, pairs, inter, last, s + at.a, s + at.as, st)));
-  } else if (gates_in_one(pairs, experts)) {
+  } else if (gates_in_one(pairs, experts, type)) {
     a.y = s + at.a; a.ys = (float*)(s + at.as); a.y_dtype = type;
     TRY_HIP(launch_product(a, type, true, st));
   } else {

@@ -352,6 +352,21 @@ def test_grouped_mm(gen, counts, m, n, behind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("counts", [[0, 3, 0, 0, 17, 1, 0, 5], [1] * 300, [40] + [0] * 9, [2, 0] * 100 + [33], [8] * 12, [7, 7, 7, 7, 20, 0, 1]], ids=lambda c: f"{len(c)}x{sum(c)}")
+@pytest.mark.parametrize("m,n", [(7, 16), (66, 784), (520, 2048), (300, 2064), (1030, 4112), (40, 16400)])
+@pytest.mark.parametrize("behind", [0, 3, 40])
+def test_grouped_mm_of_few_rows(gen, counts, m, n, behind):
+    """Several experts, and several tiles of one, to a workgroup; experts of more rows than go together; rows that LDS does not hold."""
+    R = sum(counts) + behind
+    x, w = ops.quantize_int8(randn(gen, R, n)), weight(gen, len(counts), m, n)
+    check_grouped(x, w, counts, BF16, ops.grouped_mm(x, w, _ends(counts)))
+    x[1][:] = 1.0
+    x[1][R // 2] = math.nan                            # a row without a value keeps to itself, and so does a matrix that no row asks for
+    w[1][counts.index(0) if 0 in counts else 0] = math.nan
+    check_grouped(x, w, counts, F32, ops.grouped_mm(x, w, _ends(counts), out_dtype=F32))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("counts,m", [([e * 7 % 37 for e in range(130)], 512), ([2000, 0, 3100], 4096), ([0] * 63 + [1900, 0, 2500] + [1] * 70, 1000),
                                       ([300 - 4 * e for e in range(75)], 1024), ([0] * 64 + [700], 2900)], ids=lambda c: str(len(c) if isinstance(c, list) else c))
 def test_grouped_mm_of_more_tiles_than_run_at_once(gen, counts, m):
@@ -405,7 +420,7 @@ def experts(gen, E, H, F):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF16, F16])
-@pytest.mark.parametrize("T,E,top,H,F", [(1, 4, 2, 256, 128), (5, 8, 3, 144, 400), (40, 3, 1, 256, 256), (9, 70, 8, 128, 128), (70, 2, 2, 400, 144), (60, 70, 7, 256, 16), (300, 4, 2, 32, 80)])
+@pytest.mark.parametrize("T,E,top,H,F", [(1, 4, 2, 256, 128), (5, 8, 3, 144, 400), (40, 3, 1, 256, 256), (9, 70, 8, 128, 128), (70, 2, 2, 400, 144), (60, 70, 7, 256, 16), (300, 4, 2, 32, 80), (9, 12, 5, 2064, 48), (50, 40, 6, 80, 2080)])
 @pytest.mark.parametrize("ids64", [True, False])
 def test_moe_experts_stacked(gen, dtype, T, E, top, H, F, ids64):
     x, wt = randn(gen, T, H, dtype=dtype), torch.rand(T, top, device="cuda", generator=gen)
