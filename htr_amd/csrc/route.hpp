@@ -152,33 +152,57 @@ template <int PER> __device__ __forceinline__ void route_exact(const RouteArgs& 
 // The threshold between the chosen and the others is found by halving the span of ranks (as integers): a comparison and a count of lanes to each element, until exactly
 // `top` lie above it, which takes about ten steps; the largest one by one takes a wave's maximum for each.  Whatever lies next to the threshold is a candidate, too, and
 // candidates too close to each other are ordered by their ranks in 64 bits, groups likewise.
-struct Candidate { uint32_t key; int e; float l, b; };
-template <int H> __device__ __forceinline__ void two_largest(float& first, float& second) {      // with lane ^ H
-  const float f = lane_xor_dpp<H>(first), s = lane_xor_dpp<H>(second);
-  second = fmaxf(fmaxf(second, s), fminf(first, f));
-  first = fmaxf(first, f);
+struct Candidate { float rank; int e; float l, b; };
+__device__ __forceinline__ void two_largest(uint32_t& first, uint32_t& second, uint32_t f, uint32_t s) {      // of both
+  second = max(max(second, s), min(first, f));
+  first = max(first, f);
+}
+template <int H> __device__ __forceinline__ void two_largest(uint32_t& first, uint32_t& second) {                // with lane ^ H
+  two_largest(first, second, __float_as_uint(lane_xor_dpp<H>(__uint_as_float(first))), __float_as_uint(lane_xor_dpp<H>(__uint_as_float(second))));
 }
 template <int PER> struct Route {
   const RouteArgs& a;
   const int lane, parts_log2, parts, g, p, e0;
   const bool biased, scored;      // scored: some ranks are no logits
   float l[PER], b[PER], most;     // a token's; most: the largest logit (softmax)
+  bool odd_bias;                  // one that float32 sums are not for
   __device__ __forceinline__ Route(const RouteArgs& a, int lane)
       : a(a), lane(lane), parts_log2(a.parts_log2), parts(1 << a.parts_log2), g(lane >> a.parts_log2), p(lane & ((1 << a.parts_log2) - 1)), e0(g * a.size + p),
-        biased(a.bias != nullptr), scored(a.bias != nullptr || (a.groups > 1 && a.group_best > 1)) {
+        biased(a.bias != nullptr), scored(a.bias != nullptr || (a.groups > 1 && a.group_best > 1)), odd_bias(false) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) b[i] = biased && in(i) ? ((const HTR_GLOBAL float*)a.bias)[e0 + i * parts] : 0.f;
+    for (int i = 0; i < PER; ++i) b[i] = 0.f;
+    if (biased) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) b[i] = ((const HTR_GLOBAL float*)a.bias)[at(i)];
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        b[i] = in(i) ? b[i] : 0.f;
+        odd_bias |= (magnitude(b[i]) >= 0x5D800000u) & (b[i] != -INFINITY);      // 2^60
+      }
+    }
   }
-  __device__ __forceinline__ bool in(int i) const { return g < a.groups && p + i * parts < a.size; }
+  __device__ __forceinline__ bool in(int i) const { return (g < a.groups) & (p + i * parts < a.size); }
+  __device__ __forceinline__ int at(int i) const { return min(e0 + i * parts, a.experts - 1); }      // where it may be loaded from
+  // All loads at once, none behind a condition of its lane
   __device__ __forceinline__ void load(long long token, float (&to)[PER]) const {
-    const size_t row = (size_t)(token * a.stride) + e0;
-    auto from = [&](auto type) {
+    const size_t row = (size_t)(token * a.stride);
+    if (a.dtype == HTR_F32) {
 #pragma unroll
-      for (int i = 0; i < PER; ++i) to[i] = in(i) ? load_elem_g(a.logits, decltype(type)::value, row + i * parts) : -INFINITY;
-    };
-    if (a.dtype == HTR_F32) from(std::integral_constant<int, HTR_F32>());
-    else if (a.dtype == HTR_BF16) from(std::integral_constant<int, HTR_BF16>());
-    else from(std::integral_constant<int, HTR_F16>());
+      for (int i = 0; i < PER; ++i) to[i] = ((const HTR_GLOBAL float*)a.logits)[row + at(i)];
+    } else {
+      uint32_t raw[PER];
+#pragma unroll
+      for (int i = 0; i < PER; ++i) raw[i] = ((const HTR_GLOBAL uint16_t*)a.logits)[row + at(i)];
+      if (a.dtype == HTR_BF16) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) to[i] = __uint_as_float(raw[i] << 16);
+      } else {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) to[i] = f16_bits_to_float((uint16_t)raw[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) to[i] = in(i) ? to[i] : -INFINITY;
   }
   __device__ __forceinline__ double all64() const {      // the softmax's sum
     double total = 0.0;
@@ -190,60 +214,59 @@ template <int PER> struct Route {
   // The token's candidates: their number, at least `top`; 0 where ranks are no finite numbers, or there are more than 64.  `to`(n): where they go.
   template <typename F> __device__ __forceinline__ int select(F to) {
     const int top = a.top;
-    bool odd = false;
+    bool odd = odd_bias;
     most = -INFINITY;
 #pragma unroll
     for (int i = 0; i < PER; ++i) { odd |= !(l[i] < INFINITY); most = fmaxf(most, l[i]); }
+    if (__ballot(odd)) return 0;
     if (!a.sigmoid) most = value_of_key(wave_max(key_of(most)));
-    float rank[PER], score[PER];
+    float score[PER];
+    uint32_t key[PER];      // of the ranks
     if (scored) {
-      float sum = 0.f;
+      if (a.sigmoid) {
 #pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const float e = __expf(a.sigmoid ? -l[i] : l[i] - most);
-        score[i] = a.sigmoid ? __builtin_amdgcn_rcpf(1.f + e) : e;
-        sum += e;
-      }
-      if (!a.sigmoid) {
+        for (int i = 0; i < PER; ++i) score[i] = __builtin_amdgcn_rcpf(1.f + __expf(-l[i]));
+      } else {
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) { score[i] = __expf(l[i] - most); sum += score[i]; }
         sum = 1.f / wave_sum(sum);
 #pragma unroll
         for (int i = 0; i < PER; ++i) score[i] *= sum;
       }
     }
+    if (biased) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      rank[i] = l[i];
-      if (biased) {
-        rank[i] = l[i] == -INFINITY || b[i] == -INFINITY ? -INFINITY : score[i] + b[i];
-        odd |= !(rank[i] < 0x1p60f) || (rank[i] < -0x1p60f && rank[i] != -INFINITY);
-      }
+      for (int i = 0; i < PER; ++i) key[i] = key_of(l[i] == -INFINITY ? l[i] : score[i] + b[i]);      // a bias of -inf masks, too
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) key[i] = key_of(l[i]);
     }
-    if (__ballot(odd)) return 0;
     // float32 ranks, and differences of two, are off by less: a score by 2 PER + 32 steps of 2^-24 at most (the exponential and its argument 6, the sum PER + 5, its
     // inverse and the product 3), the sum with the bias by one more of its own
     const float slack = (2 * PER + 32) * 0x1p-24f;
     bool out = g >= a.groups;
     if (a.groups > 1) {
       // a lane's two largest, then those of the group's lanes
-      float first = -INFINITY, second = -INFINITY;
-      const bool by_rank = biased || a.group_best == 1, two = a.group_best > 1 && a.size > 1;
+      uint32_t k1 = KEY_MASKED, k2 = KEY_MASKED;
+      const bool two = a.group_best > 1 && a.size > 1;
+      if (biased || a.group_best == 1) {
 #pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const float v = by_rank || rank[i] == -INFINITY ? rank[i] : score[i];
-        second = fmaxf(second, fminf(first, v));
-        first = fmaxf(first, v);
+        for (int i = 0; i < PER; ++i) two_largest(k1, k2, key[i], KEY_MASKED);
+      } else {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) two_largest(k1, k2, key[i] == KEY_MASKED ? KEY_MASKED : key_of(score[i]), KEY_MASKED);
       }
-      if (parts > 1) two_largest<1>(first, second);
-      if (parts > 2) two_largest<2>(first, second);
-      if (parts > 4) two_largest<4>(first, second);
-      if (parts > 8) two_largest<8>(first, second);
+      if (parts > 1) two_largest<1>(k1, k2);
+      if (parts > 2) two_largest<2>(k1, k2);
+      if (parts > 4) two_largest<4>(k1, k2);
+      if (parts > 8) two_largest<8>(k1, k2);
       if (parts > 16) {
-        float f0, f1, s0, s1;
-        halves16(first, f0, f1);
-        halves16(second, s0, s1);
-        second = fmaxf(fmaxf(s0, s1), fminf(f0, f1));
-        first = fmaxf(f0, f1);
+        const u2s x = __builtin_amdgcn_permlane16_swap(k1, k1, false, false), y = __builtin_amdgcn_permlane16_swap(k2, k2, false, false);
+        k1 = x.x; k2 = y.x;
+        two_largest(k1, k2, x.y, y.y);
       }
+      const float first = value_of_key(k1), second = value_of_key(k2);
       // each group's lanes compare it with as many others at once
       const unsigned long long own = ((1ull << parts) - 1) << (g << parts_log2);
       auto count_better = [&](auto mine, auto near, bool& close) {
@@ -251,8 +274,8 @@ template <int PER> struct Route {
         for (int k = 0; k < a.groups; k += parts) {
           const auto other = __shfl(mine, (k + p) << parts_log2);
           const bool there = k + p < a.groups;
-          better += (int)__builtin_popcountll(__ballot(there && (other > mine || (other == mine && k + p < g))) & own);
-          close |= there && k + p != g && !(other > mine + near) && !(other < mine - near);
+          better += (int)__builtin_popcountll(__ballot(there & ((other > mine) | ((other == mine) & (k + p < g)))) & own);
+          close |= there & (k + p != g) & !(other > mine + near) & !(other < mine - near);
         }
         return better;
       };
@@ -265,7 +288,7 @@ template <int PER> struct Route {
         double first = -INFINITY, second = -INFINITY;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-          const double v = rank[i] == -INFINITY ? -INFINITY : (a.sigmoid ? sigmoid64(l[i]) : exp((double)l[i] - (double)most) / total) + (double)b[i];
+          const double v = key[i] == KEY_MASKED ? -INFINITY : (a.sigmoid ? sigmoid64(l[i]) : exp((double)l[i] - (double)most) / total) + (double)b[i];
           second = fmax(second, fmin(first, v));
           first = fmax(first, v);
         }
@@ -278,10 +301,11 @@ template <int PER> struct Route {
       }
       out |= better >= a.top_groups;
     }
-    uint32_t key[PER], largest = 0;
+    uint32_t largest = 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      key[i] = !in(i) ? 0u : out ? KEY_MASKED : key_of(rank[i]);
+      key[i] = out ? KEY_MASKED : key[i];
+      key[i] = in(i) ? key[i] : 0u;
       largest = max(largest, key[i]);
     }
     largest = __builtin_amdgcn_readfirstlane(wave_max(largest));
@@ -306,7 +330,7 @@ template <int PER> struct Route {
       const int m = count(mid);
       if (m >= top) { lo = mid; n = m; } else hi = mid;
     }
-    unsigned long long taken[PER];
+    bool taken[PER];
     if ((biased && lo > KEY_MASKED) || n == top) {
       if (biased && lo > KEY_MASKED) {
         const float t = value_of_key(lo);
@@ -315,7 +339,7 @@ template <int PER> struct Route {
         if (n > 64) return 0;
       }
 #pragma unroll
-      for (int i = 0; i < PER; ++i) taken[i] = __ballot(key[i] >= lo);
+      for (int i = 0; i < PER; ++i) taken[i] = key[i] >= lo;
     } else {
       // lo itself is the rank of several, of which the first by number are taken
       int ahead = 0;
@@ -330,45 +354,44 @@ template <int PER> struct Route {
       for (int i = 0; i < PER; ++i) {
         const int here = ahead + (int)__builtin_popcountll(at[i] & mine & lower);
         ahead += (int)__builtin_popcountll(at[i] & mine);
-        taken[i] = __ballot(key[i] > lo || (key[i] == lo && here < top));
+        taken[i] = key[i] > lo || (key[i] == lo && here < top);
       }
       n = top;
     }
     Candidate* place = to(n);
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      if (taken[i] >> lane & 1ull)
-        place[__builtin_amdgcn_mbcnt_hi((uint32_t)(taken[i] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)taken[i], 0))] = Candidate{key[i], e0 + i * parts, l[i], b[i]};
-      place += (int)__builtin_popcountll(taken[i]);
+      const unsigned long long lanes = __ballot(taken[i]);
+      if (taken[i])
+        place[__builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0))] = Candidate{value_of_key(key[i]), e0 + i * parts, l[i], b[i]};
+      place += (int)__builtin_popcountll(lanes);
     }
     return n;
   }
 
-  // Of tokens' candidates, LANES places and lanes to each, the chosen in order with their weights.  n, most, total: of the lane's token
-  template <int LANES> __device__ __forceinline__ void finish(const Candidate* place, long long token, int n, float most, double total) const {
+  // Of tokens' candidates, LANES places and lanes to each, the chosen in order with their weights.  n, most, total: of the lane's token; most_n: the largest n
+  template <int LANES> __device__ __forceinline__ void finish(const Candidate* place, long long token, int n, int most_n, float most, double total) const {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
     const int k = lane & (LANES - 1), top = a.top;
     place += lane - k;
-    const Candidate c = k < n ? place[k] : Candidate{KEY_MASKED, 0, -INFINITY, 0.f};
-    const bool none = c.key == KEY_MASKED;
-    const float v = value_of_key(c.key), near = (2 * PER + 32) * 0x1p-24f * (1.f + fabsf(v));
-    int order = 0;
-    bool close = false;
-    for (int j = 0; j < (LANES == 64 ? n : LANES); ++j) {
-      const uint32_t key = place[j].key;
-      const int e = place[j].e;
-      order += j < n && (key > c.key || (key == c.key && e < c.e));
-      close |= j < n && j != k && fabsf(value_of_key(key) - v) <= near;
+    const Candidate c = k < n ? place[k] : Candidate{-INFINITY, 0, -INFINITY, 0.f};
+    const bool none = c.rank == -INFINITY;
+    const float near = (2 * PER + 32) * 0x1p-24f * (1.f + fabsf(c.rank));
+    int order = 0, close = 0;
+    for (int j = 0; j < most_n; ++j) {      // places without a candidate hold -inf and the highest number
+      const float r = place[j].rank;
+      order += (r > c.rank) | ((r == c.rank) & (place[j].e < c.e));
+      close += fabsf(r - c.rank) <= near;
     }
     // scores of the candidates; of the softmax over the sum of all only where that does not cancel
     double w = none ? 0.0 : a.sigmoid ? sigmoid64(c.l) : exp((double)c.l - (double)most) / total;
-    if (biased && __ballot(close && !none)) {
+    if (biased && __ballot((close > 1) & !none)) {      // one of them is itself
       const long long mine = none ? ORDER_MASKED : order_of(w + (double)c.b);
       order = 0;
-      for (int j = 0; j < LANES; ++j) {
+      for (int j = 0; j < most_n; ++j) {
         const long long other = __shfl(mine, lane - k + j);
-        order += j < n && (other > mine || (other == mine && place[j].e < c.e));
+        order += (j < n) & ((other > mine) | ((other == mine) & (place[j].e < c.e)));
       }
     }
     const bool chosen = k < n && order < top;
@@ -393,11 +416,13 @@ __global__ __launch_bounds__(ROUTE_WAVES * 64) void k_route(const RouteArgs a) {
   const long long first = ((long long)blockIdx.x * ROUTE_WAVES + wv) * TOKENS;
   if (first >= a.tokens) return;
   Candidate *together = candidates[wv], *alone = candidates[wv] + (TOKENS == 1 ? 0 : 64);
+  if (TOKENS > 1) together[lane] = Candidate{-INFINITY, 0x7FFFFFFF, 0.f, 0.f};
   Route<PER> r(a, lane);
   float logits[TOKENS][PER];
 #pragma unroll
   for (int q = 0; q < TOKENS; ++q) r.load(min(first + q, a.tokens - 1), logits[q]);
-  int n = 0;
+  int n = 0, most_n = 0;
+  uint32_t left = 0;              // tokens for route_exact
   float most = 0.f;
   double total = 1.0;
 #pragma unroll
@@ -406,15 +431,18 @@ __global__ __launch_bounds__(ROUTE_WAVES * 64) void k_route(const RouteArgs a) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) r.l[i] = logits[q][i];
     const int found = r.select([&](int n) { return TOKENS > 1 && n <= 16 ? together + 16 * q : alone; });
-    if (found == 0) { route_exact<(PER < 16 ? PER : 16)>(a, first + q, lane); continue; }
+    if (found == 0 || (TOKENS > 1 && found > 16)) { left |= 1u << q; continue; }
+    most_n = max(most_n, found);
     const double sum = !a.sigmoid && r.most > -INFINITY && (!a.renormalize || r.biased) ? r.all64() : 1.0;
-    if (TOKENS == 1 || found > 16) {
-      r.template finish<64>(alone, first + q, found, r.most, sum);
+    if (TOKENS == 1) {
+      r.template finish<64>(alone, first, found, found, r.most, sum);
     } else if (lane >> 4 == q) {
       n = found;
       most = r.most;
       total = sum;
     }
   }
-  if constexpr (TOKENS > 1) r.template finish<16>(together, first + (lane >> 4), n, most, total);
+  if constexpr (TOKENS > 1) r.template finish<16>(together, first + (lane >> 4), n, most_n, most, total);
+#pragma unroll 1
+  for (; left != 0; left &= left - 1) route_exact<(PER < 16 ? PER : 16)>(a, first + __builtin_ctz(left), lane);
 }
