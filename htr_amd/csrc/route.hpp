@@ -9,7 +9,7 @@
 // One wave to a token.  Ranks that are logits are float32 as they are; others are first formed in float32, and only those that lie within what float32 may be off of each
 // other, or of what decides, are compared in 64 bits (Route); what that does not cover is done in 64 bits throughout (route_exact).  The weights of the chosen are
 // 64 bits either way.
-constexpr int ROUTE_MOST = 1024, ROUTE_WAVES = 4, ROUTE_TOGETHER = 4096;
+constexpr int ROUTE_MOST = 1024, ROUTE_WAVES = 4;
 
 struct RouteArgs {
   const void* logits;                 // [tokens][experts], `stride` elements from token to token
@@ -43,7 +43,26 @@ template <typename V> __device__ __forceinline__ V wave_largest(V v) {
   for (int off = 1; off < 64; off <<= 1) { const V w = __shfl_xor(v, off); v = w > v ? w : v; }
   return v;
 }
-__device__ __forceinline__ double sigmoid64(float l) { return 1.0 / (1.0 + exp(-(double)l)); }
+// 1 / x for x from 2^-1000 to 2^1000, off by 2^-51 at most: the instruction's 24 bits doubled twice.  A quotient as the language defines it takes four times the instructions.
+__device__ __forceinline__ double inverse64(double x) {
+  double r = __builtin_amdgcn_rcp(x);
+  r = __builtin_fma(__builtin_fma(-x, r, 1.0), r, r);
+  return __builtin_fma(__builtin_fma(-x, r, 1.0), r, r);
+}
+// e^x for x <= 0: 2^k times the series of e^r to r^13 for r = x - k log 2, |r| <= 0.347 (the next term is 4e-18); 0 where 64 bits hold nothing else
+__device__ __forceinline__ double exp64(double x) {
+  const double k = rint(x * 1.4426950408889634);
+  const double r = __builtin_fma(k, -2.3190468138462996e-17, __builtin_fma(k, -0.6931471805599453, x));      // log 2 in two parts
+  double p = 1.0 / 6227020800.0;
+  p = __builtin_fma(p, r, 1.0 / 479001600.0); p = __builtin_fma(p, r, 1.0 / 39916800.0); p = __builtin_fma(p, r, 1.0 / 3628800.0); p = __builtin_fma(p, r, 1.0 / 362880.0);
+  p = __builtin_fma(p, r, 1.0 / 40320.0); p = __builtin_fma(p, r, 1.0 / 5040.0); p = __builtin_fma(p, r, 1.0 / 720.0); p = __builtin_fma(p, r, 1.0 / 120.0);
+  p = __builtin_fma(p, r, 1.0 / 24.0); p = __builtin_fma(p, r, 1.0 / 6.0); p = __builtin_fma(p, r, 0.5); p = __builtin_fma(p, r, 1.0); p = __builtin_fma(p, r, 1.0);
+  return x < -746.0 ? 0.0 : __builtin_ldexp(p, (int)k);
+}
+__device__ __forceinline__ double sigmoid64(double l) {
+  const double e = exp64(-fabs(l)), r = inverse64(1.0 + e);
+  return l < 0.0 ? e * r : r;
+}
 
 // ---- in 64 bits: PER consecutive experts to a lane, the largest taken one after the other
 template <int PER> __device__ __forceinline__ void route_exact(const RouteArgs& a, long long token, int lane) {
@@ -56,15 +75,15 @@ template <int PER> __device__ __forceinline__ void route_exact(const RouteArgs& 
   }
   if (a.sigmoid) {
 #pragma unroll
-    for (int j = 0; j < PER; ++j) score[j] = 1.0 / (1.0 + exp(-l[j]));
+    for (int j = 0; j < PER; ++j) score[j] = sigmoid64(l[j]);
   } else {
     most = wave_largest(most);
     double sum = 0.0;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) { score[j] = l[j] == -INFINITY ? 0.0 : exp(l[j] - most); sum += score[j]; }
+    for (int j = 0; j < PER; ++j) { score[j] = l[j] == -INFINITY ? 0.0 : exp64(l[j] - most); sum += score[j]; }
     sum = wave_sum(sum);
 #pragma unroll
-    for (int j = 0; j < PER; ++j) score[j] = sum == 0.0 ? 0.0 : score[j] / sum;
+    for (int j = 0; j < PER; ++j) score[j] = sum == 0.0 ? 0.0 : score[j] * inverse64(sum);
   }
   long long rank[PER];
 #pragma unroll
@@ -207,12 +226,12 @@ template <int PER> struct Route {
   __device__ __forceinline__ double all64() const {      // the softmax's sum
     double total = 0.0;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) total += l[i] == -INFINITY ? 0.0 : exp((double)l[i] - (double)most);
+    for (int i = 0; i < PER; ++i) total += l[i] == -INFINITY ? 0.0 : exp64((double)l[i] - (double)most);
     return wave_sum(total);
   }
 
-  // The token's candidates: their number, at least `top`; 0 where ranks are no finite numbers, or there are more than 64.  `to`(n): where they go.
-  template <typename F> __device__ __forceinline__ int select(F to) {
+  // The token's candidates: their number, at least `top`; 0 where ranks are no finite numbers, or there are more than 64
+  __device__ __forceinline__ int select(Candidate* place) {
     const int top = a.top;
     bool odd = odd_bias;
     most = -INFINITY;
@@ -284,11 +303,11 @@ template <int PER> struct Route {
       int better = count_better(mine, 2.f * slack * (1.f + fabsf(mine)), close);
       // groups so close that float32 does not tell which is better count where one of them may be in and another out
       if (scored && __ballot(close && g < a.groups && mine > -INFINITY && better <= a.top_groups && better >= a.top_groups - 1)) {
-        const double total = a.sigmoid ? 1.0 : all64();
+        const double over = a.sigmoid ? 1.0 : inverse64(all64());
         double first = -INFINITY, second = -INFINITY;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-          const double v = key[i] == KEY_MASKED ? -INFINITY : (a.sigmoid ? sigmoid64(l[i]) : exp((double)l[i] - (double)most) / total) + (double)b[i];
+          const double v = key[i] == KEY_MASKED ? -INFINITY : (a.sigmoid ? sigmoid64(l[i]) : exp64((double)l[i] - (double)most) * over) + (double)b[i];
           second = fmax(second, fmin(first, v));
           first = fmax(first, v);
         }
@@ -358,7 +377,6 @@ template <int PER> struct Route {
       }
       n = top;
     }
-    Candidate* place = to(n);
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const unsigned long long lanes = __ballot(taken[i]);
@@ -369,37 +387,36 @@ template <int PER> struct Route {
     return n;
   }
 
-  // Of tokens' candidates, LANES places and lanes to each, the chosen in order with their weights.  n, most, total: of the lane's token; most_n: the largest n
-  template <int LANES> __device__ __forceinline__ void finish(const Candidate* place, long long token, int n, int most_n, float most, double total) const {
+  // Of n candidates, one to a lane, the chosen in order with their weights
+  __device__ __forceinline__ void finish(const Candidate* place, long long token, int n) const {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    const int k = lane & (LANES - 1), top = a.top;
-    place += lane - k;
-    const Candidate c = k < n ? place[k] : Candidate{-INFINITY, 0, -INFINITY, 0.f};
+    const int top = a.top;
+    const Candidate c = lane < n ? place[lane] : Candidate{-INFINITY, 0, -INFINITY, 0.f};
     const bool none = c.rank == -INFINITY;
     const float near = (2 * PER + 32) * 0x1p-24f * (1.f + fabsf(c.rank));
     int order = 0, close = 0;
-    for (int j = 0; j < most_n; ++j) {      // places without a candidate hold -inf and the highest number
+    for (int j = 0; j < n; ++j) {
       const float r = place[j].rank;
       order += (r > c.rank) | ((r == c.rank) & (place[j].e < c.e));
-      close += fabsf(r - c.rank) <= near;
+      close += fabsf(r - c.rank) <= near;      // itself, too
     }
     // scores of the candidates; of the softmax over the sum of all only where that does not cancel
-    double w = none ? 0.0 : a.sigmoid ? sigmoid64(c.l) : exp((double)c.l - (double)most) / total;
-    if (biased && __ballot((close > 1) & !none)) {      // one of them is itself
+    double w = a.sigmoid ? sigmoid64(c.l) : exp64((double)c.l - (double)most);
+    w = none ? 0.0 : w;
+    if (!a.sigmoid && most > -INFINITY && (!a.renormalize || biased)) w *= inverse64(all64());
+    if (biased && __ballot((close > 1) & !none)) {
       const long long mine = none ? ORDER_MASKED : order_of(w + (double)c.b);
       order = 0;
-      for (int j = 0; j < most_n; ++j) {
-        const long long other = __shfl(mine, lane - k + j);
-        order += (j < n) & ((other > mine) | ((other == mine) & (place[j].e < c.e)));
+      for (int j = 0; j < n; ++j) {
+        const long long other = __shfl(mine, j);
+        order += (other > mine) | ((other == mine) & (place[j].e < c.e));
       }
     }
-    const bool chosen = k < n && order < top;
+    const bool chosen = lane < n && order < top;
     if (a.renormalize) {
-      double all = chosen ? w : 0.0;
-      if constexpr (LANES == 64) all = wave_sum(all);
-      else { all += dpp_mov64<0xB1>(all); all += dpp_mov64<0x4E>(all); all += dpp_mov64<0x141>(all); all += dpp_mov64<0x140>(all); }
-      w = all == 0.0 ? 0.0 : w / all;
+      const double all = wave_sum(chosen ? w : 0.0);
+      w = all > 0x1p-1000 ? w * inverse64(all) : all == 0.0 ? 0.0 : w / all;
     }
     if (chosen) {
       ((HTR_GLOBAL int*)a.ids)[token * top + order] = c.e;
@@ -408,41 +425,15 @@ template <int PER> struct Route {
   }
 };
 
-// TOKENS = 1, or 4 tokens to a wave, of which those with up to 16 candidates are finished together: what comes behind the selection has few lanes to a token at work
-template <int PER, int TOKENS>
+template <int PER>
 __global__ __launch_bounds__(ROUTE_WAVES * 64) void k_route(const RouteArgs a) {
-  __shared__ Candidate candidates[ROUTE_WAVES][TOKENS == 1 ? 64 : 128];
+  __shared__ Candidate candidates[ROUTE_WAVES][64];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const long long first = ((long long)blockIdx.x * ROUTE_WAVES + wv) * TOKENS;
-  if (first >= a.tokens) return;
-  Candidate *together = candidates[wv], *alone = candidates[wv] + (TOKENS == 1 ? 0 : 64);
-  if (TOKENS > 1) together[lane] = Candidate{-INFINITY, 0x7FFFFFFF, 0.f, 0.f};
+  const long long token = (long long)blockIdx.x * ROUTE_WAVES + wv;
+  if (token >= a.tokens) return;
   Route<PER> r(a, lane);
-  float logits[TOKENS][PER];
-#pragma unroll
-  for (int q = 0; q < TOKENS; ++q) r.load(min(first + q, a.tokens - 1), logits[q]);
-  int n = 0, most_n = 0;
-  uint32_t left = 0;              // tokens for route_exact
-  float most = 0.f;
-  double total = 1.0;
-#pragma unroll
-  for (int q = 0; q < TOKENS; ++q) {
-    if (first + q >= a.tokens) break;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) r.l[i] = logits[q][i];
-    const int found = r.select([&](int n) { return TOKENS > 1 && n <= 16 ? together + 16 * q : alone; });
-    if (found == 0 || (TOKENS > 1 && found > 16)) { left |= 1u << q; continue; }
-    most_n = max(most_n, found);
-    const double sum = !a.sigmoid && r.most > -INFINITY && (!a.renormalize || r.biased) ? r.all64() : 1.0;
-    if (TOKENS == 1) {
-      r.template finish<64>(alone, first, found, found, r.most, sum);
-    } else if (lane >> 4 == q) {
-      n = found;
-      most = r.most;
-      total = sum;
-    }
-  }
-  if constexpr (TOKENS > 1) r.template finish<16>(together, first + (lane >> 4), n, most_n, most, total);
-#pragma unroll 1
-  for (; left != 0; left &= left - 1) route_exact<(PER < 16 ? PER : 16)>(a, first + __builtin_ctz(left), lane);
+  r.load(token, r.l);
+  const int n = r.select(candidates[wv]);
+  if (n == 0) route_exact<(PER < 16 ? PER : 16)>(a, token, lane);
+  else r.finish(candidates[wv], token, n);
 }

@@ -363,19 +363,14 @@ struct StackedScratch {
     bytes = at;
   }
 };
-template <int PER> hipError_t launch_route(const RouteArgs& a, hipStream_t st) {
-  auto grid = [&](int tokens) { return dim3((unsigned)((a.tokens + ROUTE_WAVES * tokens - 1) / (ROUTE_WAVES * tokens))); };
-  if constexpr (PER <= 8)
-    if (a.top <= 16 && a.tokens >= ROUTE_TOGETHER) return launch(k_route<PER, 4>, grid(4), ROUTE_WAVES * 64, 0, st, a);
-  return launch(k_route<PER, 1>, grid(1), ROUTE_WAVES * 64, 0, st, a);
-}
 hipError_t launch_route(RouteArgs a, hipStream_t st) {
+  const dim3 grid((unsigned)((a.tokens + ROUTE_WAVES - 1) / ROUTE_WAVES));
   a.size = a.experts / a.groups;
   a.parts_log2 = 6;
   while ((64 >> a.parts_log2) < a.groups) --a.parts_log2;
   const int per = (a.size + (1 << a.parts_log2) - 1) >> a.parts_log2;      // below 2 ROUTE_MOST / 64
-  return per <= 1 ? launch_route<1>(a, st) : per <= 2 ? launch_route<2>(a, st) : per <= 4 ? launch_route<4>(a, st) : per <= 8 ? launch_route<8>(a, st)
-         : per <= 16 ? launch_route<16>(a, st) : launch_route<32>(a, st);
+  auto take = [&](auto kernel) { return launch(kernel, grid, ROUTE_WAVES * 64, 0, st, a); };
+  return per <= 1 ? take(k_route<1>) : per <= 2 ? take(k_route<2>) : per <= 4 ? take(k_route<4>) : per <= 8 ? take(k_route<8>) : per <= 16 ? take(k_route<16>) : take(k_route<32>);
 }
 int stacked_shape(long long tokens, int top, int experts, int hidden, int inter, int type) {
   if (tokens < 1 || top < 1 || experts < 1 || hidden < 1 || inter < 1 || top > 4096 || tokens >= (1 << 24) || inter > (1 << 28)) return HTR_ERR_SIZE;
