@@ -11,57 +11,84 @@
 // 2.3e-3 in the 2-norm, of which 1.7e-3 are its own last rounding.
 
 // One workgroup for each expert counts the pairs of smaller experts and its own, then places its own: no atomics, no order but the pairs'.  A wave takes a run of
-// consecutive pairs, 64 at a time.  A pair whose expert is out of range has position -1.  24576 pairs, 64 experts: 16 us (34 with a run to each thread).
+// consecutive pairs, 64 at a time, and keeps up to KEEP of them to a lane between the two.  A pair whose expert is out of range has position -1.  24576 pairs,
+// 64 experts: 11 us (16 with eight loads on their way at a time, read again for the second pass, and tokens by integer division).
 constexpr int ORDER_WAVES = 16;
-__global__ __launch_bounds__(ORDER_WAVES * 64) void k_expert_order(const void* __restrict__ ids, int ids64, int pairs, int top, int experts,
-                                                                   int* __restrict__ ends, int* __restrict__ token, int* __restrict__ pos_of) {
+__device__ __forceinline__ void expert_order(const void* __restrict__ ids, int ids64, int pairs, int top, int experts, int* __restrict__ ends, int* __restrict__ token,
+                                             int* __restrict__ pos_of, int e) {
   __shared__ int s_less[ORDER_WAVES], s_same[ORDER_WAVES];
-  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), e = blockIdx.x;
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int per = (pairs + ORDER_WAVES * 64 - 1) / (ORDER_WAVES * 64) * 64, p0 = min(pairs, wv * per), p1 = min(pairs, p0 + per);
-  // AHEAD loads on their way at once: -1 for an expert out of range, or no pair
-  constexpr int AHEAD = 8;
+  // -1 for an expert out of range, or no pair
+  constexpr int AHEAD = 8, KEEP = 4;
   auto load = [&](int q, int (&v)[AHEAD]) {
+    long long id[AHEAD];
+    if (ids64) {
 #pragma unroll
-    for (int k = 0; k < AHEAD; ++k) {
-      const int p = min(q + 64 * k + lane, pairs - 1);
-      const long long id = ids64 ? ((const HTR_GLOBAL long long*)ids)[p] : (long long)((const HTR_GLOBAL int*)ids)[p];
-      v[k] = id < 0 || id >= experts || q + 64 * k + lane >= p1 ? -1 : (int)id;
+      for (int k = 0; k < AHEAD; ++k) id[k] = ((const HTR_GLOBAL long long*)ids)[min(q + 64 * k + lane, pairs - 1)];
+    } else {
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) id[k] = ((const HTR_GLOBAL int*)ids)[min(q + 64 * k + lane, pairs - 1)];
     }
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) v[k] = (((unsigned long long)id[k] >= (unsigned long long)experts) | (q + 64 * k + lane >= p1)) ? -1 : (int)id[k];
   };
   int less = 0, same = 0;
-  for (int q = p0; q < p1; q += 64 * AHEAD) {
-    int v[AHEAD];
-    load(q, v);
+  auto count = [&](int q, const int (&v)[AHEAD]) {
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) {
-      less += (int)__builtin_popcountll(__ballot(v[k] >= 0 && v[k] < e));
+      less += (int)__builtin_popcountll(__ballot((uint32_t)v[k] < (uint32_t)e));      // -1 is none
       same += (int)__builtin_popcountll(__ballot(v[k] == e));
-      if (e == 0 && v[k] < 0 && q + 64 * k + lane < p1) pos_of[q + 64 * k + lane] = -1;
     }
+    if (e == 0) {
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) if (v[k] < 0 && q + 64 * k + lane < p1) pos_of[q + 64 * k + lane] = -1;
+    }
+  };
+  int at = 0;
+  const double each = 1.0 / top;
+  auto put = [&](int q, const int (&v)[AHEAD]) {
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const unsigned long long mine = __ballot(v[k] == e);
+      if (v[k] == e) {
+        const int p = q + 64 * k + lane, pos = __builtin_amdgcn_mbcnt_hi((uint32_t)(mine >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mine, at));
+        token[pos] = (int)__builtin_fma((double)p, each, 0.5 * each);      // p / top: half a pair away from the next whole number, where 64 bits are off by 2^-22 of one
+        pos_of[p] = pos;
+      }
+      at += (int)__builtin_popcountll(mine);
+    }
+  };
+  int kept[KEEP][AHEAD];
+#pragma unroll
+  for (int j = 0; j < KEEP; ++j) if (p0 + j * 64 * AHEAD < p1) load(p0 + j * 64 * AHEAD, kept[j]);
+#pragma unroll
+  for (int j = 0; j < KEEP; ++j) if (p0 + j * 64 * AHEAD < p1) count(p0 + j * 64 * AHEAD, kept[j]);
+  for (int q = p0 + KEEP * 64 * AHEAD; q < p1; q += 64 * AHEAD) {
+    int v[AHEAD];
+    load(q, v);
+    count(q, v);
   }
   if (lane == 0) { s_less[wv] = less; s_same[wv] = same; }
   __syncthreads();
-  int at = 0, total = 0;
+  int total = 0;
   for (int k = 0; k < ORDER_WAVES; ++k) {
     at += s_less[k] + (k < wv ? s_same[k] : 0);
     total += s_less[k] + s_same[k];
   }
   if (threadIdx.x == 0) ends[e] = total;
   if (same == 0) return;
-  for (int q = p0; q < p1; q += 64 * AHEAD) {
+#pragma unroll
+  for (int j = 0; j < KEEP; ++j) if (p0 + j * 64 * AHEAD < p1) put(p0 + j * 64 * AHEAD, kept[j]);
+  for (int q = p0 + KEEP * 64 * AHEAD; q < p1; q += 64 * AHEAD) {
     int v[AHEAD];
     load(q, v);
-#pragma unroll
-    for (int k = 0; k < AHEAD; ++k) {
-      const unsigned long long mine = __ballot(v[k] == e);
-      if (mine >> lane & 1ull) {
-        const int p = q + 64 * k + lane, pos = at + (int)__builtin_popcountll(mine & ((1ull << lane) - 1ull));
-        token[pos] = p / top;
-        pos_of[p] = pos;
-      }
-      at += (int)__builtin_popcountll(mine);
-    }
+    put(q, v);
   }
+}
+__global__ __launch_bounds__(ORDER_WAVES * 64) void k_expert_order(const void* __restrict__ ids, int ids64, int pairs, int top, int experts, int* __restrict__ ends,
+                                                                   int* __restrict__ token, int* __restrict__ pos_of) {
+  expert_order(ids, ids64, pairs, top, experts, ends, token, pos_of, blockIdx.x);
 }
 
 // silu(gate) * up, eight columns to a thread

@@ -106,6 +106,50 @@ __global__ __launch_bounds__(1024) void k_round_rows(const void* __restrict__ x,
   }
 }
 
+// A routed layer's beginning: pairs sorted by expert in the first `experts` workgroups, the tokens' rows rounded in the others, a wave to each.  Neither waits for the other:
+// 4096 tokens of 2048, top 6 of 64: 12 us in one launch, 11 and 8 in two.
+template <int T>
+__global__ __launch_bounds__(ORDER_WAVES * 64) void k_order_and_round(const void* __restrict__ ids, int ids64, int pairs, int top, int experts, int* __restrict__ ends,
+                                                                      int* __restrict__ token, int* __restrict__ pos_of, const void* __restrict__ x, int tokens, int n,
+                                                                      uint8_t* __restrict__ q, float* __restrict__ scales) {
+  if ((int)blockIdx.x < experts) {
+    expert_order(ids, ids64, pairs, top, experts, ends, token, pos_of, blockIdx.x);
+    return;
+  }
+  const int lane = threadIdx.x & 63;
+  const size_t row = (size_t)(blockIdx.x - experts) * ORDER_WAVES + (threadIdx.x >> 6);
+  if (row >= (size_t)tokens) return;
+  constexpr int RUNS = 8;                     // of 512 columns, in registers; longer rows are read again
+  Eight<T> v[RUNS];
+  auto load = [&](int c) {
+#pragma unroll
+    for (int i = 0; i < RUNS; ++i) if (c + 512 * i < n) v[i].load_any(x, row * n + c + 512 * i);
+  };
+  uint32_t m = 0;
+  for (int c = 8 * lane; c < n; c += 512 * RUNS) {
+    load(c);
+#pragma unroll
+    for (int i = 0; i < RUNS; ++i)
+      if (c + 512 * i < n) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) m = max(m, magnitude(v[i].get(k)));
+      }
+  }
+  const RowScale s((double)__uint_as_float(wave_max(m)), 1.0);
+  if (lane == 0) ((HTR_GLOBAL float*)scales)[row] = s.s;
+  for (int c = 8 * lane; c < n; c += 512 * RUNS) {
+    if (n > 512 * RUNS) load(c);
+#pragma unroll
+    for (int i = 0; i < RUNS; ++i)
+      if (c + 512 * i < n) {
+        float f[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) f[k] = v[i].get(k);
+        *(HTR_GLOBAL u2*)((HTR_GLOBAL uint8_t*)q + row * n + c + 512 * i) = round8(s, f);
+      }
+  }
+}
+
 // The norm of norm.hpp, rounded to int8.  NV as above.  The largest |t w| goes with the sum of squares; products of 16-bit values are exact in float32 where they do
 // not leave it, others are formed in 64 bits.
 template <int T, int NV, bool RES>

@@ -526,11 +526,16 @@ int htr_moe_stacked(const void* x, int dtype, const void* ids, int ids_int64, co
   const int pairs = (int)(tokens * top);
   int *ends = (int*)(s + at.ends), *token = (int*)(s + at.token), *pos_of = (int*)(s + at.pos_of);
   float *h = (float*)(s + at.h), *out = (float*)(s + at.out);
-  TRY_HIP(launch(k_expert_order, dim3(experts), ORDER_WAVES * 64, 0, st, ids, ids_int64, pairs, top, experts, ends, token, pos_of));
+  if (i8) {
+    const dim3 grid((unsigned)(experts + (tokens + ORDER_WAVES - 1) / ORDER_WAVES));
+    TRY_HIP(launch(dtype == HTR_BF16 ? k_order_and_round<HTR_BF16> : k_order_and_round<HTR_F16>, grid, ORDER_WAVES * 64, 0, st, ids, ids_int64, pairs, top, experts, ends, token,
+                   pos_of, x, (int)tokens, hidden, s + at.xq, (float*)(s + at.xs)));
+  } else {
+    TRY_HIP(launch(k_expert_order, dim3(experts), ORDER_WAVES * 64, 0, st, ids, ids_int64, pairs, top, experts, ends, token, pos_of));
+  }
   ProductArgs a{x, nullptr, gate_up, (const float*)gate_up_scales, nullptr, h, ends, token, pairs, 2 * inter, hidden, experts, HTR_F32, dtype, nullptr, f8};
   if (i8) {
     a.x_type = HTR_I8;
-    TRY_HIP(launch_round(x, dtype, hidden, tokens, hidden, s + at.xq, s + at.xs, st));
     a.x = s + at.xq; a.xs = (const float*)(s + at.xs);
   } else if (f8 && gates_in_one(pairs, experts, type)) {
     a.x_type = HTR_E4M3;
