@@ -36,7 +36,9 @@ __global__ __launch_bounds__(ROWS_WAVES * 64) void k_product_rows(const ProductA
 
   // The workgroup's tiles, span by span, a matrix's from first to last: `left` of them from tile mt0 of its first span on
   const long long total = (long long)mtiles * (GROUPED ? count_spans(a, 8 * CT) : 1);
-  const long long from = blockIdx.x * total / gridDim.x, to = (blockIdx.x + 1ll) * total / gridDim.x;
+  // two workgroups of a compute unit (they come 256 apart) take neighbouring runs, so that a tile more or less evens out between them
+  const int nth = gridDim.x == 512 ? (int)(blockIdx.x & 255) * 2 + (int)(blockIdx.x >> 8) : (int)blockIdx.x;
+  const long long from = nth * total / gridDim.x, to = (nth + 1ll) * total / gridDim.x;
   if (from == to) return;
   const int span0 = GROUPED ? (int)(from / mtiles) : 0, mt0 = (int)(from - (long long)span0 * mtiles);
   int left = (int)(to - from);
@@ -90,89 +92,101 @@ __global__ __launch_bounds__(ROWS_WAVES * 64) void k_product_rows(const ProductA
       to_tile();
     }
   };
+  // A span's rows of x to LDS, zeros behind them.  A row to one, two, four or all eight waves, as many as there are for it; all loads of a run of LOADS are on their way at
+  // once, and a wave's first ones ahead of the matrix's, which it would wait for otherwise.  Several waves to a row: one row for each of them, the last one again for those
+  // without, so that all come to the barrier.
+  constexpr int LOADS = X == P_I8 ? 4 : 8, UNIT = X == P_I8 ? 16 : 8;
+  u4 q8[LOADS];
+  Eight<X == P_I8 ? HTR_BF16 : X> v[LOADS];
+  auto waves_of = [](int rows) { return rows == 1 ? 8 : rows == 2 ? 4 : rows <= 4 ? 2 : 1; };
+  auto first_of = [&](int rows) { const int w = waves_of(rows); return w > 1 ? min(wv / w, rows - 1) : wv; };
+  auto row_of = [&](const Span& s, int r) { return (size_t)(a.gather != nullptr ? a.gather[s.first + r] : s.first + r); };
+  auto load_run = [&](size_t row, int k, int step) {
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) {
+      if constexpr (X == P_I8) q8[j] = k + j * step < n ? *(const HTR_GLOBAL u4*)((const HTR_GLOBAL uint8_t*)a.x + row * n + k + j * step) : u4{0u, 0u, 0u, 0u};
+      else if (k + j * step < n) v[j].load_any(a.x, row * n + k + j * step);
+    }
+  };
+  auto row_to_lds = [&](const Span& s, int r, bool loaded) {
+    const int waves = waves_of(s.count), part = wv % waves, step = UNIT * 64 * waves, k0 = UNIT * (lane + 64 * part);
+    const size_t row = row_of(s, r);
+    if (!loaded) load_run(row, k0, step);
+    if constexpr (X == P_I8) {
+      if (lane == 0 && part == 0) scale[r] = ((const HTR_GLOBAL float*)a.xs)[row];
+      for (int k = k0; k < pitch; k += LOADS * step) {
+        if (k != k0) load_run(row, k, step);
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) if (k + j * step < pitch) *(u4*)(xq + r * pitch + k + j * step) = q8[j];
+      }
+    } else {
+      uint32_t m = 0;
+      for (int k = k0; k < n; k += LOADS * step) {
+        if (k != k0) load_run(row, k, step);
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j)
+          if (k + j * step < n) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = max(m, magnitude(v[j].get(i)));
+          }
+      }
+      m = wave_max(m);
+      if (waves > 1) {
+        if (lane == 0) largest[wv] = m;
+        __syncthreads();
+        for (int w = 0; w < waves; ++w) m = max(m, largest[wv - part + w]);
+      }
+      const RowScale of_row((double)__uint_as_float(m), 1.0);
+      if (lane == 0 && part == 0) scale[r] = of_row.s;
+      for (int k = k0; k < pitch; k += LOADS * step) {
+        if (n > LOADS * step && k < n) load_run(row, k, step);
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) {
+          if (k + j * step >= pitch) continue;
+          u2 q = {0u, 0u};
+          if (k + j * step < n) {
+            float f[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = v[j].get(i);
+            q = round8(of_row, f);
+          }
+          *(u2*)(xq + r * pitch + k + j * step) = q;
+        }
+      }
+    }
+  };
+  Span s = span_of(0);
+  if (s.e < a.experts) load_run(row_of(s, min(first_of(s.count), s.count - 1)), UNIT * (lane + 64 * (wv % waves_of(s.count))), UNIT * 64 * waves_of(s.count));
   to_matrix();
   to_tile();
 #pragma unroll
   for (int p = 0; p < STAGES; ++p) load(p);
 
-  // The span's rows of x to LDS, zeros behind them.  A row to one, two, four or all eight waves, as many as there are for it; all loads of a run of LOADS are on their way at once.
-  auto rows_to_lds = [&](const Span& s) {
-    const int rows = s.count, per_row = rows == 1 ? 8 : rows == 2 ? 4 : rows <= 4 ? 2 : 1, part = wv % per_row;
-    constexpr int LOADS = 8, UNIT = X == P_I8 ? 16 : 8;
-    const int step_x = UNIT * 64 * per_row, k0 = UNIT * (lane + 64 * part);
-    // several waves to a row: one row for each of them, the last one again for those without, so that all come to the barrier
-    for (int r = per_row > 1 ? min(wv / per_row, rows - 1) : wv; r < rows; r += ROWS_WAVES) {
-      const size_t row = a.gather != nullptr ? a.gather[s.first + r] : s.first + r;
-      if constexpr (X == P_I8) {
-        for (int k = k0; k < pitch; k += LOADS * step_x) {
-          u4 v[LOADS];
-#pragma unroll
-          for (int j = 0; j < LOADS; ++j)
-            v[j] = k + j * step_x < n ? *(const HTR_GLOBAL u4*)((const HTR_GLOBAL uint8_t*)a.x + row * n + k + j * step_x) : u4{0u, 0u, 0u, 0u};
-#pragma unroll
-          for (int j = 0; j < LOADS; ++j) if (k + j * step_x < pitch) *(u4*)(xq + r * pitch + k + j * step_x) = v[j];
-        }
-        if (lane == 0 && part == 0) scale[r] = ((const HTR_GLOBAL float*)a.xs)[row];
-      } else {
-        Eight<X> v[LOADS];
-        auto load_run = [&](int k) {
-#pragma unroll
-          for (int j = 0; j < LOADS; ++j) if (k + j * step_x < n) v[j].load_any(a.x, row * n + k + j * step_x);
-        };
-        uint32_t m = 0;
-        for (int k = k0; k < n; k += LOADS * step_x) {
-          load_run(k);
-#pragma unroll
-          for (int j = 0; j < LOADS; ++j)
-            if (k + j * step_x < n) {
-#pragma unroll
-              for (int i = 0; i < 8; ++i) m = max(m, magnitude(v[j].get(i)));
-            }
-        }
-        m = wave_max(m);
-        if (per_row > 1) {
-          if (lane == 0) largest[wv] = m;
-          __syncthreads();
-          for (int w = 0; w < per_row; ++w) m = max(m, largest[wv - part + w]);
-        }
-        const RowScale s((double)__uint_as_float(m), 1.0);
-        if (lane == 0 && part == 0) scale[r] = s.s;
-        for (int k = k0; k < pitch; k += LOADS * step_x) {
-          if (n > LOADS * step_x && k < n) load_run(k);
-#pragma unroll
-          for (int j = 0; j < LOADS; ++j) {
-            if (k + j * step_x >= pitch) continue;
-            u2 q = {0u, 0u};
-            if (k + j * step_x < n) {
-              float f[8];
-#pragma unroll
-              for (int i = 0; i < 8; ++i) f[i] = v[j].get(i);
-              q = round8(s, f);
-            }
-            *(u2*)(xq + r * pitch + k + j * step_x) = q;
-          }
-        }
-      }
-    }
-    __syncthreads();
-  };
-
   // a thread's outputs of a tile: row i of the matrix, rows t, t + ROWS of x
   constexpr int ROWS = ROWS_WAVES * 64 / TR, OUT = (8 * CT + ROWS - 1) / ROWS;
   const int i = threadIdx.x % TR, t0 = threadIdx.x / TR;
   const uint8_t* xp[CT];
-  Span s;
   float xs[OUT];
-  auto to_span = [&](int k) {
-    s = span_of(k);
-    if (s.e < a.experts) rows_to_lds(s);
+  auto span_there = [&] {
+    __syncthreads();
 #pragma unroll
     for (int k = 0; k < OUT; ++k) xs[k] = t0 + k * ROWS < s.count && s.e < a.experts ? scale[t0 + k * ROWS] : 0.f;
 #pragma unroll
     for (int t = 0; t < CT; ++t) xp[t] = xq + min(8 * t + (c >> 1), s.count - 1) * pitch + (c & 1) * 64 + 16 * g;
   };
+  auto to_span = [&](int k) {
+    s = span_of(k);
+    if (s.e < a.experts)
+      for (int r = first_of(s.count); r < s.count; r += ROWS_WAVES) row_to_lds(s, r, false);
+    span_there();
+  };
+  if (s.e < a.experts) {
+    const int r0 = first_of(s.count);
+    if (r0 < s.count) row_to_lds(s, r0, true);
+    for (int r = r0 + ROWS_WAVES; r < s.count; r += ROWS_WAVES) row_to_lds(s, r, false);
+  }
+  span_there();
   int span = 0, mt = mt0;
-  to_span(0);
   auto type_of = [&](auto store) {
     if (a.y_dtype == HTR_BF16) store(std::integral_constant<int, HTR_BF16>());
     else if (a.y_dtype == HTR_F16) store(std::integral_constant<int, HTR_F16>());
@@ -183,10 +197,10 @@ __global__ __launch_bounds__(ROWS_WAVES * 64) void k_product_rows(const ProductA
   for (int t = 0; t < CT; ++t) acc[t] = i4{0, 0, 0, 0};
   int step = 0, half = 0;
   // Scales and biases of ROWS_AHEAD of the matrix's rows at once: as loads of every tile they would hold up the matrix's
-  int nth = 0, which = 1;                                                     // of the tiles since the last of these, and where they lie
+  int done = 0, which = 1;                                                    // of the tiles since the last of these, and where they lie
   auto scales_from = [&] {
     which ^= 1;
-    nth = 0;
+    done = 0;
     float* to = ahead + which * 2 * ROWS_AHEAD;
     const int r = mt * TR + threadIdx.x;
     if (threadIdx.x >= ROWS_AHEAD || r >= a.m || s.e == a.experts) return;
@@ -225,7 +239,7 @@ __global__ __launch_bounds__(ROWS_WAVES * 64) void k_product_rows(const ProductA
         int sum = 0;
 #pragma unroll
         for (int w = 0; w < KW; ++w) sum += parts[w * PART];
-        const float* of_row = ahead + which * 2 * ROWS_AHEAD + nth * TR + i;
+        const float* of_row = ahead + which * 2 * ROWS_AHEAD + done * TR + i;
         float v = (float)sum * xs[k] * of_row[0];
         if (a.bias != nullptr) v += of_row[ROWS_AHEAD];
         if (GROUPED && s.e == a.experts) v = 0.f;                             // rows behind the last expert's
@@ -236,13 +250,13 @@ __global__ __launch_bounds__(ROWS_WAVES * 64) void k_product_rows(const ProductA
       step = 0;
       half ^= 1;
       --left;
-      ++nth;
+      ++done;
       if (++mt == mtiles) {
         mt = 0;
         if (GROUPED && left > 0) to_span(++span);                             // every wave is past the products of the one before
-        nth = ROWS_AHEAD / TR;
+        done = ROWS_AHEAD / TR;
       }
-      if (nth == ROWS_AHEAD / TR && left > 0) scales_from();
+      if (done == ROWS_AHEAD / TR && left > 0) scales_from();
     }
   }
 }
