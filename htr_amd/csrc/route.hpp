@@ -31,10 +31,11 @@ __device__ __forceinline__ long long order_of(double v) {
 constexpr long long ORDER_MASKED = (long long)0x800FFFFFFFFFFFFFull;      // order_of(-inf)
 constexpr long long ORDER_NONE = (long long)0x8000000000000000ull;        // no expert, or one that is taken
 // the same of float32 that is not NaN, in unsigned numbers from 1 on (0: no expert)
-__device__ __forceinline__ uint32_t key_of(float v) {
-  const uint32_t u = __float_as_uint(v + 0.f);
+__device__ __forceinline__ uint32_t key_of_sum(float v) {                // that is not -0
+  const uint32_t u = __float_as_uint(v);
   return u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
 }
+__device__ __forceinline__ uint32_t key_of(float v) { return key_of_sum(v + 0.f); }
 __device__ __forceinline__ float value_of_key(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); }
 constexpr uint32_t KEY_MASKED = 0x007FFFFFu;                             // of -inf
 
@@ -171,7 +172,7 @@ template <int PER> __device__ __forceinline__ void route_exact(const RouteArgs& 
 // The threshold between the chosen and the others is found by halving the span of ranks (as integers): a comparison and a count of lanes to each element, until exactly
 // `top` lie above it, which takes about ten steps; the largest one by one takes a wave's maximum for each.  Whatever lies next to the threshold is a candidate, too, and
 // candidates too close to each other are ordered by their ranks in 64 bits, groups likewise.
-struct Candidate { float rank; int e; float l, b; };
+struct Candidate { uint32_t after, key; float l, b; };      // after: ~expert; with the key in front, a number for each candidate in descending order
 __device__ __forceinline__ void two_largest(uint32_t& first, uint32_t& second, uint32_t f, uint32_t s) {      // of both
   second = max(max(second, s), min(first, f));
   first = max(first, f);
@@ -201,17 +202,18 @@ template <int PER> struct Route {
     }
   }
   __device__ __forceinline__ bool in(int i) const { return (g < a.groups) & (p + i * parts < a.size); }
-  __device__ __forceinline__ int at(int i) const { return min(e0 + i * parts, a.experts - 1); }      // where it may be loaded from
+  __device__ __forceinline__ uint32_t at(int i) const { return (uint32_t)min(e0 + i * parts, a.experts - 1); }      // where it may be loaded from
   // All loads at once, none behind a condition of its lane
   __device__ __forceinline__ void load(long long token, float (&to)[PER]) const {
-    const size_t row = (size_t)(token * a.stride);
     if (a.dtype == HTR_F32) {
+      const HTR_GLOBAL float* row = (const HTR_GLOBAL float*)a.logits + token * a.stride;
 #pragma unroll
-      for (int i = 0; i < PER; ++i) to[i] = ((const HTR_GLOBAL float*)a.logits)[row + at(i)];
+      for (int i = 0; i < PER; ++i) to[i] = row[at(i)];
     } else {
+      const HTR_GLOBAL uint16_t* row = (const HTR_GLOBAL uint16_t*)a.logits + token * a.stride;
       uint32_t raw[PER];
 #pragma unroll
-      for (int i = 0; i < PER; ++i) raw[i] = ((const HTR_GLOBAL uint16_t*)a.logits)[row + at(i)];
+      for (int i = 0; i < PER; ++i) raw[i] = row[at(i)];
       if (a.dtype == HTR_BF16) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) to[i] = __uint_as_float(raw[i] << 16);
@@ -256,7 +258,7 @@ template <int PER> struct Route {
     }
     if (biased) {
 #pragma unroll
-      for (int i = 0; i < PER; ++i) key[i] = key_of(l[i] == -INFINITY ? l[i] : score[i] + b[i]);      // a bias of -inf masks, too
+      for (int i = 0; i < PER; ++i) key[i] = key_of_sum(l[i] == -INFINITY ? l[i] : score[i] + b[i]);      // a bias of -inf masks, too; scores are no -0
     } else {
 #pragma unroll
       for (int i = 0; i < PER; ++i) key[i] = key_of(l[i]);
@@ -381,46 +383,58 @@ template <int PER> struct Route {
     for (int i = 0; i < PER; ++i) {
       const unsigned long long lanes = __ballot(taken[i]);
       if (taken[i])
-        place[__builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0))] = Candidate{value_of_key(key[i]), e0 + i * parts, l[i], b[i]};
+        place[__builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0))] = Candidate{~(uint32_t)(e0 + i * parts), key[i], l[i], b[i]};
       place += (int)__builtin_popcountll(lanes);
     }
     return n;
   }
 
   // Of n candidates, one to a lane, the chosen in order with their weights
-  __device__ __forceinline__ void finish(const Candidate* place, long long token, int n) const {
+  __device__ __forceinline__ void finish(Candidate* place, long long token, int n) const {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
     const int top = a.top;
-    const Candidate c = lane < n ? place[lane] : Candidate{-INFINITY, 0, -INFINITY, 0.f};
-    const bool none = c.rank == -INFINITY;
-    const float near = (2 * PER + 32) * 0x1p-24f * (1.f + fabsf(c.rank));
-    int order = 0, close = 0;
-    for (int j = 0; j < n; ++j) {
-      const float r = place[j].rank;
-      order += (r > c.rank) | ((r == c.rank) & (place[j].e < c.e));
-      close += fabsf(r - c.rank) <= near;      // itself, too
+    const Candidate c = lane < n ? place[lane] : Candidate{0u, KEY_MASKED, -INFINITY, 0.f};
+    const bool none = c.key == KEY_MASKED;
+    const uint32_t e = ~c.after;
+    auto number = [](const Candidate& c) { return (unsigned long long)c.key << 32 | c.after; };
+    const unsigned long long mine = number(c);
+    int order = 0;
+    for (int j = 0; j < n; ++j) order += number(place[j]) > mine;
+    bool close = false;
+    if (biased) {
+      // each one's rank to its place, where the one before it looks
+      const float v = value_of_key(c.key);
+      if (lane < n) place[order].l = v;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      close = (order + 1 < n) & (fabsf(v - place[min(order + 1, 63)].l) <= (2 * PER + 32) * 0x1p-24f * (1.f + fabsf(v)));
     }
     // scores of the candidates; of the softmax over the sum of all only where that does not cancel
     double w = a.sigmoid ? sigmoid64(c.l) : exp64((double)c.l - (double)most);
     w = none ? 0.0 : w;
     if (!a.sigmoid && most > -INFINITY && (!a.renormalize || biased)) w *= inverse64(all64());
-    if (biased && __ballot((close > 1) & !none)) {
-      const long long mine = none ? ORDER_MASKED : order_of(w + (double)c.b);
+    if (__ballot(close & !none)) {
+      const long long rank = none ? ORDER_MASKED : order_of(w + (double)c.b);
       order = 0;
       for (int j = 0; j < n; ++j) {
-        const long long other = __shfl(mine, j);
-        order += (other > mine) | ((other == mine) & (place[j].e < c.e));
+        const long long other = __shfl(rank, j);
+        order += (other > rank) | ((other == rank) & (place[j].after > c.after));
       }
     }
     const bool chosen = lane < n && order < top;
     if (a.renormalize) {
-      const double all = wave_sum(chosen ? w : 0.0);
+      double all = chosen ? w : 0.0;
+      if (n > 16) {
+        all = wave_sum(all);
+      } else {      // in the first 16 lanes, which have them all
+        all += dpp_mov64<0xB1>(all); all += dpp_mov64<0x4E>(all); all += dpp_mov64<0x141>(all); all += dpp_mov64<0x140>(all);
+      }
       w = all > 0x1p-1000 ? w * inverse64(all) : all == 0.0 ? 0.0 : w / all;
     }
     if (chosen) {
-      ((HTR_GLOBAL int*)a.ids)[token * top + order] = c.e;
-      ((HTR_GLOBAL float*)a.weights)[token * top + order] = (float)(w * a.scale);
+      ((HTR_GLOBAL int*)a.ids + token * top)[order] = (int)e;
+      ((HTR_GLOBAL float*)a.weights + token * top)[order] = (float)(w * a.scale);
     }
   }
 };
