@@ -424,7 +424,8 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
       __builtin_amdgcn_global_load_lds((const HTR_GLOBAL void*)(src.scales + slab + src.scale),
                                        (__attribute__((address_space(3))) void*)(lds + stage * STAGE + (TM + TN) * 128 + min(wv, XW) * 256), 4, 0, 0);
   };
-  // int8: a tile's scales, asked for ahead of its first slab and so there with it.  One load more than `landed` counts makes it wait longer, never shorter.
+  // int8: a tile's scales, asked for NS - 1 slabs or more ahead of its first product, so that `landed` has waited for them long before its last.  One load more than it counts makes it
+  // wait longer, never shorter.
   auto issue_tile_scales = [&](const Tile& t, int which) {
     if constexpr (T == P_I8) {
 #pragma unroll
@@ -599,7 +600,12 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_product_tile(const ProductA
     if (slab + NS == slabs) {
       id += gridDim.x;
       more = find(then);
-      if (more) { source(then, src2); issue_tile_scales(then, which ^ 1); }
+      if (more) {
+        source(then, src2);
+        // with as many slabs as stages no barrier has passed since the tile before was stored: a wave may still read that half of the scales' place
+        if (T == P_I8 && slab == 0) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        issue_tile_scales(then, which ^ 1);
+      }
     }
     const int ask = slab + NS < slabs ? slab + NS : slabs >= NS ? slab + NS - slabs : slabs - 1;
     multiply(asked, src, ask, src2, slab + 2 == slabs);

@@ -320,6 +320,17 @@ def test_products_of_many_kinds_of_tiles(gen):
     assert len(seen) >= 8, seen
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [16, 48, 128, 144, 256, 272, 384, 400, 512, 528])
+@pytest.mark.parametrize("rows,m", [(5000, 6000), (1100, 9000), (400, 20000), (200, 9000)])
+def test_short_rows_of_many_tiles(gen, n, rows, m):
+    """Several tiles to a workgroup, each with fewer slabs than the ring has stages, as many, and more: a tile's scales may not reach the one before."""
+    w, x = weight(gen, m, n), ops.quantize_int8(randn(gen, rows, n) * torch.exp(randn(gen, rows, 1)))
+    want, bound = product_bound(x, w, F32)
+    for _ in range(3):
+        assert_within(ops.linear_int8(x, *w, out_dtype=F32), want, bound)
+
+
 def _ends(counts):
     return torch.tensor(counts, dtype=torch.int32).cumsum(0).to(torch.int32).cuda()
 
