@@ -223,8 +223,11 @@ template <int T, typename F> auto product_kernel(const ProductArgs& a, F take) {
       return take(Tiles<2, 2, 2, 2, 4>{});
     }
     // Rows of fewer slabs than waves leave some idle (7 rows on 15657x384 in e4m3 5.5 us by 16 rows to a workgroup of 8 waves, 4.7 by 32 to one of 4), and rows
-    // to be rounded are rounded by half as many (4 tokens over 8 of 16 experts of 1920/384 37 and 31); long rows of few workgroups need more waves to share them
-    if (wgs >= 512 && (slabs < 8 || (slabs <= 16 && T == P_F8 && a.x_type != HTR_E4M3))) return take(Stream<2, 1, 4>{});
+    // to be rounded are rounded by half as many (4 tokens over 8 of 16 experts of 1920/384 37 and 31); long rows of few workgroups need more waves to share them.
+    // In int8 what comes here has rows too long for k_product_rows.
+    if (T != P_I8 && wgs >= 512 && (slabs < 8 || (slabs <= 16 && T == P_F8 && a.x_type != HTR_E4M3))) {
+      if constexpr (T != P_I8) return take(Stream<2, 1, 4>{});
+    }
     if (wgs <= 256 && slabs >= 64) return take(Stream<1, 1, 16>{});
     return take(Stream<1, 1, 8>{});
   }

@@ -20,7 +20,7 @@ scales made here are the row's largest magnitude over 127, the values the neares
 
 Norms sum in 64 bits, products of 16-bit values in float32.  Products of e4m3 values are first added eight consecutive
 columns at a time, as the matrix instructions do: each eight is off by at most 2^-10 of the largest magnitude in x times that in the matrix (one below 2^-6 of its
-scale counts as that).  Sums of int8 products are exact.
+scale counts as that).  Sums of int8 products are exact; one is multiplied with its row's scale, then with its channel's.
 Everything beyond is float32, the product of a row's scale and a block's as well (below 2^-126 it has fewer bits, beyond float32 it is
 infinite).  Results are rounded once.  Nothing here has a derivative, as no packed linear has one in its
 activations: a call that torch would differentiate is refused.  Calls only queue kernels on the current stream of x's device, allocate with torch and

@@ -387,6 +387,22 @@ def test_grouped_mm_of_more_tiles_than_run_at_once(gen, counts, m):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("E", [15000, 28000, 40000])
+@pytest.mark.parametrize("rows_of", [lambda e: e % 3 == 0, lambda e: e * 0 + 1, lambda e: e % 5], ids=["a third", "one", "up to four"])
+def test_grouped_mm_of_tens_of_thousands_of_experts(gen, E, rows_of):
+    """Up to some sixty experts to a workgroup, and more than it takes."""
+    m, n = 20, 48
+    counts = rows_of(torch.arange(E, device="cuda")).int()
+    of, R = torch.repeat_interleave(torch.arange(E, device="cuda"), counts), int(counts.sum()) + 7
+    x, w = ops.quantize_int8(randn(gen, R, n)), weight(gen, E, m, n)
+    y = ops.grouped_mm(x, w, counts.cumsum(0).int(), out_dtype=F32)
+    R -= 7
+    want = (x[0][:R, None].double() * w[0][of].double()).sum(-1) * x[1][:R, None].double() * w[1][of].double()
+    assert_within(y[:R], want, want.abs() * 3.01 * 2.0 ** -24 * 1.01 + half_step(want, F32))
+    assert (y[R:] == 0).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("ends,meant", [([4, 2, 9], [4, 4, 9]), ([-5, 3, 100], [0, 3, 40]), ([2 ** 31 - 1, 0, 7], [40, 40, 40]), ([-1, -2, -3], [0, 0, 0])])
 def test_ends_out_of_order_or_range(gen, ends, meant):
     x, w = ops.quantize_int8(randn(gen, 40, 64)), weight(gen, 3, 40, 64)
@@ -510,6 +526,41 @@ def test_a_block_of_them_eager_on_streams_captured_and_compiled(gen):
         assert torch.equal(out[0], want[k][0]) and torch.equal(out[1], want[k][1])
     for a, b in zip(torch.compile(run, backend="eager")(*inputs[1]), want[1]):
         assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_layers_of_many_rows_on_streams_and_captured(gen):
+    """Tiles that go on from one to the next, on two streams at once and replayed."""
+    w, experts = weight(gen, 6000, 512), (weight(gen, 4, 1024, 512), weight(gen, 4, 512, 512))
+    ids, wt = torch.randint(0, 4, (1500, 2), device="cuda", generator=gen), torch.rand(1500, 2, device="cuda", generator=gen)
+
+    def run(x):
+        y = ops.moe_experts_stacked(x, ids, wt, *experts)
+        return ops.linear_int8(y, *w)
+
+    inputs = [randn(gen, 1500, 512, dtype=BF16) for _ in range(4)]
+    want = [run(x) for x in inputs]
+    side = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for k, x in enumerate(inputs):
+        side[k % 2].wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side[k % 2]):
+            got.append(run(x))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    x = inputs[0].clone()
+    with torch.cuda.stream(side[0]):
+        run(x)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(x)
+    for k in (1, 2, 3, 0, 2):
+        x.copy_(inputs[k])
+        graph.replay()
+        run(inputs[(k + 1) % 4])                        # eager work between the replays
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[k])
 
 
 @pytest.mark.gpu
