@@ -6,7 +6,8 @@
 // a half decides by as much as one outlier may be worth of the small ones: quotients are formed in 64 bits, and with halves away from zero they need no division.
 // y / s is y f with f = (1 / s)(1 + 2^-50): what is a half of an integer, exactly, lies beyond it then, and everything else is 2^-32 of itself or more away from one
 // (numerator and denominator have 24 bits).  Added to 1.5 2^52, one fused operation leaves the integer in the low bits.
-// Bound: HBM, rows read once and kept in registers between the two passes.
+// Bound: HBM, rows read once and kept in registers between the two passes: 24576 rows of 1408 float32 29 us (6.0 TB/s), the norm with a residual of 333 rows of 4096 in f16
+// 5.7 us, of one 2.6.
 
 constexpr int I8_MOST = 32768;              // columns of a row in registers: 1024 threads by four runs of eight
 

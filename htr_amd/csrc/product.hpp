@@ -298,8 +298,10 @@ __global__ __launch_bounds__(STREAM_WAVES * 64) void k_product_stream(const Prod
 // Row number 4 q + j of a wave's MFMA tiles 2 h and 2 h + 1 are its rows 32 h + 8 q + j and + 4: a lane then holds eight consecutive outputs, and four
 // lanes 64 bytes of a row in 16 bits.
 // GATED: the matrix is gate over up, m / 2 rows each; a tile takes TM / 2 of either, 32 by 32 in turn, so that a lane holds gate and up of eight consecutive
-// hidden columns; y [rows][m / 2] is silu(gate) up, in 16 bits, in float32 (int8: a row's scale is not known before its last column) or in e4m3 (then TM / 2 = 128 columns share a
-// scale); rows behind the last expert's are left.
+// hidden columns; y [rows][m / 2] is silu(gate) up, in 16 bits, in float32 (int8: a row's scale is not known before its last column, and values rounded to 16 bits before would
+// fall on another integer here and there, 0.8 % of the result's norm) or in e4m3 (then TM / 2 = 128 columns share a scale); rows behind the last expert's are left.
+// int8: the sums stay in the matrix unit's registers over all slabs, and the scales meet them at a tile's end, from LDS: 8192 rows on 14336x4096 392 to 412 us (2.33 to 2.45
+// POP/s, the library's 8192^3 product 2.36), 465 with scales loaded where they are used; 24576 rows of 64 experts of 2816x2048 110; 333 rows on 6144x4096 22.
 __device__ __forceinline__ int swizzle_w(int r) { return ((r >> 1) & 1) | ((r >> 3 & 3) << 1); }
 __device__ __forceinline__ int swizzle_x(int r) { return (r >> 1) & 7; }
 constexpr int TILE_XCDS = 8, TOGETHER = 8;

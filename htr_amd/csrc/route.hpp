@@ -9,6 +9,9 @@
 // One wave to a token.  Ranks that are logits are float32 as they are; others are first formed in float32, and only those that lie within what float32 may be off of each
 // other, or of what decides, are compared in 64 bits (Route); what that does not cover is done in 64 bits throughout (route_exact).  The weights of the chosen are
 // 64 bits either way.
+// 8 of 256 experts, sigmoid, bias, 4 of 8 groups: 16384 tokens 17 us, where their 17 MB take 2.4; 427 vector and 351 scalar instructions a token, the vector units busy in
+// four fifths of the time.  6 of 64 by softmax: 1 token 2.8 us, 500 tokens 4.7, less than the host takes for the call.  In 64 bits throughout 16384 tokens take 127; four tokens
+// to a wave, finished together, 19; a wave that goes on from token to token 31 (the 64-bit constants kept in registers leave it too few neighbours).
 constexpr int ROUTE_MOST = 1024, ROUTE_WAVES = 4;
 
 struct RouteArgs {

@@ -258,6 +258,8 @@ template <int T, typename F> auto product_kernel(const ProductArgs& a, F take) {
     default: return take(Tiles<2, 2, 2, 1, 4>{});
   }
 }
+// In int8 the tables in e4m3 fit: the tile chosen takes as long as the best one on average and 1.15 times as long at most on 84 sizes of one
+// matrix, 1.02 and 1.32 on 47 of experts.
 // ---- few rows in int8
 struct RowsGrid { int columns, kw, most, mtiles, workgroups; long long tiles; size_t lds; bool fits; };      // most: rows of a span; tiles: a bound where rows are grouped
 RowsGrid rows_grid(const ProductArgs& a) {
