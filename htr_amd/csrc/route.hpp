@@ -1,7 +1,8 @@
 // Part of unpacked.hip, included inside its anonymous namespace: a router's logits to each token's experts and their weights.
 //
 //   s_e = softmax_e(l) or 1 / (1 + exp(-l_e));   r_e = s_e + b_e, without a bias l_e, of which s_e is a growing function
-//   groups: the sum of a group's `group_best` largest s_e + b_e ranks it; experts of the best `top_groups` groups compete (one best, no bias: by l_e)
+//   groups: the sum of a group's `group_best` largest s_e + b_e ranks it; experts of the best `top_groups` groups compete (one best, no bias: by l_e).  Masked experts
+//   add nothing to it: a group with one expert left is as good as that one, one with none comes behind all others
 //   the `top` largest r_e in descending order, ties to the lowest number;  weights s_e, over their sum if `renormalize`, times `scale`
 //
 // A logit or bias of -inf masks its expert: it comes behind every other, with weight 0; a token of which every expert is masked has weights 0.  NaN ranks first.
@@ -125,7 +126,8 @@ template <int PER> __device__ __forceinline__ void route_exact(const RouteArgs& 
           if (e / size == g && e < a.experts && order_of(v[j]) == top && (top < before || e > before_e)) { first = e; value = v[j]; }
         }
         const int e = -wave_largest(-first);
-        sum += __shfl(value, e / PER);
+        value = __shfl(value, e / PER);
+        sum += k == 0 || top != ORDER_MASKED ? value : 0.0;
         before = top;
         before_e = e;
       }
@@ -303,7 +305,7 @@ template <int PER> struct Route {
         }
         return better;
       };
-      const float mine = two ? first + second : first;
+      const float mine = two && k2 != KEY_MASKED ? first + second : first;
       bool close = false, none = false;
       int better = count_better(mine, 2.f * slack * (1.f + fabsf(mine)), close);
       // groups so close that float32 does not tell which is better count where one of them may be in and another out
@@ -321,7 +323,7 @@ template <int PER> struct Route {
           second = fmax(fmax(second, s), fmin(first, f));
           first = fmax(first, f);
         }
-        better = count_better(two ? first + second : first, 0.0, none);
+        better = count_better(two && second != -INFINITY ? first + second : first, 0.0, none);
       }
       out |= better >= a.top_groups;
     }

@@ -411,7 +411,8 @@ def route_experts(logits, top, scores="softmax", bias=None, groups=1, top_groups
     the experts' load, no part of the weights), without a bias of their logits, ties to the lowest number.  With groups, E / groups consecutive experts each, only
     those of the best top_groups groups compete; a group is as good as its best expert, or with group_best=2 the sum of its two best scores + bias.  Weights are
     the scores, divided by their sum with renormalize, times scale.  Logits bfloat16, float16 or float32; scores are 64 bits.
-    A logit of -inf masks its expert, which comes behind every other, with weight 0; a token without any other expert gets weights 0.  NaN ranks first, with weight NaN.
+    A logit (or bias) of -inf masks its expert, which comes behind every other, with weight 0; a group is then as good as the experts it has left, and comes behind all others
+    without any; a token without any other expert gets weights 0.  NaN ranks first, with weight NaN.
     E up to 1024, groups and top up to 64."""
     path = _fast(logits)
     if path is not None:

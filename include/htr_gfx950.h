@@ -387,8 +387,9 @@ int htr_moe_stacked(const void* x, int dtype, const void* ids, int ids_int64, co
  * token to token, as htr_moe_stacked and htr_moe_experts take them.  Scores s_e = softmax_e(l), or 1 / (1 + exp(-l_e)) where sigmoid; experts in descending
  * order of s_e + bias_e, without a bias (NULL) of l_e; ties go to the lowest number.  With groups > 1 (consecutive experts) only those of the best top_groups groups
  * compete, a group being as good as the sum of its group_best (1 or 2) largest s_e + bias_e (one, without a bias: its largest l_e).  Weights are the scores,
- * divided by their sum if renormalize, times scale.  Scores and sums in 64 bits.  A logit, or bias, of -inf masks an expert: behind all others, weight 0, also in a
- * group's sum; a token without any other expert has weights 0.  NaN ranks first, and its weight is NaN.
+ * divided by their sum if renormalize, times scale.  Scores and sums in 64 bits.  A logit, or bias, of -inf masks an expert: it comes behind all others with weight 0 and
+ * adds nothing to its group's sum, which is then that of fewer experts; a group of masked experts alone comes behind all others, and a token without any other expert has
+ * weights 0.  NaN ranks first, and its weight is NaN.
  * experts up to 1024, top up to 64 and to the experts of top_groups groups, groups up to 64 and a divisor of experts.
  */
 int htr_route(const void* logits, int64_t stride, int dtype, int64_t tokens, int experts, int top, int sigmoid, const float* bias, int groups, int top_groups,
