@@ -61,12 +61,12 @@ template <typename V> __device__ __forceinline__ u2 round8(const RowScale& s, co
 }
 
 // Rows as they are (G = false, x [rows][n] of T, `stride` elements apart), or silu(gate) up of float32 rows [gate | up] of n columns each (G = true).
-// NV runs of eight columns to a thread; NV = 0: rows too long for that are read twice.  last: rows from last[0] on are left, NULL: none.
+// NV runs of eight columns to a thread; NV = 0: rows too long for that are read twice.  Rows from `from` on; last: rows from last[0] on are left, NULL: none.
 template <int T, int NV, bool G>
-__global__ __launch_bounds__(1024) void k_round_rows(const void* __restrict__ x, long long stride, int n, const int* __restrict__ last, uint8_t* __restrict__ q,
-                                                     float* __restrict__ scales) {
+__global__ __launch_bounds__(1024) void k_round_rows(const void* __restrict__ x, long long stride, long long from, int n, const int* __restrict__ last,
+                                                     uint8_t* __restrict__ q, float* __restrict__ scales) {
   __shared__ uint32_t s_max[16];
-  const long long row = blockIdx.x;
+  const long long row = from + blockIdx.x;
   if (last != nullptr && row >= last[0]) return;
   auto get = [&](int c, float (&f)[8]) {
     Eight<T> v;

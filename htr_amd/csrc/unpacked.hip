@@ -102,8 +102,12 @@ template <typename F> hipError_t by_runs(int n, F take) {
   return nv == 1 ? take(std::integral_constant<int, 1>(), threads) : nv == 2 ? take(std::integral_constant<int, 2>(), threads) : take(std::integral_constant<int, 4>(), threads);
 }
 template <int T, bool G> hipError_t launch_round(const void* x, long long stride, long long rows, int n, const int* last, void* q, void* scales, hipStream_t st) {
+  constexpr long long MOST = 1 << 21;      // a launch has fewer than 2^32 threads, up to 1024 of them to a row
   return by_runs(n, [&](auto nv, unsigned threads) {
-    return launch(k_round_rows<T, decltype(nv)::value, G>, dim3((unsigned)rows), threads, 0, st, x, stride, n, last, (uint8_t*)q, (float*)scales);
+    hipError_t e = hipSuccess;
+    for (long long r = 0; r < rows && e == hipSuccess; r += MOST)
+      e = launch(k_round_rows<T, decltype(nv)::value, G>, dim3((unsigned)(rows - r < MOST ? rows - r : MOST)), threads, 0, st, x, stride, r, n, last, (uint8_t*)q, (float*)scales);
+    return e;
   });
 }
 hipError_t launch_round(const void* x, int dtype, long long stride, long long rows, int n, void* q, void* scales, hipStream_t st) {
@@ -441,10 +445,7 @@ int htr_quantize_int8(const void* x, int64_t stride, int64_t rows, int n, int dt
   if (rows == 0) return HTR_OK;
   if (!x || !q || !scales) return HTR_ERR_NULL;
   if (!aligned(x, element_bytes(dtype)) || !aligned(q, 8) || !aligned(scales, 4)) return HTR_ERR_ALIGN;
-  constexpr int64_t MOST = 1 << 21;
-  for (int64_t r = 0; r < rows; r += MOST)
-    TRY_HIP(launch_round((const uint8_t*)x + r * stride * (int64_t)element_bytes(dtype), dtype, stride, rows - r < MOST ? rows - r : MOST, n, (uint8_t*)q + r * n,
-                         (float*)scales + r, (hipStream_t)stream));
+  TRY_HIP(launch_round(x, dtype, stride, rows, n, q, scales, (hipStream_t)stream));
   return HTR_OK;
 }
 
