@@ -108,3 +108,21 @@ def test_groups_of_which_one_expert_is_left(gen, E, groups, top_groups, dtype, s
         check(logits, top, bias=bias, **how)
     logits[::2, E - 1] = math.nan
     check(logits, top, bias=bias, **how)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scores,with_bias", KINDS)
+@pytest.mark.parametrize("E,groups,top_groups,top", [(1023, 3, 2, 12), (1020, 5, 3, 8), (990, 33, 9, 8), (1023, 33, 4, 64), (1022, 2, 1, 64), (256, 2, 1, 8), (512, 2, 1, 17), (512, 2, 2, 8),
+                                                     (260, 2, 1, 5), (1000, 5, 1, 33), (70, 35, 8, 10)])
+@pytest.mark.parametrize("group_best", [1, 2])
+def test_groups_of_many_lanes_and_of_one(gen, E, groups, top_groups, top, scores, with_bias, group_best):
+    """Up to 31 experts to a lane; groups of 32 lanes, of 16 and of one; ranks next to each other, where 64 bits decide."""
+    bias = randn(gen, E, scale=0.1) if with_bias else None
+    how = dict(scores=scores, bias=bias, groups=groups, top_groups=top_groups, group_best=group_best)
+    for logits in (randn(gen, 9, E, scale=2), randn(gen, 5, E, dtype=BF16), torch.randint(0, 4, (5, E), device="cuda", generator=gen).to(F16)):
+        check(logits, top, **how)
+    logits[1, 7] = math.inf
+    check(logits, top, **how)
+    # sigmoid(x) = 1/2 + x / 4 and a bias of 1/4: a quarter of float32's step at 3/4 from one to the next
+    near = 2.0 ** -24 * torch.argsort(torch.rand(6, E, device="cuda", generator=gen), -1)
+    check(near, top, **dict(how, bias=None if bias is None else torch.full((E,), 0.25, device="cuda")))
