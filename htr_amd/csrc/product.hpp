@@ -136,11 +136,16 @@ __device__ __forceinline__ float silu(float g) { return g / (1.f + __expf(-g)); 
 // latency of two loads and the sum.
 // X: the type of x; 16-bit rows with an e4m3 matrix are rounded on the way, by every workgroup for itself: about 110 instructions to a slab, beside
 // its 2 KB or more of the matrix, against a launch ahead of this one.  WIDE: e4m3 products in float32 sums.
-template <int T, int X, int R, int TT, int STREAM_WAVES, bool WIDE>
+// TAIL: rows end inside their last slab, at a multiple of 16 bytes.  Others have no test of where a row ends (us in bf16, with it and without: 12 rows of 3 experts of 4096x1408
+// 11.9 and 9.4, of 1024x4096 9.5 and 8.8, 4 rows on 4096x4096 10.1 and 9.2; 12 of 3 of 4096x8192 46.7 and 47.3, of 54 sizes the only one that was slower).  With a tail, whole
+// slabs in a form of their own cost 16 rows in 16 bits more than the test does (1 row on 4096x7600, both forms and one: 17.4 and 16.8; 8 of 8 experts of 1024x4104 17.7 and
+// 17.4, 12 of 3 of 4096x4104 27.3 and 27.9), and 32, or int8, less (128 of 4 of 512x4104 15.6 and 17.4; in int8 48 rows on 2048x4112 8.4 and 9.4, 48 of 8 of 1024x24592
+// 58.7 and 60.5).
+template <int T, int X, int R, int TT, int STREAM_WAVES, bool WIDE, bool TAIL>
 __global__ __launch_bounds__(STREAM_WAVES * 64) void k_product_stream(const ProductArgs a) {
   constexpr int P = R + TT <= 3 && !(X != T && STREAM_WAVES > 8) ? 4 : 2;      // slabs in flight
   constexpr bool ROUNDS = X != T;
-  static_assert((!ROUNDS && !WIDE) || T == P_F8, "");
+  static_assert(((!ROUNDS && !WIDE) || T == P_F8) && !(TAIL && T == P_F8), "");
   typedef typename SumOf<T>::type Sum;
   typedef typename SumOf<T>::one One;
   __shared__ One red[STREAM_WAVES][R * TT * 256];
@@ -210,10 +215,10 @@ __global__ __launch_bounds__(STREAM_WAVES * 64) void k_product_stream(const Prod
       for (int t = 0; t < TT; ++t) if constexpr (!ROUNDS) sx[p][t] = sp[t][slab];
     }
   };
-  // other than e4m3 rows may end inside the last slab, at a multiple of 16 bytes
-  const int whole_slabs = (int)(row_bytes >> 7);
   auto load = [&](int p, int slab) {
-    if (T == P_F8 || slab < whole_slabs) load_slab(p, slab, std::true_type());
+    if constexpr (!TAIL) load_slab(p, slab, std::true_type());
+    else if constexpr (TT == 1 && T != P_I8) load_slab(p, slab, std::false_type());
+    else if (((size_t)slab << 7) + 128 <= row_bytes) load_slab(p, slab, std::true_type());
     else load_slab(p, slab, std::false_type());
   };
   // a row's 128 columns lie in the four lanes c, c + 16, c + 32, c + 48

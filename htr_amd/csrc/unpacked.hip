@@ -146,11 +146,14 @@ template <int T, typename K> TileGrid tile_grid(const ProductArgs& a) {
 template <int T, int R, int TT, int WAVES> hipError_t launch_kernel(Stream<R, TT, WAVES>, const ProductArgs& a, hipStream_t st) {
   const dim3 grid((a.m + 16 * R - 1) / (16 * R), (unsigned)span_bound(a.rows, a.experts, a.ends != nullptr, 16 * TT));
   if constexpr (T == P_F8 && TT == 1) {
-    if (a.wide) return launch(a.x_type == HTR_BF16 ? k_product_stream<T, HTR_BF16, R, TT, WAVES, true> : k_product_stream<T, HTR_F16, R, TT, WAVES, true>, grid, WAVES * 64, 0, st, a);
-    if (a.x_type == HTR_BF16) return launch(k_product_stream<T, HTR_BF16, R, TT, WAVES, false>, grid, WAVES * 64, 0, st, a);
-    if (a.x_type == HTR_F16) return launch(k_product_stream<T, HTR_F16, R, TT, WAVES, false>, grid, WAVES * 64, 0, st, a);
+    if (a.wide) return launch(a.x_type == HTR_BF16 ? k_product_stream<T, HTR_BF16, R, TT, WAVES, true, false> : k_product_stream<T, HTR_F16, R, TT, WAVES, true, false>, grid, WAVES * 64, 0, st, a);
+    if (a.x_type == HTR_BF16) return launch(k_product_stream<T, HTR_BF16, R, TT, WAVES, false, false>, grid, WAVES * 64, 0, st, a);
+    if (a.x_type == HTR_F16) return launch(k_product_stream<T, HTR_F16, R, TT, WAVES, false, false>, grid, WAVES * 64, 0, st, a);
   }
-  return launch(k_product_stream<T, T, R, TT, WAVES, false>, grid, WAVES * 64, 0, st, a);
+  if constexpr (T != P_F8) {
+    if ((size_t)a.n * bytes_of<T> % 128 != 0) return launch(k_product_stream<T, T, R, TT, WAVES, false, true>, grid, WAVES * 64, 0, st, a);
+  }
+  return launch(k_product_stream<T, T, R, TT, WAVES, false, false>, grid, WAVES * 64, 0, st, a);
 }
 template <int T, int WM, int WN, int AT, int BT, int NS, bool GATED> hipError_t launch_kernel(Tiles<WM, WN, AT, BT, NS, GATED> k, const ProductArgs& a, hipStream_t st) {
   constexpr size_t LDS = decltype(k)::template LDS<T>;
@@ -237,7 +240,7 @@ template <int T, typename F> auto product_kernel(const ProductArgs& a, F take) {
   }
   // Matrices so small that each compute unit has a workgroup of 16 of their rows by 16 or 32 of x at most: many waves for each are faster than a ring for few.
   // Measured from HBM on 17 .. 384 rows of 256 .. 4096 matrix rows of 1024, 4096 and 8192 columns, 108 sizes in each type: the way taken was the fastest in all.
-  // us by 16 rows, by 32, by tiles of 64x32: 64 rows on 1024x4096 in 16 bits 10.6, 14.7, 20.8, in e4m3 7.2, 9.8, 11.9; 48 rows on 2048x4096 19.5, 15.0, 21.0 and
+  // us by 16 rows, by 32, by tiles of 64x32: 64 rows on 1024x4096 in 16 bits 10.3, 14.7, 20.8, in e4m3 7.2, 9.8, 11.9; 48 rows on 2048x4096 19.5, 13.8, 21.0 and
   // 11.8, 9.9, 11.9; beyond the limits 192 rows on 1024x4096 26.1, 26.2, 20.7 and 16.1, 18.6, 11.8, 64 rows on 4096x4096 38, 30, 22 and 21.6, 19.4, 12.6.
   auto workgroups = [&](int height) {
     const float full = (float)a.rows / height, experts = (float)(a.rows < a.experts ? a.rows : a.experts);
@@ -250,7 +253,7 @@ template <int T, typename F> auto product_kernel(const ProductArgs& a, F take) {
     if (mean <= 32) return a.m < 8192 ? take(Stream<1, 2, 8>{}) : a.m < 16384 ? take(Tiles<2, 2, 2, 1, 4>{}) : take(Tiles<4, 1, 2, 2, 4>{});
   } else if (mean <= 24) {
     // experts' rows are uneven: where 16 rows to a workgroup leave two to a compute unit they are still ahead of tiles of 128x32 (us, 192 rows of 8 experts of
-    // 512x4096 in e4m3 12.1 and 16.8, in 16 bits 19.6 and 26.7; of 512x768 4.4 and 6.1, 5.9 and 8.4; 1056 rows of 48 of 72x3200 in 16 bits 20.1 and 19.4)
+    // 512x4096 in e4m3 12.1 and 16.8, in 16 bits 18.3 and 26.7; of 512x768 4.4 and 6.1, 5.9 and 8.4; 1056 rows of 48 of 72x3200 in 16 bits 20.1 and 19.4)
     return y_fits && workgroups(16) <= 512.f ? take(Stream<1, 1, 8>{}) : take(Tiles<4, 1, 2, 2, 4>{});
   }
   switch (T == P_F8 || T == P_I8 ? best_tile(TILES_8, a, (size_t)a.n) : best_tile(TILES_16, a, (size_t)a.n * 2)) {
