@@ -2,7 +2,8 @@
 //
 //   k_expert_order    pairs (token, slot) sorted by expert, in their own order within one: ends of the experts, token of each position, position of
 //                     each pair
-//   product           silu(gate) * up of every pair, in the activations' type or in e4m3 (few pairs: gate and up in float32, then k_gated)
+//   product           silu(gate) * up of every pair, in the activations' type or in e4m3 (few pairs: gate and up in float32, then k_gated); for int8 in float32, which
+//                     k_round_rows rounds by row (few pairs: gate and up, then both by k_round_rows)
 //   product           down, float32
 //   k_weighted_sum    y_t = sum_j w_tj out(t, j), j ascending
 //

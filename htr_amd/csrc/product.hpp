@@ -15,7 +15,7 @@ template <> struct SumOf<P_I8> { typedef i4 type; typedef int one; };
 typedef int i8v __attribute__((ext_vector_type(8)));
 
 struct ProductArgs {
-  const void* x;                         // [.][n]; e4m3 matrices: also 16-bit rows, where takes_16bit_rows says so
+  const void* x;                         // [.][n]; also rows that the product rounds itself: 16 bits with e4m3 matrices (takes_16bit_rows), floating ones with an int8 one (rounds_rows)
   const float* xs;                       // e4m3 rows: [.][n / 128]; int8: [.]
   const void* w;                         // [experts][m][n]
   const float* ws;                       // e4m3: [experts][ceil(m / 128)][n / 128]; int8: [experts][m]
@@ -306,7 +306,7 @@ __global__ __launch_bounds__(STREAM_WAVES * 64) void k_product_stream(const Prod
 // hidden columns; y [rows][m / 2] is silu(gate) up, in 16 bits, in float32 (int8: a row's scale is not known before its last column, and values rounded to 16 bits before would
 // fall on another integer here and there, 0.8 % of the result's norm) or in e4m3 (then TM / 2 = 128 columns share a scale); rows behind the last expert's are left.
 // int8: the sums stay in the matrix unit's registers over all slabs, and the scales meet them at a tile's end, from LDS: 8192 rows on 14336x4096 392 to 412 us (2.33 to 2.45
-// POP/s, the library's 8192^3 product 2.36), 465 with scales loaded where they are used; 24576 rows of 64 experts of 2816x2048 110; 333 rows on 6144x4096 22.
+// POP/s, the library's 8192^3 product 2.36), 465 with scales loaded where they are used; 24576 rows of 64 experts of 2048x1408 110; 333 rows on 6144x4096 22.
 __device__ __forceinline__ int swizzle_w(int r) { return ((r >> 1) & 1) | ((r >> 3 & 3) << 1); }
 __device__ __forceinline__ int swizzle_x(int r) { return (r >> 1) & 7; }
 constexpr int TILE_XCDS = 8, TOGETHER = 8;

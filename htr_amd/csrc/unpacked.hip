@@ -309,7 +309,7 @@ hipError_t launch_rows(const ProductArgs& a, hipStream_t st) {
                            : launch_rows<P_I8, 4, 8, false>(a, g, st);
 }
 // Up to 32 rows of one matrix that LDS holds.  us by k_product_rows and by the faster of the kernels for more rows: 1 row on 1024x4096 4.9 and 5.3, on 6144x4096 7.7 and
-// 10.1, 8 on 152064x4096 101 and 125, 16 on 14336x4096 14.0 and 15.8, 32 on 28672x4096 25 and 29, on 4096x4096 9.6 and 8.8
+// 10.1, 8 on 152064x4096 101 and 125, 16 on 14336x4096 14.0 and 15.8, 32 on 28672x4096 25 and 29, but 32 on 4096x4096 9.6 and 8.8 (the matrix's height is no part of the rule)
 bool takes_rows(int64_t rows, int n) { return rows >= 1 && rows <= 32 && rows_lds((int)rows, 32, n, 8, false) <= 160 * 1024; }
 // Up to 8 of them rounded on the way, by every workgroup for itself: 1 row on 6144x4096 9.5 us, 8 rows 11.3 (rounded ahead 7.7 and 8.5, and 4.5 for that launch), 16 rows
 // on 14336x4096 19.2 (14.0 and 4.6)
@@ -319,7 +319,8 @@ bool rounds_rows(int64_t rows, int n) { return rows <= 8 && takes_rows(rows, n);
 bool few_int8(long long rows, int experts) { return rows <= 8ll * experts; }
 // the kernel for few rows, for a product in int8
 bool takes_rows(const ProductArgs& a) { return a.ends == nullptr ? takes_rows(a.rows, a.n) : few_int8(a.rows, a.experts) && rows_grid(a).fits; }
-// silu(gate) up of rows by expert, where one launch is the better way (few rows to an expert: the matrices are read by k_product_stream, k_gated follows)
+// silu(gate) up of rows by expert, where one launch is the better way (few rows to an expert: the matrices are read by k_product_stream, in int8 by k_product_rows, and
+// k_gated or k_round_rows follows)
 bool gates_in_one(long long rows, int experts, int type) { return type == HTR_I8 ? !few_int8(rows, experts) : !takes_16bit_rows(rows, experts, true); }
 template <int T, typename F> auto gated_kernel(const ProductArgs& a, F take) {
   switch (best_tile(GATED_TILES, a, (size_t)a.n * bytes_of<T>)) {

@@ -359,10 +359,11 @@ int htr_product(const void* x, int x_type, const void* x_scales, const void* w, 
                 int64_t rows, int m, int n, int experts, int type, int y_dtype, void* stream);
 /* 1 where htr_product takes 16-bit rows with e4m3 matrices and rounds them on the way (few rows), otherwise 0: htr_quantize_e4m3 first.  grouped: ends is given. */
 int htr_product_rounds(int64_t rows, int experts, int grouped);
-/* 1 where htr_product takes floating rows with one int8 matrix (ends NULL) and rounds them on the way (few rows, n up to some thousand), otherwise 0. */
+/* 1 where htr_product takes floating rows with one int8 matrix (ends NULL) and rounds them on the way, otherwise 0: up to 8 rows that a compute unit's LDS holds in int8 (one
+ * row of any n, 8 of n up to 16384). */
 int htr_product_rounds_int8(int64_t rows, int n);
 /* The kernel behind htr_product for these sizes, or (gated = 1, with grouped = 1) behind the first product of htr_moe_stacked, where gate and up are
- * one launch: m = 2 inter, more than 4 rows to an expert on average, HTR_ERR_SIZE otherwise.  out6 = {matrix rows of a tile, rows of x of a tile, waves of a workgroup,
+ * one launch: m = 2 inter, more than 4 rows to an expert on average (int8: more than 8), HTR_ERR_SIZE otherwise.  out6 = {matrix rows of a tile, rows of x of a tile, waves of a workgroup,
  * stages of its ring in LDS (0: straight from memory), workgroups, tiles (grouped: at most)}.  Where there are fewer workgroups than tiles they go on from
  * tile to tile.  For tests and tuning. */
 int htr_product_plan(int64_t rows, int m, int n, int experts, int grouped, int gated, int type, int x_type, int* out6);
